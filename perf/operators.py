@@ -115,6 +115,7 @@ def draw(rng):
             c["top"] = rng.choice((0, 0, 1, 5, 20, 32)) if rows <= 512 else 0
         return c
     width = _size(rng, 64, 8192)
+    vocab = min(vocab, (1 << 29) // width)
     tokens = _log(rng, 1, min(65536, (1 << 27) // width))
     c = {"op": op, "tokens": tokens, "width": width, "vocab": vocab, "dtype": dtype,
          "scale": rng.choice((1.0, 1.0, math.sqrt(width))), "wide_ids": rng.random() < 0.5}
