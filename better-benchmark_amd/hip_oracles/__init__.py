@@ -83,6 +83,23 @@ _SIGNATURES = {
     "hipo_batchnorm_train_fwd_f32_noalloc": (
         ctypes.c_int,
         [_c_ptr] * 8 + [_c_i64, _c_i64, _c_i64, _c_f32, _c_f32, ctypes.c_int, _c_ptr]),
+    "hipo_token_logprobs_workspace_bytes": (ctypes.c_size_t, [_c_i64] * 3),
+    "hipo_token_logprobs": (
+        ctypes.c_int,
+        [_c_ptr, ctypes.c_int, _c_ptr, ctypes.c_int] + [_c_ptr] * 5 + [_c_i64] * 3
+        + [_c_f32, _c_i64, _c_i64, _c_ptr, ctypes.c_size_t, _c_ptr]),
+    "hipo_token_logprobs_bwd": (
+        ctypes.c_int,
+        [_c_ptr, _c_ptr, ctypes.c_int, _c_ptr, ctypes.c_int] + [_c_ptr] * 5 + [_c_i64] * 4
+        + [_c_f32, _c_i64, _c_ptr]),
+    "hipo_embedding": (
+        ctypes.c_int,
+        [_c_ptr, ctypes.c_int, _c_ptr, ctypes.c_int, _c_ptr] + [_c_i64] * 4 + [_c_f32, _c_ptr]),
+    "hipo_embedding_bwd_workspace_bytes": (ctypes.c_size_t, [_c_i64] * 3),
+    "hipo_embedding_bwd": (
+        ctypes.c_int,
+        [_c_ptr, ctypes.c_int, _c_ptr, ctypes.c_int, _c_ptr, ctypes.c_int] + [_c_i64] * 3
+        + [_c_f32, _c_i64, ctypes.c_int, _c_ptr, ctypes.c_size_t, _c_ptr]),
 }
 
 _lib = None
@@ -657,6 +674,166 @@ def batchnorm_nchw_act_mean(x, gamma, beta, running_mean, running_var, *, moment
     return save_mean, save_rstd, out
 
 
+_FLOATS = (torch.bfloat16, torch.float32)
+
+
+def _require_tokens(what: str, tokens: torch.Tensor) -> None:
+    _require(tokens.dtype in (torch.int32, torch.int64) and tokens.is_contiguous(),
+             f"{what}: tokens must be contiguous int32 or int64")
+
+
+def _require_logits(what: str, logits: torch.Tensor, tokens: torch.Tensor,
+                    scale: float) -> tuple[int, int, int]:
+    _require(logits.dtype in _FLOATS and logits.dim() == 2,
+             f"{what}: logits must be 2-D bf16 or fp32")
+    rows, vocab = logits.shape
+    _require_tokens(what, tokens)
+    _require(tokens.shape == (rows,), f"{what}: tokens must be [rows]")
+    _require(0.0 < scale < float("inf"), f"{what}: scale must be positive and finite")
+    _require(logits.stride(1) == 1 or vocab <= 1, f"{what}: logits need a unit inner stride")
+    stride = logits.stride(0) if rows > 1 else vocab
+    _require(stride >= vocab, f"{what}: rows of logits overlap")
+    return rows, vocab, stride
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, scale: float = 1.0,
+                   ignore_index: int = -100, entropy: bool = False, top: int = 0):
+    """Log probabilities of tokens [R] (int32 or int64) under softmax(scale *
+    logits, -1), logits [R, V] bf16 or fp32 with any row stride >= V, in fp32.
+
+    Returns (logprob [R], lse [R]), then the distribution's entropy [R] with
+    entropy=True, then with top=k (at most 64) the k most probable tokens'
+    log probabilities [R, k] and ids [R, k] (int64; of equal logits the lower
+    id first, NaN above all).  A row whose token is ignore_index is not read:
+    its results are 0, its alternatives -inf and -1.  Any other token outside
+    [0, V) has log probability NaN.  A row with nothing above -inf has lse
+    -inf, with +inf lse +inf, with NaN lse NaN; there logprob = scale * logit -
+    lse, and the entropy is NaN."""
+    lib = _lib or load_library()
+    dev = _require_rocm(logits, tokens)
+    rows, vocab, stride = _require_logits("token_logprobs", logits, tokens, scale)
+    _require(0 <= top <= 64 and top <= vocab,
+             "token_logprobs: top must be at most 64 and at most the vocabulary")
+    _require(vocab > 0 or rows == 0, "token_logprobs: empty vocabulary")
+    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
+    lse = torch.empty(rows, dtype=torch.float32, device=dev)
+    out = [logprob, lse]
+    ptrs = [None, None, None]
+    if entropy:
+        out.append(torch.empty(rows, dtype=torch.float32, device=dev))
+        ptrs[0] = _ptr(out[-1])
+    if top:
+        out.append(torch.empty((rows, top), dtype=torch.float32, device=dev))
+        out.append(torch.empty((rows, top), dtype=torch.int64, device=dev))
+        ptrs[1:] = _ptr(out[-2]), _ptr(out[-1])
+    need = int(lib.hipo_token_logprobs_workspace_bytes(rows, vocab, top))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _call(lib.hipo_token_logprobs, "token_logprobs", dev, _ptr(logits), logits.element_size(),
+          _ptr(tokens), tokens.element_size(), _ptr(logprob), _ptr(lse), *ptrs, rows, vocab,
+          stride, float(scale), int(ignore_index), int(top), None if ws is None else _ptr(ws),
+          need)
+    return tuple(out)
+
+
+def token_logprobs_bwd(grad: torch.Tensor, logits: torch.Tensor, tokens: torch.Tensor,
+                       lse: torch.Tensor, *, scale: float = 1.0, ignore_index: int = -100,
+                       entropy: torch.Tensor | None = None,
+                       grad_entropy: torch.Tensor | None = None,
+                       grad_lse: torch.Tensor | None = None,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of token_logprobs with respect to the logits, [R, V] of their
+    type: grad, grad_entropy and grad_lse (fp32 [R]) are the gradients of its
+    logprob, entropy and lse; lse, and entropy where grad_entropy is given,
+    are its results.  Rows of ignore_index are zero, rows of another token
+    outside [0, V) NaN.  out: where the result goes, the logits themselves or
+    memory that does not overlap them (any row stride >= V)."""
+    lib = _lib or load_library()
+    rows_of = [t for t in (grad, lse, entropy, grad_entropy, grad_lse) if t is not None]
+    dev = _require_rocm(logits, tokens, *rows_of, *(() if out is None else (out,)))
+    what = "token_logprobs_bwd"
+    rows, vocab, stride = _require_logits(what, logits, tokens, scale)
+    for t in rows_of:
+        _require(t.dtype == torch.float32 and t.shape == (rows,) and t.is_contiguous(),
+                 f"{what}: grad, lse, entropy, grad_entropy and grad_lse must be contiguous "
+                 f"fp32 [rows]")
+    _require(grad_entropy is None or entropy is not None,
+             f"{what}: grad_entropy needs the entropy")
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
+    _require(out.dtype == logits.dtype and out.shape == logits.shape
+             and (out.stride(1) == 1 or vocab <= 1), f"{what}: out must match the logits")
+    out_stride = out.stride(0) if rows > 1 else vocab
+    _require(out_stride >= vocab, f"{what}: rows of out overlap")
+    _require(out.data_ptr() != logits.data_ptr() or out_stride == stride,
+             f"{what}: out and logits overlap")
+    _call(lib.hipo_token_logprobs_bwd, what, dev, _ptr(grad), _ptr(logits),
+          logits.element_size(), _ptr(tokens), tokens.element_size(), _ptr(lse),
+          *(None if t is None else _ptr(t) for t in (entropy, grad_entropy, grad_lse)),
+          _ptr(out), rows, vocab, stride, out_stride, float(scale), int(ignore_index))
+    return out
+
+
+def embedding(weight: torch.Tensor, tokens: torch.Tensor, *, scale: float = 1.0) -> torch.Tensor:
+    """scale * weight[tokens] for weight [V, D] bf16 or fp32 (any row stride >=
+    D) and int32 or int64 tokens of any shape -> [*tokens.shape, D], one fp32
+    product and one rounding per value.  A token outside [0, V) gives a row of
+    NaN."""
+    lib = _lib or load_library()
+    dev = _require_rocm(weight, tokens)
+    _require(weight.dtype in _FLOATS and weight.dim() == 2,
+             "embedding: weight must be 2-D bf16 or fp32")
+    _require_tokens("embedding", tokens)
+    vocab, width = weight.shape
+    _require(weight.stride(1) == 1 or width <= 1, "embedding: weight needs a unit inner stride")
+    stride = weight.stride(0) if vocab > 1 else width
+    _require(stride >= width, "embedding: rows of weight overlap")
+    out = torch.empty((*tokens.shape, width), dtype=weight.dtype, device=dev)
+    _call(lib.hipo_embedding, "embedding", dev, _ptr(weight), weight.element_size(),
+          _ptr(tokens), tokens.element_size(), _ptr(out), tokens.numel(), width, vocab, stride,
+          float(scale))
+    return out
+
+
+def embedding_bwd(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, scale: float = 1.0,
+                  padding_idx: int | None = None, dtype: torch.dtype | None = None,
+                  into: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of embedding with respect to its weight, [vocab, D]: scale times
+    the sum of the rows of grad [*tokens.shape, D] (contiguous, bf16 or fp32)
+    of each token, in fp32 in a fixed order (the same call gives the same
+    bits), rounded once to dtype (default: grad's).  Tokens equal to
+    padding_idx, and tokens outside [0, vocab), add nothing.  into: a
+    contiguous bf16 or fp32 [vocab, D] that the gradient is added to (before
+    the one rounding) and that is returned; its rows without tokens are not
+    touched."""
+    lib = _lib or load_library()
+    dev = _require_rocm(grad, tokens, *(() if into is None else (into,)))
+    _require(grad.dtype in _FLOATS and grad.dim() >= 1 and grad.is_contiguous(),
+             "embedding_bwd: grad must be contiguous bf16 or fp32")
+    _require_tokens("embedding_bwd", tokens)
+    _require(grad.shape[:-1] == tokens.shape, "embedding_bwd: grad must be [*tokens.shape, D]")
+    _require(vocab >= 0, "embedding_bwd: negative vocabulary")
+    _require(padding_idx is None or 0 <= padding_idx < vocab,
+             "embedding_bwd: padding_idx must be in [0, vocab)")
+    width = grad.shape[-1]
+    if into is None:
+        dtype = grad.dtype if dtype is None else dtype
+        _require(dtype in _FLOATS, "embedding_bwd: dtype must be bf16 or fp32")
+        out = torch.empty((vocab, width), dtype=dtype, device=dev)
+    else:
+        _require(dtype is None or dtype == into.dtype,
+                 "embedding_bwd: dtype and into's type differ")
+        _require(into.dtype in _FLOATS and into.shape == (vocab, width) and into.is_contiguous(),
+                 "embedding_bwd: into must be contiguous bf16 or fp32 [vocab, D]")
+        out = into
+    need = int(lib.hipo_embedding_bwd_workspace_bytes(tokens.numel(), width, vocab))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _call(lib.hipo_embedding_bwd, "embedding_bwd", dev, _ptr(grad), grad.element_size(),
+          _ptr(tokens), tokens.element_size(), _ptr(out), out.element_size(), tokens.numel(),
+          width, vocab, float(scale), -1 if padding_idx is None else int(padding_idx),
+          0 if into is None else 1, None if ws is None else _ptr(ws), need)
+    return out
+
+
 def _error_word(ws: torch.Tensor) -> torch.Tensor:
     raw = ws.view(torch.uint8) if ws.dtype != torch.uint8 else ws
     return raw[BN_ERROR_WORD_OFFSET:BN_ERROR_WORD_OFFSET + 4].view(torch.int32)
@@ -733,4 +910,5 @@ __all__ = [
     "flat_copy2",
     "hold_copy",
     "gelu_erf_bwd_colsum",
+    "token_logprobs", "token_logprobs_bwd", "embedding", "embedding_bwd",
 ]

@@ -40,6 +40,8 @@ SOURCES = [
     "gelu_flat.hip",
     "transpose.hip",
     "gelu_bwd.hip",
+    "token_logprobs.hip",
+    "embedding.hip",
 ]
 
 # Packed-FP32 VALU forms are disabled for all device code (the compiler

@@ -437,6 +437,97 @@ int hipo_gelu_erf_bwd_colsum_bf16(const uint16_t* grad, const uint16_t* x, uint1
                                   void* workspace, size_t workspace_bytes,
                                   hipStream_t stream);
 
+/*
+ * Log probabilities of given tokens.  With s_j = scale * x[r, j]:
+ *   lse[r]     = ln sum_j e^(s_j)
+ *   logprob[r] = s_t - lse[r],  t = tokens[r]
+ *   entropy[r] = -sum_j p_j ln p_j,  p_j = e^(s_j - lse)   (0 where p_j = 0)
+ *   top_token[r, 0:top], top_logprob[r, 0:top]: the `top` largest logits of
+ *                the row in falling order (of equal ones the lower index
+ *                first; NaN above all) and their s - lse
+ * in fp32 (one pass over the row).  logits is [rows, vocab] with row stride
+ * `row_stride` (>= vocab), of bf16 (elem_size 2) or fp32 (4), at any element
+ * alignment; tokens is [rows] of int32 (token_size 4) or int64 (8); the
+ * outputs are contiguous.  entropy may be NULL; top is at most 64 and at
+ * most vocab, its outputs NULL where it is 0; scale is positive and finite.
+ * A row whose token is ignore_index is not read: 0, 0, 0, and for the
+ * alternatives -inf and -1.  A token outside [0, vocab) otherwise has
+ * logprob NaN.  A row with nothing above -inf has lse -inf, one with +inf
+ * lse +inf, one with NaN lse NaN; their logprobs are s - lse, their entropy
+ * NaN.  `workspace`: at least hipo_token_logprobs_workspace_bytes bytes,
+ * 16-byte aligned, no initialisation needed (NULL when that is 0); calls
+ * that share one must be ordered.
+ * No counterpart among the reference's oracles; beside
+ * hipo_scaled_masked_softmax_bf16 as the softmax of a whole vocabulary.
+ */
+size_t hipo_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t top);
+int hipo_token_logprobs(const void* logits, int elem_size, const void* tokens,
+                        int token_size, float* logprob, float* lse, float* entropy,
+                        float* top_logprob, int64_t* top_token, int64_t rows,
+                        int64_t vocab, int64_t row_stride, float scale,
+                        int64_t ignore_index, int64_t top, void* workspace,
+                        size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Gradient of hipo_token_logprobs with respect to the logits, for the
+ * gradients grad of logprob, grad_entropy of entropy and grad_lse of lse
+ * (each fp32 [rows]; the latter two may be NULL):
+ *   dx[r, j] = scale * (grad [j = t]
+ *              + p_j (grad_lse - grad - grad_entropy (ln p_j + entropy)))
+ * fp32 arithmetic, one rounding to the logits' type.  lse, and entropy (with
+ * grad_entropy), are the forward's results.  logits and dlogits are [rows,
+ * vocab] with row strides of their own; dlogits may be logits itself (one
+ * stride), and does not overlap it otherwise.  Rows of ignore_index are
+ * zero and not read; rows of another token outside [0, vocab) are NaN.
+ * No counterpart among the reference's oracles; beside
+ * hipo_gelu_erf_bwd_colsum_bf16 as a training gradient.
+ */
+int hipo_token_logprobs_bwd(const float* grad, const void* logits, int elem_size,
+                            const void* tokens, int token_size, const float* lse,
+                            const float* entropy, const float* grad_entropy,
+                            const float* grad_lse, void* dlogits, int64_t rows,
+                            int64_t vocab, int64_t row_stride,
+                            int64_t dlogits_row_stride, float scale,
+                            int64_t ignore_index, hipStream_t stream);
+
+/*
+ * Embedding lookup with a scale:
+ *   out[i, :] = scale * weight[tokens[i], :]   (fp32 product, one rounding)
+ * weight is [vocab, width] with row stride `row_stride` (>= width), of bf16
+ * (elem_size 2) or fp32 (4), out [count, width] contiguous of the same type,
+ * both at any element alignment; tokens is [count] of int32 (token_size 4)
+ * or int64 (8).  A token outside [0, vocab) gives a row of NaN.
+ * No counterpart among the reference's oracles; the input of the
+ * residual-RMSNorm and LayerNorm families.
+ */
+int hipo_embedding(const void* weight, int elem_size, const void* tokens,
+                   int token_size, void* out, int64_t count, int64_t width,
+                   int64_t vocab, int64_t row_stride, float scale,
+                   hipStream_t stream);
+
+/*
+ * Gradient of hipo_embedding with respect to the weight:
+ *   dweight[v, :] = scale * sum_{i: tokens[i] = v} grad[i, :]
+ * in fp32, in an order that the tokens alone fix (the same call gives the
+ * same bits), rounded once.  Every row of dweight is written, zeros where no
+ * token is; with accumulate != 0 the sum is added to what dweight holds
+ * (before the rounding) and rows without tokens are not touched.  Tokens
+ * equal to padding_idx, and tokens outside [0, vocab), add nothing (an index
+ * outside [0, vocab): no padding).  grad is contiguous [count, width] of bf16
+ * (elem_size 2) or fp32 (4), dweight contiguous [vocab, width] of bf16
+ * (out_size 2) or fp32 (4).  `workspace`: at least
+ * hipo_embedding_bwd_workspace_bytes bytes, 16-byte aligned, no
+ * initialisation needed (NULL when that is 0); calls that share one must be
+ * ordered.
+ * No counterpart among the reference's oracles.
+ */
+size_t hipo_embedding_bwd_workspace_bytes(int64_t count, int64_t width, int64_t vocab);
+int hipo_embedding_bwd(const void* grad, int elem_size, const void* tokens,
+                       int token_size, void* dweight, int out_size, int64_t count,
+                       int64_t width, int64_t vocab, float scale,
+                       int64_t padding_idx, int accumulate, void* workspace,
+                       size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif
