@@ -15,12 +15,13 @@
 //      workgroups, no atomics on memory, and the scan is a small part of
 //      reading the gradient rows (8 bytes of a token from the L2 against
 //      hundreds to thousands).
-//   2. sum_pieces: tokens that occur more than kPiece times are cut into
-//      pieces of kPiece positions, each summed on its own (fp32, into the
-//      workspace).
-//   3. write_rows: a lane per piece of columns of a row of dw: the sum of its
-//      few positions, or of its pieces, or zeros.  Adding into dw only visits
-//      rows that have a token.
+//   2. sum_rows: a lane per 16 bytes of a gradient row's columns and row of dw:
+//      the sum of its few positions.  Where there are fewer tokens than rows
+//      it visits the rows that have one, and the others are zeroed by
+//      workgroups of the first launch, beside the sort.  Tokens that occur
+//      more than kPiece times are cut into pieces of kPiece positions, summed
+//      in the same launch into the workspace (fp32);
+//   3. join_pieces: their rows, the sums of their pieces.
 #include <math.h>
 
 #include <algorithm>
@@ -34,14 +35,14 @@ constexpr int kThreads = 256;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / kWave;
 constexpr int kSortLoads = 8;        // tokens per thread in flight
+constexpr int kSortList = 512;       // tokens a sorting wave keeps
 constexpr int kSortRows = 512;       // rows of dw per sorting workgroup
 constexpr int kSortRowBits = 9;
+constexpr int64_t kSortPart = int64_t{1} << (32 - kSortRowBits);  // positions a list can tell
 constexpr int kSortGroups = 256;     // at least: one workgroup per CU
-constexpr int kPiece = 64;           // positions per piece of a frequent token
+constexpr int kPiece = 32;           // positions per piece of a frequent token
+constexpr int kFillStores = 1;       // 16-byte stores of zeros per thread
 constexpr int64_t kLanes = int64_t{1} << 30;  // lanes per launch
-
-typedef uint16_t u16x4_t __attribute__((ext_vector_type(4)));
-typedef uint16_t u16x8_t __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ int64_t token_at(const void* tokens, int size, int64_t i) {
   return size == 8 ? static_cast<const int64_t*>(tokens)[i]
@@ -53,9 +54,12 @@ template <typename T, int C>
 struct Values {
   typedef T Vec __attribute__((ext_vector_type(C)));
   typedef Vec Unaligned __attribute__((aligned(sizeof(T))));
-  static_assert(sizeof(Vec) <= 16 && (sizeof(Vec) & (sizeof(Vec) - 1)) == 0, "one access");
   Vec v;
 
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] = T{0};
+  }
   __device__ __forceinline__ void load(const T* p) {
     v = *reinterpret_cast<const Unaligned*>(p);
   }
@@ -129,56 +133,120 @@ __global__ __launch_bounds__(kThreads) void embedding_rows(FwdArgs a) {
   else x.store_part(out, left);
 }
 
-// Where a row's positions are in the sorted order.
+// A token's places in the sorted order.
 struct Segment {
   int start, count;
 };
 struct Place {
   int position, row;
+  Segment token;  // all places of this row
 };
 
 struct SortArgs {
   const void* tokens;
-  Segment* segments;  // [vocab]
+  Segment* segments;  // [vocab], or null
   Place* order;       // [count]
   int* total;         // tokens that count
+  uint16_t* fill;     // zeroed by the workgroups after the sorting ones
+  int64_t fill_values;
   int64_t count, vocab, padding_idx;
-  int token_size, group_bits;  // 2^group_bits workgroups
+  int group_bits;     // 2^group_bits sorting workgroups
 };
 
+// Zeros, kFillStores 16-byte stores per thread.
+__device__ __forceinline__ void fill_zeros(const SortArgs& a, int64_t block) {
+  Values<uint16_t, 8> zero;
+  zero.clear();
+#pragma unroll
+  for (int u = 0; u < kFillStores; ++u) {
+    const int64_t at = ((block * kFillStores + u) * kSortThreads + threadIdx.x) * 8;
+    if (at + 8 <= a.fill_values) zero.store_stream(a.fill + at);
+    else if (at < a.fill_values) zero.store_part(a.fill + at, static_cast<int>(a.fill_values - at));
+  }
+}
+
+// kSortLoads tokens of a lane, 64 positions apart; past the end the last one.
+template <typename I>
+__device__ __forceinline__ void load_tokens(const SortArgs& a, int64_t at, I (&v)[kSortLoads]) {
+  const I* p = static_cast<const I*>(a.tokens);
+#pragma unroll
+  for (int u = 0; u < kSortLoads; ++u)
+    v[u] = p[at + u * kWave < a.count ? at + u * kWave : a.count - 1];
+}
+
+// A wave's next places of the rows, one row per lane (-1: none), lanes in
+// order: stable.
+__device__ __forceinline__ int take_places(int r, int* next, bool& last) {
+  uint64_t same = __ballot(r >= 0);
+#pragma unroll
+  for (int b = 0; b < kSortRowBits; ++b) {
+    const uint64_t m = __ballot((r >> b) & 1);
+    same &= ((r >> b) & 1) ? m : ~m;
+  }
+  const int rank = __popcll(same & ((uint64_t{1} << (threadIdx.x & (kWave - 1))) - 1));
+  const int place = r >= 0 ? next[r] + rank : 0;
+  last = r >= 0 && rank + 1 == __popcll(same);
+  return place;
+}
+
+// The waves of a workgroup take consecutive parts of the tokens, in order, so
+// that each has its own counts and places and none waits for another but
+// between the count and the places.  A wave keeps what it finds in a list in
+// LDS; one that finds more than the list holds reads its part again.
+template <typename I>
 __global__ __launch_bounds__(kSortThreads) void sort_tokens(SortArgs a) {
-  __shared__ int next[kSortRows];                          // count, then next place
-  __shared__ unsigned short seen[kSortWaves][kSortRows];   // a batch's counts per wave
-  __shared__ int wave_sum_[kSortWaves];
+  __shared__ int found[kSortWaves][kSortRows];  // counts, then next places
+  __shared__ Segment token[kSortRows];
+  __shared__ uint32_t list[kSortWaves][kSortList];  // place in the part, row
+  __shared__ int wave_count[kSortWaves];
   __shared__ int wave_below[kSortWaves];
-  __shared__ int found[kSortLoads * kSortWaves];
-  __shared__ int list_row[kSortLoads * kSortThreads];
-  __shared__ int list_pos[kSortLoads * kSortThreads];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6;
   const int groups = 1 << a.group_bits;
   const int mine = blockIdx.x;
-  for (int i = tid; i < kSortRows; i += kSortThreads) next[i] = 0;
-  for (int i = tid; i < kSortWaves * kSortRows; i += kSortThreads) (&seen[0][0])[i] = 0;
+  if (mine >= groups) {
+    fill_zeros(a, mine - groups);
+    return;
+  }
+  const int64_t part = (a.count + kSortThreads - 1) / kSortThreads * kWave;  // of a wave
+  const int64_t from = wave * part;
+  const int64_t to = from + part < a.count ? from + part : a.count;
+  I v[kSortLoads];
+  if (from < to) load_tokens(a, from + lane, v);
+  for (int i = tid; i < kSortWaves * kSortRows / 4; i += kSortThreads)
+    reinterpret_cast<u32x4_t*>(&found[0][0])[i] = u32x4_t{0u, 0u, 0u, 0u};
   __syncthreads();
 
-  // -1: does not count.
-  const auto row_of = [&](int64_t i) -> int64_t {
-    if (i >= a.count) return -1;
-    const int64_t v = token_at(a.tokens, a.token_size, i);
-    return v >= 0 && v < a.vocab && v != a.padding_idx ? v : -1;
+  const auto own_row = [&](I x, int64_t at) -> int {
+    const int64_t t = x;
+    return at < to && t >= 0 && t < a.vocab && t != a.padding_idx &&
+                   static_cast<int>(t & (groups - 1)) == mine
+               ? static_cast<int>(t >> a.group_bits)
+               : -1;
   };
 
-  int below = 0;
-  for (int64_t i0 = 0; i0 < a.count; i0 += kSortLoads * kSortThreads) {
-    int64_t v[kSortLoads];
+  int below = 0, held = 0;
+  for (int64_t i0 = from; i0 < to; i0 += kSortLoads * kWave) {
+    I now[kSortLoads];
 #pragma unroll
-    for (int u = 0; u < kSortLoads; ++u) v[u] = row_of(i0 + u * kSortThreads + tid);
+    for (int u = 0; u < kSortLoads; ++u) now[u] = v[u];
+    if (i0 + kSortLoads * kWave < to) load_tokens(a, i0 + kSortLoads * kWave + lane, v);
+    __builtin_amdgcn_sched_barrier(0);  // the next loads first
 #pragma unroll
     for (int u = 0; u < kSortLoads; ++u) {
-      if (v[u] < 0) continue;
-      const int g = static_cast<int>(v[u] & (groups - 1));
-      below += g < mine;
-      if (g == mine) atomicAdd(&next[v[u] >> a.group_bits], 1);
+      const int64_t at = i0 + u * kWave + lane;
+      const int64_t t = now[u];
+      below += at < to && t >= 0 && t < a.vocab && t != a.padding_idx &&
+               static_cast<int>(t & (groups - 1)) < mine;
+      const int r = own_row(now[u], at);
+      const uint64_t m = __ballot(r >= 0);
+      if (m == 0) continue;
+      const int slot = held + __popcll(m & ((uint64_t{1} << lane) - 1));
+      if (r >= 0) {
+        atomicAdd(&found[wave][r], 1);
+        if (slot < kSortList)
+          list[wave][slot] = static_cast<uint32_t>(at - from) << kSortRowBits | r;
+      }
+      held += __popcll(m);
     }
   }
 #pragma unroll
@@ -186,89 +254,73 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens(SortArgs a) {
   if (lane == 0) wave_below[wave] = below;
   __syncthreads();
 
-  // Exclusive sums of the counts, one row per thread.
-  const int n = tid < kSortRows ? next[tid] : 0;
+  // Exclusive sums over the rows, one row per thread, then over the waves.
+  int n = 0;
+  if (tid < kSortRows) {
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) n += found[w][tid];
+  }
   int sum = n;
 #pragma unroll
   for (int d = 1; d < kWave; d *= 2) {
     const int up = __shfl_up(sum, d);
     if (lane >= d) sum += up;
   }
-  if (lane == kWave - 1) wave_sum_[wave] = sum;
+  if (lane == kWave - 1) wave_count[wave] = sum;
   __syncthreads();
   int start = sum - n;
+#pragma unroll
   for (int w = 0; w < kSortWaves; ++w) {
     start += wave_below[w];
-    if (w < wave) start += wave_sum_[w];
+    if (w < wave) start += wave_count[w];
   }
   if (tid < kSortRows) {
-    next[tid] = start;
+    const Segment g{start, n};
+    token[tid] = g;
+    int next = start;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      const int c = found[w][tid];
+      found[w][tid] = next;
+      next += c;
+    }
     const int64_t row = (static_cast<int64_t>(tid) << a.group_bits) + mine;
-    if (row < a.vocab) a.segments[row] = Segment{start, n};
+    if (a.segments != nullptr && row < a.vocab) a.segments[row] = g;
     if (mine == groups - 1 && tid == kSortRows - 1) *a.total = start + n;
   }
   __syncthreads();
 
-  for (int64_t i0 = 0; i0 < a.count; i0 += kSortLoads * kSortThreads) {
-    // This batch's tokens, in order of position, into the list.
-    int row[kSortLoads], before[kSortLoads];
-#pragma unroll
-    for (int u = 0; u < kSortLoads; ++u) {
-      const int64_t v = row_of(i0 + u * kSortThreads + tid);
-      row[u] = v >= 0 && (v & (groups - 1)) == mine ? static_cast<int>(v >> a.group_bits) : -1;
+  const auto write = [&](int r, int64_t at) {
+    bool last;
+    const int place = take_places(r, found[wave], last);
+    if (r >= 0) {
+      a.order[place] = Place{static_cast<int>(at), (r << a.group_bits) + mine, token[r]};
+      if (last) found[wave][r] = place + 1;
     }
-#pragma unroll
-    for (int u = 0; u < kSortLoads; ++u) {
-      const uint64_t m = __ballot(row[u] >= 0);
-      before[u] = __popcll(m & ((uint64_t{1} << lane) - 1));
-      if (lane == 0) found[u * kSortWaves + wave] = __popcll(m);
+    __builtin_amdgcn_wave_barrier();  // the wave's other lanes read it next
+  };
+  if (held <= kSortList && part <= kSortPart) {
+    for (int l0 = 0; l0 < held; l0 += kWave) {
+      const bool in = l0 + lane < held;
+      const uint32_t e = in ? list[wave][l0 + lane] : 0;
+      write(in ? static_cast<int>(e & (kSortRows - 1)) : -1, from + (e >> kSortRowBits));
     }
-    __syncthreads();
-    int total = 0;
-    {
-      int at[kSortLoads];
+  } else {
+    load_tokens(a, from + lane, v);
+    for (int64_t i0 = from; i0 < to; i0 += kSortLoads * kWave) {
+      I now[kSortLoads];
 #pragma unroll
+      for (int u = 0; u < kSortLoads; ++u) now[u] = v[u];
+      if (i0 + kSortLoads * kWave < to) load_tokens(a, i0 + kSortLoads * kWave + lane, v);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
       for (int u = 0; u < kSortLoads; ++u) {
-        for (int w = 0; w < kSortWaves; ++w) {
-          if (w == wave) at[u] = total;
-          total += found[u * kSortWaves + w];
-        }
-      }
+        const int64_t at = i0 + u * kWave + lane;
+        I x = now[0];  // now[u], kept in registers
 #pragma unroll
-      for (int u = 0; u < kSortLoads; ++u) {
-        if (row[u] < 0) continue;
-        list_row[at[u] + before[u]] = row[u];
-        list_pos[at[u] + before[u]] = static_cast<int>(i0) + u * kSortThreads + tid;
+        for (int k = 1; k < kSortLoads; ++k) x = u == k ? now[k] : x;
+        write(own_row(x, at), at);
       }
-    }
-    __syncthreads();
-    // Places: after what came before in the tokens, the waves before in this
-    // round of 1024, and the lanes before with the same row.
-    for (int l0 = 0; l0 < total; l0 += kSortThreads) {
-      const int i = l0 + tid;
-      const bool in = i < total;
-      const int r = in ? list_row[i] : -1;
-      uint64_t same = __ballot(in);
-#pragma unroll
-      for (int b = 0; b < kSortRowBits; ++b) {
-        const uint64_t m = __ballot((r >> b) & 1);
-        same &= ((r >> b) & 1) ? m : ~m;
-      }
-      const int rank = __popcll(same & ((uint64_t{1} << lane) - 1));
-      const bool last = in && rank + 1 == __popcll(same);
-      if (last) seen[wave][r] = static_cast<unsigned short>(rank + 1);
-      __syncthreads();
-      if (in) {
-        int at = next[r] + rank;
-        for (int w = 0; w < wave; ++w) at += seen[w][r];
-        a.order[at] = Place{list_pos[i], (r << a.group_bits) + mine};
-      }
-      __syncthreads();
-      if (last) {
-        atomicAdd(&next[r], rank + 1);
-        seen[wave][r] = 0;
-      }
-      __syncthreads();
     }
   }
 }
@@ -279,8 +331,9 @@ struct BwdArgs {
   const Segment* segments;
   const Place* order;
   const int* total;
-  float* sums;  // [2 * bins][width], see sum_pieces
-  int64_t first, count;  // rows of dw, places or pieces of this launch
+  float* sums;           // [2 * bins][width], see first_piece
+  int64_t first, count;  // slots of this launch
+  int64_t places;        // in order, of which *total are filled
   int64_t bins;          // of kPiece places
   DivMagic by_pieces;
   int width, pieces;     // pieces of C columns per row
@@ -288,121 +341,81 @@ struct BwdArgs {
 };
 
 // sum[c] += grad[position][col + c] over order[from, to), in order, with
-// eight rows' loads in flight.
-template <typename T, int C, bool WHOLE>
+// FLIGHT rows' loads in flight.
+template <typename T, int C, bool WHOLE, int FLIGHT>
 __device__ __forceinline__ void add_rows(float (&sum)[C], const BwdArgs& a, int from, int to,
                                          int col) {
-  constexpr int kFlight = 8;
   const T* grad = static_cast<const T*>(a.grad) + col;
   const int left = a.width - col;
-  for (int i0 = from; i0 < to; i0 += kFlight) {
-    int64_t at[kFlight];
-    Values<T, C> x[kFlight];
+  for (int i0 = from; i0 < to; i0 += FLIGHT) {
+    // The barriers: or the compiler waits for each load before it issues the
+    // next.  No load where there is no row: most tokens occur once or twice.
+    int at[FLIGHT];
+    Values<T, C> x[FLIGHT];
 #pragma unroll
-    for (int k = 0; k < kFlight; ++k)
-      at[k] = static_cast<int64_t>(a.order[i0 + k < to ? i0 + k : to - 1].position) * a.width;
-#pragma unroll
-    for (int k = 0; k < kFlight; ++k) {
-      if (WHOLE || left >= C) x[k].load_stream(grad + at[k]);
-      else x[k].load_part(grad + at[k], left);
+    for (int k = 0; k < FLIGHT; ++k) {
+      at[k] = 0;
+      if (i0 + k < to) at[k] = a.order[i0 + k].position;
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int k = 0; k < kFlight; ++k) {
+    for (int k = 0; k < FLIGHT; ++k) {
+      x[k].clear();
+      if (i0 + k < to) {
+        const T* p = grad + static_cast<int64_t>(at[k]) * a.width;
+        if (WHOLE || left >= C) x[k].load_stream(p);
+        else x[k].load_part(p, left);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int c = 0; c < C; ++c) sum[c] += i0 + k < to ? x[k].get(c) : 0.0f;
+    for (int k = 0; k < FLIGHT; ++k) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) sum[c] += x[k].get(c);
     }
   }
 }
 
-// The sum of each piece of kPiece positions of a token with more than that.
-// Pieces are counted from the token's first place s, and the sorted places are
-// cut into bins of kPiece: a bin holds the start of at most one piece after a
-// token's first (kept in sums[bin]) and of at most one first piece (in
-// sums[bins + bin]; its token reaches into the next bin).
-template <typename T, int C, bool WHOLE>
-__global__ __launch_bounds__(kThreads) void sum_pieces(BwdArgs a) {
-  const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
-  const uint32_t slot = div_by(id, a.by_pieces);
-  if (slot >= a.count) return;
-  const int col = static_cast<int>(id - slot * a.pieces) * C;
-  const int64_t s = a.first + slot;
-  const bool first = s >= a.bins;
-  const int bin = static_cast<int>(first ? s - a.bins : s);
+// Tokens with more than kPiece places are summed in pieces of kPiece places,
+// counted from the token's first place.  The sorted places are cut into bins
+// of kPiece: a bin holds the start of at most one piece after a token's first
+// (its sum is kept in sums[bin]) and of at most one first piece (in sums[bins +
+// bin]; its token reaches into the next bin).  The token of a bin's first
+// piece, count 0 if there is none:
+__device__ __forceinline__ Segment first_piece(const BwdArgs& a, int bin) {
+  const int64_t probe = (int64_t{bin} + 1) * kPiece;
   const int total = *a.total;
-  const int64_t probe = (static_cast<int64_t>(bin) + (first ? 1 : 0)) * kPiece;
-  if (probe >= total) return;
-  const Segment g = a.segments[a.order[probe].row];
-  if (g.count <= kPiece) return;
-  int from;
-  if (first) {
-    if (g.start < bin * kPiece || g.start >= probe) return;
+  const Segment g = a.order[probe < a.places ? probe : a.places - 1].token;
+  const bool here = probe < total && g.count > kPiece && g.start >= bin * kPiece &&
+                    g.start < probe;
+  return here ? g : Segment{0, 0};
+}
+
+// The places of slot's piece, from == to if there is none.
+__device__ __forceinline__ void piece_places(const BwdArgs& a, int64_t slot, int& from, int& to) {
+  from = to = 0;
+  Segment g;
+  if (slot >= a.bins) {
+    g = first_piece(a, static_cast<int>(slot - a.bins));
+    if (g.count == 0) return;
     from = g.start;
   } else {
-    from = g.start + (static_cast<int>(probe) - g.start + kPiece - 1) / kPiece * kPiece;
-    if (from == g.start || from >= g.start + g.count) return;
+    const int64_t probe = slot * kPiece;
+    const int total = *a.total;
+    g = a.order[probe].token;
+    if (probe >= total || g.count <= kPiece) return;
+    const int at = g.start + (static_cast<int>(probe) - g.start + kPiece - 1) / kPiece * kPiece;
+    if (at == g.start || at >= g.start + g.count) return;
+    from = at;
   }
-  float sum[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) sum[c] = 0.0f;
-  add_rows<T, C, WHOLE>(sum, a, from, std::min(from + kPiece, g.start + g.count), col);
-  float* to = a.sums + s * a.width + col;
-  Values<float, 4> v;
-#pragma unroll
-  for (int c = 0; c < C; c += 4) {
-    const float part[4] = {sum[c], sum[c + 1], sum[c + 2], sum[c + 3]};
-    v.set(part);
-    const int left = a.width - col - c;
-    if (WHOLE || left >= 4) v.store(to + c);
-    else if (left > 0) v.store_part(to + c, left);
-  }
+  to = std::min(from + kPiece, g.start + g.count);
 }
 
-// ADD: rows are those of the places that start a token, added to dw; otherwise
-// rows of dw, written.
-template <typename T, typename O, int C, bool WHOLE, bool ADD>
-__global__ __launch_bounds__(kThreads) void write_rows(BwdArgs a) {
-  const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
-  const uint32_t r = div_by(id, a.by_pieces);
-  if (r >= a.count) return;
-  const int col = static_cast<int>(id - r * a.pieces) * C;
-  int64_t row = a.first + r;
-  if constexpr (ADD) {
-    const int64_t place = row;
-    if (place >= *a.total) return;
-    row = a.order[place].row;
-    if (a.segments[row].start != place) return;
-  }
-  const Segment g = a.segments[row];
-  float sum[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) sum[c] = 0.0f;
-  const int left = a.width - col;
-  if (g.count <= kPiece) {
-    add_rows<T, C, WHOLE>(sum, a, g.start, g.start + g.count, col);
-  } else {
-    constexpr int kFlight = 8;
-    const int n = (g.count + kPiece - 1) / kPiece;
-    for (int j0 = 0; j0 < n; j0 += kFlight) {
-      Values<float, 4> x[kFlight][C / 4];
-#pragma unroll
-      for (int k = 0; k < kFlight; ++k) {
-        const int j = j0 + k < n ? j0 + k : n - 1;
-        const int64_t slot = (j == 0 ? a.bins : 0) + (g.start + j * kPiece) / kPiece;
-        const float* p = a.sums + slot * a.width + col;
-#pragma unroll
-        for (int c = 0; c < C; c += 4) {
-          if (WHOLE || left >= c + 4) x[k][c / 4].load(p + c);
-          else x[k][c / 4].load_part(p + c, left - c);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < kFlight; ++k) {
-#pragma unroll
-        for (int c = 0; c < C; ++c) sum[c] += j0 + k < n ? x[k][c / 4].get(c % 4) : 0.0f;
-      }
-    }
-  }
+template <typename O, int C, bool WHOLE, bool ADD>
+__device__ __forceinline__ void write_row(const BwdArgs& a, int64_t row, int col,
+                                          float (&sum)[C]) {
   O* dw = static_cast<O*>(a.dw) + row * a.width + col;
+  const int left = a.width - col;
   Values<O, C> v;
   if constexpr (ADD) {
     if (WHOLE || left >= C) v.load(dw);
@@ -413,6 +426,95 @@ __global__ __launch_bounds__(kThreads) void write_rows(BwdArgs a) {
   v.set(sum);
   if (WHOLE || left >= C) v.store_stream(dw);
   else v.store_part(dw, left);
+}
+
+// A lane per C columns of a piece (the first 2 * bins slots) or of a row of
+// dw.  PLACES: the rows of the places that start a token (those without one
+// are zeros already, or stay); otherwise every row.  Rows of tokens in pieces
+// are left to join_pieces.  ADD: added to dw.
+template <typename T, typename O, int C, bool WHOLE, bool PLACES, bool ADD>
+__global__ __launch_bounds__(kThreads) void sum_rows(BwdArgs a) {
+  const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
+  const uint32_t r = div_by(id, a.by_pieces);
+  if (r >= a.count) return;
+  const int col = static_cast<int>(id - r * a.pieces) * C;
+  const int left = a.width - col;
+  const int64_t slot = a.first + r;
+  int64_t row = slot - 2 * a.bins;
+  int from, to;
+  float sum[C] = {};
+  if (row < 0) {
+    piece_places(a, slot, from, to);
+    if (from == to) return;
+  } else if constexpr (PLACES) {
+    const int total = *a.total;
+    // One load for all of it, beside the total's.
+    const Place p = __builtin_bit_cast(Place, *reinterpret_cast<const u32x4_t*>(a.order + row));
+    if (row >= total || p.token.start != row || p.token.count > kPiece) return;
+    from = p.token.start + 1;
+    to = p.token.start + p.token.count;
+    row = p.row;
+    // Its first position is in hand.
+    const T* grad = static_cast<const T*>(a.grad) + int64_t{p.position} * a.width + col;
+    Values<T, C> x;
+    if (WHOLE || left >= C) x.load_stream(grad);
+    else x.load_part(grad, left);
+#pragma unroll
+    for (int c = 0; c < C; ++c) sum[c] += x.get(c);
+  } else {
+    const Segment g = a.segments[row];
+    if (g.count > kPiece) return;
+    from = g.start;
+    to = g.start + g.count;
+  }
+  add_rows<T, C, WHOLE, 8>(sum, a, from, to, col);
+  if (row >= 0) {
+    write_row<O, C, WHOLE, ADD>(a, row, col, sum);
+  } else {
+    float* p = a.sums + slot * a.width + col;
+    Values<float, C> v;
+    v.set(sum);
+    if (WHOLE || left >= C) v.store(p);
+    else v.store_part(p, left);
+  }
+}
+
+// The rows of tokens in pieces: a lane per C columns and bin.
+template <typename O, int C, bool WHOLE, bool ADD>
+__global__ __launch_bounds__(kThreads) void join_pieces(BwdArgs a) {
+  constexpr int kFlight = 8;
+  const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
+  const uint32_t r = div_by(id, a.by_pieces);
+  if (r >= a.count) return;
+  const int col = static_cast<int>(id - r * a.pieces) * C;
+  const int left = a.width - col;
+  const int bin = static_cast<int>(a.first + r);
+  const Segment g = first_piece(a, bin);
+  if (g.count == 0) return;
+  const int row = a.order[g.start].row;
+  const float* sums = a.sums + col;
+  const int n = (g.count + kPiece - 1) / kPiece;
+  float sum[C] = {};
+  for (int j0 = 0; j0 < n; j0 += kFlight) {
+    Values<float, C> x[kFlight];
+#pragma unroll
+    for (int k = 0; k < kFlight; ++k) {
+      x[k].clear();
+      const int j = j0 + k;
+      if (j < n) {
+        const float* p = sums + ((j == 0 ? a.bins : 0) + int64_t{bin} + j) * a.width;
+        if (WHOLE || left >= C) x[k].load(p);
+        else x[k].load_part(p, left);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int k = 0; k < kFlight; ++k) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) sum[c] += x[k].get(c);
+    }
+  }
+  write_row<O, C, WHOLE, ADD>(a, row, col, sum);
 }
 
 // Workspace: the order, the rows' segments, the number of places, the sums of
@@ -434,7 +536,7 @@ inline Layout layout(int64_t count, int64_t width, int64_t vocab) {
   return l;
 }
 
-// LAUNCH(first, count, blocks) over `rows` rows of `pieces` lanes each.
+// launch(first, count, blocks) over `rows` rows of `pieces` lanes each.
 template <typename F>
 void for_lanes(int64_t rows, int64_t pieces, F&& launch) {
   const int64_t step = std::max<int64_t>(1, kLanes / pieces);
@@ -445,28 +547,49 @@ void for_lanes(int64_t rows, int64_t pieces, F&& launch) {
 }
 
 template <typename T, typename O>
-void launch_bwd(BwdArgs a, const SortArgs& s, bool accumulate, hipStream_t stream) {
-  constexpr int C = 16 / std::max(sizeof(T), sizeof(O));
+void launch_bwd(BwdArgs a, SortArgs s, int token_size, bool accumulate, hipStream_t stream) {
+  constexpr int C = 16 / sizeof(T);
   const bool whole = a.width % C == 0;
   a.pieces = (a.width + C - 1) / C;
   a.by_pieces = div_magic(a.pieces);
-  if (s.count > 0 || !accumulate) {
-    sort_tokens<<<dim3(1u << s.group_bits), dim3(kSortThreads), 0, stream>>>(s);
+  const bool fill = !accumulate && s.count < s.vocab;
+  const bool places = accumulate || fill;
+  int64_t fill_blocks = 0;
+  if (fill) {
+    constexpr int64_t kPerBlock = int64_t{kSortThreads} * kFillStores * 8;
+    s.fill = static_cast<uint16_t*>(a.dw);
+    s.fill_values = s.vocab * a.width * static_cast<int64_t>(sizeof(O) / 2);
+    fill_blocks = (s.fill_values + kPerBlock - 1) / kPerBlock;
   }
-  const auto run = [&](auto kernel, int64_t rows) {
-    for_lanes(rows, a.pieces, [&](int64_t first, int64_t n, dim3 grid) {
+  if (places) s.segments = nullptr;
+  if (s.count > 0 || fill) {
+    auto kernel = token_size == 8 ? sort_tokens<int64_t> : sort_tokens<int32_t>;
+    kernel<<<dim3(static_cast<unsigned>((int64_t{1} << s.group_bits) + fill_blocks)),
+             dim3(kSortThreads), 0, stream>>>(s);
+  }
+  const auto run = [&](auto kernel, int64_t slots) {
+    for_lanes(slots, a.pieces, [&](int64_t first, int64_t n, dim3 grid) {
       a.first = first;
       a.count = n;
       kernel<<<grid, dim3(kThreads), 0, stream>>>(a);
     });
   };
-  if (s.count > kPiece) {
-    run(whole ? sum_pieces<T, C, true> : sum_pieces<T, C, false>, 2 * a.bins);
+  a.places = s.count;
+  if (s.count <= kPiece) a.bins = 0;
+  if (accumulate) {
+    run(whole ? sum_rows<T, O, C, true, true, true> : sum_rows<T, O, C, false, true, true>,
+        2 * a.bins + s.count);
+  } else if (fill) {
+    run(whole ? sum_rows<T, O, C, true, true, false> : sum_rows<T, O, C, false, true, false>,
+        2 * a.bins + s.count);
+  } else {
+    run(whole ? sum_rows<T, O, C, true, false, false> : sum_rows<T, O, C, false, false, false>,
+        2 * a.bins + s.vocab);
   }
   if (accumulate) {
-    run(whole ? write_rows<T, O, C, true, true> : write_rows<T, O, C, false, true>, s.count);
+    run(whole ? join_pieces<O, C, true, true> : join_pieces<O, C, false, true>, a.bins);
   } else {
-    run(whole ? write_rows<T, O, C, true, false> : write_rows<T, O, C, false, false>, s.vocab);
+    run(whole ? join_pieces<O, C, true, false> : join_pieces<O, C, false, false>, a.bins);
   }
 }
 
@@ -544,17 +667,17 @@ extern "C" int hipo_embedding_bwd(const void* grad, int elem_size, const void* t
   a.width = static_cast<int>(width);
   a.scale = scale;
   SortArgs s{tokens, reinterpret_cast<Segment*>(ws + l.segments), reinterpret_cast<Place*>(ws),
-             reinterpret_cast<int*>(ws + l.total), count, vocab, padding_idx, token_size, 0};
+             reinterpret_cast<int*>(ws + l.total), nullptr, 0, count, vocab, padding_idx, 0};
   while ((int64_t{1} << s.group_bits) < kSortGroups ||
          (int64_t{kSortRows} << s.group_bits) < vocab) {
     ++s.group_bits;
   }
   if (elem_size == 2) {
-    if (out_size == 2) launch_bwd<uint16_t, uint16_t>(a, s, accumulate != 0, stream);
-    else launch_bwd<uint16_t, float>(a, s, accumulate != 0, stream);
+    if (out_size == 2) launch_bwd<uint16_t, uint16_t>(a, s, token_size, accumulate != 0, stream);
+    else launch_bwd<uint16_t, float>(a, s, token_size, accumulate != 0, stream);
   } else {
-    if (out_size == 2) launch_bwd<float, uint16_t>(a, s, accumulate != 0, stream);
-    else launch_bwd<float, float>(a, s, accumulate != 0, stream);
+    if (out_size == 2) launch_bwd<float, uint16_t>(a, s, token_size, accumulate != 0, stream);
+    else launch_bwd<float, float>(a, s, token_size, accumulate != 0, stream);
   }
   return check_launch("embedding_bwd");
 }
