@@ -689,7 +689,7 @@ def _require_logits(what: str, logits: torch.Tensor, tokens: torch.Tensor,
     rows, vocab = logits.shape
     _require_tokens(what, tokens)
     _require(tokens.shape == (rows,), f"{what}: tokens must be [rows]")
-    _require(0.0 < scale < float("inf"), f"{what}: scale must be positive and finite")
+    _require(2.0 ** -100 <= scale <= 2.0 ** 100, f"{what}: scale must be from 2^-100 to 2^100")
     _require(logits.stride(1) == 1 or vocab <= 1, f"{what}: logits need a unit inner stride")
     stride = logits.stride(0) if rows > 1 else vocab
     _require(stride >= vocab, f"{what}: rows of logits overlap")

@@ -7,12 +7,23 @@
 //   dx_j = scale * (g [j = t] + p_j (g_lse - g - g_H (ln p_j + H))),
 //   p_j = e^(s_j - lse),  p_j ln p_j = 0 where p_j = 0.
 //
-// The maximum and the two sums are kept while the row streams by (a running
-// maximum; the sums are rescaled when it rises), so a row is read once.
-// (s_j - m) is formed as scale * (x_j - m): the type's lowest value in every
-// place, a row masked by it, then is a row of equal logits and not an
-// overflow.
+// Forward: HBM-bound, the row is read once.  Each lane keeps a running
+// maximum and the two sums relative to it (rescaled when it rises, once per
+// 32 values); lanes, waves and slices of a row are then joined by the same
+// rescaling.  A workgroup takes a row, or a slice of one where there are too
+// few rows to fill the chip, whose parts a second launch joins.
+//
+// The alternatives cost nothing while the row streams by: the lanes' maxima
+// say where the largest values are.  The k-th largest of 64 groups' maxima is
+// a lower bound of the k-th largest value, few values reach it, and they lie
+// in lanes whose maximum does: only these lanes' values are read again (k = 20
+// of 64 groups: about 24 lanes of 256).
+//
+// Backward: HBM-bound, one pass, a value's gradient needs its logit and a few
+// numbers of its row.
 #include <math.h>
+
+#include <algorithm>
 
 #include "hipo_common.h"
 
@@ -20,67 +31,151 @@ namespace hipo {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kFlight = 4;         // 16-byte loads per lane in flight
 constexpr int kMaxTop = 64;
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kMaxSlices = 64;     // of a row
+constexpr int kCandidates = 1024;  // values that a slice can rank at once
+constexpr int64_t kMaxVocab = 0x7fffffff - 4096;
+constexpr int64_t kMaxBlocks = 1 << 23;  // of a launch
+constexpr int64_t kFill = 1024;    // workgroups that fill the chip
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kInf = __builtin_inff();
+constexpr float kHuge = 0x1p100f;
 
+// C consecutive logits in 16 bytes.
 template <typename T>
-__device__ __forceinline__ float to_f32(T v);
-template <>
-__device__ __forceinline__ float to_f32<uint16_t>(uint16_t v) {
-  return bf16_to_f32(v);
+struct Logits {
+  static constexpr int C = 16 / sizeof(T);
+  typedef T Vec __attribute__((ext_vector_type(C)));
+  typedef Vec Unaligned __attribute__((aligned(sizeof(T))));
+};
+
+__device__ __forceinline__ float to_f32(uint16_t v) { return bf16_to_f32(v); }
+__device__ __forceinline__ float to_f32(float v) { return v; }
+
+__device__ __forceinline__ void unpack(u32x4_t v, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = bf16lo(v[i]);
+    x[2 * i + 1] = bf16hi(v[i]);
+  }
 }
-template <>
-__device__ __forceinline__ float to_f32<float>(float v) {
-  return v;
+__device__ __forceinline__ void unpack(u32x4_t v, float (&x)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(v[i]);
 }
 
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ uint16_t from_f32<uint16_t>(float v) {
-  return static_cast<uint16_t>(pack_bf16x2(v, 0.0f) & 0xffffu);
+__device__ __forceinline__ u32x4_t pack(const float (&x)[8]) {
+  return u32x4_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                 pack_bf16x2(x[6], x[7])};
 }
-template <>
-__device__ __forceinline__ float from_f32<float>(float v) {
-  return v;
+__device__ __forceinline__ u32x4_t pack(const float (&x)[4]) {
+  return u32x4_t{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+                 __float_as_uint(x[3])};
 }
 
-// The running maximum of x with Z = sum 2^u and U = sum 2^u u over
-// u = c (x - m), c = scale log2(e).
+__device__ __forceinline__ float maximum(float a, float b) {
+  return __builtin_elementwise_maximum(a, b);
+}
+
+__device__ __forceinline__ int64_t token_at(const void* tokens, int size, int64_t i) {
+  return size == 8 ? static_cast<const int64_t*>(tokens)[i]
+                   : static_cast<const int32_t*>(tokens)[i];
+}
+
+// ---------------------------------------------------------------------------
+// Statistics: the maximum m of x, Z = sum 2^w and U = sum 2^w w over
+// w = c x - round(c m), c = scale log2(e), one FMA per value.  Against a row
+// maximum whose c m is not below 2^100 (the type's lowest value in every
+// place: a row masked by it) values are equal to it or vanish, and w is not
+// formed.  m = -inf: nothing yet.
+// ---------------------------------------------------------------------------
+
 struct Stats {
   float m, z, u;
 };
 
-// u of one value; the clamp keeps 2^u u from being 0 * inf (2^-200 is 0).
-__device__ __forceinline__ float exponent(float x, float m, float c) {
-  return __builtin_elementwise_maximum((x - m) * c, -200.0f);
+// -round(c m); 0 for -inf, so that w of -inf is -inf.
+__device__ __forceinline__ float offset(float m, float c) { return m == -kInf ? 0.0f : -(m * c); }
+
+__device__ __forceinline__ bool is_huge(float o) { return !(fabsf(o) < kHuge); }  // NaN too
+
+// 2^w w without 0 * inf (2^-200 is 0).
+__device__ __forceinline__ float weighted(float e, float w) { return e * maximum(w, -200.0f); }
+
+// s relative to the maximum m >= s.m instead.
+__device__ __forceinline__ Stats rescale(Stats s, float m, float c) {
+  const float o = offset(m, c);
+  if (is_huge(o)) return s.m == m ? s : Stats{m, 0.0f, 0.0f};
+  // s.m = -inf: its sums are 0, and 2^d is at most 1.
+  const float d = __builtin_elementwise_minimum(maximum(o - offset(s.m, c), -200.0f), 0.0f);
+  const float f = s.m == m ? 1.0f : __builtin_amdgcn_exp2f(d);
+  return Stats{m, s.z * f, s.m == m ? s.u : f * __builtin_fmaf(d, s.z, s.u)};
 }
 
-__device__ __forceinline__ Stats merge(Stats a, Stats b, float c) {
-  const float m = __builtin_elementwise_maximum(a.m, b.m);
-  // Nothing above -inf on either side, or +inf or NaN on one: finish() needs
-  // the maximum alone.
-  if (!(fabsf(m) < kInf)) return Stats{m, 0.0f, 0.0f};
-  const float ua = exponent(a.m, m, c), ub = exponent(b.m, m, c);
-  const float ea = __builtin_amdgcn_exp2f(ua), eb = __builtin_amdgcn_exp2f(ub);
-  // sum 2^(u + ua) (u + ua) = 2^ua (U + ua Z)
-  return Stats{m, a.z * ea + b.z * eb, ea * (a.u + ua * a.z) + eb * (b.u + ub * b.z)};
+template <int N, bool ENTROPY>
+__device__ __forceinline__ void add_values(Stats& s, const float (&x)[N], float c) {
+  float top = x[0];
+#pragma unroll
+  for (int i = 1; i + 1 < N; i += 2) top = maximum(maximum(top, x[i]), x[i + 1]);
+  if constexpr (N % 2 == 0) top = maximum(top, x[N - 1]);
+  const float m = maximum(s.m, top);
+  const float o = offset(m, c);
+  if (__builtin_expect(__any(is_huge(o)), 0)) {
+    if (is_huge(o)) {
+      s = rescale(s, m, c);
+#pragma unroll
+      for (int i = 0; i < N; ++i) s.z += x[i] == m ? 1.0f : 0.0f;
+      return;
+    }
+  }
+  s = rescale(s, m, c);
+  float z[2] = {0.0f, 0.0f}, u[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float w = __builtin_fmaf(x[i], c, o);
+    const float e = __builtin_amdgcn_exp2f(w);
+    z[i & 1] += e;
+    if constexpr (ENTROPY) u[i & 1] += weighted(e, w);
+  }
+  s.z += z[0] + z[1];
+  if constexpr (ENTROPY) s.u += u[0] + u[1];
 }
 
-// What a row's statistics say: its lse and entropy, and s - lse of a value.
+// Of all lanes of a wave, and of a workgroup's waves; every lane has it.
+__device__ __forceinline__ Stats join_wave(Stats s, float c) {
+  const float m = wave_maximum(s.m);
+  s = rescale(s, m, c);
+  return Stats{m, wave_sum(s.z), wave_sum(s.u)};
+}
+
+__device__ __forceinline__ Stats join(const Stats* part, int n, float c) {
+  float m = part[0].m;
+  for (int i = 1; i < n; ++i) m = maximum(m, part[i].m);
+  Stats all{m, 0.0f, 0.0f};
+  for (int i = 0; i < n; ++i) {
+    const Stats s = rescale(part[i], m, c);
+    all.z += s.z;
+    all.u += s.u;
+  }
+  return all;
+}
+
 struct Row {
   float m, log_z, lse, entropy;
 };
 
-__device__ __forceinline__ Row finish(Stats s, float scale) {
+__device__ __forceinline__ Row finish(Stats s, float scale, float c) {
   Row r;
   r.m = s.m;
   if (fabsf(s.m) < kInf) {
-    r.log_z = kLn2 * __builtin_amdgcn_logf(s.z);
+    const float o = offset(s.m, c);
+    const float log2_z = __builtin_amdgcn_logf(s.z);
+    // Z is relative to round(c m): what it is off c m by, exactly.
+    r.log_z = kLn2 * (is_huge(o) ? log2_z : log2_z + __builtin_fmaf(-s.m, c, -o));
     r.lse = __builtin_fmaf(scale, s.m, r.log_z);
-    r.entropy = r.log_z - kLn2 * (s.u / s.z);
+    r.entropy = kLn2 * (log2_z - s.u / s.z);
   } else {  // -inf: nothing is left; +inf; NaN
     r.log_z = 0.0f;
     r.lse = s.m;
@@ -89,100 +184,430 @@ __device__ __forceinline__ Row finish(Stats s, float scale) {
   return r;
 }
 
-// In fp64: x - m of the type's lowest and largest value overflows fp32 where
-// their scaled difference need not.
+// s - lse of a value.  In fp64: x - m of the type's lowest and largest value
+// overflows fp32 where their scaled difference need not.
 __device__ __forceinline__ float log_prob(float x, const Row& r, float scale) {
   const double s = scale;
   return static_cast<float>(fabsf(r.m) < kInf ? s * (double{x} - double{r.m}) - double{r.log_z}
                                               : s * double{x} - double{r.lse});
 }
 
-// Order of the alternatives as a whole number: the larger value first (NaN
+// ---------------------------------------------------------------------------
+// Order of the alternatives as whole numbers: the larger value first (NaN
 // above all, -0 with 0), of equal ones the lower index.  0 is no value's.
-__device__ __forceinline__ uint64_t order_key(float x, uint32_t index) {
-  uint32_t b = __float_as_uint(x + 0.0f);
-  b = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-  if (x != x) b = 0xffffffffu;
-  return (static_cast<uint64_t>(b) << 32) | (0xffffffffu - index);
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return x != x ? 0xffffffffu : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t o) {
+  return o == 0xffffffffu ? __builtin_nanf("")
+                          : __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+}
+__device__ __forceinline__ uint64_t order_key(uint32_t order, uint32_t index) {
+  return (static_cast<uint64_t>(order) << 32) | (0xffffffffu - index);
+}
+__device__ __forceinline__ uint32_t key_order(uint64_t key) {
+  return static_cast<uint32_t>(key >> 32);
 }
 __device__ __forceinline__ uint32_t key_index(uint64_t key) {
   return 0xffffffffu - static_cast<uint32_t>(key);
 }
 
-__device__ __forceinline__ int64_t token_at(const void* tokens, int size, int64_t i) {
-  return size == 8 ? static_cast<const int64_t*>(tokens)[i]
-                   : static_cast<const int32_t*>(tokens)[i];
+// The k-th largest of a wave's 64 orders (0 if fewer than k are not 0).
+__device__ __forceinline__ uint32_t kth_of_wave(uint32_t order, int k) {
+  int above = 0;
+#pragma unroll
+  for (int l = 0; l < kWave; ++l)
+    above += static_cast<uint32_t>(__builtin_amdgcn_readlane(order, l)) > order ? 1 : 0;
+  // The smallest of those with fewer than k above.
+  uint32_t v = above < k ? order : 0xffffffffu;
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) v = std::min(v, static_cast<uint32_t>(__shfl_xor(v, d)));
+  return v;
 }
+
+// Writes the k largest of n keys in falling order to sorted (all of a
+// workgroup's threads; keys are distinct, n >= k).
+__device__ __forceinline__ void sort_top(const uint64_t* keys, int n, int k, uint64_t* sorted) {
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const uint64_t key = keys[i];
+    int above = 0;
+    for (int l = 0; l < n; ++l) above += keys[l] > key ? 1 : 0;
+    if (above < k) sorted[above] = key;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Forward
+// ---------------------------------------------------------------------------
 
 struct FwdArgs {
   const void* x;
   const void* tokens;
   float *logprob, *lse, *entropy, *top_logprob;
   int64_t* top_token;
-  int64_t rows, vocab, row_stride, ignore_index;
-  float scale;
-  int token_size, top;
+  Stats* parts;      // [rows][slices]
+  uint64_t* keys;    // [rows][slices][top]
+  int64_t first, vocab, row_stride, ignore_index;
+  float scale, c;
+  int token_size, top, slices, span;  // of span 16-byte vectors
+  DivMagic by_slices;
 };
 
-// A workgroup per row.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void logprobs_rows(FwdArgs a) {
-  __shared__ Stats part[kThreads];
-  __shared__ uint64_t best[kThreads];
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x;
-  const int64_t token = token_at(a.tokens, a.token_size, row);
-  if (token == a.ignore_index) {
-    if (tid == 0) {
-      a.logprob[row] = 0.0f;
-      a.lse[row] = 0.0f;
-      if (a.entropy) a.entropy[row] = 0.0f;
-    }
-    for (int i = tid; i < a.top; i += kThreads) {
-      a.top_logprob[row * a.top + i] = -kInf;
-      a.top_token[row * a.top + i] = -1;
-    }
-    return;
+__device__ __forceinline__ void write_ignored(const FwdArgs& a, int64_t row) {
+  if (threadIdx.x == 0) {
+    a.logprob[row] = 0.0f;
+    a.lse[row] = 0.0f;
+    if (a.entropy) a.entropy[row] = 0.0f;
   }
-  const T* x = static_cast<const T*>(a.x) + row * a.row_stride;
-  const float c = a.scale * kLog2e;
-  Stats s{-kInf, 0.0f, 0.0f};
-  for (int64_t j = tid; j < a.vocab; j += kThreads) s = merge(s, Stats{to_f32(x[j]), 1.0f, 0.0f}, c);
-  part[tid] = s;
-  __syncthreads();
-  for (int w = kThreads / 2; w > 0; w /= 2) {
-    if (tid < w) part[tid] = merge(part[tid], part[tid + w], c);
-    __syncthreads();
+  for (int i = threadIdx.x; i < a.top; i += kThreads) {
+    a.top_logprob[row * a.top + i] = -kInf;
+    a.top_token[row * a.top + i] = -1;
   }
-  const Row r = finish(part[0], a.scale);
-  if (tid == 0) {
-    a.logprob[row] = token >= 0 && token < a.vocab ? log_prob(to_f32(x[token]), r, a.scale)
-                                                   : __builtin_nanf("");
+}
+
+__device__ __forceinline__ void write_row(const FwdArgs& a, int64_t row, int64_t token, float at,
+                                          const Row& r, const uint64_t* sorted) {
+  if (threadIdx.x == 0) {
+    a.logprob[row] =
+        token >= 0 && token < a.vocab ? log_prob(at, r, a.scale) : __builtin_nanf("");
     a.lse[row] = r.lse;
     if (a.entropy) a.entropy[row] = r.entropy;
   }
-  uint64_t last = ~uint64_t{0};
-  for (int i = 0; i < a.top; ++i) {
-    uint64_t key = 0;
-    for (int64_t j = tid; j < a.vocab; j += kThreads) {
-      const uint64_t k = order_key(to_f32(x[j]), static_cast<uint32_t>(j));
-      if (k < last && k > key) key = k;
-    }
-    best[tid] = key;
-    __syncthreads();
-    for (int w = kThreads / 2; w > 0; w /= 2) {
-      if (tid < w && best[tid + w] > best[tid]) best[tid] = best[tid + w];
-      __syncthreads();
-    }
-    last = best[0];
-    __syncthreads();
-    if (tid == 0) {
-      const uint32_t j = key_index(last);
-      a.top_logprob[row * a.top + i] = log_prob(to_f32(x[j]), r, a.scale);
-      a.top_token[row * a.top + i] = j;
-    }
+  for (int i = threadIdx.x; i < a.top; i += kThreads) {
+    const uint64_t key = sorted[i];
+    a.top_logprob[row * a.top + i] = log_prob(value_of(key_order(key)), r, a.scale);
+    a.top_token[row * a.top + i] = key_index(key);
   }
 }
+
+// A slice of a row: 16-byte vectors lo..hi of those that are aligned in
+// memory, and for the row's first slice the values before the first and after
+// the last of them, one per lane.
+template <typename T>
+struct Slice {
+  const T* x;      // the row
+  const T* vec;    // its first aligned vector
+  int head;        // values before it
+  int lo, hi;
+  int odd;         // this lane's odd value's index, -1: none
+
+  static constexpr int C = Logits<T>::C;
+
+  __device__ __forceinline__ Slice(const FwdArgs& a, int64_t row, int slice) {
+    x = static_cast<const T*>(a.x) + row * a.row_stride;
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
+    const int vocab = static_cast<int>(a.vocab);
+    head = std::min(off == 0 ? 0 : C - off, vocab);
+    vec = x + head;
+    const int n = (vocab - head) / C;
+    lo = std::min(n, slice * a.span);
+    hi = slice == a.slices - 1 ? n : std::min(n, lo + a.span);
+    const int tail = vocab - head - n * C;
+    const int tid = threadIdx.x;
+    odd = slice != 0 || tid >= head + tail ? -1 : tid < head ? tid : vocab - tail + tid - head;
+  }
+  __device__ __forceinline__ u32x4_t load(int v) const {
+    return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(vec) + v);
+  }
+  __device__ __forceinline__ int index(int v) const { return head + v * C; }
+};
+
+// Collects the values of a slice whose order is at least (STRICT: above) tau
+// into keys; returns how many there are (which may be more than keys holds).
+// All threads; lane_order: the order of the thread's maximum.
+template <bool STRICT, typename T>
+__device__ __forceinline__ int collect(const Slice<T>& s, uint32_t lane_order, uint32_t tau,
+                                       uint64_t* keys, int* count) {
+  constexpr int C = Logits<T>::C;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  const auto reaches = [&](uint32_t o) { return STRICT ? o > tau : o >= tau; };
+  const auto take = [&](float x, int index) {
+    const uint32_t o = order_of(x);
+    if (!reaches(o)) return;
+    const int at = atomicAdd(count, 1);
+    if (at < kCandidates) keys[at] = order_key(o, static_cast<uint32_t>(index));
+  };
+  if (threadIdx.x == 0) *count = 0;
+  __syncthreads();
+  if (s.odd >= 0) take(to_f32(s.x[s.odd]), s.odd);
+  // A lane's vectors are kThreads apart; a group of `per` lanes reads those
+  // of one lane that reaches tau.
+  const int rounds = (s.hi - s.lo + kThreads - 1) / kThreads;
+  int per = 1;
+  while (per < rounds && per < kWave) per *= 2;
+  uint64_t who = __ballot(lane_order != 0 && reaches(lane_order));
+  while (who != 0) {
+    int mine = -1;
+    for (int g = 0; g < kWave && who != 0; g += per) {
+      const int l = __builtin_ctzll(who);
+      who &= who - 1;
+      if (lane >= g && lane < g + per) mine = l;
+    }
+    if (mine < 0) continue;
+    for (int r = lane & (per - 1); r < rounds; r += per) {
+      const int v = s.lo + r * kThreads + wave * kWave + mine;
+      if (v >= s.hi) continue;
+      float x[C];
+      unpack(s.load(v), x);
+#pragma unroll
+      for (int i = 0; i < C; ++i) take(x[i], s.index(v) + i);
+    }
+  }
+  __syncthreads();
+  return *count;
+}
+
+// Appends the `want` lowest indexes of values whose order is tau to keys.
+template <typename T>
+__device__ __forceinline__ void collect_equal(const Slice<T>& s, uint32_t tau, int want,
+                                              uint64_t* keys, int* wave_count) {
+  constexpr int C = Logits<T>::C;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  int have = 0;
+  // One value per thread, in order of the index: before the vectors, they,
+  // and after them.
+  const auto step = [&](bool equal, int index) {
+    const uint64_t m = __ballot(equal);
+    __syncthreads();
+    if (lane == 0) wave_count[wave] = __popcll(m);
+    __syncthreads();
+    int at = have + __popcll(m & ((uint64_t{1} << lane) - 1));
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) at += wave_count[w];
+      have += wave_count[w];
+    }
+    if (equal && at < want) keys[at] = order_key(tau, static_cast<uint32_t>(index));
+  };
+  const auto is = [&](int index) { return order_of(to_f32(s.x[index])) == tau; };
+  step(s.odd >= 0 && s.odd < s.head && is(s.odd), s.odd);
+  for (int i = s.lo * C; i < s.hi * C && have < want; i += kThreads) {
+    const int at = i + static_cast<int>(threadIdx.x);
+    step(at < s.hi * C && is(s.head + at), s.head + at);
+  }
+  step(s.odd >= s.head && s.odd >= 0 && is(s.odd), s.odd);
+  __syncthreads();
+}
+
+struct TopMemory {
+  uint64_t keys[kCandidates + kMaxTop];
+  uint64_t sorted[kMaxTop];
+  uint32_t lane_order[kThreads];
+  int count;
+  int wave_count[kWaves];
+};
+
+// The slice's k largest keys into mem.sorted, in falling order, 0 where it
+// has fewer values.  All threads; x: the lane's maximum.
+template <typename T>
+__device__ __forceinline__ void slice_top(const Slice<T>& s, float x, bool any, int k,
+                                          TopMemory& mem) {
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const uint32_t mine = any ? order_of(x) : 0;
+  mem.lane_order[tid] = mine;
+  if (tid < kMaxTop) mem.sorted[tid] = 0;
+  __syncthreads();
+  uint32_t group = mem.lane_order[lane];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) group = std::max(group, mem.lane_order[w * kWave + lane]);
+  const uint32_t tau = kth_of_wave(group, k);
+  int n = collect<false>(s, mine, tau, mem.keys, &mem.count);
+  if (n > kCandidates) {
+    // Many values are equal to tau: those above it, and the first of the others.
+    __syncthreads();
+    n = collect<true>(s, mine, tau, mem.keys, &mem.count);
+    if (n < k) {
+      collect_equal(s, tau, k - n, mem.keys + n, mem.wave_count);
+      n = k;
+    }
+  }
+  if (n <= kCandidates) {
+    sort_top(mem.keys, n, k, mem.sorted);
+    __syncthreads();
+    return;
+  }
+  // Still too many, all in a few lanes: one by one.
+  uint64_t last = ~uint64_t{0};
+  for (int i = 0; i < k; ++i) {
+    uint64_t best = 0;
+    const auto look = [&](float v, int index) {
+      const uint64_t key = order_key(order_of(v), static_cast<uint32_t>(index));
+      if (key < last && key > best) best = key;
+    };
+    if (s.odd >= 0) look(to_f32(s.x[s.odd]), s.odd);
+    for (int v = s.lo + tid; v < s.hi; v += kThreads) {
+      float y[Logits<T>::C];
+      unpack(s.load(v), y);
+#pragma unroll
+      for (int e = 0; e < Logits<T>::C; ++e) look(y[e], s.index(v) + e);
+    }
+    mem.keys[tid] = best;
+    __syncthreads();
+    for (int w = kThreads / 2; w > 0; w /= 2) {
+      if (tid < w) mem.keys[tid] = std::max(mem.keys[tid], mem.keys[tid + w]);
+      __syncthreads();
+    }
+    last = mem.keys[0];
+    if (tid == 0) mem.sorted[i] = last;
+    __syncthreads();
+  }
+}
+
+// A workgroup per row and slice.
+template <typename T, bool ENTROPY, bool TOP>
+__global__ __launch_bounds__(kThreads) void logprobs_slices(FwdArgs a) {
+  constexpr int C = Logits<T>::C;
+  __shared__ Stats wave_stats[kWaves];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & (kWave - 1);
+  const uint32_t r = div_by(blockIdx.x, a.by_slices);
+  const int slice = static_cast<int>(blockIdx.x - r * a.slices);
+  const int64_t row = a.first + r;
+  const int64_t token = token_at(a.tokens, a.token_size, row);
+  if (token == a.ignore_index) {
+    if (a.slices == 1) write_ignored(a, row);
+    return;
+  }
+  const Slice<T> s(a, row, slice);
+  Stats stats{-kInf, 0.0f, 0.0f};
+  // Rounds of kFlight vectors per lane, the next round's loads before this
+  // one's values.
+  constexpr int kRound = kThreads * kFlight;
+  u32x4_t next[kFlight];
+  const auto load = [&](int v0) {
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const int v = v0 + f * kThreads + tid;
+      next[f] = s.load(v < s.hi ? v : s.hi - 1);
+    }
+  };
+  if (s.lo < s.hi) load(s.lo);
+  __builtin_amdgcn_sched_barrier(0);
+  float at = 0.0f;
+  if (tid == 0 && a.slices == 1 && token >= 0 && token < a.vocab) at = to_f32(s.x[token]);
+  float odd[1] = {-kInf};
+  if (s.odd >= 0) odd[0] = to_f32(s.x[s.odd]);
+  for (int v0 = s.lo; v0 < s.hi; v0 += kRound) {
+    u32x4_t now[kFlight];
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) now[f] = next[f];
+    if (v0 + kRound < s.hi) load(v0 + kRound);
+    __builtin_amdgcn_sched_barrier(0);
+    float x[kFlight * C];
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      float y[C];
+      unpack(now[f], y);
+#pragma unroll
+      for (int i = 0; i < C; ++i) x[f * C + i] = y[i];
+    }
+    if (v0 + kRound > s.hi) {
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f) {
+        if (v0 + f * kThreads + tid >= s.hi) {
+#pragma unroll
+          for (int i = 0; i < C; ++i) x[f * C + i] = -kInf;
+        }
+      }
+    }
+    add_values<kFlight * C, ENTROPY>(stats, x, a.c);
+  }
+  const float lane_max = stats.m;  // of its vectors
+  if (slice == 0 && wave == 0) add_values<1, ENTROPY>(stats, odd, a.c);
+
+  const Stats w = join_wave(stats, a.c);
+  if (lane == 0) wave_stats[wave] = w;
+  __syncthreads();
+  const Stats all = join(wave_stats, kWaves, a.c);
+
+  const uint64_t* sorted = nullptr;
+  if constexpr (TOP) {
+    __shared__ TopMemory mem;
+    // A lane with an odd value alone takes part with it.
+    const bool vectors = s.lo + tid < s.hi;
+    const float m = s.odd >= 0 ? (vectors ? maximum(lane_max, odd[0]) : odd[0]) : lane_max;
+    slice_top(s, m, vectors || s.odd >= 0, a.top, mem);
+    sorted = mem.sorted;
+  }
+  if (a.slices == 1) {
+    write_row(a, row, token, at, finish(all, a.scale, a.c), sorted);
+    return;
+  }
+  const int64_t part = row * a.slices + slice;
+  if (tid == 0) a.parts[part] = all;
+  if constexpr (TOP) {
+    if (tid < a.top) a.keys[part * a.top + tid] = sorted[tid];
+  }
+}
+
+// Joins the slices of a row: a workgroup per row.
+template <typename T, bool TOP>
+__global__ __launch_bounds__(kThreads) void join_slices(FwdArgs a) {
+  __shared__ Stats parts[kMaxSlices];
+  const int tid = threadIdx.x;
+  const int64_t row = a.first + blockIdx.x;
+  const int64_t token = token_at(a.tokens, a.token_size, row);
+  if (token == a.ignore_index) {
+    write_ignored(a, row);
+    return;
+  }
+  float at = 0.0f;
+  if (tid == 0 && token >= 0 && token < a.vocab)
+    at = to_f32(static_cast<const T*>(a.x)[row * a.row_stride + token]);
+  if (tid < a.slices) parts[tid] = a.parts[row * a.slices + tid];
+  const uint64_t* best = nullptr;
+  if constexpr (TOP) {
+    // Of the slices' keys those that reach the k-th largest of 64 groups'
+    // maxima, sorted.
+    __shared__ uint64_t keys[kMaxSlices * kMaxTop];
+    __shared__ uint64_t few[kMaxSlices * kMaxTop];
+    __shared__ uint64_t sorted[kMaxTop];
+    __shared__ int count;
+    const int n = a.slices * a.top;
+    for (int i = tid; i < n; i += kThreads) keys[i] = a.keys[row * n + i];
+    if (tid == 0) count = 0;
+    if (tid < kMaxTop) sorted[tid] = 0;
+    __syncthreads();
+    uint32_t group = 0;
+    for (int i = tid & (kWave - 1); i < n; i += kWave) group = std::max(group, key_order(keys[i]));
+    const uint32_t tau = kth_of_wave(group, a.top);
+    for (int i = tid; i < n; i += kThreads) {
+      if (keys[i] != 0 && key_order(keys[i]) >= tau) few[atomicAdd(&count, 1)] = keys[i];
+    }
+    __syncthreads();
+    sort_top(few, count, a.top, sorted);
+    best = sorted;
+  }
+  __syncthreads();
+  write_row(a, row, token, at, finish(join(parts, a.slices, a.c), a.scale, a.c), best);
+}
+
+// Slices per row and vectors per slice: enough workgroups to fill the chip,
+// each with at least two vectors per lane.
+struct Plan {
+  int slices, span;
+};
+
+inline Plan plan(int64_t rows, int64_t vocab, int elem_size) {
+  const int64_t vectors = vocab / (16 / elem_size);
+  const int64_t want = std::min<int64_t>((kFill + rows - 1) / rows, kMaxSlices);
+  const int64_t most = std::max<int64_t>(1, vectors / (2 * kThreads));
+  Plan p;
+  const int64_t slices = std::min(want, most);
+  p.span = static_cast<int>(
+      ((vectors + slices - 1) / slices + kThreads - 1) / kThreads * kThreads);
+  p.slices = p.span == 0 ? 1 : static_cast<int>(std::max<int64_t>(1, (vectors + p.span - 1) / p.span));
+  return p;
+}
+
+inline size_t parts_bytes(int64_t rows, int slices) {
+  return (rows * slices * sizeof(Stats) + 15) / 16 * 16;
+}
+
+// ---------------------------------------------------------------------------
+// Backward
+// ---------------------------------------------------------------------------
 
 struct BwdArgs {
   const float* grad;
@@ -195,36 +620,99 @@ struct BwdArgs {
   int token_size;
 };
 
-// A workgroup per row.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void logprobs_bwd_rows(BwdArgs a) {
-  const int64_t row = blockIdx.x;
+constexpr int kBwdVectors = 2;  // per lane
+constexpr int kBwdRows = 32768;  // rows per grid layer
+
+// The gradient of a logit, without the token's own term.  e^-104 is 0: the
+// bound keeps p ln p from being 0 * inf.
+template <bool ENTROPY>
+__device__ __forceinline__ float logit_grad(float x, float scale, float lse, float factor,
+                                            float gh, float h) {
+  const float lp = maximum(__builtin_fmaf(scale, x, -lse), -104.0f);
+  const float p = exp_f32(lp);
+  return p * (ENTROPY ? factor - gh * (lp + h) : factor);
+}
+
+// A workgroup per row and chunk of it: blockIdx.x the chunk, y and z the row.
+template <typename T, bool ENTROPY>
+__global__ __launch_bounds__(kThreads) void logprobs_bwd_chunks(BwdArgs a) {
+  constexpr int C = Logits<T>::C;
+  typedef typename Logits<T>::Unaligned Unaligned;
+  const int64_t row = static_cast<int64_t>(blockIdx.z) * kBwdRows + blockIdx.y;
+  if (row >= a.rows) return;
   const T* x = static_cast<const T*>(a.x) + row * a.row_stride;
   T* dx = static_cast<T*>(a.dx) + row * a.dx_row_stride;
+  const int vocab = static_cast<int>(a.vocab);
+  // Vectors are aligned in dx.
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(dx) % 16 / sizeof(T));
+  const int head = std::min(off == 0 ? 0 : C - off, vocab);
+  const int n = (vocab - head) / C;
+  const int tail = vocab - head - n * C;
+  const int tid = threadIdx.x;
+  int odd = -1;
+  if (blockIdx.x == 0 && tid < head + tail) odd = tid < head ? tid : vocab - tail + tid - head;
+  const int v0 = static_cast<int>(blockIdx.x) * (kThreads * kBwdVectors) + tid;
+
   const int64_t token = token_at(a.tokens, a.token_size, row);
   if (token == a.ignore_index) {
-    for (int64_t j = threadIdx.x; j < a.vocab; j += kThreads) dx[j] = from_f32<T>(0.0f);
+#pragma unroll
+    for (int k = 0; k < kBwdVectors; ++k) {
+      const int v = v0 + k * kThreads;
+      if (v < n)
+        __builtin_nontemporal_store(u32x4_t{0u, 0u, 0u, 0u},
+                                    reinterpret_cast<u32x4_t*>(dx + head) + v);
+    }
+    if (odd >= 0) dx[odd] = T{0};
     return;
+  }
+  u32x4_t in[kBwdVectors];
+#pragma unroll
+  for (int k = 0; k < kBwdVectors; ++k) {
+    const int v = v0 + k * kThreads;
+    if (v < n)
+      in[k] = __builtin_bit_cast(
+          u32x4_t,
+          __builtin_nontemporal_load(reinterpret_cast<const Unaligned*>(x + head + v * C)));
   }
   const bool known = token >= 0 && token < a.vocab;
   const float g = known ? a.grad[row] : __builtin_nanf("");
   const float lse = a.lse[row];
-  const float gh = a.grad_entropy ? a.grad_entropy[row] : 0.0f;
-  const float h = a.grad_entropy ? a.entropy[row] : 0.0f;
+  const float gh = ENTROPY ? a.grad_entropy[row] : 0.0f;
+  const float h = ENTROPY ? a.entropy[row] : 0.0f;
   const float factor = (a.grad_lse ? a.grad_lse[row] : 0.0f) - g;
-  for (int64_t j = threadIdx.x; j < a.vocab; j += kThreads) {
-    // The clamp (e^-104 is 0) also keeps p ln p from being 0 * inf.
-    const float lp = exp_domain(__builtin_fmaf(a.scale, to_f32(x[j]), -lse));
-    float d = exp_f32(lp) * (factor - gh * (lp + h));
-    if (j == token) d += g;
-    dx[j] = from_f32<T>(a.scale * d);
+  const int hot = known ? static_cast<int>(token) : -1;
+  const auto gradient = [&](float v, int index) {
+    const float d = logit_grad<ENTROPY>(v, a.scale, lse, factor, gh, h);
+    return a.scale * (index == hot ? d + g : d);
+  };
+#pragma unroll
+  for (int k = 0; k < kBwdVectors; ++k) {
+    const int v = v0 + k * kThreads;
+    if (v >= n) continue;
+    float f[C];
+    unpack(in[k], f);
+#pragma unroll
+    for (int i = 0; i < C; ++i) f[i] = gradient(f[i], head + v * C + i);
+    __builtin_nontemporal_store(pack(f), reinterpret_cast<u32x4_t*>(dx + head) + v);
+  }
+  if (odd >= 0) {
+    const float d = gradient(to_f32(x[odd]), odd);
+    if constexpr (sizeof(T) == 2) dx[odd] = static_cast<T>(pack_bf16x2(d, 0.0f) & 0xffffu);
+    else dx[odd] = d;
   }
 }
 
 }  // namespace
 }  // namespace hipo
 
-extern "C" size_t hipo_token_logprobs_workspace_bytes(int64_t, int64_t, int64_t) { return 0; }
+extern "C" size_t hipo_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int64_t top) {
+  using namespace hipo;
+  if (rows <= 0 || vocab <= 0 || top < 0 || rows > 0x7fffffff || vocab > 0x7fffffff) return 0;
+  // The most of either element size.
+  const int slices = std::max(plan(rows, vocab, 2).slices, plan(rows, vocab, 4).slices);
+  if (slices == 1) return 0;
+  return parts_bytes(rows, slices) + rows * slices * top * sizeof(uint64_t);
+}
 
 extern "C" int hipo_token_logprobs(const void* logits, int elem_size, const void* tokens,
                                    int token_size, float* logprob, float* lse, float* entropy,
@@ -237,9 +725,10 @@ extern "C" int hipo_token_logprobs(const void* logits, int elem_size, const void
   HIPO_REQUIRE(rows >= 0 && vocab >= 0, "token_logprobs: negative size");
   HIPO_REQUIRE(elem_size == 2 || elem_size == 4, "token_logprobs: elem_size must be 2 or 4");
   HIPO_REQUIRE(token_size == 4 || token_size == 8, "token_logprobs: token_size must be 4 or 8");
-  HIPO_REQUIRE(scale > 0.0f && scale < __builtin_inff(),
-               "token_logprobs: scale must be positive and finite");
-  HIPO_REQUIRE(vocab <= 0x7fffffff && rows <= 0x7fffffff, "token_logprobs: size over 2^31");
+  HIPO_REQUIRE(scale >= 0x1p-100f && scale <= 0x1p100f,
+               "token_logprobs: scale must be from 2^-100 to 2^100");
+  HIPO_REQUIRE(vocab <= kMaxVocab && rows <= 0x7fffffff,
+               "token_logprobs: vocab over 2^31 - 4096 or rows over 2^31");
   HIPO_REQUIRE(row_stride >= vocab, "token_logprobs: row_stride %lld < vocab %lld",
                (long long)row_stride, (long long)vocab);
   HIPO_REQUIRE(top >= 0 && top <= kMaxTop && top <= vocab,
@@ -250,12 +739,33 @@ extern "C" int hipo_token_logprobs(const void* logits, int elem_size, const void
                "token_logprobs: null pointer");
   HIPO_REQUIRE(top == 0 || (top_logprob != nullptr && top_token != nullptr),
                "token_logprobs: null pointer (top)");
-  HIPO_REQUIRE(workspace_bytes >= hipo_token_logprobs_workspace_bytes(rows, vocab, top),
-               "token_logprobs: workspace too small");
-  const FwdArgs a{logits, tokens, logprob, lse, entropy, top_logprob, top_token, rows, vocab,
-                  row_stride, ignore_index, scale, token_size, static_cast<int>(top)};
-  auto kernel = elem_size == 2 ? logprobs_rows<uint16_t> : logprobs_rows<float>;
-  kernel<<<dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, stream>>>(a);
+  const size_t need = hipo_token_logprobs_workspace_bytes(rows, vocab, top);
+  HIPO_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need),
+               "token_logprobs: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  HIPO_REQUIRE(need == 0 || aligned16(workspace),
+               "token_logprobs: workspace must be 16-byte aligned");
+  const Plan p = plan(rows, vocab, elem_size);
+  FwdArgs a{logits, tokens, logprob, lse, entropy, top_logprob, top_token,
+                  static_cast<Stats*>(workspace),
+                  reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) +
+                                              parts_bytes(rows, p.slices)),
+                  0, vocab, row_stride, ignore_index, scale, scale * kLog2eHi, token_size,
+                  static_cast<int>(top), p.slices, p.span,
+                  div_magic(static_cast<uint32_t>(p.slices))};
+  const bool bf16 = elem_size == 2, ent = entropy != nullptr;
+#define HIPO_LP(T_)                                                            \
+  (top ? (ent ? logprobs_slices<T_, true, true> : logprobs_slices<T_, false, true>) \
+       : (ent ? logprobs_slices<T_, true, false> : logprobs_slices<T_, false, false>))
+  auto kernel = bf16 ? HIPO_LP(uint16_t) : HIPO_LP(float);
+#undef HIPO_LP
+  auto join = bf16 ? (top ? join_slices<uint16_t, true> : join_slices<uint16_t, false>)
+                   : (top ? join_slices<float, true> : join_slices<float, false>);
+  const int64_t step = kMaxBlocks / p.slices;
+  for (; a.first < rows; a.first += step) {
+    const unsigned n = static_cast<unsigned>(std::min(step, rows - a.first));
+    kernel<<<dim3(n * p.slices), dim3(kThreads), 0, stream>>>(a);
+    if (p.slices > 1) join<<<dim3(n), dim3(kThreads), 0, stream>>>(a);
+  }
   return check_launch("token_logprobs");
 }
 
@@ -272,9 +782,10 @@ extern "C" int hipo_token_logprobs_bwd(const float* grad, const void* logits, in
   HIPO_REQUIRE(elem_size == 2 || elem_size == 4, "token_logprobs_bwd: elem_size must be 2 or 4");
   HIPO_REQUIRE(token_size == 4 || token_size == 8,
                "token_logprobs_bwd: token_size must be 4 or 8");
-  HIPO_REQUIRE(scale > 0.0f && scale < __builtin_inff(),
-               "token_logprobs_bwd: scale must be positive and finite");
-  HIPO_REQUIRE(vocab <= 0x7fffffff && rows <= 0x7fffffff, "token_logprobs_bwd: size over 2^31");
+  HIPO_REQUIRE(scale >= 0x1p-100f && scale <= 0x1p100f,
+               "token_logprobs_bwd: scale must be from 2^-100 to 2^100");
+  HIPO_REQUIRE(vocab <= kMaxVocab && rows <= 0x7fffffff,
+               "token_logprobs_bwd: vocab over 2^31 - 4096 or rows over 2^31");
   HIPO_REQUIRE(row_stride >= vocab && dlogits_row_stride >= vocab,
                "token_logprobs_bwd: row_stride < vocab %lld", (long long)vocab);
   HIPO_REQUIRE(grad_entropy == nullptr || entropy != nullptr,
@@ -287,7 +798,15 @@ extern "C" int hipo_token_logprobs_bwd(const float* grad, const void* logits, in
                "token_logprobs_bwd: null pointer");
   const BwdArgs a{grad, logits, tokens, lse, entropy, grad_entropy, grad_lse, dlogits, rows,
                   vocab, row_stride, dlogits_row_stride, ignore_index, scale, token_size};
-  auto kernel = elem_size == 2 ? logprobs_bwd_rows<uint16_t> : logprobs_bwd_rows<float>;
-  kernel<<<dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, stream>>>(a);
+  const int64_t chunk = int64_t{kThreads} * kBwdVectors * (16 / elem_size);
+  const dim3 grid(static_cast<unsigned>((vocab + chunk - 1) / chunk),
+                  static_cast<unsigned>(std::min<int64_t>(rows, kBwdRows)),
+                  static_cast<unsigned>((rows + kBwdRows - 1) / kBwdRows));
+  const bool ent = grad_entropy != nullptr;
+  auto kernel = elem_size == 2 ? (ent ? logprobs_bwd_chunks<uint16_t, true>
+                                      : logprobs_bwd_chunks<uint16_t, false>)
+                               : (ent ? logprobs_bwd_chunks<float, true>
+                                      : logprobs_bwd_chunks<float, false>);
+  kernel<<<grid, dim3(kThreads), 0, stream>>>(a);
   return check_launch("token_logprobs_bwd");
 }

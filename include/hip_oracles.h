@@ -449,7 +449,7 @@ int hipo_gelu_erf_bwd_colsum_bf16(const uint16_t* grad, const uint16_t* x, uint1
  * `row_stride` (>= vocab), of bf16 (elem_size 2) or fp32 (4), at any element
  * alignment; tokens is [rows] of int32 (token_size 4) or int64 (8); the
  * outputs are contiguous.  entropy may be NULL; top is at most 64 and at
- * most vocab, its outputs NULL where it is 0; scale is positive and finite.
+ * most vocab, its outputs NULL where it is 0; scale is from 2^-100 to 2^100.
  * A row whose token is ignore_index is not read: 0, 0, 0, and for the
  * alternatives -inf and -1.  A token outside [0, vocab) otherwise has
  * logprob NaN.  A row with nothing above -inf has lse -inf, one with +inf
