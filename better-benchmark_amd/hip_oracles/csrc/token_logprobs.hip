@@ -15,9 +15,9 @@
 //
 // The alternatives cost nothing while the row streams by: the lanes' maxima
 // say where the largest values are.  The k-th largest of 64 groups' maxima is
-// a lower bound of the k-th largest value, few values reach it, and they lie
-// in lanes whose maximum does: only these lanes' values are read again (k = 20
-// of 64 groups: about 24 lanes of 256).
+// a lower bound of the k-th largest value, few values reach it (k = 20: about
+// 24), and they lie in lanes whose maximum does: only these lanes' values are
+// read again, shared out over the workgroup, and ranked by counting.
 //
 // Backward: HBM-bound, one pass, a value's gradient needs its logit and a few
 // numbers of its row.
@@ -31,14 +31,13 @@ namespace hipo {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
+constexpr int kLarge = 1024;       // threads of a workgroup where rows are few
 constexpr int kFlight = 4;         // 16-byte loads per lane in flight
 constexpr int kMaxTop = 64;
-constexpr int kMaxSlices = 64;     // of a row
+constexpr int64_t kMaxSlices = 64;    // of a row
 constexpr int kCandidates = 1024;  // values that a slice can rank at once
 constexpr int64_t kMaxVocab = 0x7fffffff - 4096;
 constexpr int64_t kMaxBlocks = 1 << 23;  // of a launch
-constexpr int64_t kFill = 1024;    // workgroups that fill the chip
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kInf = __builtin_inff();
 constexpr float kHuge = 0x1p100f;
@@ -150,16 +149,10 @@ __device__ __forceinline__ Stats join_wave(Stats s, float c) {
   return Stats{m, wave_sum(s.z), wave_sum(s.u)};
 }
 
-__device__ __forceinline__ Stats join(const Stats* part, int n, float c) {
-  float m = part[0].m;
-  for (int i = 1; i < n; ++i) m = maximum(m, part[i].m);
-  Stats all{m, 0.0f, 0.0f};
-  for (int i = 0; i < n; ++i) {
-    const Stats s = rescale(part[i], m, c);
-    all.z += s.z;
-    all.u += s.u;
-  }
-  return all;
+// Of n <= 64 parts, a part per lane; every lane has it.
+__device__ __forceinline__ Stats join_parts(const Stats* part, int n, float c) {
+  const int lane = threadIdx.x & (kWave - 1);
+  return join_wave(lane < n ? part[lane] : Stats{-kInf, 0.0f, 0.0f}, c);
 }
 
 struct Row {
@@ -215,25 +208,28 @@ __device__ __forceinline__ uint32_t key_index(uint64_t key) {
   return 0xffffffffu - static_cast<uint32_t>(key);
 }
 
-// The k-th largest of a wave's 64 orders (0 if fewer than k are not 0).
+// The k-th largest of a wave's 64 orders (0 if fewer than k are not 0), bit by
+// bit the largest number that k of them reach; with 16 BITS its upper ones,
+// a lower bound (bf16 values have no others).
+template <int BITS>
 __device__ __forceinline__ uint32_t kth_of_wave(uint32_t order, int k) {
-  int above = 0;
+  uint32_t v = 0;
 #pragma unroll
-  for (int l = 0; l < kWave; ++l)
-    above += static_cast<uint32_t>(__builtin_amdgcn_readlane(order, l)) > order ? 1 : 0;
-  // The smallest of those with fewer than k above.
-  uint32_t v = above < k ? order : 0xffffffffu;
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) v = std::min(v, static_cast<uint32_t>(__shfl_xor(v, d)));
+  for (int b = 31; b >= 32 - BITS; --b) {
+    const uint32_t higher = v | (1u << b);
+    if (__popcll(__ballot(order >= higher)) >= k) v = higher;
+  }
   return v;
 }
 
 // Writes the k largest of n keys in falling order to sorted (all of a
 // workgroup's threads; keys are distinct, n >= k).
+template <int NT>
 __device__ __forceinline__ void sort_top(const uint64_t* keys, int n, int k, uint64_t* sorted) {
-  for (int i = threadIdx.x; i < n; i += kThreads) {
+  for (int i = threadIdx.x; i < n; i += NT) {
     const uint64_t key = keys[i];
     int above = 0;
+#pragma unroll 8
     for (int l = 0; l < n; ++l) above += keys[l] > key ? 1 : 0;
     if (above < k) sorted[above] = key;
   }
@@ -249,25 +245,28 @@ struct FwdArgs {
   float *logprob, *lse, *entropy, *top_logprob;
   int64_t* top_token;
   Stats* parts;      // [rows][slices]
-  uint64_t* keys;    // [rows][slices][top]
+  uint64_t* keys;    // [rows][slices][kMaxTop]
   int64_t first, vocab, row_stride, ignore_index;
   float scale, c;
   int token_size, top, slices, span;  // of span 16-byte vectors
-  DivMagic by_slices;
+  int rounds;                         // vectors per lane in a slice
+  DivMagic by_slices, by_rounds;
 };
 
+template <int NT>
 __device__ __forceinline__ void write_ignored(const FwdArgs& a, int64_t row) {
   if (threadIdx.x == 0) {
     a.logprob[row] = 0.0f;
     a.lse[row] = 0.0f;
     if (a.entropy) a.entropy[row] = 0.0f;
   }
-  for (int i = threadIdx.x; i < a.top; i += kThreads) {
+  for (int i = threadIdx.x; i < a.top; i += NT) {
     a.top_logprob[row * a.top + i] = -kInf;
     a.top_token[row * a.top + i] = -1;
   }
 }
 
+template <int NT>
 __device__ __forceinline__ void write_row(const FwdArgs& a, int64_t row, int64_t token, float at,
                                           const Row& r, const uint64_t* sorted) {
   if (threadIdx.x == 0) {
@@ -276,7 +275,7 @@ __device__ __forceinline__ void write_row(const FwdArgs& a, int64_t row, int64_t
     a.lse[row] = r.lse;
     if (a.entropy) a.entropy[row] = r.entropy;
   }
-  for (int i = threadIdx.x; i < a.top; i += kThreads) {
+  for (int i = threadIdx.x; i < a.top; i += NT) {
     const uint64_t key = sorted[i];
     a.top_logprob[row * a.top + i] = log_prob(value_of(key_order(key)), r, a.scale);
     a.top_token[row * a.top + i] = key_index(key);
@@ -315,53 +314,82 @@ struct Slice {
   __device__ __forceinline__ int index(int v) const { return head + v * C; }
 };
 
+template <int NT>
+struct TopMemory {
+  uint64_t keys[kCandidates + kMaxTop];
+  uint64_t sorted[kMaxTop];
+  uint32_t lane_order[NT];
+  int lanes[NT];  // those whose maximum reaches the bound
+  int lane_count, count;
+  int wave_count[NT / kWave];
+};
+
 // Collects the values of a slice whose order is at least (STRICT: above) tau
-// into keys; returns how many there are (which may be more than keys holds).
+// into mem.keys; returns how many there are (which may be more than it holds).
 // All threads; lane_order: the order of the thread's maximum.
-template <bool STRICT, typename T>
-__device__ __forceinline__ int collect(const Slice<T>& s, uint32_t lane_order, uint32_t tau,
-                                       uint64_t* keys, int* count) {
+template <bool STRICT, int NT, typename T>
+__device__ __forceinline__ int collect(const Slice<T>& s, DivMagic by_rounds, int rounds,
+                                       uint32_t lane_order, uint32_t tau, TopMemory<NT>& mem) {
   constexpr int C = Logits<T>::C;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
-  const auto reaches = [&](uint32_t o) { return STRICT ? o > tau : o >= tau; };
-  const auto take = [&](float x, int index) {
-    const uint32_t o = order_of(x);
-    if (!reaches(o)) return;
-    const int at = atomicAdd(count, 1);
-    if (at < kCandidates) keys[at] = order_key(o, static_cast<uint32_t>(index));
-  };
-  if (threadIdx.x == 0) *count = 0;
+  constexpr int kLoads = 4;
+  // Not below the bound as a value: the same (a NaN bound, of an order below
+  // that of -inf or a NaN's, leaves nothing out).
+  const float bound = value_of(tau);
+  const auto reaches = [&](float v) { return STRICT ? order_of(v) > tau : !(v < bound); };
+  if (threadIdx.x == 0) mem.lane_count = mem.count = 0;
   __syncthreads();
-  if (s.odd >= 0) take(to_f32(s.x[s.odd]), s.odd);
-  // A lane's vectors are kThreads apart; a group of `per` lanes reads those
-  // of one lane that reaches tau.
-  const int rounds = (s.hi - s.lo + kThreads - 1) / kThreads;
-  int per = 1;
-  while (per < rounds && per < kWave) per *= 2;
-  uint64_t who = __ballot(lane_order != 0 && reaches(lane_order));
-  while (who != 0) {
-    int mine = -1;
-    for (int g = 0; g < kWave && who != 0; g += per) {
-      const int l = __builtin_ctzll(who);
-      who &= who - 1;
-      if (lane >= g && lane < g + per) mine = l;
-    }
-    if (mine < 0) continue;
-    for (int r = lane & (per - 1); r < rounds; r += per) {
-      const int v = s.lo + r * kThreads + wave * kWave + mine;
-      if (v >= s.hi) continue;
-      float x[C];
-      unpack(s.load(v), x);
-#pragma unroll
-      for (int i = 0; i < C; ++i) take(x[i], s.index(v) + i);
+  if (lane_order != 0 && (STRICT ? lane_order > tau : lane_order >= tau))
+    mem.lanes[atomicAdd(&mem.lane_count, 1)] = threadIdx.x;
+  if (s.odd >= 0) {
+    const float x = to_f32(s.x[s.odd]);
+    if (reaches(x)) {
+      const int at = atomicAdd(&mem.count, 1);
+      if (at < kCandidates) mem.keys[at] = order_key(order_of(x), static_cast<uint32_t>(s.odd));
     }
   }
   __syncthreads();
-  return *count;
+  // Their vectors, NT apart, shared out over all threads.
+  const int n = mem.lane_count * rounds;
+  for (int j0 = threadIdx.x; j0 < n; j0 += NT * kLoads) {
+    int v[kLoads];
+    u32x4_t raw[kLoads];
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      const int j = j0 + k * NT;
+      v[k] = s.hi;
+      if (j < n) {
+        const int l = static_cast<int>(div_by(j, by_rounds));
+        v[k] = s.lo + (j - l * rounds) * NT + mem.lanes[l];
+      }
+      if (v[k] < s.hi) raw[k] = s.load(v[k]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+      if (v[k] >= s.hi) continue;
+      float x[C];
+      unpack(raw[k], x);
+      uint32_t hits = 0;
+#pragma unroll
+      for (int i = 0; i < C; ++i) hits |= reaches(x[i]) ? 1u << i : 0u;
+      if (hits == 0) continue;
+      int at = atomicAdd(&mem.count, __popc(hits));
+      for (; hits != 0; hits &= hits - 1, ++at) {
+        const int i = __builtin_ctz(hits);
+        float y = x[0];  // x[i], kept in registers
+#pragma unroll
+        for (int c = 1; c < C; ++c) y = i == c ? x[c] : y;
+        if (at < kCandidates)
+          mem.keys[at] = order_key(order_of(y), static_cast<uint32_t>(s.index(v[k]) + i));
+      }
+    }
+  }
+  __syncthreads();
+  return mem.count;
 }
 
 // Appends the `want` lowest indexes of values whose order is tau to keys.
-template <typename T>
+template <int NT, typename T>
 __device__ __forceinline__ void collect_equal(const Slice<T>& s, uint32_t tau, int want,
                                               uint64_t* keys, int* wave_count) {
   constexpr int C = Logits<T>::C;
@@ -375,7 +403,7 @@ __device__ __forceinline__ void collect_equal(const Slice<T>& s, uint32_t tau, i
     if (lane == 0) wave_count[wave] = __popcll(m);
     __syncthreads();
     int at = have + __popcll(m & ((uint64_t{1} << lane) - 1));
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < NT / kWave; ++w) {
       if (w < wave) at += wave_count[w];
       have += wave_count[w];
     }
@@ -383,7 +411,7 @@ __device__ __forceinline__ void collect_equal(const Slice<T>& s, uint32_t tau, i
   };
   const auto is = [&](int index) { return order_of(to_f32(s.x[index])) == tau; };
   step(s.odd >= 0 && s.odd < s.head && is(s.odd), s.odd);
-  for (int i = s.lo * C; i < s.hi * C && have < want; i += kThreads) {
+  for (int i = s.lo * C; i < s.hi * C && have < want; i += NT) {
     const int at = i + static_cast<int>(threadIdx.x);
     step(at < s.hi * C && is(s.head + at), s.head + at);
   }
@@ -391,19 +419,13 @@ __device__ __forceinline__ void collect_equal(const Slice<T>& s, uint32_t tau, i
   __syncthreads();
 }
 
-struct TopMemory {
-  uint64_t keys[kCandidates + kMaxTop];
-  uint64_t sorted[kMaxTop];
-  uint32_t lane_order[kThreads];
-  int count;
-  int wave_count[kWaves];
-};
-
-// The slice's k largest keys into mem.sorted, in falling order, 0 where it
-// has fewer values.  All threads; x: the lane's maximum.
-template <typename T>
-__device__ __forceinline__ void slice_top(const Slice<T>& s, float x, bool any, int k,
-                                          TopMemory& mem) {
+// The slice's k largest keys: with sort they alone, in falling order, without
+// it at most kMaxTop keys with them among them; returns where, and in n how
+// many.  All threads; x: the lane's maximum.
+template <int NT, typename T>
+__device__ __forceinline__ const uint64_t* slice_top(const Slice<T>& s, DivMagic by_rounds,
+                                                     int rounds, float x, bool any, int k,
+                                                     bool sort, TopMemory<NT>& mem, int& n) {
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const uint32_t mine = any ? order_of(x) : 0;
   mem.lane_order[tid] = mine;
@@ -411,22 +433,26 @@ __device__ __forceinline__ void slice_top(const Slice<T>& s, float x, bool any, 
   __syncthreads();
   uint32_t group = mem.lane_order[lane];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) group = std::max(group, mem.lane_order[w * kWave + lane]);
-  const uint32_t tau = kth_of_wave(group, k);
-  int n = collect<false>(s, mine, tau, mem.keys, &mem.count);
+  for (int w = 1; w < NT / kWave; ++w) group = std::max(group, mem.lane_order[w * kWave + lane]);
+  uint32_t tau = kth_of_wave<16>(group, k);
+  n = collect<false, NT>(s, by_rounds, rounds, mine, tau, mem);
+  if (!sort && n <= kMaxTop) return mem.keys;
   if (n > kCandidates) {
-    // Many values are equal to tau: those above it, and the first of the others.
+    // Many values are equal to the bound, or near it: those above the exact one,
+    // and the first of those equal to it.
+    tau = kth_of_wave<32>(group, k);
     __syncthreads();
-    n = collect<true>(s, mine, tau, mem.keys, &mem.count);
+    n = collect<true, NT>(s, by_rounds, rounds, mine, tau, mem);
     if (n < k) {
-      collect_equal(s, tau, k - n, mem.keys + n, mem.wave_count);
+      collect_equal<NT>(s, tau, k - n, mem.keys + n, mem.wave_count);
       n = k;
     }
   }
   if (n <= kCandidates) {
-    sort_top(mem.keys, n, k, mem.sorted);
+    sort_top<NT>(mem.keys, n, k, mem.sorted);
     __syncthreads();
-    return;
+    n = std::min(n, k);
+    return mem.sorted;
   }
   // Still too many, all in a few lanes: one by one.
   uint64_t last = ~uint64_t{0};
@@ -437,7 +463,7 @@ __device__ __forceinline__ void slice_top(const Slice<T>& s, float x, bool any, 
       if (key < last && key > best) best = key;
     };
     if (s.odd >= 0) look(to_f32(s.x[s.odd]), s.odd);
-    for (int v = s.lo + tid; v < s.hi; v += kThreads) {
+    for (int v = s.lo + tid; v < s.hi; v += NT) {
       float y[Logits<T>::C];
       unpack(s.load(v), y);
 #pragma unroll
@@ -445,7 +471,7 @@ __device__ __forceinline__ void slice_top(const Slice<T>& s, float x, bool any, 
     }
     mem.keys[tid] = best;
     __syncthreads();
-    for (int w = kThreads / 2; w > 0; w /= 2) {
+    for (int w = NT / 2; w > 0; w /= 2) {
       if (tid < w) mem.keys[tid] = std::max(mem.keys[tid], mem.keys[tid + w]);
       __syncthreads();
     }
@@ -453,32 +479,34 @@ __device__ __forceinline__ void slice_top(const Slice<T>& s, float x, bool any, 
     if (tid == 0) mem.sorted[i] = last;
     __syncthreads();
   }
+  n = k;
+  return mem.sorted;
 }
 
 // A workgroup per row and slice.
-template <typename T, bool ENTROPY, bool TOP>
-__global__ __launch_bounds__(kThreads) void logprobs_slices(FwdArgs a) {
+template <int NT, typename T, bool ENTROPY, bool TOP>
+__global__ __launch_bounds__(NT) void logprobs_slices(FwdArgs a) {
   constexpr int C = Logits<T>::C;
-  __shared__ Stats wave_stats[kWaves];
+  __shared__ Stats wave_stats[NT / kWave];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & (kWave - 1);
   const uint32_t r = div_by(blockIdx.x, a.by_slices);
   const int slice = static_cast<int>(blockIdx.x - r * a.slices);
   const int64_t row = a.first + r;
   const int64_t token = token_at(a.tokens, a.token_size, row);
   if (token == a.ignore_index) {
-    if (a.slices == 1) write_ignored(a, row);
+    if (a.slices == 1) write_ignored<NT>(a, row);
     return;
   }
   const Slice<T> s(a, row, slice);
   Stats stats{-kInf, 0.0f, 0.0f};
   // Rounds of kFlight vectors per lane, the next round's loads before this
   // one's values.
-  constexpr int kRound = kThreads * kFlight;
+  constexpr int kRound = NT * kFlight;
   u32x4_t next[kFlight];
   const auto load = [&](int v0) {
 #pragma unroll
     for (int f = 0; f < kFlight; ++f) {
-      const int v = v0 + f * kThreads + tid;
+      const int v = v0 + f * NT + tid;
       next[f] = s.load(v < s.hi ? v : s.hi - 1);
     }
   };
@@ -505,7 +533,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_slices(FwdArgs a) {
     if (v0 + kRound > s.hi) {
 #pragma unroll
       for (int f = 0; f < kFlight; ++f) {
-        if (v0 + f * kThreads + tid >= s.hi) {
+        if (v0 + f * NT + tid >= s.hi) {
 #pragma unroll
           for (int i = 0; i < C; ++i) x[f * C + i] = -kInf;
         }
@@ -519,37 +547,40 @@ __global__ __launch_bounds__(kThreads) void logprobs_slices(FwdArgs a) {
   const Stats w = join_wave(stats, a.c);
   if (lane == 0) wave_stats[wave] = w;
   __syncthreads();
-  const Stats all = join(wave_stats, kWaves, a.c);
+  const Stats all = NT == kWave ? w : join_parts(wave_stats, NT / kWave, a.c);
 
-  const uint64_t* sorted = nullptr;
+  const uint64_t* best = nullptr;
+  int n = 0;
   if constexpr (TOP) {
-    __shared__ TopMemory mem;
+    __shared__ TopMemory<NT> mem;
     // A lane with an odd value alone takes part with it.
     const bool vectors = s.lo + tid < s.hi;
     const float m = s.odd >= 0 ? (vectors ? maximum(lane_max, odd[0]) : odd[0]) : lane_max;
-    slice_top(s, m, vectors || s.odd >= 0, a.top, mem);
-    sorted = mem.sorted;
+    best = slice_top(s, a.by_rounds, a.rounds, m, vectors || s.odd >= 0, a.top, a.slices == 1, mem,
+                     n);
   }
   if (a.slices == 1) {
-    write_row(a, row, token, at, finish(all, a.scale, a.c), sorted);
+    write_row<NT>(a, row, token, at, finish(all, a.scale, a.c), best);
     return;
   }
   const int64_t part = row * a.slices + slice;
   if (tid == 0) a.parts[part] = all;
   if constexpr (TOP) {
-    if (tid < a.top) a.keys[part * a.top + tid] = sorted[tid];
+    // 0 where there is none.
+    if (tid < kMaxTop) a.keys[part * kMaxTop + tid] = tid < n ? best[tid] : 0;
   }
 }
 
 // Joins the slices of a row: a workgroup per row.
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kThreads) void join_slices(FwdArgs a) {
+  constexpr int NT = kThreads;
   __shared__ Stats parts[kMaxSlices];
   const int tid = threadIdx.x;
   const int64_t row = a.first + blockIdx.x;
   const int64_t token = token_at(a.tokens, a.token_size, row);
   if (token == a.ignore_index) {
-    write_ignored(a, row);
+    write_ignored<NT>(a, row);
     return;
   }
   float at = 0.0f;
@@ -564,40 +595,60 @@ __global__ __launch_bounds__(kThreads) void join_slices(FwdArgs a) {
     __shared__ uint64_t few[kMaxSlices * kMaxTop];
     __shared__ uint64_t sorted[kMaxTop];
     __shared__ int count;
-    const int n = a.slices * a.top;
-    for (int i = tid; i < n; i += kThreads) keys[i] = a.keys[row * n + i];
+    const int n = a.slices * kMaxTop;
+    for (int i = tid; i < n; i += NT) keys[i] = a.keys[row * n + i];
     if (tid == 0) count = 0;
     if (tid < kMaxTop) sorted[tid] = 0;
     __syncthreads();
     uint32_t group = 0;
-    for (int i = tid & (kWave - 1); i < n; i += kWave) group = std::max(group, key_order(keys[i]));
-    const uint32_t tau = kth_of_wave(group, a.top);
-    for (int i = tid; i < n; i += kThreads) {
+    // (A slice's first places are the filled ones: another lane's in each.)
+    for (int i = 0; i < a.slices; ++i)
+      group = std::max(group, key_order(keys[i * kMaxTop + ((tid + 23 * i) & (kMaxTop - 1))]));
+    const uint32_t tau = kth_of_wave<16>(group, a.top);
+    for (int i = tid; i < n; i += NT) {
       if (keys[i] != 0 && key_order(keys[i]) >= tau) few[atomicAdd(&count, 1)] = keys[i];
     }
     __syncthreads();
-    sort_top(few, count, a.top, sorted);
+    sort_top<NT>(few, count, a.top, sorted);
     best = sorted;
   }
   __syncthreads();
-  write_row(a, row, token, at, finish(join(parts, a.slices, a.c), a.scale, a.c), best);
+  write_row<NT>(a, row, token, at, finish(join_parts(parts, a.slices, a.c), a.scale, a.c), best);
 }
 
-// Slices per row and vectors per slice: enough workgroups to fill the chip,
-// each with at least two vectors per lane.
+// Threads per workgroup, slices per row and 16-byte vectors per slice, us of
+// graph replays on one card (bf16; 0 / 20 alternatives):
+//   one wave per row where rows are short and many: [8192, 1000] 8.6 at 64
+//   threads, 24.4 at 256; [8192, 8192] 25.4, 25.2; fewer rows only up to 2048
+//   values, for the search that one wave does alone ([512, 8192] 6.2 / 13.6 at
+//   64, 5.5 / 8.6 at 256).  What is asked for does not enter: the statistics
+//   are the same bits with and without alternatives;
+//   1024 threads for rows of 64 KB and more, up to one per CU ([256, 50001]
+//   10.0 / 13.2, 256 threads 9.8 / 14.7; [512, 32000] 9.7 / 19.1, 9.5 / 13.6);
+//   slices of 16 KB and more of still longer rows where that fills the chip
+//   no more than twice: [64, 128000] one slice of 1024 threads 11.9 / 15.8, 4
+//   slices 8.9 / 13.7, 8 slices 8.5 / 12.9, 16 slices 8.6 / 14.5; [1, 200000]
+//   16.6 / 19.5, 8 slices 7.3 / 11.5, 16 slices 6.1 / 11.0; [256, 128000] 15.6 /
+//   19.3, 2 slices 16.5 / 23.6.
 struct Plan {
-  int slices, span;
+  int threads, slices, span;
 };
 
 inline Plan plan(int64_t rows, int64_t vocab, int elem_size) {
   const int64_t vectors = vocab / (16 / elem_size);
-  const int64_t want = std::min<int64_t>((kFill + rows - 1) / rows, kMaxSlices);
-  const int64_t most = std::max<int64_t>(1, vectors / (2 * kThreads));
+  int64_t slices = 1;
   Plan p;
-  const int64_t slices = std::min(want, most);
+  if (vectors <= (rows >= 1024 ? 1024 : 256)) {
+    p.threads = kWave;
+  } else if (rows <= 128 && vectors >= 6144) {
+    p.threads = kThreads;
+    slices = std::min({std::max<int64_t>(4, 512 / rows), vectors / 1024, kMaxSlices});
+  } else {
+    p.threads = rows <= 256 && vectors >= 4000 ? kLarge : kThreads;
+  }
   p.span = static_cast<int>(
-      ((vectors + slices - 1) / slices + kThreads - 1) / kThreads * kThreads);
-  p.slices = p.span == 0 ? 1 : static_cast<int>(std::max<int64_t>(1, (vectors + p.span - 1) / p.span));
+      ((vectors + slices - 1) / slices + p.threads - 1) / p.threads * p.threads);
+  p.slices = slices == 1 ? 1 : static_cast<int>((vectors + p.span - 1) / p.span);
   return p;
 }
 
@@ -711,7 +762,7 @@ extern "C" size_t hipo_token_logprobs_workspace_bytes(int64_t rows, int64_t voca
   // The most of either element size.
   const int slices = std::max(plan(rows, vocab, 2).slices, plan(rows, vocab, 4).slices);
   if (slices == 1) return 0;
-  return parts_bytes(rows, slices) + rows * slices * top * sizeof(uint64_t);
+  return parts_bytes(rows, slices) + (top ? rows * slices * kMaxTop * sizeof(uint64_t) : 0);
 }
 
 extern "C" int hipo_token_logprobs(const void* logits, int elem_size, const void* tokens,
@@ -751,19 +802,24 @@ extern "C" int hipo_token_logprobs(const void* logits, int elem_size, const void
                                               parts_bytes(rows, p.slices)),
                   0, vocab, row_stride, ignore_index, scale, scale * kLog2eHi, token_size,
                   static_cast<int>(top), p.slices, p.span,
-                  div_magic(static_cast<uint32_t>(p.slices))};
+                  std::max(1, p.span / p.threads), div_magic(static_cast<uint32_t>(p.slices)),
+                  div_magic(static_cast<uint32_t>(std::max(1, p.span / p.threads)))};
   const bool bf16 = elem_size == 2, ent = entropy != nullptr;
-#define HIPO_LP(T_)                                                            \
-  (top ? (ent ? logprobs_slices<T_, true, true> : logprobs_slices<T_, false, true>) \
-       : (ent ? logprobs_slices<T_, true, false> : logprobs_slices<T_, false, false>))
-  auto kernel = bf16 ? HIPO_LP(uint16_t) : HIPO_LP(float);
+#define HIPO_LP(N_, T_)                                                                    \
+  (top ? (ent ? logprobs_slices<N_, T_, true, true> : logprobs_slices<N_, T_, false, true>) \
+       : (ent ? logprobs_slices<N_, T_, true, false> : logprobs_slices<N_, T_, false, false>))
+#define HIPO_LP_N(N_) (bf16 ? HIPO_LP(N_, uint16_t) : HIPO_LP(N_, float))
+  auto kernel = p.threads == kWave      ? HIPO_LP_N(kWave)
+                : p.threads == kThreads ? HIPO_LP_N(kThreads)
+                                        : HIPO_LP_N(kLarge);
+#undef HIPO_LP_N
 #undef HIPO_LP
   auto join = bf16 ? (top ? join_slices<uint16_t, true> : join_slices<uint16_t, false>)
                    : (top ? join_slices<float, true> : join_slices<float, false>);
   const int64_t step = kMaxBlocks / p.slices;
   for (; a.first < rows; a.first += step) {
     const unsigned n = static_cast<unsigned>(std::min(step, rows - a.first));
-    kernel<<<dim3(n * p.slices), dim3(kThreads), 0, stream>>>(a);
+    kernel<<<dim3(n * p.slices), dim3(p.threads), 0, stream>>>(a);
     if (p.slices > 1) join<<<dim3(n), dim3(kThreads), 0, stream>>>(a);
   }
   return check_launch("token_logprobs");
