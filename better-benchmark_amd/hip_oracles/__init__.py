@@ -675,25 +675,51 @@ def batchnorm_nchw_act_mean(x, gamma, beta, running_mean, running_var, *, moment
 
 
 _FLOATS = (torch.bfloat16, torch.float32)
+_TOKENS = (torch.int32, torch.int64)
 
 
 def _require_tokens(what: str, tokens: torch.Tensor) -> None:
-    _require(tokens.dtype in (torch.int32, torch.int64) and tokens.is_contiguous(),
-             f"{what}: tokens must be contiguous int32 or int64")
+    if not (tokens.dtype in _TOKENS and tokens.is_contiguous()):
+        raise ValueError(f"{what}: tokens must be contiguous int32 or int64")
 
 
 def _require_logits(what: str, logits: torch.Tensor, tokens: torch.Tensor,
                     scale: float) -> tuple[int, int, int]:
+    """(rows, vocab, row stride).  One condition first: the messages are built
+    where it does not hold (a string per check costs a call 0.5 us)."""
+    if logits.dim() == 2:
+        rows, vocab = logits.shape
+        stride, inner = logits.stride()
+        if rows <= 1:
+            stride = vocab
+        if (logits.dtype in _FLOATS and tokens.shape == (rows,)
+                and tokens.dtype in _TOKENS and tokens.is_contiguous()
+                and 2.0 ** -100 <= scale <= 2.0 ** 100 and (inner == 1 or vocab <= 1)
+                and stride >= vocab):
+            return rows, vocab, stride
     _require(logits.dtype in _FLOATS and logits.dim() == 2,
              f"{what}: logits must be 2-D bf16 or fp32")
-    rows, vocab = logits.shape
     _require_tokens(what, tokens)
     _require(tokens.shape == (rows,), f"{what}: tokens must be [rows]")
     _require(2.0 ** -100 <= scale <= 2.0 ** 100, f"{what}: scale must be from 2^-100 to 2^100")
-    _require(logits.stride(1) == 1 or vocab <= 1, f"{what}: logits need a unit inner stride")
-    stride = logits.stride(0) if rows > 1 else vocab
+    _require(inner == 1 or vocab <= 1, f"{what}: logits need a unit inner stride")
     _require(stride >= vocab, f"{what}: rows of logits overlap")
-    return rows, vocab, stride
+    raise AssertionError(what)
+
+
+def _rows_apart_or_same(a: torch.Tensor, a_stride: int, b: torch.Tensor, b_stride: int,
+                        rows: int, cols: int) -> bool:
+    """Whether [rows, cols] at a and b, of one type, are the same memory or share none."""
+    size = a.element_size()
+    off = a.data_ptr() - b.data_ptr()
+    if rows == 0 or cols == 0 or (off == 0 and a_stride == b_stride):
+        return True
+    if (off >= ((rows - 1) * b_stride + cols) * size
+            or -off >= ((rows - 1) * a_stride + cols) * size):
+        return True
+    # Columns of one buffer's rows.
+    gap = off % (a_stride * size)
+    return a_stride == b_stride and cols * size <= gap <= (a_stride - cols) * size
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, scale: float = 1.0,
@@ -753,19 +779,22 @@ def token_logprobs_bwd(grad: torch.Tensor, logits: torch.Tensor, tokens: torch.T
     what = "token_logprobs_bwd"
     rows, vocab, stride = _require_logits(what, logits, tokens, scale)
     for t in rows_of:
-        _require(t.dtype == torch.float32 and t.shape == (rows,) and t.is_contiguous(),
-                 f"{what}: grad, lse, entropy, grad_entropy and grad_lse must be contiguous "
-                 f"fp32 [rows]")
+        if not (t.dtype == torch.float32 and t.shape == (rows,) and t.is_contiguous()):
+            raise ValueError(f"{what}: grad, lse, entropy, grad_entropy and grad_lse must be "
+                             f"contiguous fp32 [rows]")
     _require(grad_entropy is None or entropy is not None,
-             f"{what}: grad_entropy needs the entropy")
+             "token_logprobs_bwd: grad_entropy needs the entropy")
     if out is None:
         out = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
-    _require(out.dtype == logits.dtype and out.shape == logits.shape
-             and (out.stride(1) == 1 or vocab <= 1), f"{what}: out must match the logits")
-    out_stride = out.stride(0) if rows > 1 else vocab
-    _require(out_stride >= vocab, f"{what}: rows of out overlap")
-    _require(out.data_ptr() != logits.data_ptr() or out_stride == stride,
-             f"{what}: out and logits overlap")
+        out_stride = vocab
+    else:
+        _require(out.dtype == logits.dtype and out.shape == logits.shape
+                 and (out.stride(1) == 1 or vocab <= 1),
+                 "token_logprobs_bwd: out must match the logits")
+        out_stride = out.stride(0) if rows > 1 else vocab
+        _require(out_stride >= vocab, "token_logprobs_bwd: rows of out overlap")
+        _require(_rows_apart_or_same(out, out_stride, logits, stride, rows, vocab),
+                 "token_logprobs_bwd: out and logits overlap")
     _call(lib.hipo_token_logprobs_bwd, what, dev, _ptr(grad), _ptr(logits),
           logits.element_size(), _ptr(tokens), tokens.element_size(), _ptr(lse),
           *(None if t is None else _ptr(t) for t in (entropy, grad_entropy, grad_lse)),
