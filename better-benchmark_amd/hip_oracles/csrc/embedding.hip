@@ -19,8 +19,8 @@
 //      the sum of its few positions.  Where there are fewer tokens than rows
 //      it visits the rows that have one, and the others are zeroed by
 //      workgroups of the first launch, beside the sort.  Tokens that occur
-//      more than kPiece times are cut into pieces of kPiece positions, summed
-//      in the same launch into the workspace (fp32);
+//      more often than a piece is long are cut into pieces, summed in the same
+//      launch into the workspace (fp32);
 //   3. join_pieces: their rows, the sums of their pieces.
 #include <math.h>
 
@@ -216,32 +216,40 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens(SortArgs a) {
     reinterpret_cast<u32x4_t*>(&found[0][0])[i] = u32x4_t{0u, 0u, 0u, 0u};
   __syncthreads();
 
-  const auto own_row = [&](I x, int64_t at) -> int {
-    const int64_t t = x;
-    return at < to && t >= 0 && t < a.vocab && t != a.padding_idx &&
-                   static_cast<int>(t & (groups - 1)) == mine
-               ? static_cast<int>(t >> a.group_bits)
-               : -1;
+  // A token that counts is a 32-bit number; what it leaves modulo the number
+  // of groups, or no group's number.
+  const uint32_t vocab = static_cast<uint32_t>(a.vocab);
+  const uint32_t padding = a.padding_idx >= 0 && a.padding_idx < a.vocab
+                               ? static_cast<uint32_t>(a.padding_idx)
+                               : 0xffffffffu;
+  const uint32_t mask = static_cast<uint32_t>(groups) - 1;
+  const auto group_of = [&](I x, bool in) -> uint32_t {
+    const uint32_t t = static_cast<uint32_t>(x);
+    bool counts = in && t < vocab && t != padding;
+    if constexpr (sizeof(I) == 8) counts = counts && static_cast<uint64_t>(x) >> 32 == 0;
+    return counts ? t & mask : 0xffffffffu;
   };
+  const auto row_of = [&](I x) { return static_cast<int>(static_cast<uint32_t>(x) >> a.group_bits); };
 
-  int below = 0, held = 0;
+  int below = 0, held = 0;  // of the wave
   for (int64_t i0 = from; i0 < to; i0 += kSortLoads * kWave) {
     I now[kSortLoads];
 #pragma unroll
     for (int u = 0; u < kSortLoads; ++u) now[u] = v[u];
     if (i0 + kSortLoads * kWave < to) load_tokens(a, i0 + kSortLoads * kWave + lane, v);
     __builtin_amdgcn_sched_barrier(0);  // the next loads first
+    const bool whole = i0 + kSortLoads * kWave <= to;
 #pragma unroll
     for (int u = 0; u < kSortLoads; ++u) {
       const int64_t at = i0 + u * kWave + lane;
-      const int64_t t = now[u];
-      below += at < to && t >= 0 && t < a.vocab && t != a.padding_idx &&
-               static_cast<int>(t & (groups - 1)) < mine;
-      const int r = own_row(now[u], at);
-      const uint64_t m = __ballot(r >= 0);
+      const uint32_t g = group_of(now[u], whole || at < to);
+      below += __popcll(__ballot(g < static_cast<uint32_t>(mine)));
+      const bool own = g == static_cast<uint32_t>(mine);
+      const uint64_t m = __ballot(own);
       if (m == 0) continue;
       const int slot = held + __popcll(m & ((uint64_t{1} << lane) - 1));
-      if (r >= 0) {
+      if (own) {
+        const int r = row_of(now[u]);
         atomicAdd(&found[wave][r], 1);
         if (slot < kSortList)
           list[wave][slot] = static_cast<uint32_t>(at - from) << kSortRowBits | r;
@@ -249,8 +257,6 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens(SortArgs a) {
       held += __popcll(m);
     }
   }
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) below += __shfl_xor(below, d);
   if (lane == 0) wave_below[wave] = below;
   __syncthreads();
 
@@ -319,7 +325,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens(SortArgs a) {
         I x = now[0];  // now[u], kept in registers
 #pragma unroll
         for (int k = 1; k < kSortLoads; ++k) x = u == k ? now[k] : x;
-        write(own_row(x, at), at);
+        write(group_of(x, at < to) == static_cast<uint32_t>(mine) ? row_of(x) : -1, at);
       }
     }
   }
@@ -376,18 +382,18 @@ __device__ __forceinline__ void add_rows(float (&sum)[C], const BwdArgs& a, int 
   }
 }
 
-// Tokens with more than kPiece places are summed in pieces of kPiece places,
+// Tokens with more than kPiece places are summed in pieces of that many,
 // counted from the token's first place.  The sorted places are cut into bins
-// of kPiece: a bin holds the start of at most one piece after a token's first
-// (its sum is kept in sums[bin]) and of at most one first piece (in sums[bins +
-// bin]; its token reaches into the next bin).  The token of a bin's first
-// piece, count 0 if there is none:
+// of the same size: a bin holds the start of at most one piece after a token's
+// first (its sum is kept in sums[bin]) and of at most one first piece (in
+// sums[bins + bin]; its token reaches into the next bin).  The token of a bin's
+// first piece, count 0 if there is none:
 __device__ __forceinline__ Segment first_piece(const BwdArgs& a, int bin) {
   const int64_t probe = (int64_t{bin} + 1) * kPiece;
   const int total = *a.total;
   const Segment g = a.order[probe < a.places ? probe : a.places - 1].token;
-  const bool here = probe < total && g.count > kPiece && g.start >= bin * kPiece &&
-                    g.start < probe;
+  const bool here = probe < total && g.count > kPiece &&
+                    g.start >= bin * kPiece && g.start < probe;
   return here ? g : Segment{0, 0};
 }
 
@@ -404,7 +410,7 @@ __device__ __forceinline__ void piece_places(const BwdArgs& a, int64_t slot, int
     const int total = *a.total;
     g = a.order[probe].token;
     if (probe >= total || g.count <= kPiece) return;
-    const int at = g.start + (static_cast<int>(probe) - g.start + kPiece - 1) / kPiece * kPiece;
+    const int at = g.start + ((static_cast<int>(probe) - g.start + kPiece - 1) & -kPiece);
     if (at == g.start || at >= g.start + g.count) return;
     from = at;
   }
@@ -479,40 +485,54 @@ __global__ __launch_bounds__(kThreads) void sum_rows(BwdArgs a) {
   }
 }
 
-// The rows of tokens in pieces: a lane per C columns and bin.
+// The rows of tokens in pieces: a workgroup per bin and 64 lanes of C columns
+// each, its waves a quarter of the pieces each, added in order.
 template <typename O, int C, bool WHOLE, bool ADD>
 __global__ __launch_bounds__(kThreads) void join_pieces(BwdArgs a) {
-  constexpr int kFlight = 8;
-  const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
-  const uint32_t r = div_by(id, a.by_pieces);
-  if (r >= a.count) return;
-  const int col = static_cast<int>(id - r * a.pieces) * C;
+  constexpr int kWaves = kThreads / kWave, kFlight = 8;
+  __shared__ float part[kWaves][C][kWave];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+  const uint32_t r = div_by(blockIdx.x, a.by_pieces);
+  const int col = (static_cast<int>(blockIdx.x - r * a.pieces) * kWave + lane) * C;
   const int left = a.width - col;
   const int bin = static_cast<int>(a.first + r);
   const Segment g = first_piece(a, bin);
-  if (g.count == 0) return;
+  if (g.count == 0) return;  // the whole workgroup
   const int row = a.order[g.start].row;
   const float* sums = a.sums + col;
   const int n = (g.count + kPiece - 1) / kPiece;
+  const int each = (n + kWaves - 1) / kWaves;
+  const int to = std::min(n, (wave + 1) * each);
   float sum[C] = {};
-  for (int j0 = 0; j0 < n; j0 += kFlight) {
-    Values<float, C> x[kFlight];
+  if (left > 0) {
+    for (int j0 = wave * each; j0 < to; j0 += kFlight) {
+      Values<float, C> x[kFlight];
 #pragma unroll
-    for (int k = 0; k < kFlight; ++k) {
-      x[k].clear();
-      const int j = j0 + k;
-      if (j < n) {
-        const float* p = sums + ((j == 0 ? a.bins : 0) + int64_t{bin} + j) * a.width;
-        if (WHOLE || left >= C) x[k].load(p);
-        else x[k].load_part(p, left);
+      for (int k = 0; k < kFlight; ++k) {
+        x[k].clear();
+        const int j = j0 + k;
+        if (j < to) {
+          const float* p = sums + ((j == 0 ? a.bins : 0) + int64_t{bin} + j) * a.width;
+          if (WHOLE || left >= C) x[k].load(p);
+          else x[k].load_part(p, left);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) sum[c] += x[k].get(c);
       }
     }
-    __builtin_amdgcn_sched_barrier(0);
+  }
 #pragma unroll
-    for (int k = 0; k < kFlight; ++k) {
+  for (int c = 0; c < C; ++c) part[wave][c][lane] = sum[c];
+  __syncthreads();
+  if (wave != 0 || left <= 0) return;
 #pragma unroll
-      for (int c = 0; c < C; ++c) sum[c] += x[k].get(c);
-    }
+  for (int w = 1; w < kWaves; ++w) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) sum[c] += part[w][c][lane];
   }
   write_row<O, C, WHOLE, ADD>(a, row, col, sum);
 }
@@ -531,8 +551,9 @@ inline Layout layout(int64_t count, int64_t width, int64_t vocab) {
   l.segments = up(count * sizeof(Place));
   l.total = l.segments + up(vocab * sizeof(Segment));
   l.sums = l.total + 16;
-  // A token with more than kPiece places needs that many.
-  l.bytes = l.sums + (count > kPiece ? 2 * l.bins * width * sizeof(float) : 0);
+  // A token with more places than a piece needs that many.
+  if (count <= kPiece) l.bins = 0;
+  l.bytes = l.sums + 2 * l.bins * width * sizeof(float);
   return l;
 }
 
@@ -575,7 +596,6 @@ void launch_bwd(BwdArgs a, SortArgs s, int token_size, bool accumulate, hipStrea
     });
   };
   a.places = s.count;
-  if (s.count <= kPiece) a.bins = 0;
   if (accumulate) {
     run(whole ? sum_rows<T, O, C, true, true, true> : sum_rows<T, O, C, false, true, true>,
         2 * a.bins + s.count);
@@ -586,10 +606,16 @@ void launch_bwd(BwdArgs a, SortArgs s, int token_size, bool accumulate, hipStrea
     run(whole ? sum_rows<T, O, C, true, false, false> : sum_rows<T, O, C, false, false, false>,
         2 * a.bins + s.vocab);
   }
-  if (accumulate) {
-    run(whole ? join_pieces<O, C, true, true> : join_pieces<O, C, false, true>, a.bins);
-  } else {
-    run(whole ? join_pieces<O, C, true, false> : join_pieces<O, C, false, false>, a.bins);
+  if (a.bins == 0) return;
+  auto join = accumulate
+                  ? (whole ? join_pieces<O, C, true, true> : join_pieces<O, C, false, true>)
+                  : (whole ? join_pieces<O, C, true, false> : join_pieces<O, C, false, false>);
+  a.pieces = (a.pieces + kWave - 1) / kWave;  // workgroups per row
+  a.by_pieces = div_magic(a.pieces);
+  const int64_t step = std::max<int64_t>(1, kLanes / kThreads / a.pieces);
+  for (a.first = 0; a.first < a.bins; a.first += step) {
+    const int64_t n = std::min(step, a.bins - a.first) * a.pieces;
+    join<<<dim3(static_cast<unsigned>(n)), dim3(kThreads), 0, stream>>>(a);
   }
 }
 
@@ -646,7 +672,7 @@ extern "C" int hipo_embedding_bwd(const void* grad, int elem_size, const void* t
   HIPO_REQUIRE((elem_size == 2 || elem_size == 4) && (out_size == 2 || out_size == 4),
                "embedding_bwd: elem_size and out_size must be 2 or 4");
   HIPO_REQUIRE(token_size == 4 || token_size == 8, "embedding_bwd: token_size must be 4 or 8");
-  HIPO_REQUIRE(count <= 0x7fffffff - kPiece && width <= 0x7fffffff && vocab <= 0x7fffffff,
+  HIPO_REQUIRE(count <= 0x7fffffff - 4096 && width <= 0x7fffffff && vocab <= 0x7fffffff,
                "embedding_bwd: size over 2^31");
   if (width == 0 || vocab == 0) return 0;
   HIPO_REQUIRE(dweight != nullptr && (count == 0 || (grad != nullptr && tokens != nullptr)),
