@@ -25,6 +25,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "hipo_common.h"
 
@@ -165,13 +166,21 @@ __device__ __forceinline__ void fill_zeros(const SortArgs& a, int64_t block) {
   }
 }
 
-// kSortLoads tokens of a lane, 64 positions apart; past the end the last one.
+// kSortLoads tokens of a lane, 64 positions apart from `at` (of the wave) on;
+// past the end the last one.
 template <typename I>
 __device__ __forceinline__ void load_tokens(const SortArgs& a, int64_t at, I (&v)[kSortLoads]) {
-  const I* p = static_cast<const I*>(a.tokens);
+  const I* p = static_cast<const I*>(a.tokens) + at;
+  const int lane = threadIdx.x & (kWave - 1);
+  if (at + kSortLoads * kWave <= a.count) {
 #pragma unroll
-  for (int u = 0; u < kSortLoads; ++u)
-    v[u] = p[at + u * kWave < a.count ? at + u * kWave : a.count - 1];
+    for (int u = 0; u < kSortLoads; ++u) v[u] = p[lane + u * kWave];
+  } else {
+    const int last = static_cast<int>(a.count - 1 - at);
+#pragma unroll
+    for (int u = 0; u < kSortLoads; ++u) v[u] = p[std::min(lane + u * kWave, last)];
+  }
+  __builtin_amdgcn_sched_barrier(0);  // the loads first
 }
 
 // A wave's next places of the rows, one row per lane (-1: none), lanes in
@@ -194,13 +203,14 @@ __device__ __forceinline__ int take_places(int r, int* next, bool& last) {
 // between the count and the places.  A wave keeps what it finds in a list in
 // LDS; one that finds more than the list holds reads its part again.
 template <typename I>
-__global__ __launch_bounds__(kSortThreads) void sort_tokens(SortArgs a) {
+__global__ __launch_bounds__(kSortThreads, 8) void sort_tokens(SortArgs a) {
   __shared__ int found[kSortWaves][kSortRows];  // counts, then next places
   __shared__ Segment token[kSortRows];
   __shared__ uint32_t list[kSortWaves][kSortList];  // place in the part, row
   __shared__ int wave_count[kSortWaves];
   __shared__ int wave_below[kSortWaves];
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int groups = 1 << a.group_bits;
   const int mine = blockIdx.x;
   if (mine >= groups) {
@@ -210,8 +220,9 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens(SortArgs a) {
   const int64_t part = (a.count + kSortThreads - 1) / kSortThreads * kWave;  // of a wave
   const int64_t from = wave * part;
   const int64_t to = from + part < a.count ? from + part : a.count;
-  I v[kSortLoads];
-  if (from < to) load_tokens(a, from + lane, v);
+  constexpr int kBatch = kSortLoads * kWave;
+  I v[2][kSortLoads];  // a batch and the one after it
+  if (from < to) load_tokens(a, from, v[0]);
   for (int i = tid; i < kSortWaves * kSortRows / 4; i += kSortThreads)
     reinterpret_cast<u32x4_t*>(&found[0][0])[i] = u32x4_t{0u, 0u, 0u, 0u};
   __syncthreads();
@@ -232,30 +243,35 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens(SortArgs a) {
   const auto row_of = [&](I x) { return static_cast<int>(static_cast<uint32_t>(x) >> a.group_bits); };
 
   int below = 0, held = 0;  // of the wave
-  for (int64_t i0 = from; i0 < to; i0 += kSortLoads * kWave) {
-    I now[kSortLoads];
-#pragma unroll
-    for (int u = 0; u < kSortLoads; ++u) now[u] = v[u];
-    if (i0 + kSortLoads * kWave < to) load_tokens(a, i0 + kSortLoads * kWave + lane, v);
-    __builtin_amdgcn_sched_barrier(0);  // the next loads first
-    const bool whole = i0 + kSortLoads * kWave <= to;
+  const auto scan = [&](auto whole, const I (&x)[kSortLoads], int64_t i0) {
+    const int left = static_cast<int>(std::min<int64_t>(to - i0, kBatch));
+    const uint32_t part_at = static_cast<uint32_t>(i0 - from) + lane;
 #pragma unroll
     for (int u = 0; u < kSortLoads; ++u) {
-      const int64_t at = i0 + u * kWave + lane;
-      const uint32_t g = group_of(now[u], whole || at < to);
+      const uint32_t g = group_of(x[u], whole || u * kWave + lane < left);
       below += __popcll(__ballot(g < static_cast<uint32_t>(mine)));
       const bool own = g == static_cast<uint32_t>(mine);
       const uint64_t m = __ballot(own);
       if (m == 0) continue;
       const int slot = held + __popcll(m & ((uint64_t{1} << lane) - 1));
       if (own) {
-        const int r = row_of(now[u]);
+        const int r = row_of(x[u]);
         atomicAdd(&found[wave][r], 1);
-        if (slot < kSortList)
-          list[wave][slot] = static_cast<uint32_t>(at - from) << kSortRowBits | r;
+        if (slot < kSortList) list[wave][slot] = (part_at + u * kWave) << kSortRowBits | r;
       }
       held += __popcll(m);
     }
+  };
+  const auto scan_batch = [&](const I (&x)[kSortLoads], int64_t i0) {
+    if (i0 + kBatch <= to) scan(std::true_type{}, x, i0);
+    else scan(std::false_type{}, x, i0);
+  };
+  for (int64_t i0 = from; i0 < to; i0 += 2 * kBatch) {
+    if (i0 + kBatch < to) load_tokens(a, i0 + kBatch, v[1]);
+    scan_batch(v[0], i0);
+    if (i0 + kBatch >= to) break;
+    if (i0 + 2 * kBatch < to) load_tokens(a, i0 + 2 * kBatch, v[0]);
+    scan_batch(v[1], i0 + kBatch);
   }
   if (lane == 0) wave_below[wave] = below;
   __syncthreads();
@@ -312,20 +328,16 @@ __global__ __launch_bounds__(kSortThreads) void sort_tokens(SortArgs a) {
       write(in ? static_cast<int>(e & (kSortRows - 1)) : -1, from + (e >> kSortRowBits));
     }
   } else {
-    load_tokens(a, from + lane, v);
-    for (int64_t i0 = from; i0 < to; i0 += kSortLoads * kWave) {
-      I now[kSortLoads];
-#pragma unroll
-      for (int u = 0; u < kSortLoads; ++u) now[u] = v[u];
-      if (i0 + kSortLoads * kWave < to) load_tokens(a, i0 + kSortLoads * kWave + lane, v);
-      __builtin_amdgcn_sched_barrier(0);
+    for (int64_t i0 = from; i0 < to; i0 += kBatch) {
+      load_tokens(a, i0, v[0]);
+      const int left = static_cast<int>(std::min<int64_t>(to - i0, kBatch));
 #pragma unroll 1
       for (int u = 0; u < kSortLoads; ++u) {
-        const int64_t at = i0 + u * kWave + lane;
-        I x = now[0];  // now[u], kept in registers
+        I x = v[0][0];  // v[0][u], kept in registers
 #pragma unroll
-        for (int k = 1; k < kSortLoads; ++k) x = u == k ? now[k] : x;
-        write(group_of(x, at < to) == static_cast<uint32_t>(mine) ? row_of(x) : -1, at);
+        for (int k = 1; k < kSortLoads; ++k) x = u == k ? v[0][k] : x;
+        const uint32_t g = group_of(x, u * kWave + lane < left);
+        write(g == static_cast<uint32_t>(mine) ? row_of(x) : -1, i0 + u * kWave + lane);
       }
     }
   }
