@@ -742,11 +742,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, scale: float =
              "token_logprobs: top must be at most 64 and at most the vocabulary")
     _require(vocab > 0 or rows == 0, "token_logprobs: empty vocabulary")
     logprob = torch.empty(rows, dtype=torch.float32, device=dev)
-    lse = torch.empty(rows, dtype=torch.float32, device=dev)
+    lse = torch.empty_like(logprob)
     out = [logprob, lse]
     ptrs = [None, None, None]
     if entropy:
-        out.append(torch.empty(rows, dtype=torch.float32, device=dev))
+        out.append(torch.empty_like(logprob))
         ptrs[0] = _ptr(out[-1])
     if top:
         out.append(torch.empty((rows, top), dtype=torch.float32, device=dev))
@@ -813,8 +813,10 @@ def embedding(weight: torch.Tensor, tokens: torch.Tensor, *, scale: float = 1.0)
              "embedding: weight must be 2-D bf16 or fp32")
     _require_tokens("embedding", tokens)
     vocab, width = weight.shape
-    _require(weight.stride(1) == 1 or width <= 1, "embedding: weight needs a unit inner stride")
-    stride = weight.stride(0) if vocab > 1 else width
+    stride, inner = weight.stride()
+    _require(inner == 1 or width <= 1, "embedding: weight needs a unit inner stride")
+    if vocab <= 1:
+        stride = width
     _require(stride >= width, "embedding: rows of weight overlap")
     out = torch.empty((*tokens.shape, width), dtype=weight.dtype, device=dev)
     _call(lib.hipo_embedding, "embedding", dev, _ptr(weight), weight.element_size(),
