@@ -133,6 +133,37 @@ def test_forward_ignored_and_unknown_tokens(rows, vocab, dtype, rocm_device, ho)
     assert (got[0][t == t[4]] == 0).all() and (got[3][t.to(rocm_device) == t[4]] == -1).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab", [
+    (511, 2049), (1023, 4100), (1024, 4096), (1024, 8200), (300, 2048), (128, 24600), (129, 24600),
+    (127, 49160), (129, 49152), (256, 32000), (257, 32003), (5, 49151), (40, 60001)])
+def test_forward_where_the_workgroups_change(rows, vocab, dtype, rocm_device, ho):
+    x, t = make_logits(rows, vocab, dtype, "plain", vocab - rows)
+    check_forward(ho, rocm_device, x, t, top=3, shift=rows % 2, what=f"[{rows}, {vocab}] {dtype}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab", [(2, 4096), (3, 30000), (130, 32768), (2, 131072)])
+def test_alternatives_that_a_few_lanes_hold(rows, vocab, dtype, rocm_device, ho):
+    """Every second run of 32 16-byte vectors far above the others: the largest
+    of 64 lanes' values say little."""
+    g = torch.Generator().manual_seed(vocab)
+    run = 32 * 16 // dtype.itemsize
+    x = torch.randn(rows, vocab, generator=g) + 50.0 * ((torch.arange(vocab) // run) % 2)
+    t = torch.randint(0, vocab, (rows,), generator=g)
+    for top in (20, 33, 64):
+        check_forward(ho, rocm_device, x.to(dtype), t, top=top, what=f"stripes {vocab} {top}")
+
+
+@pytest.mark.parametrize("rows,vocab", [(4, 5000), (3, 70000)])
+def test_alternatives_where_one_number_fills_the_row(rows, vocab, rocm_device, ho):
+    """fp32 logits that no bf16 value is near: a mask of -1e9 with fewer places
+    left than alternatives asked for, the rest ties."""
+    x = torch.full((rows, vocab), -1e9)
+    x[:, 7::vocab // 5] = torch.randn(rows, len(range(7, vocab, vocab // 5)))
+    check_forward(ho, rocm_device, x, torch.full((rows,), 7), top=20, what="masked by -1e9")
+
+
 def test_forward_is_the_same_alone_and_in_a_batch_of_its_kind(rocm_device, ho):
     x, t = make_logits(300, 9001, BF16, "plain", 8)
     xd, td = x.to(rocm_device), t.to(rocm_device)
@@ -265,13 +296,28 @@ def ids_of(kind, count, vocab, g):
     return t
 
 
+def test_ids_past_32_bits(rocm_device, ho):
+    """int64 ids whose lower half alone would be one of the vocabulary."""
+    far = torch.tensor([3 + (1 << 32), 3 - (1 << 32), 2, 3 + (1 << 40), 3])
+    x, _ = make_logits(5, 50, F32, "plain", 1)
+    lp = ho.token_logprobs(x.to(rocm_device), far.to(rocm_device))[0].cpu()
+    assert lp.isnan().tolist() == [True, True, False, True, False]
+    w = torch.randn(50, 8, device=rocm_device)
+    e = ho.embedding(w, far.to(rocm_device))
+    assert e.isnan().all(-1).tolist() == [True, True, False, True, False]
+    dw = ho.embedding_bwd(torch.ones(5, 8, device=rocm_device), far.to(rocm_device), 50)
+    assert dw[2].eq(1).all() and dw[3].eq(1).all() and float(dw.sum()) == 16.0
+
+
 @pytest.mark.parametrize("dtype,out", [(BF16, BF16), (BF16, F32), (F32, F32), (F32, BF16)])
 @pytest.mark.parametrize("count,width,vocab,kind", [
     (0, 64, 50, "uniform"), (1, 1, 1, "one"), (1, 64, 1000, "uniform"), (7, 5, 3, "uniform"),
     (64, 96, 64, "runs"), (65, 768, 3000, "text"), (1000, 1001, 517, "text"),
     (4096, 40, 50001, "text"), (5000, 264, 70, "uniform"), (20000, 16, 3, "uniform"),
     (70001, 8, 1025, "text"), (3000, 2048, 11, "one"), (9000, 8, 2000, "one"),
-    (300, 4096, 100, "unknown"), (2049, 33, 131073, "uniform")])
+    (300, 4096, 100, "unknown"), (2049, 33, 131073, "uniform"), (32, 24, 1, "one"),
+    (33, 24, 1, "one"), (64, 24, 2, "one"), (96, 24, 3, "runs"), (16384, 24, 9000, "text"),
+    (33000, 8, 300000, "text"), (8193, 64, 8192, "runs")])
 def test_embedding_backward(count, width, vocab, kind, dtype, out, rocm_device, ho):
     g = torch.Generator().manual_seed(count + width)
     t = ids_of(kind, count, vocab, g)
@@ -333,6 +379,9 @@ def test_refusals(rocm_device, ho):
         lambda: ho.token_logprobs_bwd(f, x, t, f, out=x[:, :8]),
         lambda: ho.token_logprobs_bwd(f, x.view(-1)[:32].view(4, 8), t, f,
                                       out=x.view(-1)[:64].view(4, 16)[:, :8]),
+        lambda: ho.token_logprobs_bwd(f, x.view(-1)[:32].view(4, 8), t, f,
+                                      out=x.view(-1)[1:33].view(4, 8)),
+        lambda: ho.token_logprobs_bwd(f, x[:, :8], t, f, out=x[:, 4:12]),
         lambda: ho.embedding(x.half(), t), lambda: ho.embedding(x, t.float()),
         lambda: ho.embedding(x.t(), t), lambda: ho.embedding(x[0], t),
         lambda: ho.embedding(x[:1].expand(4, 16), t),
@@ -349,6 +398,17 @@ def test_refusals(rocm_device, ho):
         with pytest.raises(ValueError):
             call()
             print(f"refusal {k} was not one")
+
+
+def test_backward_into_other_columns_of_the_logits_buffer(rocm_device, ho):
+    x, t = make_logits(6, 200, F32, "plain", 4)
+    buf = torch.zeros(6, 400, device=rocm_device)
+    buf[:, :200] = x.to(rocm_device)
+    g = torch.ones(6, device=rocm_device)
+    _, lse = ho.token_logprobs(buf[:, :200], t.to(rocm_device))
+    want = ho.token_logprobs_bwd(g, x.to(rocm_device), t.to(rocm_device), lse)
+    ho.token_logprobs_bwd(g, buf[:, :200], t.to(rocm_device), lse, out=buf[:, 200:])
+    assert torch.equal(buf[:, 200:], want) and torch.equal(buf[:, :200].cpu(), x)
 
 
 def test_empty_calls(rocm_device, ho):
