@@ -14,15 +14,19 @@
 //      order of position.  A workgroup owns the tokens with one remainder
 //      modulo the number of workgroups (a vocabulary is ordered by frequency:
 //      ranges of it would give one workgroup most of the tokens) and scans all
-//      tokens twice, for the counts and for the places: no exchange between
-//      workgroups, no atomics on memory, and the scan is a small part of
-//      reading the gradient rows (8 bytes of a token from the L2 against
-//      hundreds to thousands).
-//   2. sum_rows: a lane per 16 bytes of a gradient row's columns and row of dw:
-//      the sum of its few positions.  Where there are fewer tokens than rows
-//      it visits the rows that have one, and the others are zeroed by
-//      workgroups of the first launch, beside the sort.  Tokens that occur
-//      more often than a piece is long are cut into pieces, summed in the same
+//      tokens, counting the smaller remainders on the way: no exchange between
+//      workgroups, no atomics on memory.  Arithmetic bounds the scan, about
+//      200 cycles per 64 tokens and SIMD: 6.6 us at 8192 tokens, 21 us at
+//      65536.
+//      Other workgroups of the same launch write zeros to all of dw: most of
+//      the bytes where tokens are fewer than rows ([128000, 4096] bf16 170 us,
+//      6.2 TB/s), and beside the sort hardly any time where they are not (rows
+//      without a token found and zeroed by sum_rows instead: [65536, 2048] into
+//      [32000, 2048] 106.5 us against 101.4, [65536, 64] into [1696, 64] 38.2
+//      against 39.1).
+//   2. sum_rows: a lane per 16 bytes of a gradient row's columns and place that
+//      starts a token: the sum of its few positions.  Tokens that occur more
+//      often than a piece is long are cut into pieces, summed in the same
 //      launch into the workspace (fp32);
 //   3. join_pieces: their rows, the sums of their pieces.
 #include <math.h>
@@ -45,7 +49,6 @@ constexpr int kSortRowBits = 9;
 constexpr int64_t kSortPart = int64_t{1} << (32 - kSortRowBits);  // positions a list can tell
 constexpr int kSortGroups = 256;     // at least: one workgroup per CU
 constexpr int kPiece = 32;           // positions per piece of a frequent token
-constexpr int kFillStores = 1;       // 16-byte stores of zeros per thread
 constexpr int64_t kLanes = int64_t{1} << 30;  // lanes per launch
 
 __device__ __forceinline__ int64_t token_at(const void* tokens, int size, int64_t i) {
@@ -148,7 +151,6 @@ struct Place {
 
 struct SortArgs {
   const void* tokens;
-  Segment* segments;  // [vocab], or null
   Place* order;       // [count]
   int* total;         // tokens that count
   uint16_t* fill;     // zeroed by the workgroups after the sorting ones
@@ -157,16 +159,13 @@ struct SortArgs {
   int group_bits;     // 2^group_bits sorting workgroups
 };
 
-// Zeros, kFillStores 16-byte stores per thread.
+// Zeros, 16 bytes per thread (64: [128000, 4096] bf16 221 us instead of 173).
 __device__ __forceinline__ void fill_zeros(const SortArgs& a, int64_t block) {
   Values<uint16_t, 8> zero;
   zero.clear();
-#pragma unroll
-  for (int u = 0; u < kFillStores; ++u) {
-    const int64_t at = ((block * kFillStores + u) * kSortThreads + threadIdx.x) * 8;
-    if (at + 8 <= a.fill_values) zero.store_stream(a.fill + at);
-    else if (at < a.fill_values) zero.store_part(a.fill + at, static_cast<int>(a.fill_values - at));
-  }
+  const int64_t at = (block * kSortThreads + threadIdx.x) * 8;
+  if (at + 8 <= a.fill_values) zero.store_stream(a.fill + at);
+  else if (at < a.fill_values) zero.store_part(a.fill + at, static_cast<int>(a.fill_values - at));
 }
 
 // kSortLoads tokens of a lane, 64 positions apart from `at` (of the wave) on;
@@ -309,8 +308,6 @@ __global__ __launch_bounds__(kSortThreads, 8) void sort_tokens(SortArgs a) {
       found[w][tid] = next;
       next += c;
     }
-    const int64_t row = (static_cast<int64_t>(tid) << a.group_bits) + mine;
-    if (a.segments != nullptr && row < a.vocab) a.segments[row] = g;
     if (mine == groups - 1 && tid == kSortRows - 1) *a.total = start + n;
   }
   __syncthreads();
@@ -349,7 +346,6 @@ __global__ __launch_bounds__(kSortThreads, 8) void sort_tokens(SortArgs a) {
 struct BwdArgs {
   const void* grad;
   void* dw;
-  const Segment* segments;
   const Place* order;
   const int* total;
   float* sums;           // [2 * bins][width], see first_piece
@@ -434,28 +430,36 @@ __device__ __forceinline__ void piece_places(const BwdArgs& a, int64_t slot, int
   to = std::min(from + kPiece, g.start + g.count);
 }
 
+// A lane's C columns of a row of dw.
 template <typename O, int C, bool WHOLE, bool ADD>
-__device__ __forceinline__ void write_row(const BwdArgs& a, int64_t row, int col,
-                                          float (&sum)[C]) {
-  O* dw = static_cast<O*>(a.dw) + row * a.width + col;
-  const int left = a.width - col;
-  Values<O, C> v;
-  if constexpr (ADD) {
-    if (WHOLE || left >= C) v.load(dw);
-    else v.load_part(dw, left);
-  }
-#pragma unroll
-  for (int c = 0; c < C; ++c) sum[c] = ADD ? v.get(c) + sum[c] * a.scale : sum[c] * a.scale;
-  v.set(sum);
-  if (WHOLE || left >= C) v.store_stream(dw);
-  else v.store_part(dw, left);
-}
+struct Row {
+  O* dw;
+  int left;
+  Values<O, C> had;
 
-// A lane per C columns of a piece (the first 2 * bins slots) or of a row of
-// dw.  PLACES: the rows of the places that start a token (those without one
-// are zeros already, or stay); otherwise every row.  Rows of tokens in pieces
-// are left to join_pieces.  ADD: added to dw.
-template <typename T, typename O, int C, bool WHOLE, bool PLACES, bool ADD>
+  // What is there is loaded at once: beside the gradient rows, not after them.
+  __device__ __forceinline__ Row(const BwdArgs& a, int64_t row, int col)
+      : dw(static_cast<O*>(a.dw) + row * a.width + col), left(a.width - col) {
+    if constexpr (ADD) {
+      if (WHOLE || left >= C) had.load(dw);
+      else had.load_part(dw, left);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  __device__ __forceinline__ void write(float (&sum)[C], float scale) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) sum[c] = ADD ? had.get(c) + sum[c] * scale : sum[c] * scale;
+    had.set(sum);
+    if (WHOLE || left >= C) had.store_stream(dw);
+    else had.store_part(dw, left);
+  }
+};
+
+// A lane per C columns of a piece (the first 2 * bins slots) or of a place:
+// one that starts a token sums and writes its row.  Tokens in pieces are left
+// to join_pieces; rows without a token are zeros already, or stay.  ADD: added
+// to dw.
+template <typename T, typename O, int C, bool WHOLE, bool ADD>
 __global__ __launch_bounds__(kThreads) void sum_rows(BwdArgs a) {
   const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
   const uint32_t r = div_by(id, a.by_pieces);
@@ -463,43 +467,35 @@ __global__ __launch_bounds__(kThreads) void sum_rows(BwdArgs a) {
   const int col = static_cast<int>(id - r * a.pieces) * C;
   const int left = a.width - col;
   const int64_t slot = a.first + r;
-  int64_t row = slot - 2 * a.bins;
-  int from, to;
   float sum[C] = {};
-  if (row < 0) {
+  if (slot < 2 * a.bins) {
+    int from, to;
     piece_places(a, slot, from, to);
     if (from == to) return;
-  } else if constexpr (PLACES) {
-    const int total = *a.total;
-    // One load for all of it, beside the total's.
-    const Place p = __builtin_bit_cast(Place, *reinterpret_cast<const u32x4_t*>(a.order + row));
-    if (row >= total || p.token.start != row || p.token.count > kPiece) return;
-    from = p.token.start + 1;
-    to = p.token.start + p.token.count;
-    row = p.row;
-    // Its first position is in hand.
-    const T* grad = static_cast<const T*>(a.grad) + int64_t{p.position} * a.width + col;
-    Values<T, C> x;
-    if (WHOLE || left >= C) x.load_stream(grad);
-    else x.load_part(grad, left);
-#pragma unroll
-    for (int c = 0; c < C; ++c) sum[c] += x.get(c);
-  } else {
-    const Segment g = a.segments[row];
-    if (g.count > kPiece) return;
-    from = g.start;
-    to = g.start + g.count;
-  }
-  add_rows<T, C, WHOLE, 8>(sum, a, from, to, col);
-  if (row >= 0) {
-    write_row<O, C, WHOLE, ADD>(a, row, col, sum);
-  } else {
+    add_rows<T, C, WHOLE, 8>(sum, a, from, to, col);
     float* p = a.sums + slot * a.width + col;
     Values<float, C> v;
     v.set(sum);
     if (WHOLE || left >= C) v.store(p);
     else v.store_part(p, left);
+    return;
   }
+  const int64_t place = slot - 2 * a.bins;
+  const int total = *a.total;
+  // One load for all of it, beside the total's.
+  const Place p = __builtin_bit_cast(Place, *reinterpret_cast<const u32x4_t*>(a.order + place));
+  const Segment g = p.token;
+  if (place >= total || g.start != place || g.count > kPiece) return;
+  // Its first position is in hand.
+  const T* grad = static_cast<const T*>(a.grad) + int64_t{p.position} * a.width + col;
+  Values<T, C> x;
+  if (WHOLE || left >= C) x.load_stream(grad);
+  else x.load_part(grad, left);
+  Row<O, C, WHOLE, ADD> out(a, p.row, col);
+#pragma unroll
+  for (int c = 0; c < C; ++c) sum[c] += x.get(c);
+  add_rows<T, C, WHOLE, 8>(sum, a, g.start + 1, g.start + g.count, col);
+  out.write(sum, a.scale);
 }
 
 // The rows of tokens in pieces: a workgroup per bin and 64 lanes of C columns
@@ -551,22 +547,21 @@ __global__ __launch_bounds__(kThreads) void join_pieces(BwdArgs a) {
 #pragma unroll
     for (int c = 0; c < C; ++c) sum[c] += part[w][c][lane];
   }
-  write_row<O, C, WHOLE, ADD>(a, row, col, sum);
+  Row<O, C, WHOLE, ADD>(a, row, col).write(sum, a.scale);
 }
 
-// Workspace: the order, the rows' segments, the number of places, the sums of
-// pieces; each 16-byte aligned.
+// Workspace: the order, the number of places, the sums of pieces; each 16-byte
+// aligned.
 struct Layout {
   int64_t bins;
-  size_t segments, total, sums, bytes;
+  size_t total, sums, bytes;
 };
 
-inline Layout layout(int64_t count, int64_t width, int64_t vocab) {
+inline Layout layout(int64_t count, int64_t width) {
   const auto up = [](size_t n) { return (n + 15) / 16 * 16; };
   Layout l;
   l.bins = (count + kPiece - 1) / kPiece;
-  l.segments = up(count * sizeof(Place));
-  l.total = l.segments + up(vocab * sizeof(Segment));
+  l.total = up(count * sizeof(Place));
   l.sums = l.total + 16;
   // A token with more places than a piece needs that many.
   if (count <= kPiece) l.bins = 0;
@@ -590,39 +585,27 @@ void launch_bwd(BwdArgs a, SortArgs s, int token_size, bool accumulate, hipStrea
   const bool whole = a.width % C == 0;
   a.pieces = (a.width + C - 1) / C;
   a.by_pieces = div_magic(a.pieces);
-  const bool fill = !accumulate && s.count < s.vocab;
-  const bool places = accumulate || fill;
+  if (accumulate && s.count == 0) return;
   int64_t fill_blocks = 0;
-  if (fill) {
-    constexpr int64_t kPerBlock = int64_t{kSortThreads} * kFillStores * 8;
+  if (!accumulate) {
+    constexpr int64_t kPerBlock = int64_t{kSortThreads} * 8;
     s.fill = static_cast<uint16_t*>(a.dw);
     s.fill_values = s.vocab * a.width * static_cast<int64_t>(sizeof(O) / 2);
     fill_blocks = (s.fill_values + kPerBlock - 1) / kPerBlock;
   }
-  if (places) s.segments = nullptr;
-  if (s.count > 0 || fill) {
-    auto kernel = token_size == 8 ? sort_tokens<int64_t> : sort_tokens<int32_t>;
-    kernel<<<dim3(static_cast<unsigned>((int64_t{1} << s.group_bits) + fill_blocks)),
-             dim3(kSortThreads), 0, stream>>>(s);
-  }
-  const auto run = [&](auto kernel, int64_t slots) {
-    for_lanes(slots, a.pieces, [&](int64_t first, int64_t n, dim3 grid) {
-      a.first = first;
-      a.count = n;
-      kernel<<<grid, dim3(kThreads), 0, stream>>>(a);
-    });
-  };
+  auto sort = token_size == 8 ? sort_tokens<int64_t> : sort_tokens<int32_t>;
+  sort<<<dim3(static_cast<unsigned>((int64_t{1} << s.group_bits) + fill_blocks)),
+         dim3(kSortThreads), 0, stream>>>(s);
+  if (s.count == 0) return;
   a.places = s.count;
-  if (accumulate) {
-    run(whole ? sum_rows<T, O, C, true, true, true> : sum_rows<T, O, C, false, true, true>,
-        2 * a.bins + s.count);
-  } else if (fill) {
-    run(whole ? sum_rows<T, O, C, true, true, false> : sum_rows<T, O, C, false, true, false>,
-        2 * a.bins + s.count);
-  } else {
-    run(whole ? sum_rows<T, O, C, true, false, false> : sum_rows<T, O, C, false, false, false>,
-        2 * a.bins + s.vocab);
-  }
+  auto rows = accumulate
+                  ? (whole ? sum_rows<T, O, C, true, true> : sum_rows<T, O, C, false, true>)
+                  : (whole ? sum_rows<T, O, C, true, false> : sum_rows<T, O, C, false, false>);
+  for_lanes(2 * a.bins + s.count, a.pieces, [&](int64_t first, int64_t n, dim3 grid) {
+    a.first = first;
+    a.count = n;
+    rows<<<grid, dim3(kThreads), 0, stream>>>(a);
+  });
   if (a.bins == 0) return;
   auto join = accumulate
                   ? (whole ? join_pieces<O, C, true, true> : join_pieces<O, C, false, true>)
@@ -675,7 +658,7 @@ extern "C" int hipo_embedding(const void* weight, int elem_size, const void* tok
 extern "C" size_t hipo_embedding_bwd_workspace_bytes(int64_t count, int64_t width,
                                                      int64_t vocab) {
   if (count < 0 || width <= 0 || vocab <= 0) return 0;
-  return hipo::layout(count, width, vocab).bytes;
+  return hipo::layout(count, width).bytes;
 }
 
 extern "C" int hipo_embedding_bwd(const void* grad, int elem_size, const void* tokens,
@@ -694,7 +677,7 @@ extern "C" int hipo_embedding_bwd(const void* grad, int elem_size, const void* t
   if (width == 0 || vocab == 0) return 0;
   HIPO_REQUIRE(dweight != nullptr && (count == 0 || (grad != nullptr && tokens != nullptr)),
                "embedding_bwd: null pointer");
-  const Layout l = layout(count, width, vocab);
+  const Layout l = layout(count, width);
   HIPO_REQUIRE(workspace != nullptr && workspace_bytes >= l.bytes,
                "embedding_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, l.bytes);
   HIPO_REQUIRE(aligned16(workspace), "embedding_bwd: workspace must be 16-byte aligned");
@@ -703,13 +686,12 @@ extern "C" int hipo_embedding_bwd(const void* grad, int elem_size, const void* t
   a.grad = grad;
   a.dw = dweight;
   a.order = reinterpret_cast<Place*>(ws);
-  a.segments = reinterpret_cast<Segment*>(ws + l.segments);
   a.total = reinterpret_cast<int*>(ws + l.total);
   a.sums = reinterpret_cast<float*>(ws + l.sums);
   a.bins = l.bins;
   a.width = static_cast<int>(width);
   a.scale = scale;
-  SortArgs s{tokens, reinterpret_cast<Segment*>(ws + l.segments), reinterpret_cast<Place*>(ws),
+  SortArgs s{tokens, reinterpret_cast<Place*>(ws),
              reinterpret_cast<int*>(ws + l.total), nullptr, 0, count, vocab, padding_idx, 0};
   while ((int64_t{1} << s.group_bits) < kSortGroups ||
          (int64_t{kSortRows} << s.group_bits) < vocab) {
