@@ -50,6 +50,7 @@ constexpr int64_t kSortPart = int64_t{1} << (32 - kSortRowBits);  // positions a
 constexpr int kSortGroups = 256;     // at least: one workgroup per CU
 constexpr int kPiece = 32;           // positions per piece of a frequent token
 constexpr int64_t kLanes = int64_t{1} << 30;  // lanes per launch
+constexpr int64_t kFillBlocks = int64_t{1} << 21;  // with 2^21 sorting ones 2^32 threads
 
 __device__ __forceinline__ int64_t token_at(const void* tokens, int size, int64_t i) {
   return size == 8 ? static_cast<const int64_t*>(tokens)[i]
@@ -159,13 +160,16 @@ struct SortArgs {
   int group_bits;     // 2^group_bits sorting workgroups
 };
 
-// Zeros, 16 bytes per thread (64: [128000, 4096] bf16 221 us instead of 173).
-__device__ __forceinline__ void fill_zeros(const SortArgs& a, int64_t block) {
+// Zeros, 16 bytes per thread (64: [128000, 4096] bf16 221 us instead of 173);
+// more where dw is over kFillBlocks * 16 KiB.
+__device__ __forceinline__ void fill_zeros(const SortArgs& a, int64_t block, int64_t blocks) {
   Values<uint16_t, 8> zero;
   zero.clear();
-  const int64_t at = (block * kSortThreads + threadIdx.x) * 8;
-  if (at + 8 <= a.fill_values) zero.store_stream(a.fill + at);
-  else if (at < a.fill_values) zero.store_part(a.fill + at, static_cast<int>(a.fill_values - at));
+  for (int64_t at = (block * kSortThreads + threadIdx.x) * 8; at < a.fill_values;
+       at += blocks * kSortThreads * 8) {
+    if (at + 8 <= a.fill_values) zero.store_stream(a.fill + at);
+    else zero.store_part(a.fill + at, static_cast<int>(a.fill_values - at));
+  }
 }
 
 // kSortLoads tokens of a lane, 64 positions apart from `at` (of the wave) on;
@@ -216,7 +220,7 @@ __global__ __launch_bounds__(kSortThreads, 8) void sort_tokens(SortArgs a) {
   const int groups = 1 << a.group_bits;
   const int mine = blockIdx.x;
   if (mine >= groups) {
-    fill_zeros(a, mine - groups);
+    fill_zeros(a, mine - groups, gridDim.x - groups);
     return;
   }
   const int64_t part = (a.count + kSortThreads - 1) / kSortThreads * kWave;  // of a wave
@@ -591,7 +595,7 @@ void launch_bwd(BwdArgs a, SortArgs s, int token_size, bool accumulate, hipStrea
     constexpr int64_t kPerBlock = int64_t{kSortThreads} * 8;
     s.fill = static_cast<uint16_t*>(a.dw);
     s.fill_values = s.vocab * a.width * static_cast<int64_t>(sizeof(O) / 2);
-    fill_blocks = (s.fill_values + kPerBlock - 1) / kPerBlock;
+    fill_blocks = std::min((s.fill_values + kPerBlock - 1) / kPerBlock, kFillBlocks);
   }
   auto sort = token_size == 8 ? sort_tokens<int64_t> : sort_tokens<int32_t>;
   sort<<<dim3(static_cast<unsigned>((int64_t{1} << s.group_bits) + fill_blocks)),
@@ -672,8 +676,8 @@ extern "C" int hipo_embedding_bwd(const void* grad, int elem_size, const void* t
   HIPO_REQUIRE((elem_size == 2 || elem_size == 4) && (out_size == 2 || out_size == 4),
                "embedding_bwd: elem_size and out_size must be 2 or 4");
   HIPO_REQUIRE(token_size == 4 || token_size == 8, "embedding_bwd: token_size must be 4 or 8");
-  HIPO_REQUIRE(count <= 0x7fffffff - 4096 && width <= 0x7fffffff && vocab <= 0x7fffffff,
-               "embedding_bwd: size over 2^31");
+  HIPO_REQUIRE(count <= 0x7fffffff - 4096 && width <= 0x7fffffff && vocab <= (1 << 30),
+               "embedding_bwd: count over 2^31 - 4096, width over 2^31 or vocab over 2^30");
   if (width == 0 || vocab == 0) return 0;
   HIPO_REQUIRE(dweight != nullptr && (count == 0 || (grad != nullptr && tokens != nullptr)),
                "embedding_bwd: null pointer");

@@ -675,7 +675,7 @@ struct BwdArgs {
 // bf16 635 / 667 / 728, [1501, 50001] fp32 101 / 95 / 102.
 template <typename T>
 constexpr int kBwdVectors = 8 / Logits<T>::C;
-constexpr int kBwdRows = 32768;     // rows per grid layer
+constexpr int kBwdRows = 49152;     // rows per grid layer
 constexpr int kBwdLineFrom = 1024;  // vectors of a row from which on lines count
 
 // The gradient of a logit, without the token's own term.  e^-104 is 0: the
