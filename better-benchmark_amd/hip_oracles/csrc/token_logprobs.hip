@@ -32,7 +32,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kLarge = 1024;       // threads of a workgroup where rows are few
-constexpr int kFlight = 4;         // 16-byte loads per lane in flight
 constexpr int kMaxTop = 64;
 constexpr int64_t kMaxSlices = 64;    // of a row
 constexpr int kCandidates = 1024;  // values that a slice can rank at once
@@ -483,8 +482,9 @@ __device__ __forceinline__ const uint64_t* slice_top(const Slice<T>& s, DivMagic
   return mem.sorted;
 }
 
-// A workgroup per row and slice.
-template <int NT, typename T, bool ENTROPY, bool TOP>
+// A workgroup of NT threads per row and slice, kFlight 16-byte loads per lane
+// and round.
+template <int NT, int kFlight, typename T, bool ENTROPY, bool TOP>
 __global__ __launch_bounds__(NT) void logprobs_slices(FwdArgs a) {
   constexpr int C = Logits<T>::C;
   __shared__ Stats wave_stats[NT / kWave];
@@ -492,15 +492,10 @@ __global__ __launch_bounds__(NT) void logprobs_slices(FwdArgs a) {
   const uint32_t r = div_by(blockIdx.x, a.by_slices);
   const int slice = static_cast<int>(blockIdx.x - r * a.slices);
   const int64_t row = a.first + r;
-  const int64_t token = token_at(a.tokens, a.token_size, row);
-  if (token == a.ignore_index) {
-    if (a.slices == 1) write_ignored<NT>(a, row);
-    return;
-  }
   const Slice<T> s(a, row, slice);
   Stats stats{-kInf, 0.0f, 0.0f};
-  // Rounds of kFlight vectors per lane, the next round's loads before this
-  // one's values.
+  // The next round's loads before this one's values.  (Two sets of registers
+  // instead of the copy, so that no load waits for another, measured the same.)
   constexpr int kRound = NT * kFlight;
   u32x4_t next[kFlight];
   const auto load = [&](int v0) {
@@ -510,8 +505,14 @@ __global__ __launch_bounds__(NT) void logprobs_slices(FwdArgs a) {
       next[f] = s.load(v < s.hi ? v : s.hi - 1);
     }
   };
+  // The first round beside the token, and for nothing where that is ignored.
   if (s.lo < s.hi) load(s.lo);
   __builtin_amdgcn_sched_barrier(0);
+  const int64_t token = token_at(a.tokens, a.token_size, row);
+  if (token == a.ignore_index) {
+    if (a.slices == 1) write_ignored<NT>(a, row);
+    return;
+  }
   float at = 0.0f;
   if (tid == 0 && a.slices == 1 && token >= 0 && token < a.vocab) at = to_f32(s.x[token]);
   float odd[1] = {-kInf};
@@ -630,8 +631,12 @@ __global__ __launch_bounds__(kThreads) void join_slices(FwdArgs a) {
 //   slices 8.9 / 13.7, 8 slices 8.5 / 12.9, 16 slices 8.6 / 14.5; [1, 200000]
 //   16.6 / 19.5, 8 slices 7.3 / 11.5, 16 slices 6.1 / 11.0; [256, 128000] 15.6 /
 //   19.3, 2 slices 16.5 / 23.6.
+//   Loads in flight: 2 per lane where a wave has a row ([16384, 1000] 10.2,
+//   with 4 12.6), 8 for many rows of bf16 (2 / 4 / 8: [8192, 50001] - / 136 / 130,
+//   [8192, 32000] - / 86 / 81; [512, 32000] 13.8 / 13.4 / 13.5 with 20
+//   alternatives, [700, 32000] - / 16.2 / 17.2; fp32 the same either way).
 struct Plan {
-  int threads, slices, span;
+  int threads, slices, span, flight;
 };
 
 inline Plan plan(int64_t rows, int64_t vocab, int elem_size) {
@@ -646,6 +651,7 @@ inline Plan plan(int64_t rows, int64_t vocab, int elem_size) {
   } else {
     p.threads = rows <= 256 && vectors >= 4000 ? kLarge : kThreads;
   }
+  p.flight = rows >= 2048 && elem_size == 2 ? 8 : 4;
   p.span = static_cast<int>(
       ((vectors + slices - 1) / slices + p.threads - 1) / p.threads * p.threads);
   p.slices = slices == 1 ? 1 : static_cast<int>((vectors + p.span - 1) / p.span);
@@ -815,13 +821,16 @@ extern "C" int hipo_token_logprobs(const void* logits, int elem_size, const void
                   std::max(1, p.span / p.threads), div_magic(static_cast<uint32_t>(p.slices)),
                   div_magic(static_cast<uint32_t>(std::max(1, p.span / p.threads)))};
   const bool bf16 = elem_size == 2, ent = entropy != nullptr;
-#define HIPO_LP(N_, T_)                                                                    \
-  (top ? (ent ? logprobs_slices<N_, T_, true, true> : logprobs_slices<N_, T_, false, true>) \
-       : (ent ? logprobs_slices<N_, T_, true, false> : logprobs_slices<N_, T_, false, false>))
-#define HIPO_LP_N(N_) (bf16 ? HIPO_LP(N_, uint16_t) : HIPO_LP(N_, float))
-  auto kernel = p.threads == kWave      ? HIPO_LP_N(kWave)
-                : p.threads == kThreads ? HIPO_LP_N(kThreads)
-                                        : HIPO_LP_N(kLarge);
+#define HIPO_LP(N_, F_, T_)                                   \
+  (top ? (ent ? logprobs_slices<N_, F_, T_, true, true>       \
+              : logprobs_slices<N_, F_, T_, false, true>)     \
+       : (ent ? logprobs_slices<N_, F_, T_, true, false>      \
+              : logprobs_slices<N_, F_, T_, false, false>))
+#define HIPO_LP_N(N_, F_) (bf16 ? HIPO_LP(N_, F_, uint16_t) : HIPO_LP(N_, F_, float))
+  auto kernel = p.threads == kWave    ? HIPO_LP_N(kWave, 2)
+                : p.threads == kLarge ? HIPO_LP_N(kLarge, 4)
+                : p.flight == 8       ? HIPO_LP(kThreads, 8, uint16_t)
+                                      : HIPO_LP_N(kThreads, 4);
 #undef HIPO_LP_N
 #undef HIPO_LP
   auto join = bf16 ? (top ? join_slices<uint16_t, true> : join_slices<uint16_t, false>)
