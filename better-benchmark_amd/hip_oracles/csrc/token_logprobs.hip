@@ -39,7 +39,7 @@ constexpr int64_t kMaxVocab = 0x7fffffff - 4096;
 constexpr int64_t kMaxBlocks = 1 << 23;  // of a launch
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kInf = __builtin_inff();
-constexpr float kHuge = 0x1p100f;
+constexpr float kFar = 0x1p20f;
 
 // C consecutive logits in 16 bytes.
 template <typename T>
@@ -83,11 +83,13 @@ __device__ __forceinline__ int64_t token_at(const void* tokens, int size, int64_
 }
 
 // ---------------------------------------------------------------------------
-// Statistics: the maximum m of x, Z = sum 2^w and U = sum 2^w w over
-// w = c x - round(c m), c = scale log2(e), one FMA per value.  Against a row
-// maximum whose c m is not below 2^100 (the type's lowest value in every
-// place: a row masked by it) values are equal to it or vanish, and w is not
-// formed.  m = -inf: nothing yet.
+// Statistics: the maximum m of x, Z = sum 2^w and U = sum 2^w w, where w is
+// c x less a reference near c m, c = scale log2(e).  Near (c m below 2^20) the
+// reference is c m rounded, and w one FMA per value: exact before its one
+// rounding, and 2^-5 off c (x - m) at most, which finish() puts back.  Far (a
+// row of nothing but mask values of -1e9, or of the type's lowest) it is c m
+// itself and w = c (x - m): the rounding of c m could be any number there.
+// m = -inf: nothing yet.
 // ---------------------------------------------------------------------------
 
 struct Stats {
@@ -97,19 +99,26 @@ struct Stats {
 // -round(c m); 0 for -inf, so that w of -inf is -inf.
 __device__ __forceinline__ float offset(float m, float c) { return m == -kInf ? 0.0f : -(m * c); }
 
-__device__ __forceinline__ bool is_huge(float o) { return !(fabsf(o) < kHuge); }  // NaN too
+__device__ __forceinline__ bool is_far(float o) { return !(fabsf(o) < kFar); }  // NaN too
 
 // 2^w w without 0 * inf (2^-200 is 0).
 __device__ __forceinline__ float weighted(float e, float w) { return e * maximum(w, -200.0f); }
 
 // s relative to the maximum m >= s.m instead.
 __device__ __forceinline__ Stats rescale(Stats s, float m, float c) {
-  const float o = offset(m, c);
-  if (is_huge(o)) return s.m == m ? s : Stats{m, 0.0f, 0.0f};
-  // s.m = -inf: its sums are 0, and 2^d is at most 1.
-  const float d = __builtin_elementwise_minimum(maximum(o - offset(s.m, c), -200.0f), 0.0f);
-  const float f = s.m == m ? 1.0f : __builtin_amdgcn_exp2f(d);
-  return Stats{m, s.z * f, s.m == m ? s.u : f * __builtin_fmaf(d, s.z, s.u)};
+  if (s.m == m) return s;
+  const float o = offset(m, c), had = offset(s.m, c);
+  // The old reference less the new one, in one rounding each.
+  float d = o - had;
+  if (__builtin_expect(is_far(o) || is_far(had), 0)) {
+    d = !is_far(o)    ? __builtin_fmaf(s.m, c, o)
+        : is_far(had) ? (s.m - m) * c
+                      : __builtin_fmaf(-m, c, -had);
+  }
+  // s.m = -inf: its sums are 0, and 2^d is at most 1 (a NaN m stays in m).
+  d = __builtin_elementwise_minimum(maximum(d, -200.0f), 0.0f);
+  const float f = __builtin_amdgcn_exp2f(d);
+  return Stats{m, s.z * f, f * __builtin_fmaf(d, s.z, s.u)};
 }
 
 template <int N, bool ENTROPY>
@@ -119,23 +128,28 @@ __device__ __forceinline__ void add_values(Stats& s, const float (&x)[N], float 
   for (int i = 1; i + 1 < N; i += 2) top = maximum(maximum(top, x[i]), x[i + 1]);
   if constexpr (N % 2 == 0) top = maximum(top, x[N - 1]);
   const float m = maximum(s.m, top);
-  const float o = offset(m, c);
-  if (__builtin_expect(__any(is_huge(o)), 0)) {
-    if (is_huge(o)) {
-      s = rescale(s, m, c);
-#pragma unroll
-      for (int i = 0; i < N; ++i) s.z += x[i] == m ? 1.0f : 0.0f;
-      return;
-    }
-  }
   s = rescale(s, m, c);
+  const float o = offset(m, c);
   float z[2] = {0.0f, 0.0f}, u[2] = {0.0f, 0.0f};
+  if (__builtin_expect(is_far(o), 0)) {
+#pragma unroll 1
+    for (int i = 0; i < N; ++i) {
+      float v = x[0];  // x[i], kept in registers
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float w = __builtin_fmaf(x[i], c, o);
-    const float e = __builtin_amdgcn_exp2f(w);
-    z[i & 1] += e;
-    if constexpr (ENTROPY) u[i & 1] += weighted(e, w);
+      for (int k = 1; k < N; ++k) v = i == k ? x[k] : v;
+      const float w = maximum((v - m) * c, -200.0f);
+      const float e = __builtin_amdgcn_exp2f(w);
+      z[0] += e;
+      u[0] += e * w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float w = __builtin_fmaf(x[i], c, o);
+      const float e = __builtin_amdgcn_exp2f(w);
+      z[i & 1] += e;
+      if constexpr (ENTROPY) u[i & 1] += weighted(e, w);
+    }
   }
   s.z += z[0] + z[1];
   if constexpr (ENTROPY) s.u += u[0] + u[1];
@@ -164,8 +178,8 @@ __device__ __forceinline__ Row finish(Stats s, float scale, float c) {
   if (fabsf(s.m) < kInf) {
     const float o = offset(s.m, c);
     const float log2_z = __builtin_amdgcn_logf(s.z);
-    // Z is relative to round(c m): what it is off c m by, exactly.
-    r.log_z = kLn2 * (is_huge(o) ? log2_z : log2_z + __builtin_fmaf(-s.m, c, -o));
+    // Z is relative to round(c m) where that is near: what it is off c m by.
+    r.log_z = kLn2 * (is_far(o) ? log2_z : log2_z + __builtin_fmaf(-s.m, c, -o));
     r.lse = __builtin_fmaf(scale, s.m, r.log_z);
     r.entropy = kLn2 * (log2_z - s.u / s.z);
   } else {  // -inf: nothing is left; +inf; NaN

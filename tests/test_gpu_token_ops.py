@@ -155,6 +155,25 @@ def test_alternatives_that_a_few_lanes_hold(rows, vocab, dtype, rocm_device, ho)
         check_forward(ho, rocm_device, x.to(dtype), t, top=top, what=f"stripes {vocab} {top}")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab", [(14, 40), (14, 3000), (14, 66000), (1100, 2100)])
+def test_logits_far_from_zero(rows, vocab, dtype, rocm_device, ho):
+    """Rows of nothing but a mask value, logits around large numbers, maxima that
+    rise past where the statistics change their form (c x = 2^20)."""
+    g = torch.Generator().manual_seed(vocab)
+    at = [-1e4, -65504.0, -1e6, -1e9, -1e10, -1e20, -1e30, 3e5, 1e6, 5e7, -7.2e5, 726000.0, 1e5]
+    x = torch.randn(rows, vocab, generator=g) * 3
+    for r in range(len(at)):
+        x[r] = at[r] if r in (3, 4, 5, 6) else at[r] + x[r]
+    x[11] += torch.arange(vocab) * (3000.0 / vocab)
+    x[12, vocab // 2] = 9e5   # near, then far
+    x[13, :vocab // 2] = -1e9
+    t = torch.randint(0, vocab, (rows,), generator=g)
+    for scale in (1.0, 0.7):
+        check_forward(ho, rocm_device, x.to(dtype), t, scale=scale, top=4,
+                      what=f"far [{rows}, {vocab}] {dtype} {scale}")
+
+
 @pytest.mark.parametrize("rows,vocab", [(4, 5000), (3, 70000)])
 def test_alternatives_where_one_number_fills_the_row(rows, vocab, rocm_device, ho):
     """fp32 logits that no bf16 value is near: a mask of -1e9 with fewer places
