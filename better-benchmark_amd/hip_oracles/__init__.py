@@ -707,6 +707,12 @@ def _require_logits(what: str, logits: torch.Tensor, tokens: torch.Tensor,
     raise AssertionError(what)
 
 
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share no memory."""
+    p, q = a.data_ptr(), b.data_ptr()
+    return p + a.numel() * a.element_size() <= q or q + b.numel() * b.element_size() <= p
+
+
 def _rows_apart_or_same(a: torch.Tensor, a_stride: int, b: torch.Tensor, b_stride: int,
                         rows: int, cols: int) -> bool:
     """Whether [rows, cols] at a and b, of one type, are the same memory or share none."""
@@ -835,7 +841,7 @@ def embedding_bwd(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, scale
     padding_idx, and tokens outside [0, vocab), add nothing.  into: a
     contiguous bf16 or fp32 [vocab, D] that the gradient is added to (before
     the one rounding) and that is returned; its rows without tokens are not
-    touched."""
+    touched.  It does not overlap grad or the tokens."""
     lib = _lib or load_library()
     dev = _require_rocm(grad, tokens, *(() if into is None else (into,)))
     _require(grad.dtype in _FLOATS and grad.dim() >= 1 and grad.is_contiguous(),
@@ -855,6 +861,8 @@ def embedding_bwd(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, scale
                  "embedding_bwd: dtype and into's type differ")
         _require(into.dtype in _FLOATS and into.shape == (vocab, width) and into.is_contiguous(),
                  "embedding_bwd: into must be contiguous bf16 or fp32 [vocab, D]")
+        _require(_apart(into, grad) and _apart(into, tokens),
+                 "embedding_bwd: into overlaps grad or tokens")
         out = into
     need = int(lib.hipo_embedding_bwd_workspace_bytes(tokens.numel(), width, vocab))
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None

@@ -412,6 +412,8 @@ def test_refusals(rocm_device, ho):
         lambda: ho.embedding_bwd(x, t, 9, into=torch.zeros(8, 16, device=dev)),
         lambda: ho.embedding_bwd(x, t, 9, into=torch.zeros(16, 9, device=dev).t()),
         lambda: ho.embedding_bwd(x, t, 9, dtype=BF16, into=torch.zeros(9, 16, device=dev)),
+        lambda: ho.embedding_bwd(x, t, 4, into=x),
+        lambda: ho.embedding_bwd(x, t, 3, into=x[1:]),
     ]
     for k, call in enumerate(bad):
         with pytest.raises(ValueError):
