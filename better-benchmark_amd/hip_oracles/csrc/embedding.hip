@@ -51,7 +51,6 @@ constexpr int64_t kSortPart = int64_t{1} << (32 - kSortRowBits);  // positions a
 // 768] 20.1 us instead of 19.1, [65536, 2048] into [32000, 2048] 104.7 instead of
 // 101.1; nothing else within 2 %).
 constexpr int kSortGroups = 128;
-constexpr int kPiece = 32;           // positions per piece of a frequent token
 constexpr int64_t kLanes = int64_t{1} << 30;  // lanes per launch
 constexpr int64_t kFillBlocks = int64_t{1} << 21;  // with 2^21 sorting ones 2^32 threads
 
@@ -358,7 +357,8 @@ struct BwdArgs {
   float* sums;           // [2 * bins][width], see first_piece
   int64_t first, count;  // slots of this launch
   int64_t places;        // in order, of which *total are filled
-  int64_t bins;          // of kPiece places
+  int64_t bins;          // of 2^bits places
+  int bits;              // of a piece
   DivMagic by_pieces;
   int width, pieces;     // pieces of C columns per row
   float scale;
@@ -402,23 +402,28 @@ __device__ __forceinline__ void add_rows(float (&sum)[C], const BwdArgs& a, int 
   }
 }
 
-// Tokens with more than kPiece places are summed in pieces of that many,
+// Tokens with more than 2^bits places are summed in pieces of that many,
 // counted from the token's first place.  The sorted places are cut into bins
 // of the same size: a bin holds the start of at most one piece after a token's
 // first (its sum is kept in sums[bin]) and of at most one first piece (in
-// sums[bins + bin]; its token reaches into the next bin).  The token of a bin's
-// first piece, count 0 if there is none:
+// sums[bins + bin]; its token reaches into the next bin).
+__device__ __forceinline__ bool in_pieces(const BwdArgs& a, Segment token) {
+  return token.count > 1 << a.bits;
+}
+
+// The token of a bin's first piece, count 0 if there is none.
 __device__ __forceinline__ Segment first_piece(const BwdArgs& a, int bin) {
-  const int64_t probe = (int64_t{bin} + 1) * kPiece;
+  const int64_t probe = (int64_t{bin} + 1) << a.bits;
   const int total = *a.total;
   const Segment g = a.order[probe < a.places ? probe : a.places - 1].token;
-  const bool here = probe < total && g.count > kPiece &&
-                    g.start >= bin * kPiece && g.start < probe;
+  const bool here = probe < total && in_pieces(a, g) && g.start < probe &&
+                    g.start >= probe - (1 << a.bits);
   return here ? g : Segment{0, 0};
 }
 
 // The places of slot's piece, from == to if there is none.
 __device__ __forceinline__ void piece_places(const BwdArgs& a, int64_t slot, int& from, int& to) {
+  const int size = 1 << a.bits;
   from = to = 0;
   Segment g;
   if (slot >= a.bins) {
@@ -426,15 +431,15 @@ __device__ __forceinline__ void piece_places(const BwdArgs& a, int64_t slot, int
     if (g.count == 0) return;
     from = g.start;
   } else {
-    const int64_t probe = slot * kPiece;
+    const int64_t probe = slot << a.bits;
     const int total = *a.total;
     g = a.order[probe].token;
-    if (probe >= total || g.count <= kPiece) return;
-    const int at = g.start + ((static_cast<int>(probe) - g.start + kPiece - 1) & -kPiece);
+    if (probe >= total || !in_pieces(a, g)) return;
+    const int at = g.start + ((static_cast<int>(probe) - g.start + size - 1) & -size);
     if (at == g.start || at >= g.start + g.count) return;
     from = at;
   }
-  to = std::min(from + kPiece, g.start + g.count);
+  to = std::min(from + size, g.start + g.count);
 }
 
 // A lane's C columns of a row of dw.
@@ -492,7 +497,7 @@ __global__ __launch_bounds__(kThreads) void sum_rows(BwdArgs a) {
   // One load for all of it, beside the total's.
   const Place p = __builtin_bit_cast(Place, *reinterpret_cast<const u32x4_t*>(a.order + place));
   const Segment g = p.token;
-  if (place >= total || g.start != place || g.count > kPiece) return;
+  if (place >= total || g.start != place || in_pieces(a, g)) return;
   // Its first position is in hand.
   const T* grad = static_cast<const T*>(a.grad) + int64_t{p.position} * a.width + col;
   Values<T, C> x;
@@ -520,7 +525,7 @@ __global__ __launch_bounds__(kThreads) void join_pieces(BwdArgs a) {
   if (g.count == 0) return;  // the whole workgroup
   const int row = a.order[g.start].row;
   const float* sums = a.sums + col;
-  const int n = (g.count + kPiece - 1) / kPiece;
+  const int n = (g.count + (1 << a.bits) - 1) >> a.bits;
   const int each = (n + kWaves - 1) / kWaves;
   const int to = std::min(n, (wave + 1) * each);
   float sum[C] = {};
@@ -560,6 +565,7 @@ __global__ __launch_bounds__(kThreads) void join_pieces(BwdArgs a) {
 // Workspace: the order, the number of places, the sums of pieces; each 16-byte
 // aligned.
 struct Layout {
+  int bits;
   int64_t bins;
   size_t total, sums, bytes;
 };
@@ -567,11 +573,17 @@ struct Layout {
 inline Layout layout(int64_t count, int64_t width) {
   const auto up = [](size_t n) { return (n + 15) / 16 * 16; };
   Layout l;
-  l.bins = (count + kPiece - 1) / kPiece;
+  // A piece is as long a chain of loads as the whole call waits for where there
+  // is little to read: 8 / 16 / 32 places, us: [2048, 768] into [32000, 768] 16.5
+  // / 17.5 / 19.4, [16384, 512] added into [32000, 512] 24.1 / 22.7 / 23.9,
+  // [8192, 2048] 26.2 / 26.1 / 26.2, [65536, 2048] into [32000, 2048] 121 / 108 /
+  // 102, [65536, 64] into [1696, 64] 55 / 43 / 40.
+  l.bits = count <= 32768 && count * width <= 1 << 24 ? 4 : 5;
+  l.bins = (count + (1 << l.bits) - 1) >> l.bits;
   l.total = up(count * sizeof(Place));
   l.sums = l.total + 16;
   // A token with more places than a piece needs that many.
-  if (count <= kPiece) l.bins = 0;
+  if (count <= 1 << l.bits) l.bins = 0;
   l.bytes = l.sums + 2 * l.bins * width * sizeof(float);
   return l;
 }
@@ -696,6 +708,7 @@ extern "C" int hipo_embedding_bwd(const void* grad, int elem_size, const void* t
   a.total = reinterpret_cast<int*>(ws + l.total);
   a.sums = reinterpret_cast<float*>(ws + l.sums);
   a.bins = l.bins;
+  a.bits = l.bits;
   a.width = static_cast<int>(width);
   a.scale = scale;
   SortArgs s{tokens, reinterpret_cast<Place*>(ws),
