@@ -736,8 +736,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, scale: float =
     Returns (logprob [R], lse [R]), then the distribution's entropy [R] with
     entropy=True, then with top=k (at most 64) the k most probable tokens'
     log probabilities [R, k] and ids [R, k] (int64; of equal logits the lower
-    id first, NaN above all).  A row whose token is ignore_index is not read:
-    its results are 0, its alternatives -inf and -1.  Any other token outside
+    id first, NaN above all).  A row whose token is ignore_index is left out,
+    whatever its logits hold: its results are 0, its alternatives -inf and -1.  Any other token outside
     [0, V) has log probability NaN.  A row with nothing above -inf has lse
     -inf, with +inf lse +inf, with NaN lse NaN; there logprob = scale * logit -
     lse, and the entropy is NaN."""

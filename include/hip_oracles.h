@@ -450,8 +450,8 @@ int hipo_gelu_erf_bwd_colsum_bf16(const uint16_t* grad, const uint16_t* x, uint1
  * alignment; tokens is [rows] of int32 (token_size 4) or int64 (8); the
  * outputs are contiguous.  entropy may be NULL; top is at most 64 and at
  * most vocab, its outputs NULL where it is 0; scale is from 2^-100 to 2^100.
- * A row whose token is ignore_index is not read: 0, 0, 0, and for the
- * alternatives -inf and -1.  A token outside [0, vocab) otherwise has
+ * A row whose token is ignore_index is left out, whatever its logits hold:
+ * 0, 0, 0, and for the alternatives -inf and -1.  A token outside [0, vocab) otherwise has
  * logprob NaN.  A row with nothing above -inf has lse -inf, one with +inf
  * lse +inf, one with NaN lse NaN; their logprobs are s - lse, their entropy
  * NaN.  `workspace`: at least hipo_token_logprobs_workspace_bytes bytes,
@@ -478,7 +478,7 @@ int hipo_token_logprobs(const void* logits, int elem_size, const void* tokens,
  * grad_entropy), are the forward's results.  logits and dlogits are [rows,
  * vocab] with row strides of their own; dlogits may be logits itself (one
  * stride), and does not overlap it otherwise.  Rows of ignore_index are
- * zero and not read; rows of another token outside [0, vocab) are NaN.
+ * zero, whatever they hold; rows of another token outside [0, vocab) are NaN.
  * No counterpart among the reference's oracles; beside
  * hipo_gelu_erf_bwd_colsum_bf16 as a training gradient.
  */
