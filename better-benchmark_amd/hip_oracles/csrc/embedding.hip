@@ -29,6 +29,7 @@
 //      often than a piece is long are cut into pieces, summed in the same
 //      launch into the workspace (fp32);
 //   3. join_pieces: their rows, the sums of their pieces.
+// Few tokens take one launch instead, sum_few.
 #include <math.h>
 
 #include <algorithm>
@@ -51,6 +52,8 @@ constexpr int64_t kSortPart = int64_t{1} << (32 - kSortRowBits);  // positions a
 // 768] 20.1 us instead of 19.1, [65536, 2048] into [32000, 2048] 104.7 instead of
 // 101.1; nothing else within 2 %).
 constexpr int kSortGroups = 128;
+constexpr int kFewTokens = 1024;     // summed without a sort
+constexpr int kFewThreads = 512;
 constexpr int64_t kLanes = int64_t{1} << 30;  // lanes per launch
 constexpr int64_t kFillBlocks = int64_t{1} << 21;  // with 2^21 sorting ones 2^32 threads
 
@@ -562,6 +565,112 @@ __global__ __launch_bounds__(kThreads) void join_pieces(BwdArgs a) {
   Row<O, C, WHOLE, ADD>(a, row, col).write(sum, a.scale);
 }
 
+// ---------------------------------------------------------------------------
+// Few tokens: no sort.  A workgroup per position and 64 lanes' columns looks
+// through all tokens: where its own occurs first it sums all of that token's
+// rows, each wave a part of them.
+// ---------------------------------------------------------------------------
+
+__global__ __launch_bounds__(kSortThreads) void zero_values(SortArgs a) {
+  fill_zeros(a, blockIdx.x, gridDim.x);
+}
+
+struct FewArgs {
+  const void* grad;
+  const void* tokens;
+  void* dw;
+  int64_t vocab, padding_idx;
+  DivMagic by_chunks;
+  int count, width, chunks;  // workgroups per row
+  float scale;
+  int token_size;
+};
+
+template <typename T, typename O, int C, bool WHOLE, bool ADD>
+__global__ __launch_bounds__(kFewThreads) void sum_few(FewArgs f) {
+  constexpr int kWaves = kFewThreads / kWave, kLooks = kFewTokens / kFewThreads, kFlight = 8;
+  __shared__ uint64_t same[kLooks * kWaves];  // of each 64 positions
+  __shared__ int list[kFewTokens];
+  __shared__ float part[kWaves][C][kWave];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6;
+  const int t = static_cast<int>(div_by(blockIdx.x, f.by_chunks));
+  const int col = ((static_cast<int>(blockIdx.x) - t * f.chunks) * kWave + lane) * C;
+  const int64_t token = token_at(f.tokens, f.token_size, t);
+  uint64_t m[kLooks];
+#pragma unroll
+  for (int k = 0; k < kLooks; ++k) {
+    const int i = k * kFewThreads + tid;
+    m[k] = __ballot(i < f.count && token_at(f.tokens, f.token_size, i) == token);
+    if (lane == 0) same[k * kWaves + wave] = m[k];
+  }
+  if (token < 0 || token >= f.vocab || token == f.padding_idx) return;  // the workgroup
+  __syncthreads();
+  int n = 0, first = f.count, before[kLooks];
+#pragma unroll
+  for (int j = 0; j < kLooks * kWaves; ++j) {
+    const uint64_t b = same[j];
+    if (j % kWaves == wave) before[j / kWaves] = n;
+    if (n == 0 && b != 0) first = j * kWave + __builtin_ctzll(b);
+    n += __popcll(b);
+  }
+  if (first != t) return;  // the workgroup
+#pragma unroll
+  for (int k = 0; k < kLooks; ++k) {
+    if ((m[k] >> lane) & 1)
+      list[before[k] + __popcll(m[k] & ((uint64_t{1} << lane) - 1))] = k * kFewThreads + tid;
+  }
+  __syncthreads();
+  BwdArgs a{};
+  a.dw = f.dw;
+  a.width = f.width;
+  const bool columns = col < f.width;
+  const int left = f.width - col;
+  const int each = (n + kWaves - 1) / kWaves;
+  const int to = std::min(n, (wave + 1) * each);
+  float sum[C] = {};
+  if (columns) {
+    const T* grad = static_cast<const T*>(f.grad) + col;
+    for (int i0 = wave * each; i0 < to; i0 += kFlight) {
+      Values<T, C> x[kFlight];
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+        x[k].clear();
+        if (i0 + k < to) {
+          const T* p = grad + int64_t{list[i0 + k]} * f.width;
+          if (WHOLE || left >= C) x[k].load_stream(p);
+          else x[k].load_part(p, left);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int k = 0; k < kFlight; ++k) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) sum[c] += x[k].get(c);
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < C; ++c) part[wave][c][lane] = sum[c];
+  __syncthreads();
+  if (wave != 0 || !columns) return;
+  Row<O, C, WHOLE, ADD> out(a, token, col);
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) sum[c] += part[w][c][lane];
+  }
+  out.write(sum, f.scale);
+}
+
+// Up to so many tokens and gradient values there is no sort (one launch, two
+// where the rest is zeroed, and no workspace).  Graph replays of bf16, us, with the
+// sort / this: added [128, 768] 9.0 / 4.7, [512, 512] 11.0 / 5.6, [1024, 64] 13.1 /
+// 7.4, [1024, 768] 12.6 / 11.4; of one token alone 10.5 / 5.4, 11.4 / 9.8, 13.3 /
+// 16.1, 14.0 / 20.2.  [512, 512] with 256 threads 5.0 and 14.9, with 1024 7.1 and 9.4.
+inline bool few_tokens(int64_t count, int64_t width) {
+  return count <= kFewTokens && count * width <= 1 << 19;
+}
+
 // Workspace: the order, the number of places, the sums of pieces; each 16-byte
 // aligned.
 struct Layout {
@@ -598,24 +707,38 @@ void for_lanes(int64_t rows, int64_t pieces, F&& launch) {
   }
 }
 
+inline int64_t fill_blocks(const SortArgs& s) {
+  constexpr int64_t kPerBlock = int64_t{kSortThreads} * 8;
+  return std::min((s.fill_values + kPerBlock - 1) / kPerBlock, kFillBlocks);
+}
+
+template <typename T, typename O>
+void launch_few(const BwdArgs& a, const SortArgs& s, int token_size, bool accumulate,
+                hipStream_t stream) {
+  constexpr int C = 16 / sizeof(T);
+  const bool whole = a.width % C == 0;
+  if (!accumulate)
+    zero_values<<<dim3(static_cast<unsigned>(fill_blocks(s))), dim3(kSortThreads), 0, stream>>>(s);
+  if (s.count == 0) return;
+  const int chunks = (a.width + C * kWave - 1) / (C * kWave);
+  const FewArgs f{a.grad, s.tokens, a.dw, s.vocab, s.padding_idx, div_magic(chunks),
+                  static_cast<int>(s.count), a.width, chunks, a.scale, token_size};
+  auto kernel = accumulate
+                    ? (whole ? sum_few<T, O, C, true, true> : sum_few<T, O, C, false, true>)
+                    : (whole ? sum_few<T, O, C, true, false> : sum_few<T, O, C, false, false>);
+  kernel<<<dim3(static_cast<unsigned>(f.count * chunks)), dim3(kFewThreads), 0, stream>>>(f);
+}
+
 template <typename T, typename O>
 void launch_bwd(BwdArgs a, SortArgs s, int token_size, bool accumulate, hipStream_t stream) {
   constexpr int C = 16 / sizeof(T);
   const bool whole = a.width % C == 0;
   a.pieces = (a.width + C - 1) / C;
   a.by_pieces = div_magic(a.pieces);
-  if (accumulate && s.count == 0) return;
-  int64_t fill_blocks = 0;
-  if (!accumulate) {
-    constexpr int64_t kPerBlock = int64_t{kSortThreads} * 8;
-    s.fill = static_cast<uint16_t*>(a.dw);
-    s.fill_values = s.vocab * a.width * static_cast<int64_t>(sizeof(O) / 2);
-    fill_blocks = std::min((s.fill_values + kPerBlock - 1) / kPerBlock, kFillBlocks);
-  }
   auto sort = token_size == 8 ? sort_tokens<int64_t> : sort_tokens<int32_t>;
-  sort<<<dim3(static_cast<unsigned>((int64_t{1} << s.group_bits) + fill_blocks)),
-         dim3(kSortThreads), 0, stream>>>(s);
-  if (s.count == 0) return;
+  const int64_t fill = accumulate ? 0 : fill_blocks(s);
+  sort<<<dim3(static_cast<unsigned>((int64_t{1} << s.group_bits) + fill)), dim3(kSortThreads), 0,
+         stream>>>(s);
   a.places = s.count;
   auto rows = accumulate
                   ? (whole ? sum_rows<T, O, C, true, true> : sum_rows<T, O, C, false, true>)
@@ -676,7 +799,7 @@ extern "C" int hipo_embedding(const void* weight, int elem_size, const void* tok
 
 extern "C" size_t hipo_embedding_bwd_workspace_bytes(int64_t count, int64_t width,
                                                      int64_t vocab) {
-  if (count < 0 || width <= 0 || vocab <= 0) return 0;
+  if (count < 0 || width <= 0 || vocab <= 0 || hipo::few_tokens(count, width)) return 0;
   return hipo::layout(count, width).bytes;
 }
 
@@ -696,33 +819,53 @@ extern "C" int hipo_embedding_bwd(const void* grad, int elem_size, const void* t
   if (width == 0 || vocab == 0) return 0;
   HIPO_REQUIRE(dweight != nullptr && (count == 0 || (grad != nullptr && tokens != nullptr)),
                "embedding_bwd: null pointer");
+  BwdArgs a{};
+  a.grad = grad;
+  a.dw = dweight;
+  a.width = static_cast<int>(width);
+  a.scale = scale;
+  SortArgs s{};
+  s.tokens = tokens;
+  s.count = count;
+  s.vocab = vocab;
+  s.padding_idx = padding_idx;
+  if (!accumulate) {
+    s.fill = static_cast<uint16_t*>(dweight);
+    s.fill_values = vocab * width * (out_size / 2);
+  }
+  const auto run = [&](auto launch) {
+    if (elem_size == 2) {
+      if (out_size == 2) launch(uint16_t{}, uint16_t{});
+      else launch(uint16_t{}, float{});
+    } else {
+      if (out_size == 2) launch(float{}, uint16_t{});
+      else launch(float{}, float{});
+    }
+  };
+  if (few_tokens(count, width)) {
+    run([&](auto t, auto o) {
+      launch_few<decltype(t), decltype(o)>(a, s, token_size, accumulate != 0, stream);
+    });
+    return check_launch("embedding_bwd");
+  }
   const Layout l = layout(count, width);
   HIPO_REQUIRE(workspace != nullptr && workspace_bytes >= l.bytes,
                "embedding_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, l.bytes);
   HIPO_REQUIRE(aligned16(workspace), "embedding_bwd: workspace must be 16-byte aligned");
   char* ws = static_cast<char*>(workspace);
-  BwdArgs a{};
-  a.grad = grad;
-  a.dw = dweight;
-  a.order = reinterpret_cast<Place*>(ws);
-  a.total = reinterpret_cast<int*>(ws + l.total);
+  s.order = reinterpret_cast<Place*>(ws);
+  s.total = reinterpret_cast<int*>(ws + l.total);
+  a.order = s.order;
+  a.total = s.total;
   a.sums = reinterpret_cast<float*>(ws + l.sums);
   a.bins = l.bins;
   a.bits = l.bits;
-  a.width = static_cast<int>(width);
-  a.scale = scale;
-  SortArgs s{tokens, reinterpret_cast<Place*>(ws),
-             reinterpret_cast<int*>(ws + l.total), nullptr, 0, count, vocab, padding_idx, 0};
   while ((int64_t{1} << s.group_bits) < kSortGroups ||
          (int64_t{kSortRows} << s.group_bits) < vocab) {
     ++s.group_bits;
   }
-  if (elem_size == 2) {
-    if (out_size == 2) launch_bwd<uint16_t, uint16_t>(a, s, token_size, accumulate != 0, stream);
-    else launch_bwd<uint16_t, float>(a, s, token_size, accumulate != 0, stream);
-  } else {
-    if (out_size == 2) launch_bwd<float, uint16_t>(a, s, token_size, accumulate != 0, stream);
-    else launch_bwd<float, float>(a, s, token_size, accumulate != 0, stream);
-  }
+  run([&](auto t, auto o) {
+    launch_bwd<decltype(t), decltype(o)>(a, s, token_size, accumulate != 0, stream);
+  });
   return check_launch("embedding_bwd");
 }

@@ -334,8 +334,10 @@ def test_ids_past_32_bits(rocm_device, ho):
     (64, 96, 64, "runs"), (65, 768, 3000, "text"), (1000, 1001, 517, "text"),
     (4096, 40, 50001, "text"), (5000, 264, 70, "uniform"), (20000, 16, 3, "uniform"),
     (70001, 8, 1025, "text"), (3000, 2048, 11, "one"), (9000, 8, 2000, "one"),
-    (300, 4096, 100, "unknown"), (2049, 33, 131073, "uniform"), (16, 8, 2, "one"), (17, 8, 2, "one"), (32, 24, 1, "one"),
-    (33, 24, 1, "one"), (64, 24, 2, "one"), (96, 24, 3, "runs"), (16384, 24, 9000, "text"),
+    (300, 4096, 100, "unknown"), (2049, 33, 131073, "uniform"), (16, 8, 2, "one"), (17, 8, 2, "one"),
+    (1024, 512, 3000, "text"), (1024, 513, 3000, "text"), (1025, 16, 3000, "text"),
+    (1023, 100, 7, "uniform"), (513, 700, 40, "one"), (1000, 5, 300, "unknown"),
+    (16, 32769, 5, "text"), (16, 32768, 5, "text"), (32, 24, 1, "one"), (33, 24, 1, "one"), (64, 24, 2, "one"), (96, 24, 3, "runs"), (16384, 24, 9000, "text"),
     (33000, 8, 300000, "text"), (8193, 64, 8192, "runs")])
 def test_embedding_backward(count, width, vocab, kind, dtype, out, rocm_device, ho):
     g = torch.Generator().manual_seed(count + width)

@@ -85,6 +85,9 @@ def test_workspaces_are_checked(lib):
             assert emb_bwd(lib, **kw, ws=ws, wb=wb) == HIPO_EINVAL
             assert b"workspace" in lib.hipo_last_error()
     assert lib.hipo_token_logprobs_workspace_bytes(0, 100, 0) == 0
+    assert lib.hipo_embedding_bwd_workspace_bytes(1024, 512, 32000) == 0  # no sort
+    assert lib.hipo_embedding_bwd_workspace_bytes(1024, 513, 32000) > 0
+    assert lib.hipo_embedding_bwd_workspace_bytes(1025, 8, 32000) > 0
 
 
 def test_empty_calls_are_no_ops(lib):
