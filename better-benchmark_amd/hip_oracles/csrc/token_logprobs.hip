@@ -887,13 +887,15 @@ extern "C" int hipo_token_logprobs_bwd(const float* grad, const void* logits, in
                "token_logprobs_bwd: null pointer");
   const BwdArgs a{grad, logits, tokens, lse, entropy, grad_entropy, grad_lse, dlogits, rows,
                   vocab, row_stride, dlogits_row_stride, ignore_index, scale, token_size};
-  // Short rows take fewer waves; one vector more, and where lines count one
-  // line, than the row is long.
+  // One vector more, and where lines count one line, than the row is long.  A
+  // row's workgroups are alike, so that no half empty one ends it ([15320, 2945]
+  // bf16 37.1 us instead of 44.6, [8192, 4097] 25.2 instead of 27.6).
   const int64_t c = 16 / elem_size, per_lane = 8 / c;
   const int64_t vectors = vocab / c + (vocab / c < kBwdLineFrom ? 1 : 9);
   const int64_t lanes = (vectors + per_lane - 1) / per_lane;
+  const int64_t groups = (lanes + kThreads - 1) / kThreads;
   const unsigned threads = static_cast<unsigned>(
-      std::min<int64_t>(kThreads, (lanes + kWave - 1) / kWave * kWave));
+      ((lanes + groups - 1) / groups + kWave - 1) / kWave * kWave);
   const dim3 grid(static_cast<unsigned>((lanes + threads - 1) / threads),
                   static_cast<unsigned>(std::min<int64_t>(rows, kBwdRows)),
                   static_cast<unsigned>((rows + kBwdRows - 1) / kBwdRows));

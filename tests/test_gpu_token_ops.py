@@ -206,7 +206,8 @@ def bwd_inputs(rows, vocab, dtype, kind, seed):
 @pytest.mark.parametrize("rows,vocab,kind", [
     (1, 1, "plain"), (3, 7, "plain"), (5, 64, "plain"), (4, 1000, "masked"), (3, 8191, "plain"),
     (2, 50001, "plain"), (1, 131072, "peaked"), (700, 517, "plain"), (7, 4099, "ties"),
-    (9, 16384, "masked")])
+    (9, 16384, "masked"), (5, 2049, "plain"), (6, 2945, "ties"), (3, 4100, "masked"),
+    (4, 6145, "plain")])
 def test_backward(rows, vocab, kind, dtype, rocm_device, ho):
     x, t, (g, gh, gl), _, _ = bwd_inputs(rows, vocab, dtype, kind, rows + vocab)
     for k, (use_h, use_l) in enumerate(((0, 0), (1, 0), (0, 1), (1, 1))):
