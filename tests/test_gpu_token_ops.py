@@ -366,9 +366,10 @@ def test_embedding_backward(count, width, vocab, kind, dtype, out, rocm_device, 
         assert buf.cpu()[~touched].isnan().all()
 
 
-def test_embedding_backward_keeps_what_lies_behind(rocm_device, ho):
+@pytest.mark.parametrize("count", [500, 1500])  # without and with a sort
+def test_embedding_backward_keeps_what_lies_behind(count, rocm_device, ho):
     """Rows of an odd width at the end of a larger buffer."""
-    count, width, vocab = 500, 37, 41
+    width, vocab = 37, 41
     g = torch.Generator().manual_seed(1)
     t = ids_of("text", count, vocab, g).to(rocm_device)
     grad = torch.randn(count, width, generator=g).to(BF16).to(rocm_device)
@@ -479,6 +480,8 @@ def test_offsets_past_32_bits(rocm_device, ho):
     dw = ho.embedding_bwd(e, t, vocab)
     assert torch.equal(dw[-1], (2 * e[0].float()).to(BF16)) and torch.equal(dw[-2], e[2])
     assert torch.equal(dw[0], e[1]) and int((dw != 0).any(-1).sum()) == 3
+    far = torch.cat([t, torch.full((1100,), -1, device=rocm_device)])  # sorted
+    assert torch.equal(ho.embedding_bwd(torch.cat([e, w[:1100]]), far, vocab), dw)
     t = torch.full(((1 << 20) + 9,), 3, dtype=torch.int32, device=rocm_device)
     t[-1] = vocab - 1
     e = ho.embedding(w, t)
@@ -491,7 +494,8 @@ def test_other_streams_and_no_change_of_device_state(rocm_device, ho):
     xd, td = x.to(rocm_device), t.to(rocm_device)
     w = torch.randn(9001, 96, device=rocm_device)
     a = [*ho.token_logprobs(xd, td, top=4), ho.embedding(w, td)]
-    a.append(ho.embedding_bwd(a[-1], td, 9001))
+    many, wide = td.repeat(30), torch.randn(1500, 96, device=rocm_device)
+    a += [ho.embedding_bwd(a[-1], td, 9001), ho.embedding_bwd(wide, many, 9001)]
     streams = [torch.cuda.Stream() for _ in range(2)]
     torch.cuda.synchronize()
     outs = []
@@ -499,7 +503,7 @@ def test_other_streams_and_no_change_of_device_state(rocm_device, ho):
         for s in streams:
             with torch.cuda.stream(s):
                 b = [*ho.token_logprobs(xd, td, top=4), ho.embedding(w, td)]
-                b.append(ho.embedding_bwd(b[-1], td, 9001))
+                b += [ho.embedding_bwd(b[-1], td, 9001), ho.embedding_bwd(wide, many, 9001)]
                 outs.append(b)
     torch.cuda.synchronize()
     for b in outs:
@@ -552,9 +556,10 @@ def test_a_run_of_all_of_them(rocm_device, ho):
     ref.close(dw, want, tol, "tied gradient")
 
 
-def test_the_run_in_a_graph(rocm_device, ho):
+@pytest.mark.parametrize("rows", [120, 1100])
+def test_the_run_in_a_graph(rows, rocm_device, ho):
     """Captured once and replayed on new tokens, with eager work between."""
-    m = Model(ho, rocm_device, 120, 128, 2003, 2)
+    m = Model(ho, rocm_device, rows, 128, 2003, 2)
     s = torch.cuda.Stream()
     with torch.cuda.stream(s):
         m.step()
