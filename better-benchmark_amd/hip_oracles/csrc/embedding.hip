@@ -19,8 +19,8 @@
 //      200 cycles per 64 tokens and SIMD: 6.6 us at 8192 tokens, 21 us at
 //      65536.
 //      Other workgroups of the same launch write zeros to all of dw: most of
-//      the bytes where tokens are fewer than rows ([128000, 4096] bf16 170 us,
-//      6.2 TB/s), and beside the sort hardly any time where they are not (rows
+//      the bytes where tokens are fewer than rows ([128000, 4096] bf16 160 us,
+//      6.5 TB/s), and beside the sort hardly any time where they are not (rows
 //      without a token found and zeroed by sum_rows instead: [65536, 2048] into
 //      [32000, 2048] 106.5 us against 101.4, [65536, 64] into [1696, 64] 38.2
 //      against 39.1).
@@ -54,6 +54,7 @@ constexpr int64_t kSortPart = int64_t{1} << (32 - kSortRowBits);  // positions a
 constexpr int kSortGroups = 128;
 constexpr int kFewTokens = 1024;     // summed without a sort
 constexpr int kFewThreads = 512;
+constexpr int kFewFill = 2;          // zeros: 16-byte pieces per thread
 constexpr int64_t kLanes = int64_t{1} << 30;  // lanes per launch
 constexpr int64_t kFillBlocks = int64_t{1} << 21;  // with 2^21 sorting ones 2^32 threads
 
@@ -166,12 +167,14 @@ struct SortArgs {
 };
 
 // Zeros, 16 bytes per thread (64: [128000, 4096] bf16 221 us instead of 173);
-// more where dw is over kFillBlocks * 16 KiB.
-__device__ __forceinline__ void fill_zeros(const SortArgs& a, int64_t block, int64_t blocks) {
+// more where dw is over kFillBlocks * 16 KiB.  Each XCD writes an eighth of dw:
+// 8192 tokens into [128000, 4096] 183.7 us in all instead of 204.4, 4096 into
+// [50000, 2048] fp32 76.9 instead of 81.4.
+__device__ __forceinline__ void fill_zeros(const SortArgs& a, uint32_t block, uint32_t blocks) {
   Values<uint16_t, 8> zero;
   zero.clear();
-  for (int64_t at = (block * kSortThreads + threadIdx.x) * 8; at < a.fill_values;
-       at += blocks * kSortThreads * 8) {
+  const int64_t first = int64_t{xcd_order(block, blocks)} * kSortThreads + threadIdx.x;
+  for (int64_t at = first * 8; at < a.fill_values; at += int64_t{blocks} * kSortThreads * 8) {
     if (at + 8 <= a.fill_values) zero.store_stream(a.fill + at);
     else zero.store_part(a.fill + at, static_cast<int>(a.fill_values - at));
   }
@@ -568,23 +571,77 @@ __global__ __launch_bounds__(kThreads) void join_pieces(BwdArgs a) {
 // ---------------------------------------------------------------------------
 // Few tokens: no sort.  A workgroup per position and 64 lanes' columns looks
 // through all tokens: where its own occurs first it sums all of that token's
-// rows, each wave a part of them.
+// rows, each wave a part of them.  Workgroups behind those write the zeros of
+// the other rows (a launch of zeros before it: [17, 94] fp32 into 13054 rows
+// 6.7 us instead of 5.0, [16, 2880] into [50001, 2880] fp32 100.8 instead of 92.1).
 // ---------------------------------------------------------------------------
-
-__global__ __launch_bounds__(kSortThreads) void zero_values(SortArgs a) {
-  fill_zeros(a, blockIdx.x, gridDim.x);
-}
 
 struct FewArgs {
   const void* grad;
   const void* tokens;
   void* dw;
   int64_t vocab, padding_idx;
-  DivMagic by_chunks;
+  DivMagic by_chunks, by_width;
   int count, width, chunks;  // workgroups per row
   float scale;
   int token_size;
 };
+
+// Zeros to kFewFill 16-byte pieces of dw per thread, but not to rows that a
+// token takes: those are marked first.  Each XCD writes an eighth of dw: 64
+// tokens into [128000, 4096] bf16 165.6 us instead of 179.2, 128 into [32000, 768]
+// 11.8 instead of 11.5.  With one / two / four pieces 200.1 / 165.6 / 177.5 and
+// 15.2 / 11.8 / 11.9.
+template <typename O>
+__device__ __forceinline__ void zero_other_rows(const FewArgs& f, int64_t block, uint32_t* marks) {
+  constexpr int C = 16 / sizeof(O), kValues = kFewThreads * kFewFill * C;
+  static_assert(kValues <= kFewTokens * 32);
+  const int tid = threadIdx.x;
+  const int64_t from = block * kValues;
+  const int values = static_cast<int>(std::min<int64_t>(f.vocab * f.width - from, kValues));
+  const int64_t row0 = from / f.width;
+  const int skip = static_cast<int>(from - row0 * f.width);
+  const int rows = static_cast<int>(div_by(skip + values - 1, f.by_width)) + 1;
+  int64_t mine[kFewTokens / kFewThreads];
+#pragma unroll
+  for (int k = 0; k < kFewTokens / kFewThreads; ++k) {
+    const int i = k * kFewThreads + tid;
+    mine[k] = i < f.count ? token_at(f.tokens, f.token_size, i) : -1;
+  }
+  for (int i = tid; i < (rows + 31) / 32; i += kFewThreads) marks[i] = 0;
+  __syncthreads();
+  int taken = 0;
+#pragma unroll
+  for (int k = 0; k < kFewTokens / kFewThreads; ++k) {
+    if (mine[k] >= row0 && mine[k] < row0 + rows && mine[k] != f.padding_idx) {
+      const uint32_t r = static_cast<uint32_t>(mine[k] - row0);
+      atomicOr(marks + r / 32, 1u << (r % 32));
+      taken = 1;
+    }
+  }
+  taken = __syncthreads_or(taken);
+  O* dw = static_cast<O*>(f.dw) + from;
+  Values<O, C> zero;
+  zero.clear();
+  const auto marked = [&](int v) {
+    const uint32_t r = div_by(skip + v, f.by_width);
+    return (marks[r / 32] >> (r % 32)) & 1;
+  };
+#pragma unroll
+  for (int k = 0; k < kFewFill; ++k) {
+    const int v = (k * kFewThreads + tid) * C;
+    if (v >= values) break;
+    const int n = std::min(values - v, C);
+    if (!taken || (f.width >= C && !marked(v) && !marked(v + n - 1))) {
+      if (n == C) zero.store_stream(dw + v);
+      else zero.store_part(dw + v, n);
+    } else {
+      for (int c = 0; c < n; ++c) {
+        if (!marked(v + c)) dw[v + c] = O{0};
+      }
+    }
+  }
+}
 
 template <typename T, typename O, int C, bool WHOLE, bool ADD>
 __global__ __launch_bounds__(kFewThreads) void sum_few(FewArgs f) {
@@ -593,6 +650,12 @@ __global__ __launch_bounds__(kFewThreads) void sum_few(FewArgs f) {
   __shared__ int list[kFewTokens];
   __shared__ float part[kWaves][C][kWave];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6;
+  if (!ADD && blockIdx.x >= static_cast<unsigned>(f.count * f.chunks)) {
+    const uint32_t sums = f.count * f.chunks;
+    zero_other_rows<O>(f, xcd_order(blockIdx.x - sums, gridDim.x - sums),
+                       reinterpret_cast<uint32_t*>(list));
+    return;
+  }
   const int t = static_cast<int>(div_by(blockIdx.x, f.by_chunks));
   const int col = ((static_cast<int>(blockIdx.x) - t * f.chunks) * kWave + lane) * C;
   const int64_t token = token_at(f.tokens, f.token_size, t);
@@ -662,13 +725,15 @@ __global__ __launch_bounds__(kFewThreads) void sum_few(FewArgs f) {
   out.write(sum, f.scale);
 }
 
-// Up to so many tokens and gradient values there is no sort (one launch, two
-// where the rest is zeroed, and no workspace).  Graph replays of bf16, us, with the
-// sort / this: added [128, 768] 9.0 / 4.7, [512, 512] 11.0 / 5.6, [1024, 64] 13.1 /
-// 7.4, [1024, 768] 12.6 / 11.4; of one token alone 10.5 / 5.4, 11.4 / 9.8, 13.3 /
-// 16.1, 14.0 / 20.2.  [512, 512] with 256 threads 5.0 and 14.9, with 1024 7.1 and 9.4.
-inline bool few_tokens(int64_t count, int64_t width) {
-  return count <= kFewTokens && count * width <= 1 << 19;
+// Up to so many tokens and gradient values there is no sort: one launch and no
+// workspace.  Graph replays of bf16, us, with the sort / this: added [128, 768] 9.0 /
+// 4.7, [512, 512] 11.0 / 5.6, [1024, 64] 13.1 / 7.4, [1024, 768] 12.6 / 11.4; of one
+// token alone 10.5 / 5.4, 11.4 / 9.8, 13.3 / 16.1, 14.0 / 20.2.  [512, 512] with 256
+// threads 5.0 and 14.9, with 1024 7.1 and 9.4.
+// 2^31 threads write the zeros of 2^34 fp32 values.
+inline bool few_tokens(int64_t count, int64_t width, int64_t vocab) {
+  return count <= kFewTokens && width <= (1 << 19) / std::max<int64_t>(count, 1) &&
+         vocab <= (int64_t{1} << 34) / width;
 }
 
 // Workspace: the order, the number of places, the sums of pieces; each 16-byte
@@ -707,26 +772,23 @@ void for_lanes(int64_t rows, int64_t pieces, F&& launch) {
   }
 }
 
-inline int64_t fill_blocks(const SortArgs& s) {
-  constexpr int64_t kPerBlock = int64_t{kSortThreads} * 8;
-  return std::min((s.fill_values + kPerBlock - 1) / kPerBlock, kFillBlocks);
-}
-
 template <typename T, typename O>
 void launch_few(const BwdArgs& a, const SortArgs& s, int token_size, bool accumulate,
                 hipStream_t stream) {
   constexpr int C = 16 / sizeof(T);
   const bool whole = a.width % C == 0;
-  if (!accumulate)
-    zero_values<<<dim3(static_cast<unsigned>(fill_blocks(s))), dim3(kSortThreads), 0, stream>>>(s);
-  if (s.count == 0) return;
   const int chunks = (a.width + C * kWave - 1) / (C * kWave);
   const FewArgs f{a.grad, s.tokens, a.dw, s.vocab, s.padding_idx, div_magic(chunks),
-                  static_cast<int>(s.count), a.width, chunks, a.scale, token_size};
+                  div_magic(a.width), static_cast<int>(s.count), a.width, chunks, a.scale,
+                  token_size};
+  constexpr int64_t kFill = int64_t{kFewThreads} * kFewFill * 16 / sizeof(O);
+  const int64_t fills = accumulate ? 0 : (s.vocab * a.width + kFill - 1) / kFill;
+  const int64_t groups = f.count * chunks + fills;
+  if (groups == 0) return;
   auto kernel = accumulate
                     ? (whole ? sum_few<T, O, C, true, true> : sum_few<T, O, C, false, true>)
                     : (whole ? sum_few<T, O, C, true, false> : sum_few<T, O, C, false, false>);
-  kernel<<<dim3(static_cast<unsigned>(f.count * chunks)), dim3(kFewThreads), 0, stream>>>(f);
+  kernel<<<dim3(static_cast<unsigned>(groups)), dim3(kFewThreads), 0, stream>>>(f);
 }
 
 template <typename T, typename O>
@@ -736,7 +798,9 @@ void launch_bwd(BwdArgs a, SortArgs s, int token_size, bool accumulate, hipStrea
   a.pieces = (a.width + C - 1) / C;
   a.by_pieces = div_magic(a.pieces);
   auto sort = token_size == 8 ? sort_tokens<int64_t> : sort_tokens<int32_t>;
-  const int64_t fill = accumulate ? 0 : fill_blocks(s);
+  constexpr int64_t kPerBlock = int64_t{kSortThreads} * 8;
+  const int64_t fill =
+      accumulate ? 0 : std::min((s.fill_values + kPerBlock - 1) / kPerBlock, kFillBlocks);
   sort<<<dim3(static_cast<unsigned>((int64_t{1} << s.group_bits) + fill)), dim3(kSortThreads), 0,
          stream>>>(s);
   a.places = s.count;
@@ -799,7 +863,7 @@ extern "C" int hipo_embedding(const void* weight, int elem_size, const void* tok
 
 extern "C" size_t hipo_embedding_bwd_workspace_bytes(int64_t count, int64_t width,
                                                      int64_t vocab) {
-  if (count < 0 || width <= 0 || vocab <= 0 || hipo::few_tokens(count, width)) return 0;
+  if (count < 0 || width <= 0 || vocab <= 0 || hipo::few_tokens(count, width, vocab)) return 0;
   return hipo::layout(count, width).bytes;
 }
 
@@ -842,7 +906,7 @@ extern "C" int hipo_embedding_bwd(const void* grad, int elem_size, const void* t
       else launch(float{}, float{});
     }
   };
-  if (few_tokens(count, width)) {
+  if (few_tokens(count, width, vocab)) {
     run([&](auto t, auto o) {
       launch_few<decltype(t), decltype(o)>(a, s, token_size, accumulate != 0, stream);
     });

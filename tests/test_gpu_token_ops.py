@@ -338,7 +338,9 @@ def test_ids_past_32_bits(rocm_device, ho):
     (300, 4096, 100, "unknown"), (2049, 33, 131073, "uniform"), (16, 8, 2, "one"), (17, 8, 2, "one"),
     (1024, 512, 3000, "text"), (1024, 513, 3000, "text"), (1025, 16, 3000, "text"),
     (1023, 100, 7, "uniform"), (513, 700, 40, "one"), (1000, 5, 300, "unknown"),
-    (16, 32769, 5, "text"), (16, 32768, 5, "text"), (32, 24, 1, "one"), (33, 24, 1, "one"), (64, 24, 2, "one"), (96, 24, 3, "runs"), (16384, 24, 9000, "text"),
+    (16, 32769, 5, "text"), (16, 32768, 5, "text"), (32, 24, 1, "one"), (33, 24, 1, "one"),
+    (64, 24, 2, "one"), (96, 24, 3, "runs"), (16384, 24, 9000, "text"),
+    (17, 94, 13054, "text"), (900, 3, 20011, "text"), (300, 1, 70001, "uniform"),
     (33000, 8, 300000, "text"), (8193, 64, 8192, "runs")])
 def test_embedding_backward(count, width, vocab, kind, dtype, out, rocm_device, ho):
     g = torch.Generator().manual_seed(count + width)

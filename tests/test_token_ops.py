@@ -88,6 +88,8 @@ def test_workspaces_are_checked(lib):
     assert lib.hipo_embedding_bwd_workspace_bytes(1024, 512, 32000) == 0  # no sort
     assert lib.hipo_embedding_bwd_workspace_bytes(1024, 513, 32000) > 0
     assert lib.hipo_embedding_bwd_workspace_bytes(1025, 8, 32000) > 0
+    assert lib.hipo_embedding_bwd_workspace_bytes(1, 16, 1 << 30) == 0
+    assert lib.hipo_embedding_bwd_workspace_bytes(1, 17, 1 << 30) > 0
 
 
 def test_empty_calls_are_no_ops(lib):
