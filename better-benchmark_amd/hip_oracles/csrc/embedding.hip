@@ -4,10 +4,13 @@
 // end.  Both move rows: HBM bounds them.
 //
 // Lookup: a lane per 16-byte piece of the output, pieces in memory order, so
-// no lane is idle whatever the width.  Non-temporal stores (cached ones: 2.5
-// times as long); [8192, 4096] bf16 16.1 us, 6.1 TB/s, with two / four pieces
-// per lane 17.2 / 17.5; rows off 16 bytes lose a fifth ([20011, 1001] fp32 20.5
-// us, [20011, 1000] 18.7; pieces aligned in the output instead: 21.4).
+// no lane is idle whatever the width.  Non-temporal stores (cached ones: 1.6
+// times as long); [8192, 4096] bf16 16.4 us, 6.0 TB/s.  Each XCD writes an eighth
+// of the output, so that lines that two rows share are merged in one L2: us, by
+// XCD / in the launch's order, [20011, 1001] fp32 19.0 / 20.4, [20011, 2001] bf16
+// 21.0 / 22.7, [20011, 1000] fp32 18.1 / 18.7, [8192, 4096] bf16 16.4 / 16.0.  In
+// the launch's order two / four pieces per lane took 17.2 / 17.5 there, pieces
+// aligned in the output 21.4 at [20011, 1001].
 //
 // Gradient, three launches:
 //   1. sort_tokens: the positions in order of their token, equal tokens in
@@ -19,8 +22,8 @@
 //      200 cycles per 64 tokens and SIMD: 6.6 us at 8192 tokens, 21 us at
 //      65536.
 //      Other workgroups of the same launch write zeros to all of dw: most of
-//      the bytes where tokens are fewer than rows ([128000, 4096] bf16 160 us,
-//      6.5 TB/s), and beside the sort hardly any time where they are not (rows
+//      the bytes where tokens are fewer than rows ([128000, 4096] bf16 158 us,
+//      6.6 TB/s), and beside the sort hardly any time where they are not (rows
 //      without a token found and zeroed by sum_rows instead: [65536, 2048] into
 //      [32000, 2048] 106.5 us against 101.4, [65536, 64] into [1696, 64] 38.2
 //      against 39.1).
@@ -127,7 +130,7 @@ struct FwdArgs {
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void embedding_rows(FwdArgs a) {
   constexpr int C = 16 / sizeof(T);
-  const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
+  const uint32_t id = xcd_order(blockIdx.x, gridDim.x) * kThreads + threadIdx.x;
   const uint32_t t = div_by(id, a.by_pieces);
   if (t >= a.count) return;
   const int col = static_cast<int>(id - t * a.pieces) * C;
