@@ -6,7 +6,6 @@ Each case is one call.  Where `own` is false, run() computes it with
 elementary torch operations in fp32; where it is true, run() calls the
 library's functions of the same meaning.
 """
-import functools
 import math
 import os
 import sys
@@ -21,9 +20,7 @@ _BYTES = {"bf16": 2, "f32": 4}
 IGNORE = -100
 
 
-@functools.lru_cache(maxsize=None)
 def _library():
-    """The library, imported once, as a program does."""
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     pkg = os.path.join(root, "better-benchmark_amd")
     if pkg not in sys.path:
