@@ -580,3 +580,19 @@ def test_the_run_in_a_graph(rows, rocm_device, ho):
         torch.cuda.synchronize()
         for k, (u, v) in enumerate(zip(captured, eager)):
             assert torch.equal(u, v), f"replay {seed}, output {k}"
+
+
+def test_embedding_backward_into_the_largest_vocabulary(rocm_device, ho):
+    """2^30 rows, 36 GB of gradient: the most workgroups that sort beside the
+    most that write zeros."""
+    width, vocab = 17, 1 << 30
+    t = torch.tensor([vocab - 1, 0, 1 << 29, vocab - 1], device=rocm_device)
+    grad = torch.randn(4, width, device=rocm_device).to(BF16)
+    dw = ho.embedding_bwd(grad, t, vocab)
+    torch.cuda.synchronize()
+    print("largest vocabulary: launched", flush=True)
+    assert torch.equal(dw[0], grad[1]) and torch.equal(dw[1 << 29], grad[2])
+    assert torch.equal(dw[-1], (grad[0].float() + grad[3].float()).to(BF16))
+    dw[t] = 0
+    flat = dw.view(-1)
+    assert not any(bool(part.any()) for part in flat.split(1 << 30))

@@ -1,0 +1,47 @@
+"""The launches of the token operators, without a GPU: a small program whose own
+functions stand in for HIP's records them.  A launch has fewer than 2^32
+threads along each axis, and one that is refused is not followed by those that
+read its results."""
+import subprocess
+
+import pytest
+
+import hip_oracles
+from conftest import ROOT
+
+
+@pytest.fixture(scope="module")
+def launches(tmp_path_factory):
+    program = tmp_path_factory.mktemp("recorder") / "launch_recorder"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-rdynamic",
+                    str(ROOT / "tests" / "launch_recorder.cpp"), str(hip_oracles.LIB_PATH),
+                    f"-Wl,-rpath,{hip_oracles.LIB_PATH.parent}", "-Wl,--allow-shlib-undefined",
+                    "-o", str(program)], check=True, capture_output=True)
+
+    def run(op, *numbers, fail=-1):
+        """([(kernel, grid, block)], return code)"""
+        out = subprocess.run([str(program), str(fail), op, *map(str, numbers)], check=True,
+                             capture_output=True, text=True).stdout.splitlines()
+        made = [line.split() for line in out[:-1]]
+        return ([(m[0], tuple(map(int, m[1:4])), tuple(map(int, m[4:7]))) for m in made],
+                int(out[-1].split()[1]))
+
+    return run
+
+
+def assert_launchable(made):
+    for kernel, grid, block in made:
+        assert block[0] * block[1] * block[2] <= 1024, (kernel, block)
+        assert grid[1] <= 65535 and grid[2] <= 65535 and min(grid) > 0, (kernel, grid)
+        assert all(g * b < 1 << 32 for g, b in zip(grid, block)), (kernel, grid, block)
+
+
+@pytest.mark.parametrize("out", [2, 4])
+@pytest.mark.parametrize("vocab", [(1 << 30), (1 << 29) + 1, 1 << 29, 10 ** 7, 32000])
+@pytest.mark.parametrize("count,width", [(1, 17), (1, 32), (1025, 8), (2000, 4096), (0, 1 << 20),
+                                         (70001, 1 << 16)])
+def test_embedding_gradients_of_large_vocabularies(count, width, vocab, out, launches):
+    for accumulate in (0, 1):
+        made, rc = launches("embedding_bwd", count, width, vocab, 2, out, accumulate)
+        assert rc == 0 and (made or count == 0)
+        assert_launchable(made)
