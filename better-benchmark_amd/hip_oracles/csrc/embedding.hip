@@ -778,8 +778,8 @@ void for_lanes(int64_t rows, int64_t pieces, F&& launch) {
 }
 
 template <typename T, typename O>
-void launch_few(const BwdArgs& a, const SortArgs& s, int token_size, bool accumulate,
-                hipStream_t stream) {
+int launch_few(const BwdArgs& a, const SortArgs& s, int token_size, bool accumulate,
+               hipStream_t stream) {
   constexpr int C = 16 / sizeof(T);
   const bool whole = a.width % C == 0;
   const int chunks = (a.width + C * kWave - 1) / (C * kWave);
@@ -789,15 +789,17 @@ void launch_few(const BwdArgs& a, const SortArgs& s, int token_size, bool accumu
   constexpr int64_t kFill = int64_t{kFewThreads} * kFewFill * 16 / sizeof(O);
   const int64_t fills = accumulate ? 0 : (s.vocab * a.width + kFill - 1) / kFill;
   const int64_t groups = f.count * chunks + fills;
-  if (groups == 0) return;
+  if (groups == 0) return 0;
   auto kernel = accumulate
                     ? (whole ? sum_few<T, O, C, true, true> : sum_few<T, O, C, false, true>)
                     : (whole ? sum_few<T, O, C, true, false> : sum_few<T, O, C, false, false>);
   kernel<<<dim3(static_cast<unsigned>(groups)), dim3(kFewThreads), 0, stream>>>(f);
+  return check_launch("embedding_bwd");
 }
 
+// Each launch reads what the one before it wrote: none follows one that was refused.
 template <typename T, typename O>
-void launch_bwd(BwdArgs a, SortArgs s, int token_size, bool accumulate, hipStream_t stream) {
+int launch_bwd(BwdArgs a, SortArgs s, int token_size, bool accumulate, hipStream_t stream) {
   constexpr int C = 16 / sizeof(T);
   const bool whole = a.width % C == 0;
   a.pieces = (a.width + C - 1) / C;
@@ -808,6 +810,7 @@ void launch_bwd(BwdArgs a, SortArgs s, int token_size, bool accumulate, hipStrea
       accumulate ? 0 : std::min((s.fill_values + kPerBlock - 1) / kPerBlock, kFillBlocks);
   sort<<<dim3(static_cast<unsigned>((int64_t{1} << s.group_bits) + fill)), dim3(kSortThreads), 0,
          stream>>>(s);
+  if (const int rc = check_launch("embedding_bwd")) return rc;
   a.places = s.count;
   auto rows = accumulate
                   ? (whole ? sum_rows<T, O, C, true, true> : sum_rows<T, O, C, false, true>)
@@ -817,7 +820,8 @@ void launch_bwd(BwdArgs a, SortArgs s, int token_size, bool accumulate, hipStrea
     a.count = n;
     rows<<<grid, dim3(kThreads), 0, stream>>>(a);
   });
-  if (a.bins == 0) return;
+  if (const int rc = check_launch("embedding_bwd")) return rc;
+  if (a.bins == 0) return 0;
   auto join = accumulate
                   ? (whole ? join_pieces<O, C, true, true> : join_pieces<O, C, false, true>)
                   : (whole ? join_pieces<O, C, true, false> : join_pieces<O, C, false, false>);
@@ -828,6 +832,7 @@ void launch_bwd(BwdArgs a, SortArgs s, int token_size, bool accumulate, hipStrea
     const int64_t n = std::min(step, a.bins - a.first) * a.pieces;
     join<<<dim3(static_cast<unsigned>(n)), dim3(kThreads), 0, stream>>>(a);
   }
+  return check_launch("embedding_bwd");
 }
 
 }  // namespace
@@ -903,19 +908,14 @@ extern "C" int hipo_embedding_bwd(const void* grad, int elem_size, const void* t
     s.fill_values = vocab * width * (out_size / 2);
   }
   const auto run = [&](auto launch) {
-    if (elem_size == 2) {
-      if (out_size == 2) launch(uint16_t{}, uint16_t{});
-      else launch(uint16_t{}, float{});
-    } else {
-      if (out_size == 2) launch(float{}, uint16_t{});
-      else launch(float{}, float{});
-    }
+    if (elem_size == 2)
+      return out_size == 2 ? launch(uint16_t{}, uint16_t{}) : launch(uint16_t{}, float{});
+    return out_size == 2 ? launch(float{}, uint16_t{}) : launch(float{}, float{});
   };
   if (few_tokens(count, width, vocab)) {
-    run([&](auto t, auto o) {
-      launch_few<decltype(t), decltype(o)>(a, s, token_size, accumulate != 0, stream);
+    return run([&](auto t, auto o) {
+      return launch_few<decltype(t), decltype(o)>(a, s, token_size, accumulate != 0, stream);
     });
-    return check_launch("embedding_bwd");
   }
   const Layout l = layout(count, width);
   HIPO_REQUIRE(workspace != nullptr && workspace_bytes >= l.bytes,
@@ -933,8 +933,7 @@ extern "C" int hipo_embedding_bwd(const void* grad, int elem_size, const void* t
          (int64_t{kSortRows} << s.group_bits) < vocab) {
     ++s.group_bits;
   }
-  run([&](auto t, auto o) {
-    launch_bwd<decltype(t), decltype(o)>(a, s, token_size, accumulate != 0, stream);
+  return run([&](auto t, auto o) {
+    return launch_bwd<decltype(t), decltype(o)>(a, s, token_size, accumulate != 0, stream);
   });
-  return check_launch("embedding_bwd");
 }

@@ -45,3 +45,15 @@ def test_embedding_gradients_of_large_vocabularies(count, width, vocab, out, lau
         made, rc = launches("embedding_bwd", count, width, vocab, 2, out, accumulate)
         assert rc == 0 and (made or count == 0)
         assert_launchable(made)
+
+
+@pytest.mark.parametrize("accumulate", [0, 1])
+def test_a_refused_launch_ends_an_embedding_gradient(accumulate, launches):
+    """sum_rows reads the order that the sort writes, and the pieces that are
+    joined are sum_rows's."""
+    call = ("embedding_bwd", 2000, 64, 5000, 2, 4, accumulate)
+    made, rc = launches(*call)
+    assert rc == 0 and len(made) == len({kernel for kernel, _, _ in made}) == 3
+    for n in range(3):
+        again, rc = launches(*call, fail=n)
+        assert rc == 9 and again == made[:n + 1]
