@@ -853,7 +853,9 @@ extern "C" int hipo_token_logprobs(const void* logits, int elem_size, const void
   for (; a.first < rows; a.first += step) {
     const unsigned n = static_cast<unsigned>(std::min(step, rows - a.first));
     kernel<<<dim3(n * p.slices), dim3(p.threads), 0, stream>>>(a);
-    if (p.slices > 1) join<<<dim3(n), dim3(kThreads), 0, stream>>>(a);
+    if (p.slices == 1) continue;
+    if (const int rc = check_launch("token_logprobs")) return rc;  // nothing to join
+    join<<<dim3(n), dim3(kThreads), 0, stream>>>(a);
   }
   return check_launch("token_logprobs");
 }

@@ -57,3 +57,11 @@ def test_a_refused_launch_ends_an_embedding_gradient(accumulate, launches):
     for n in range(3):
         again, rc = launches(*call, fail=n)
         assert rc == 9 and again == made[:n + 1]
+
+
+def test_a_refused_launch_ends_sliced_log_probabilities(launches):
+    call = ("token_logprobs", 2, 1 << 20, 2, 8)
+    made, rc = launches(*call)
+    assert rc == 0 and len(made) == 2
+    again, rc = launches(*call, fail=0)
+    assert rc == 9 and again == made[:1]
