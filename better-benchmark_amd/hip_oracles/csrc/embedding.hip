@@ -888,8 +888,11 @@ extern "C" int hipo_embedding_bwd(const void* grad, int elem_size, const void* t
   HIPO_REQUIRE((elem_size == 2 || elem_size == 4) && (out_size == 2 || out_size == 4),
                "embedding_bwd: elem_size and out_size must be 2 or 4");
   HIPO_REQUIRE(token_size == 4 || token_size == 8, "embedding_bwd: token_size must be 4 or 8");
-  HIPO_REQUIRE(count <= 0x7fffffff - 4096 && width <= 0x7fffffff && vocab <= (1 << 30),
-               "embedding_bwd: count over 2^31 - 4096, width over 2^31 or vocab over 2^30");
+  // A workgroup counts its lanes' columns past the last, a batch of places past
+  // the end, in 32 bits.
+  constexpr int64_t kMost = 0x7fffffff - 4096;
+  HIPO_REQUIRE(count <= kMost && width <= kMost && vocab <= (1 << 30),
+               "embedding_bwd: count or width over 2^31 - 4097 or vocab over 2^30");
   if (width == 0 || vocab == 0) return 0;
   HIPO_REQUIRE(dweight != nullptr && (count == 0 || (grad != nullptr && tokens != nullptr)),
                "embedding_bwd: null pointer");

@@ -515,8 +515,9 @@ int hipo_embedding(const void* weight, int elem_size, const void* tokens,
  * equal to padding_idx, and tokens outside [0, vocab), add nothing (an index
  * outside [0, vocab): no padding).  grad is contiguous [count, width] of bf16
  * (elem_size 2) or fp32 (4), dweight contiguous [vocab, width] of bf16
- * (out_size 2) or fp32 (4), the two apart; vocab is at most 2^30.  `workspace`:
- * at least hipo_embedding_bwd_workspace_bytes bytes, 16-byte aligned, no
+ * (out_size 2) or fp32 (4), the two apart; count and width are at most
+ * 2^31 - 4097, vocab 2^30.  `workspace`: at least
+ * hipo_embedding_bwd_workspace_bytes bytes, 16-byte aligned, no
  * initialisation needed (NULL when that is 0); calls that share one must be
  * ordered.
  * No counterpart among the reference's oracles.

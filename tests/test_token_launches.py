@@ -65,3 +65,19 @@ def test_a_refused_launch_ends_sliced_log_probabilities(launches):
     assert rc == 0 and len(made) == 2
     again, rc = launches(*call, fail=0)
     assert rc == 9 and again == made[:1]
+
+
+def test_the_widest_embedding_gradients(launches):
+    """Columns are counted in 32 bits, up to a workgroup's columns past the last."""
+    most = (1 << 31) - 4097
+    for elem in (2, 4):
+        pieces = -(-most * elem // 16)
+        made, rc = launches("embedding_bwd", 33, most, 3, elem, 4, 1)
+        assert rc == 0
+        assert_launchable(made)
+        # 33 places, and the sums of two pieces of 32 in two forms.
+        lanes = sum(grid[0] * block[0] for kernel, grid, block in made if "sum_rows" in kernel)
+        assert lanes >= pieces * (33 + 2 * 2)
+        for width in (most + 1, (1 << 31) - 1):
+            made, rc = launches("embedding_bwd", 33, width, 3, elem, 4, 1)
+            assert rc == 1000 and not made
