@@ -473,7 +473,8 @@ __device__ __forceinline__ const uint64_t* slice_top(const Slice<T>& s, DivMagic
     uint64_t best = 0;
     const auto look = [&](float v, int index) {
       const uint64_t key = order_key(order_of(v), static_cast<uint32_t>(index));
-      if (key < last && key > best) best = key;
+      // (A NaN at index 0 has the largest key there is.)
+      if ((i == 0 || key < last) && key > best) best = key;
     };
     if (s.odd >= 0) look(to_f32(s.x[s.odd]), s.odd);
     for (int v = s.lo + tid; v < s.hi; v += NT) {

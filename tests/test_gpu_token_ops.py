@@ -596,3 +596,21 @@ def test_embedding_backward_into_the_largest_vocabulary(rocm_device, ho):
     dw[t] = 0
     flat = dw.view(-1)
     assert not any(bool(part.any()) for part in flat.split(1 << 30))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab", [(2, 4096), (3, 30000), (130, 32768), (2, 131072)])
+def test_alternatives_that_a_few_lanes_hold_with_nan(rows, vocab, dtype, rocm_device, ho):
+    """As above, and the first value, whose key is the largest there is, is NaN;
+    then others too."""
+    g = torch.Generator().manual_seed(vocab)
+    run = 32 * 16 // dtype.itemsize
+    x = torch.randn(rows, vocab, generator=g)
+    t = torch.randint(0, vocab, (rows,), generator=g)
+    for high in (0, 1):
+        y = (x + 50.0 * ((torch.arange(vocab) // run + high) % 2)).to(dtype)
+        y[:, 0] = NAN
+        for top in (1, 33, 34, 64):
+            check_forward(ho, rocm_device, y, t, top=top, what=f"stripes {vocab} {top} {high}")
+        y[1:, ::run] = NAN
+        check_forward(ho, rocm_device, y, t, top=64, what=f"stripes {vocab} {high}, more NaN")
