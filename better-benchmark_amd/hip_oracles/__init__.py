@@ -740,7 +740,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, scale: float =
     whatever its logits hold: its results are 0, its alternatives -inf and -1.  Any other token outside
     [0, V) has log probability NaN.  A row with nothing above -inf has lse
     -inf, with +inf lse +inf, with NaN lse NaN; there logprob = scale * logit -
-    lse, and the entropy is NaN."""
+    lse, and the entropy is NaN.  Elsewhere no log probability is above 0, no
+    entropy below."""
     lib = _lib or load_library()
     dev = _require_rocm(logits, tokens)
     rows, vocab, stride = _require_logits("token_logprobs", logits, tokens, scale)

@@ -172,16 +172,21 @@ struct Row {
   float m, log_z, lse, entropy;
 };
 
+// Z and U relative to m itself.  The largest value's own term is e_m = 2^(w of
+// m), the same bits here as in Z, and sums of positive terms never fall below
+// one of them: Z / e_m >= 1, and exactly 1 where one value is all there is.  So
+// ln Z >= 0: no log probability is above 0, no entropy below.
 __device__ __forceinline__ Row finish(Stats s, float scale, float c) {
+  // U - w_m Z, two roundings of one product: 0 where one value is all there is.
+#pragma clang fp contract(off)
   Row r;
   r.m = s.m;
   if (fabsf(s.m) < kInf) {
     const float o = offset(s.m, c);
-    const float log2_z = __builtin_amdgcn_logf(s.z);
-    // Z is relative to round(c m) where that is near: what it is off c m by.
-    r.log_z = kLn2 * (is_far(o) ? log2_z : log2_z + __builtin_fmaf(-s.m, c, -o));
+    const float w_m = is_far(o) ? 0.0f : __builtin_fmaf(s.m, c, o);
+    r.log_z = maximum(kLn2 * __builtin_amdgcn_logf(s.z / __builtin_amdgcn_exp2f(w_m)), 0.0f);
     r.lse = __builtin_fmaf(scale, s.m, r.log_z);
-    r.entropy = kLn2 * (log2_z - s.u / s.z);
+    r.entropy = maximum(r.log_z + kLn2 * ((w_m * s.z - s.u) / s.z), 0.0f);
   } else {  // -inf: nothing is left; +inf; NaN
     r.log_z = 0.0f;
     r.lse = s.m;

@@ -454,7 +454,8 @@ int hipo_gelu_erf_bwd_colsum_bf16(const uint16_t* grad, const uint16_t* x, uint1
  * 0, 0, 0, and for the alternatives -inf and -1.  A token outside [0, vocab) otherwise has
  * logprob NaN.  A row with nothing above -inf has lse -inf, one with +inf
  * lse +inf, one with NaN lse NaN; their logprobs are s - lse, their entropy
- * NaN.  `workspace`: at least hipo_token_logprobs_workspace_bytes bytes,
+ * NaN.  Of the others no logprob is above 0 and no entropy below, and both are
+ * 0 where one value above -inf is all there is.  `workspace`: at least hipo_token_logprobs_workspace_bytes bytes,
  * 16-byte aligned, no initialisation needed (NULL when that is 0); calls
  * that share one must be ordered.
  * No counterpart among the reference's oracles; beside

@@ -614,3 +614,30 @@ def test_alternatives_that_a_few_lanes_hold_with_nan(rows, vocab, dtype, rocm_de
             check_forward(ho, rocm_device, y, t, top=top, what=f"stripes {vocab} {top} {high}")
         y[1:, ::run] = NAN
         check_forward(ho, rocm_device, y, t, top=64, what=f"stripes {vocab} {high}, more NaN")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab", [
+    (40, 70), (64, 2001), (1100, 4097), (300, 9001), (40, 33000), (6, 262147), (2048, 8200)])
+@pytest.mark.parametrize("scale", [1.0, 0.7, 1.25])
+def test_no_probability_above_one(rows, vocab, scale, dtype, rocm_device, ho):
+    """Rows that one token decides, alone or 17 to 30 above 200 others: no log
+    probability above 0, no entropy below, lse not below the largest value; of
+    a token that is alone exactly 0."""
+    g = torch.Generator().manual_seed(vocab)
+    t = torch.randint(0, vocab, (rows,), generator=g)
+    high = torch.randn(rows, generator=g) * 30.0
+    high[::20] *= 1e5  # far from zero too
+    x = torch.full((rows, vocab), -INF)
+    for r in range(1, rows, 2):
+        others = torch.randint(0, vocab, (200,), generator=g)
+        x[r, others] = high[r] - 17.0 - r % 14 + torch.randn(200, generator=g)
+    x[torch.arange(rows), t] = high
+    x = x.to(dtype)
+    lp, lse, ent, tv, _ = (v.cpu() for v in ho.token_logprobs(
+        x.to(rocm_device), t.to(rocm_device), scale=scale, entropy=True, top=3))
+    assert (lp <= 0).all() and (tv <= 0).all()
+    assert (ent >= 0).all()
+    largest = x.double().amax(-1) * float(torch.tensor(scale))
+    assert (lse >= largest.float()).all()
+    assert (lp[::2] == 0).all() and (ent[::2] == 0).all()
