@@ -728,6 +728,18 @@ def _rows_apart_or_same(a: torch.Tensor, a_stride: int, b: torch.Tensor, b_strid
     return a_stride == b_stride and cols * size <= gap <= (a_stride - cols) * size
 
 
+def _apart_from_rows(t: torch.Tensor, a: torch.Tensor, stride: int, rows: int, cols: int) -> bool:
+    """Whether contiguous t shares no memory with [rows, cols] at a."""
+    size = a.element_size()
+    off = t.data_ptr() - a.data_ptr()  # of t from a's first row
+    length = t.numel() * t.element_size()
+    if length == 0 or cols == 0:
+        return True
+    # The first row that ends after t begins: it, if there is one, begins after t ends.
+    row = max(0, (off - cols * size) // (stride * size) + 1)
+    return row >= rows or row * stride * size >= off + length
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, scale: float = 1.0,
                    ignore_index: int = -100, entropy: bool = False, top: int = 0):
     """Log probabilities of tokens [R] (int32 or int64) under softmax(scale *
@@ -779,7 +791,8 @@ def token_logprobs_bwd(grad: torch.Tensor, logits: torch.Tensor, tokens: torch.T
     logprob, entropy and lse; lse, and entropy where grad_entropy is given,
     are its results.  Rows of ignore_index are zero, rows of another token
     outside [0, V) NaN.  out: where the result goes, the logits themselves or
-    memory that does not overlap them (any row stride >= V)."""
+    memory that does not overlap them (any row stride >= V); it does not
+    overlap the other inputs."""
     lib = _lib or load_library()
     rows_of = [t for t in (grad, lse, entropy, grad_entropy, grad_lse) if t is not None]
     dev = _require_rocm(logits, tokens, *rows_of, *(() if out is None else (out,)))
@@ -802,6 +815,10 @@ def token_logprobs_bwd(grad: torch.Tensor, logits: torch.Tensor, tokens: torch.T
         _require(out_stride >= vocab, "token_logprobs_bwd: rows of out overlap")
         _require(_rows_apart_or_same(out, out_stride, logits, stride, rows, vocab),
                  "token_logprobs_bwd: out and logits overlap")
+        for t in (tokens, *rows_of):
+            if not _apart_from_rows(t, out, out_stride, rows, vocab):
+                raise ValueError(f"{what}: out overlaps tokens, grad, lse, entropy, grad_entropy "
+                                 f"or grad_lse")
     _call(lib.hipo_token_logprobs_bwd, what, dev, _ptr(grad), _ptr(logits),
           logits.element_size(), _ptr(tokens), tokens.element_size(), _ptr(lse),
           *(None if t is None else _ptr(t) for t in (entropy, grad_entropy, grad_lse)),

@@ -478,8 +478,8 @@ int hipo_token_logprobs(const void* logits, int elem_size, const void* tokens,
  * fp32 arithmetic, one rounding to the logits' type.  lse, and entropy (with
  * grad_entropy), are the forward's results.  logits and dlogits are [rows,
  * vocab] with row strides of their own; dlogits may be logits itself (one
- * stride), and does not overlap it otherwise.  Rows of ignore_index are
- * zero, whatever they hold; rows of another token outside [0, vocab) are NaN.
+ * stride), and does not overlap it otherwise, nor the other inputs.  Rows of
+ * ignore_index are zero, whatever they hold; rows of another token outside [0, vocab) are NaN.
  * No counterpart among the reference's oracles; beside
  * hipo_gelu_erf_bwd_colsum_bf16 as a training gradient.
  */

@@ -641,3 +641,25 @@ def test_no_probability_above_one(rows, vocab, scale, dtype, rocm_device, ho):
     largest = x.double().amax(-1) * float(torch.tensor(scale))
     assert (lse >= largest.float()).all()
     assert (lp[::2] == 0).all() and (ent[::2] == 0).all()
+
+
+def test_a_gradient_over_its_other_inputs_is_refused(rocm_device, ho):
+    """fp32 vectors, and tokens, in the memory that the gradient is written to."""
+    rows, vocab = 4, 16
+    x = torch.zeros(rows, vocab, device=rocm_device)
+    t = torch.zeros(rows, dtype=torch.int64, device=rocm_device)
+    f = torch.zeros(rows, device=rocm_device)
+    out = torch.zeros(rows, 2 * vocab, device=rocm_device)
+    inside, between = out[1, 4:8], out[1, vocab:vocab + rows]
+    ids = out[0, :2 * rows].view(torch.int64)
+    for kw in (dict(grad=inside), dict(lse=inside), dict(tokens=ids),
+               dict(entropy=inside, grad_entropy=f), dict(entropy=f, grad_entropy=inside),
+               dict(grad_lse=inside), dict(lse=out[0, vocab - 1:vocab + 3])):
+        with pytest.raises(ValueError, match="overlaps"):
+            ho.token_logprobs_bwd(**{"grad": f, "logits": x, "tokens": t, "lse": f,
+                                     "out": out[:, :vocab], **kw})
+    # Between the rows there is room.
+    f += 2.0
+    between.copy_(f)
+    got = ho.token_logprobs_bwd(f, x, t, between, out=out[:, :vocab])
+    assert torch.equal(got, ho.token_logprobs_bwd(f, x, t, f)) and (between == 2.0).all()

@@ -163,3 +163,19 @@ def test_reference_embedding_gradient_against_differences():
     (torch.nn.functional.embedding(t, wd) * 1.5 * go.double()).sum().backward()
     assert torch.allclose(got, wd.grad, atol=1e-12)
     assert touched.tolist() == [True, True, False, False, True, False]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.int64])
+def test_vectors_beside_rows_of_a_buffer(dtype):
+    """Every place of a vector in and about rows with a gap, against the bytes."""
+    stride, cols, rows = 12, 7, 3
+    buf = torch.zeros(64, dtype=torch.bfloat16)
+    a = buf[8:8 + rows * stride].view(rows, stride)[:, :cols]
+    held = torch.zeros(64, dtype=torch.bool)
+    held[8:8 + rows * stride].view(rows, stride)[:, :cols] = True
+    step = dtype.itemsize // 2
+    for at in range(0, 64, step):
+        for n in range(0, (64 - at) // step + 1):
+            t = buf[at:at + n * step].view(dtype)
+            want = not bool(held[at:at + n * step].any())
+            assert hip_oracles._apart_from_rows(t, a, stride, rows, cols) == want, (at, n)
