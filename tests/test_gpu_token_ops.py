@@ -663,3 +663,113 @@ def test_a_gradient_over_its_other_inputs_is_refused(rocm_device, ho):
     between.copy_(f)
     got = ho.token_logprobs_bwd(f, x, t, between, out=out[:, :vocab])
     assert torch.equal(got, ho.token_logprobs_bwd(f, x, t, f)) and (between == 2.0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("rows,vocab", [(2048, 8200), (2049, 16421), (2500, 50001)])
+def test_forward_of_many_long_rows(rows, vocab, shift, dtype, rocm_device, ho):
+    """The kernel of a training batch, with and without each option; every 61st
+    row against the reference, ignored and unknown tokens among them."""
+    g = torch.Generator(device=rocm_device).manual_seed(vocab)
+    buf = torch.empty(rows * (vocab + 3) + shift, dtype=dtype, device=rocm_device)
+    x = buf[shift:].view(rows, vocab + 3)[:, :vocab]
+    x.copy_(torch.randn(rows, vocab, generator=g, device=rocm_device) * 3)
+    t = torch.randint(0, vocab, (rows,), generator=g, device=rocm_device)
+    some = torch.arange(0, rows, 61, device=rocm_device)
+    t[some[1]], t[some[2]], x[some[1]] = IGNORE, vocab, NAN
+    x[some[3], :vocab // 2] = -INF
+    want, tol = ref.token_logprobs(x[some], t[some], 0.7, top=3)
+    for top in (0, 3):
+        for entropy in (False, True):
+            got = list(ho.token_logprobs(x, t, scale=0.7, entropy=entropy, top=top))
+            torch.cuda.synchronize()
+            what = f"[{rows}, {vocab}] {dtype} top {top} entropy {entropy}"
+            if not entropy:
+                got.insert(2, None)
+            for k in range(3 + (top > 0)):
+                if got[k] is not None:
+                    ref.close(got[k][some], want[k], tol[k], f"{what} {k}")
+            if top:
+                assert torch.equal(got[4][some].cpu(), want[4]), what
+
+
+def test_rows_do_not_depend_on_their_batch(rocm_device, ho):
+    """A row has the same bits in other batches of the same plan wherever it
+    begins at the same place of 16 bytes.  (Its values are added by the 16-byte
+    vectors that they lie in: elsewhere in another order, within the bound.)"""
+    for rows, vocab, part in ((300, 9001, slice(7, 270)), (1500, 700, slice(100, 1300)),
+                              (60, 50001, slice(3, 61)), (100, 9000, slice(11, 12))):
+        for dtype in DTYPES:
+            x, t = make_logits(rows, vocab, dtype, "plain", rows)
+            xd, td = x.to(rocm_device), t.to(rocm_device)
+            begins = (torch.arange(rows) * vocab * dtype.itemsize) % 16
+            whole = ho.token_logprobs(xd, td, entropy=True, top=8)
+            order = torch.randperm(rows, generator=torch.Generator().manual_seed(1))
+            want, tol = ref.token_logprobs(x, t, top=8)
+            for some in (torch.arange(rows)[part], order):
+                what = f"[{rows}, {vocab}] {dtype}"
+                got = ho.token_logprobs(xd[some], td[some], entropy=True, top=8)
+                same = begins[some] == begins[:len(some)]
+                assert bool(same.any()) or some is not order, what
+                for k, (u, v) in enumerate(zip(whole, got)):
+                    assert torch.equal(u[some][same], v[same]), f"{what}: bits"
+                    if k < 4:
+                        ref.close(v, want[k][some], tol[k][some], what)
+                assert torch.equal(got[4].cpu(), want[4][some]), what
+            # The same rows where they are.
+            for u, v in zip(whole, ho.token_logprobs(xd[part], td[part], entropy=True, top=8)):
+                assert torch.equal(u[part], v), what
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab", [(49153, 9), (100000, 17), (98305, 700)])
+def test_backward_of_more_rows_than_a_grid_layer(rows, vocab, dtype, rocm_device, ho):
+    x, t = make_logits(rows, vocab, dtype, "plain", vocab)
+    t[::7], t[5::11] = IGNORE, -1
+    x[::14] = NAN  # ignored
+    g = torch.Generator().manual_seed(rows)
+    grads = [torch.randn(rows, generator=g) for _ in range(3)]
+    (_, lse, ent, _, _), _ = ref.token_logprobs(x, t)
+    lse, ent = lse.float(), ent.float()
+    kw = dict(entropy=ent, grad_entropy=grads[1], grad_lse=grads[2])
+    want, tol = ref.token_logprobs_bwd(grads[0], x, t, lse, **kw)
+    dev = {k: v.to(rocm_device) for k, v in kw.items()}
+    got = ho.token_logprobs_bwd(*(v.to(rocm_device) for v in (grads[0], x, t, lse)), **dev)
+    ref.close(got, want, tol, f"[{rows}, {vocab}] {dtype}")
+
+
+def test_more_rows_than_a_launch(rocm_device, ho):
+    """2^23 workgroups in a launch of the forward, 2^30 lanes in one of the
+    lookup and of the embedding gradient: the rest in launches of their own."""
+    g = torch.Generator(device=rocm_device).manual_seed(1)
+    rows, vocab = (1 << 23) + 1001, 5
+    x = torch.randn(rows, vocab, generator=g, device=rocm_device)
+    t = torch.randint(0, vocab, (rows,), generator=g, device=rocm_device)
+    lp, lse, best, which = ho.token_logprobs(x, t, top=1)
+    ls = torch.log_softmax(x.double(), -1)
+    # |x| < 8: a few halves of a step of numbers below 16.
+    tol = 16 * 16 * ref.U
+    assert float((lp - ls.gather(1, t[:, None])[:, 0]).abs().max()) < tol
+    assert float((lse - torch.logsumexp(x.double(), -1)).abs().max()) < tol
+    assert torch.equal(which[:, 0], x.argmax(-1))
+    assert float((best - ls.amax(-1, keepdim=True)).abs().max()) < tol
+    del x, t, lp, lse, best, which, ls
+    print("launches: forward", flush=True)
+    count = (1 << 30) + 1001
+    w = torch.randn(7, 1, generator=g, device=rocm_device)
+    t = torch.arange(count, dtype=torch.int32, device=rocm_device) % 7
+    e = ho.embedding(w, t)
+    for part in range(0, count, 1 << 28):
+        some = slice(part, part + (1 << 28))
+        assert torch.equal(e[some], w[t[some].long()])
+    del t, e
+    print("launches: embedding", flush=True)
+    count, width, vocab = 40000, 1 << 18, 3
+    t = torch.randint(0, vocab, (count,), generator=g, device=rocm_device)
+    t[-1000:] = vocab  # adds nothing
+    grad = torch.empty(count, width, dtype=BF16, device=rocm_device).normal_(generator=g)
+    dw = ho.embedding_bwd(grad, t, vocab, dtype=F32)
+    for cols in (slice(0, 9), slice(width // 2 - 4, width // 2 + 4), slice(width - 9, width)):
+        want, tol, _ = ref.embedding_bwd(grad[:, cols], t, vocab)
+        ref.close(dw[:, cols], want, tol, f"columns {cols}")

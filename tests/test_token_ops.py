@@ -179,3 +179,12 @@ def test_vectors_beside_rows_of_a_buffer(dtype):
             t = buf[at:at + n * step].view(dtype)
             want = not bool(held[at:at + n * step].any())
             assert hip_oracles._apart_from_rows(t, a, stride, rows, cols) == want, (at, n)
+
+
+def test_workspaces_are_needed_where_rows_or_tokens_are_split():
+    """What the sizes' checks above stand on."""
+    lib = hip_oracles.load_library()
+    for rows, vocab, top in ((1, 1 << 20, 8), (1, 1 << 20, 0), (64, 128000, 20)):
+        assert lib.hipo_token_logprobs_workspace_bytes(rows, vocab, top) > 0
+    assert lib.hipo_token_logprobs_workspace_bytes(2048, 8200, 3) == 0
+    assert lib.hipo_embedding_bwd_workspace_bytes(4096, 768, 32000) >= 4096 * 16
