@@ -644,8 +644,13 @@ __global__ __launch_bounds__(kThreads) void join_slices(FwdArgs a) {
 //   values, for the search that one wave does alone ([512, 8192] 6.2 / 13.6 at
 //   64, 5.5 / 8.6 at 256).  What is asked for does not enter: the statistics
 //   are the same bits with and without alternatives;
-//   1024 threads for rows of 64 KB and more, up to one per CU ([256, 50001]
-//   10.0 / 13.2, 256 threads 9.8 / 14.7; [512, 32000] 9.7 / 19.1, 9.5 / 13.6);
+//   1024 threads for up to a row per CU where 256 take four rounds of loads or
+//   more (256 / 1024 threads, with 20 alternatives: rows of 2900 vectors, three
+//   rounds, [1] 7.7 / 8.3, [64] 8.4 / 9.2, [256] 9.8 / 10.4; of 3400, four, [1] 8.3 /
+//   8.1, [64] 9.3 / 9.1, [256] 10.5 / 10.4, fp32 9.8 / 9.3; of 8192, [256] 15.1 /
+//   12.4; without alternatives 3400 [1] 5.3 / 5.1, [256] 6.7 / 7.1, fp32 6.2 / 6.0.
+//   Just past a round of 1024 they lose: 4600 [256] 7.3 / 9.3, 11.7 / 12.5, fp32 7.1 /
+//   7.5, 10.9 / 10.8).  [512, 32000] 9.7 / 19.1 at 1024, 9.5 / 13.6 at 256;
 //   slices of 16 KB and more of still longer rows where that fills the chip
 //   no more than twice: [64, 128000] one slice of 1024 threads 11.9 / 15.8, 4
 //   slices 8.9 / 13.7, 8 slices 8.5 / 12.9, 16 slices 8.6 / 14.5; [1, 200000]
@@ -669,7 +674,8 @@ inline Plan plan(int64_t rows, int64_t vocab, int elem_size) {
     p.threads = kThreads;
     slices = std::min({std::max<int64_t>(4, 512 / rows), vectors / 1024, kMaxSlices});
   } else {
-    p.threads = rows <= 256 && vectors >= 4000 ? kLarge : kThreads;
+    const int64_t round = kThreads * 4;
+    p.threads = rows <= 256 && (vectors + round - 1) / round >= 4 ? kLarge : kThreads;
   }
   p.flight = rows >= 2048 && elem_size == 2 ? 8 : 4;
   p.span = static_cast<int>(

@@ -773,3 +773,14 @@ def test_more_rows_than_a_launch(rocm_device, ho):
     for cols in (slice(0, 9), slice(width // 2 - 4, width // 2 + 4), slice(width - 9, width)):
         want, tol, _ = ref.embedding_bwd(grad[:, cols], t, vocab)
         ref.close(dw[:, cols], want, tol, f"columns {cols}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 130, 256])
+def test_forward_where_the_threads_of_a_row_change(rows, dtype, rocm_device, ho):
+    """Three and four rounds of 256 threads' loads, and a value less and more."""
+    values = 256 * 4 * 16 // dtype.itemsize
+    for vocab in (2 * values + 1, 3 * values - 1, 3 * values + 16 // dtype.itemsize,
+                  4 * values - 1, 4 * values + 1):
+        x, t = make_logits(rows, vocab, dtype, "plain", vocab)
+        check_forward(ho, rocm_device, x, t, top=20, shift=1, what=f"[{rows}, {vocab}] {dtype}")

@@ -81,3 +81,16 @@ def test_the_widest_embedding_gradients(launches):
         for width in (most + 1, (1 << 31) - 1):
             made, rc = launches("embedding_bwd", 33, width, 3, elem, 4, 1)
             assert rc == 1000 and not made
+
+
+def test_a_rows_threads_change_at_whole_rounds_of_loads(launches):
+    """Rows few enough for 1024 threads get them where 256 threads with four
+    16-byte loads each take more than three rounds."""
+    for elem in (2, 4):
+        per_round = 256 * 4 * 16 // elem
+        for rows in (1, 100, 256):
+            for rounds in (2, 3, 4, 5):
+                threads = 256 if rounds < 4 else 1024
+                for vocab in ((rounds - 1) * per_round + 16 // elem, rounds * per_round):
+                    made, rc = launches("token_logprobs", rows, vocab, elem, 0)
+                    assert rc == 0 and [m[1:] for m in made] == [((rows, 1, 1), (threads, 1, 1))]
