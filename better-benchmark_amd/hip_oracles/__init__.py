@@ -749,11 +749,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, scale: float =
     entropy=True, then with top=k (at most 64) the k most probable tokens'
     log probabilities [R, k] and ids [R, k] (int64; of equal logits the lower
     id first, NaN above all).  A row whose token is ignore_index is left out,
-    whatever its logits hold: its results are 0, its alternatives -inf and -1.  Any other token outside
-    [0, V) has log probability NaN.  A row with nothing above -inf has lse
-    -inf, with +inf lse +inf, with NaN lse NaN; there logprob = scale * logit -
-    lse, and the entropy is NaN.  Elsewhere no log probability is above 0, no
-    entropy below."""
+    whatever its logits hold: its results are 0, its alternatives -inf and -1.
+    Any other token outside [0, V) has log probability NaN.  A row with nothing
+    above -inf has lse -inf, with +inf lse +inf, with NaN lse NaN; there
+    logprob = scale * logit - lse, and the entropy is NaN.  Elsewhere no log
+    probability is above 0, no entropy below.  A row's results do not depend on
+    the other rows' values."""
     lib = _lib or load_library()
     dev = _require_rocm(logits, tokens)
     rows, vocab, stride = _require_logits("token_logprobs", logits, tokens, scale)
@@ -790,9 +791,11 @@ def token_logprobs_bwd(grad: torch.Tensor, logits: torch.Tensor, tokens: torch.T
     type: grad, grad_entropy and grad_lse (fp32 [R]) are the gradients of its
     logprob, entropy and lse; lse, and entropy where grad_entropy is given,
     are its results.  Rows of ignore_index are zero, rows of another token
-    outside [0, V) NaN.  out: where the result goes, the logits themselves or
-    memory that does not overlap them (any row stride >= V); it does not
-    overlap the other inputs."""
+    outside [0, V), with NaN or with nothing above -inf NaN.  Probabilities are
+    e^(scale * logit - lse) of the fp32 lse: where |lse| is 2^24 and more (a row
+    of nothing but a mask of -1e9) they are none; leave such rows out.  out:
+    where the result goes, the logits themselves or memory that does not overlap
+    them (any row stride >= V); it does not overlap the other inputs."""
     lib = _lib or load_library()
     rows_of = [t for t in (grad, lse, entropy, grad_entropy, grad_lse) if t is not None]
     dev = _require_rocm(logits, tokens, *rows_of, *(() if out is None else (out,)))

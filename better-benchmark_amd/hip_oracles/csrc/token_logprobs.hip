@@ -8,16 +8,23 @@
 //   p_j = e^(s_j - lse),  p_j ln p_j = 0 where p_j = 0.
 //
 // Forward: HBM-bound, the row is read once.  Each lane keeps a running
-// maximum and the two sums relative to it (rescaled when it rises, once per
-// 32 values); lanes, waves and slices of a row are then joined by the same
-// rescaling.  A workgroup takes a row, or a slice of one where there are too
+// maximum and the two sums relative to it (rescaled when it rises, at most once
+// per round of 8 to 64 values); lanes, waves and slices of a row are then joined
+// by the same rescaling, so that a row's bits depend on its values, on where in 16
+// bytes it begins and on the plan, on no other row.  A workgroup takes a row, or a slice of one where there are too
 // few rows to fill the chip, whose parts a second launch joins.
 //
-// The alternatives cost nothing while the row streams by: the lanes' maxima
+// For the alternatives nothing is kept while the row streams by: the lanes' maxima
 // say where the largest values are.  The k-th largest of 64 groups' maxima is
 // a lower bound of the k-th largest value, few values reach it (k = 20: about
 // 24), and they lie in lanes whose maximum does: only these lanes' values are
-// read again, shared out over the workgroup, and ranked by counting.
+// read again, shared out over the workgroup, and ranked by counting.  With 0 / 20 /
+// 33 / 64 alternatives, us, bf16: [1, 32000] 5.6 / 8.7 / 9.0 / 12.8, [64, 128000] 9.2 /
+// 13.6 / 15.3 / 57, [4096, 16384] 25 / 38 / 45 / 140.  Rows of one value cost a
+// second search for its first places (20 alternatives: 28, 42, 165).  Where more
+// than 1024 values lie above all but a few lanes' they are found one by one, a pass
+// over the row or slice each (every second run of 32 vectors far above the others:
+// 33 alternatives 160, 269, 1256; 64 alternatives 286, 491, 2295).
 //
 // Backward: HBM-bound, one pass, a value's gradient needs its logit and a few
 // numbers of its row.
@@ -707,7 +714,9 @@ struct BwdArgs {
 // bf16 635 / 667 / 728, [1501, 50001] fp32 101 / 95 / 102.
 template <typename T>
 constexpr int kBwdVectors = 8 / Logits<T>::C;
-constexpr int kBwdRows = 49152;     // rows per grid layer
+// Rows per grid layer.  The last layer's workgroups past the rows end at once: just
+// past 49152 rows nearly half of all.
+constexpr int kBwdRows = 49152;
 constexpr int kBwdLineFrom = 1024;  // vectors of a row from which on lines count
 
 // The gradient of a logit, without the token's own term.  e^-104 is 0: the

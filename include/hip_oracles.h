@@ -451,13 +451,15 @@ int hipo_gelu_erf_bwd_colsum_bf16(const uint16_t* grad, const uint16_t* x, uint1
  * outputs are contiguous.  entropy may be NULL; top is at most 64 and at
  * most vocab, its outputs NULL where it is 0; scale is from 2^-100 to 2^100.
  * A row whose token is ignore_index is left out, whatever its logits hold:
- * 0, 0, 0, and for the alternatives -inf and -1.  A token outside [0, vocab) otherwise has
- * logprob NaN.  A row with nothing above -inf has lse -inf, one with +inf
+ * 0, 0, 0, and for the alternatives -inf and -1.  A token outside [0, vocab)
+ * otherwise has logprob NaN.  A row with nothing above -inf has lse -inf, one with +inf
  * lse +inf, one with NaN lse NaN; their logprobs are s - lse, their entropy
  * NaN.  Of the others no logprob is above 0 and no entropy below, and both are
  * 0 where one value above -inf is all there is.  `workspace`: at least hipo_token_logprobs_workspace_bytes bytes,
  * 16-byte aligned, no initialisation needed (NULL when that is 0); calls
- * that share one must be ordered.
+ * that share one must be ordered.  Alternatives cost up to twice the pass for
+ * top <= 33, more beyond; rows whose largest values crowd into a few runs of
+ * 16-byte vectors can take a pass per alternative.
  * No counterpart among the reference's oracles; beside
  * hipo_scaled_masked_softmax_bf16 as the softmax of a whole vocabulary.
  */
@@ -479,7 +481,11 @@ int hipo_token_logprobs(const void* logits, int elem_size, const void* tokens,
  * grad_entropy), are the forward's results.  logits and dlogits are [rows,
  * vocab] with row strides of their own; dlogits may be logits itself (one
  * stride), and does not overlap it otherwise, nor the other inputs.  Rows of
- * ignore_index are zero, whatever they hold; rows of another token outside [0, vocab) are NaN.
+ * ignore_index are zero, whatever they hold; rows of another token outside
+ * [0, vocab) are NaN, and so are rows with NaN or with nothing above -inf, and
+ * a +inf's own place.  p_j is e^(s_j - lse) of the fp32 lse: off by a factor of
+ * about 1 + |lse| 2^-24, and no probability where |lse| is 2^24 and more (a row
+ * of nothing but a mask of -1e9): leave such rows out.
  * No counterpart among the reference's oracles; beside
  * hipo_gelu_erf_bwd_colsum_bf16 as a training gradient.
  */
@@ -517,7 +523,9 @@ int hipo_embedding(const void* weight, int elem_size, const void* tokens,
  * outside [0, vocab): no padding).  grad is contiguous [count, width] of bf16
  * (elem_size 2) or fp32 (4), dweight contiguous [vocab, width] of bf16
  * (out_size 2) or fp32 (4), the two apart; count and width are at most
- * 2^31 - 4097, vocab 2^30.  `workspace`: at least
+ * 2^31 - 4097, vocab 2^30.  The time grows with vocab also where accumulate
+ * leaves rows alone: every 512 rows past 65536 scan the tokens once more (2048
+ * tokens: 12 us into 65536 rows, 262 into 10^7).  `workspace`: at least
  * hipo_embedding_bwd_workspace_bytes bytes, 16-byte aligned, no
  * initialisation needed (NULL when that is 0); calls that share one must be
  * ordered.

@@ -784,3 +784,18 @@ def test_forward_where_the_threads_of_a_row_change(rows, dtype, rocm_device, ho)
                   4 * values - 1, 4 * values + 1):
         x, t = make_logits(rows, vocab, dtype, "plain", vocab)
         check_forward(ho, rocm_device, x, t, top=20, shift=1, what=f"[{rows}, {vocab}] {dtype}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_backward_of_rows_with_infinities(dtype, rocm_device, ho):
+    """As its description says: NaN rows with NaN or with nothing left, and the
+    place of a +inf."""
+    x, t = make_logits(9, 2100, dtype, "special", 3)
+    t[:] = 7
+    xd, td = x.to(rocm_device), t.to(rocm_device)
+    g = torch.ones(9, device=rocm_device)
+    _, lse = ho.token_logprobs(xd, td)
+    got = ho.token_logprobs_bwd(g, xd, td, lse).cpu()
+    assert got[0].isnan().all() and got[4].isnan().all()
+    assert got[3].isnan().nonzero()[:, 0].tolist() == [2099] and got[3, 7] == 1
+    assert torch.isfinite(got[[1, 2, 5, 6, 7, 8]]).all()
