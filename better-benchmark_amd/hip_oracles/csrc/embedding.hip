@@ -63,8 +63,8 @@ constexpr int kFewTokens = 1024;     // summed without a sort
 constexpr int kFewThreads = 512;
 constexpr int kFewFill = 2;          // zeros: 16-byte pieces per thread
 constexpr int64_t kLanes = int64_t{1} << 30;  // lanes per launch
-// A launch has fewer than 2^32 threads: with the 2^21 sorting workgroups of 2^30 rows
-// one of 1024 less than 2^22, and a multiple of the XCDs.
+// A launch has fewer than 2^32 threads, fewer than 2^22 workgroups of 1024: 2^21 sort
+// where there are 2^30 rows; of the others as many as are left and 8 XCDs can share.
 constexpr int64_t kFillBlocks = (int64_t{1} << 21) - 8;
 
 __device__ __forceinline__ int64_t token_at(const void* tokens, int size, int64_t i) {

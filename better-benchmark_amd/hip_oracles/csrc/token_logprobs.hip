@@ -11,8 +11,9 @@
 // maximum and the two sums relative to it (rescaled when it rises, at most once
 // per round of 8 to 64 values); lanes, waves and slices of a row are then joined
 // by the same rescaling, so that a row's bits depend on its values, on where in 16
-// bytes it begins and on the plan, on no other row.  A workgroup takes a row, or a slice of one where there are too
-// few rows to fill the chip, whose parts a second launch joins.
+// bytes it begins and on the plan, on no other row.  A workgroup takes a row, or a
+// slice of one where there are too few rows to fill the chip, whose parts a second
+// launch joins.
 //
 // For the alternatives nothing is kept while the row streams by: the lanes' maxima
 // say where the largest values are.  The k-th largest of 64 groups' maxima is

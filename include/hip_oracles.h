@@ -452,14 +452,16 @@ int hipo_gelu_erf_bwd_colsum_bf16(const uint16_t* grad, const uint16_t* x, uint1
  * most vocab, its outputs NULL where it is 0; scale is from 2^-100 to 2^100.
  * A row whose token is ignore_index is left out, whatever its logits hold:
  * 0, 0, 0, and for the alternatives -inf and -1.  A token outside [0, vocab)
- * otherwise has logprob NaN.  A row with nothing above -inf has lse -inf, one with +inf
- * lse +inf, one with NaN lse NaN; their logprobs are s - lse, their entropy
- * NaN.  Of the others no logprob is above 0 and no entropy below, and both are
- * 0 where one value above -inf is all there is.  `workspace`: at least hipo_token_logprobs_workspace_bytes bytes,
- * 16-byte aligned, no initialisation needed (NULL when that is 0); calls
- * that share one must be ordered.  Alternatives cost up to twice the pass for
- * top <= 33, more beyond; rows whose largest values crowd into a few runs of
- * 16-byte vectors can take a pass per alternative.
+ * otherwise has logprob NaN.  A row with nothing above -inf has lse -inf, one
+ * with +inf lse +inf, one with NaN lse NaN; their logprobs are s - lse, their
+ * entropy NaN.  In the others no logprob is above 0 and no entropy below; where
+ * one value is above -inf, its logprob and the entropy are 0.  `workspace`: at
+ * least hipo_token_logprobs_workspace_bytes bytes, 16-byte aligned, no
+ * initialisation needed (NULL when that is 0); calls that share one must be
+ * ordered.  A call with top <= 33 takes about twice the time of one without,
+ * with more alternatives or many equal values several times as long; where the
+ * largest values crowd into a few runs of 16-byte vectors, up to a pass over
+ * the row for each alternative.
  * No counterpart among the reference's oracles; beside
  * hipo_scaled_masked_softmax_bf16 as the softmax of a whole vocabulary.
  */

@@ -799,3 +799,27 @@ def test_backward_of_rows_with_infinities(dtype, rocm_device, ho):
     assert got[0].isnan().all() and got[4].isnan().all()
     assert got[3].isnan().nonzero()[:, 0].tolist() == [2099] and got[3, 7] == 1
     assert torch.isfinite(got[[1, 2, 5, 6, 7, 8]]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("power", [-100, -40, 100])
+@pytest.mark.parametrize("rows,vocab", [(40, 700), (300, 9001), (6, 100003)])
+def test_scales_that_are_powers_of_two(rows, vocab, power, dtype, rocm_device, ho):
+    """Logits and a scale that cancel are the logits with scale 1, bit by bit;
+    the gradient is that times the scale, but for what is below 2^-126."""
+    x, t = make_logits(rows, vocab, dtype, "masked", 6)
+    t[0] = vocab // 2
+    xd, td = x.to(rocm_device), t.to(rocm_device)
+    far = xd * 2.0 ** -power
+    assert torch.equal(far.float() * 2.0 ** power, xd.float())
+    one = ho.token_logprobs(xd, td, entropy=True, top=5)
+    got = ho.token_logprobs(far, td, scale=2.0 ** power, entropy=True, top=5)
+    for u, v in zip(one, got):
+        assert torch.equal(u, v)
+    g = torch.randn(3, rows, generator=torch.Generator().manual_seed(1)).to(rocm_device)
+    kw = dict(entropy=one[2], grad_entropy=g[1], grad_lse=g[2])
+    want = ho.token_logprobs_bwd(g[0], xd, td, one[1], **kw).double() * 2.0 ** power
+    dx = ho.token_logprobs_bwd(g[0], far, td, one[1], scale=2.0 ** power, **kw).double()
+    normal = want.abs() >= 2.0 ** -125
+    assert torch.equal(dx[normal], want[normal])
+    assert float((dx - want)[~normal].abs().max()) <= 2.0 ** -126
