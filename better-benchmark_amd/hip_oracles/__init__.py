@@ -100,6 +100,27 @@ _SIGNATURES = {
         ctypes.c_int,
         [_c_ptr, ctypes.c_int, _c_ptr, ctypes.c_int, _c_ptr, ctypes.c_int] + [_c_i64] * 3
         + [_c_f32, _c_i64, ctypes.c_int, _c_ptr, ctypes.c_size_t, _c_ptr]),
+    "hipo_block_norms": (
+        ctypes.c_int,
+        [_c_ptr, _c_ptr, ctypes.c_int] + [_c_ptr] * 8 + [_c_i64] * 3 + [_c_f32] * 3
+        + [ctypes.c_int, _c_ptr]),
+    "hipo_block_norms_bwd_workspace_bytes": (ctypes.c_size_t, [_c_i64] * 2),
+    "hipo_block_norms_bwd": (
+        ctypes.c_int,
+        [_c_ptr] * 5 + [ctypes.c_int] + [_c_ptr] * 12 + [_c_i64] * 3 + [_c_f32] * 2
+        + [ctypes.c_int, _c_ptr, ctypes.c_size_t, _c_ptr]),
+    "hipo_linear_cross_entropy_workspace_bytes": (
+        ctypes.c_size_t, [_c_ptr, ctypes.c_int] + [_c_i64] * 4),
+    "hipo_linear_cross_entropy": (
+        ctypes.c_int,
+        [_c_ptr, _c_ptr, ctypes.c_int, _c_ptr, ctypes.c_int, _c_ptr, _c_ptr] + [_c_i64] * 5
+        + [_c_f32, _c_i64, _c_ptr, ctypes.c_size_t, _c_ptr]),
+    "hipo_linear_cross_entropy_bwd_workspace_bytes": (
+        ctypes.c_size_t, [_c_ptr, ctypes.c_int] + [_c_i64] * 4),
+    "hipo_linear_cross_entropy_bwd": (
+        ctypes.c_int,
+        [_c_ptr, _c_ptr, _c_ptr, ctypes.c_int, _c_ptr, ctypes.c_int] + [_c_ptr] * 4
+        + [_c_i64] * 5 + [_c_f32, _c_i64, _c_ptr, ctypes.c_size_t, _c_ptr]),
 }
 
 _lib = None
@@ -894,6 +915,182 @@ def embedding_bwd(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, scale
     return out
 
 
+def _require_block_norms(what, x, rows_of, post, post_bias, pre, pre_bias, gate, norm):
+    """(device, rows, cols, gate rows, layer) of block_norms and its gradient."""
+    vectors = [t for t in (post, post_bias, pre, pre_bias) if t is not None]
+    dev = _require_rocm(x, *rows_of, *vectors, *(() if gate is None else (gate,)))
+    _require(x.dtype in _FLOATS and x.dim() == 2, f"{what}: 2-D bf16 or fp32 rows required")
+    rows, cols = x.shape
+    for t in (x, *rows_of):
+        if not (t.dtype == x.dtype and t.shape == x.shape and t.is_contiguous()):
+            raise ValueError(f"{what}: the rows must be contiguous [R, C] of one type")
+    for t in vectors:
+        if not (t.dtype == x.dtype and t.shape == (cols,) and t.is_contiguous()):
+            raise ValueError(f"{what}: weights and biases must be contiguous [C] of the rows' type")
+    _require(norm in ("rms", "layer"), f"{what}: norm must be 'rms' or 'layer'")
+    gates = 0
+    if gate is not None:
+        _require(gate.dtype == x.dtype and gate.dim() in (1, 2) and gate.shape[-1] == cols
+                 and gate.is_contiguous(),
+                 f"{what}: gate must be contiguous [C] or [G, C] of the rows' type")
+        gates = gate.shape[0] if gate.dim() == 2 else 1
+        _require(gates > 0 and rows % gates == 0, f"{what}: gate's rows must divide the rows")
+    return dev, rows, cols, gates, 1 if norm == "layer" else 0
+
+
+def _optional(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def block_norms(x: torch.Tensor, residual: torch.Tensor, *, post: torch.Tensor | None = None,
+                post_bias: torch.Tensor | None = None, pre: torch.Tensor | None = None,
+                pre_bias: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                norm: str = "rms", scale: float = 1.0, offset: float = 0.0, eps: float = 1e-6):
+    """The norms around a residual block, fused with its gate and the sum: x
+    [R, C] is the block's output, residual the stream, both contiguous bf16 or
+    fp32 (8 <= C <= 16384).  With norm(v; w, b) RMSNorm ("rms", without biases)
+    or LayerNorm ("layer") over the last dim, times offset + w, plus b:
+
+        n = norm(x; post, post_bias), or x where post is None
+        h = residual + scale * gate * n          (rounded to the rows' type)
+        y = norm(h; pre, pre_bias), or None where pre is None
+
+    Returns (h, y, stats): h the new stream, y the next block's input, stats fp32
+    [R, 4] for block_norms_bwd (mean and 1 / deviation of x and of h, 0 and 1
+    where there is no norm).  One of post and pre at least; weights, biases and
+    gate are of the rows' type.  gate: [C], or [G, C] where G divides R, for
+    R / G consecutive rows each (a sample's, or G = R)."""
+    lib = _lib or load_library()
+    what = "block_norms"
+    dev, rows, cols, gates, layer = _require_block_norms(
+        what, x, (residual,), post, post_bias, pre, pre_bias, gate, norm)
+    h = torch.empty_like(x)
+    y = None if pre is None else torch.empty_like(x)
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
+    _call(lib.hipo_block_norms, what, dev, _ptr(x), _ptr(residual), x.element_size(),
+          _optional(post), _optional(post_bias), _optional(pre), _optional(pre_bias),
+          _optional(gate), _ptr(h), _optional(y), _ptr(stats), rows, cols, gates, float(scale),
+          float(offset), float(eps), layer)
+    return h, y, stats
+
+
+def block_norms_bwd(grad_h: torch.Tensor | None, grad_y: torch.Tensor | None,
+                    x: torch.Tensor, h: torch.Tensor | None, stats: torch.Tensor, *,
+                    post: torch.Tensor | None = None, post_bias: torch.Tensor | None = None,
+                    pre: torch.Tensor | None = None, pre_bias: torch.Tensor | None = None,
+                    gate: torch.Tensor | None = None, norm: str = "rms", scale: float = 1.0,
+                    offset: float = 0.0):
+    """Gradients of block_norms for grad_h and grad_y, those of h and y (grad_h
+    may be None where pre is not: nothing else uses the stream; grad_y is None
+    where pre is): (dx, dresidual, dgate, dpost, dpost_bias, dpre, dpre_bias),
+    None where the operand is.  x, the weights and the options are the forward's
+    operands, h and stats its results (h may be None without pre).  Sums over
+    rows are fp32, in an order that the sizes and the GPU fix, and rounded once."""
+    lib = _lib or load_library()
+    what = "block_norms_bwd"
+    _require((pre is None) == (grad_y is None) and (pre is None or h is not None),
+             "block_norms_bwd: pre, h and grad_y go together")
+    _require(pre is not None or grad_h is not None, "block_norms_bwd: no gradient given")
+    rows_of = [t for t in (grad_h, grad_y, h) if t is not None]
+    dev, rows, cols, gates, layer = _require_block_norms(
+        what, x, rows_of, post, post_bias, pre, pre_bias, gate, norm)
+    _require_rocm(x, stats)
+    _require(stats.dtype == torch.float32 and stats.shape == (rows, 4) and stats.is_contiguous(),
+             "block_norms_bwd: stats must be contiguous fp32 [R, 4]")
+    dx, dresidual = torch.empty_like(x), torch.empty_like(x)
+    made = torch.empty_like if rows else torch.zeros_like  # no rows: nothing is written
+    sums = [None if t is None else made(t) for t in (gate, post, post_bias, pre, pre_bias)]
+    need = int(lib.hipo_block_norms_bwd_workspace_bytes(rows, cols))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _call(lib.hipo_block_norms_bwd, what, dev, _optional(grad_h), _optional(grad_y), _ptr(x),
+          _optional(h), _ptr(stats), x.element_size(), _optional(post), _optional(post_bias),
+          _optional(pre), _optional(pre_bias), _optional(gate), _ptr(dx), _ptr(dresidual),
+          *(_optional(t) for t in sums), rows, cols, gates, float(scale), float(offset), layer,
+          _optional(ws), need)
+    return (dx, dresidual, *sums)
+
+
+def _require_output_layer(what, hidden, weight, tokens, scale):
+    """(rows, width, vocab, row stride of hidden, of weight)."""
+    _require(hidden.dtype in _FLOATS and hidden.dim() == 2,
+             f"{what}: hidden must be 2-D bf16 or fp32")
+    _require(weight.dtype == hidden.dtype and weight.dim() == 2
+             and weight.shape[1] == hidden.shape[1],
+             f"{what}: weight must be [V, D] of hidden's type")
+    _require_tokens(what, tokens)
+    rows, width = hidden.shape
+    vocab = weight.shape[0]
+    _require(tokens.shape == (rows,), f"{what}: tokens must be [R]")
+    _require(vocab > 0 and width > 0, f"{what}: empty vocabulary or width")
+    _require(2.0 ** -100 <= scale <= 2.0 ** 100, f"{what}: scale must be from 2^-100 to 2^100")
+    strides = []
+    for t, n in ((hidden, rows), (weight, vocab)):
+        _require(t.stride(1) == 1 or width == 1, f"{what}: unit inner strides required")
+        stride = t.stride(0) if n > 1 else width
+        _require(stride >= width, f"{what}: rows overlap")
+        strides.append(stride)
+    return rows, width, vocab, *strides
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor, *,
+                         scale: float = 1.0, ignore_index: int = -100):
+    """Softmax cross entropy of tokens [R] (int32 or int64) under the logits
+    scale * hidden @ weight.T, which are never in memory: hidden [R, D] and weight
+    [V, D] of bf16 or fp32 with any row strides >= D.  Returns (loss [R], lse
+    [R]) in fp32: lse = ln sum_j e^logit_j, loss = lse - logit_token.
+
+    A row whose token is ignore_index is left out, whatever it holds: 0 and 0.
+    Any other token outside [0, V) has loss NaN; a row with a NaN logit has both
+    NaN.  token_logprobs gives the negative loss of logits that are in memory."""
+    lib = _lib or load_library()
+    what = "linear_cross_entropy"
+    dev = _require_rocm(hidden, weight, tokens)
+    rows, width, vocab, hstride, wstride = _require_output_layer(what, hidden, weight, tokens,
+                                                                 scale)
+    loss = torch.empty(rows, dtype=torch.float32, device=dev)
+    lse = torch.empty_like(loss)
+    need = int(lib.hipo_linear_cross_entropy_workspace_bytes(
+        _ptr(weight), weight.element_size(), rows, width, vocab, wstride))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _call(lib.hipo_linear_cross_entropy, what, dev, _ptr(hidden), _ptr(weight),
+          hidden.element_size(), _ptr(tokens), tokens.element_size(), _ptr(loss), _ptr(lse), rows,
+          width, vocab, hstride, wstride, float(scale), int(ignore_index), _optional(ws), need)
+    return loss, lse
+
+
+def linear_cross_entropy_bwd(grad: torch.Tensor, hidden: torch.Tensor, weight: torch.Tensor,
+                             tokens: torch.Tensor, lse: torch.Tensor, *, scale: float = 1.0,
+                             ignore_index: int = -100, grad_lse: torch.Tensor | None = None):
+    """Gradients (dhidden [R, D], dweight [V, D]) of linear_cross_entropy, of the
+    operands' type: grad and grad_lse (fp32 [R]) are the gradients of its loss and
+    lse (1 / R each of the mean loss, 2 c lse / R of a penalty c lse^2), lse is
+    its result.  The logits are computed once more, in pieces of the vocabulary;
+    with bf16 operands their gradients are rounded to bf16 for the products with
+    hidden and weight, whose sums are fp32.  Rows of ignore_index have gradient
+    zero and add nothing to dweight, whatever they hold; a row of another token
+    outside [0, V) is NaN and makes dweight NaN."""
+    lib = _lib or load_library()
+    what = "linear_cross_entropy_bwd"
+    rows_of = [t for t in (grad, lse, grad_lse) if t is not None]
+    dev = _require_rocm(hidden, weight, tokens, *rows_of)
+    rows, width, vocab, hstride, wstride = _require_output_layer(what, hidden, weight, tokens,
+                                                                 scale)
+    for t in rows_of:
+        if not (t.dtype == torch.float32 and t.shape == (rows,) and t.is_contiguous()):
+            raise ValueError(f"{what}: grad, lse and grad_lse must be contiguous fp32 [R]")
+    made = torch.empty if rows else torch.zeros  # no rows: nothing is written
+    dhidden = made((rows, width), dtype=hidden.dtype, device=dev)
+    dweight = made((vocab, width), dtype=hidden.dtype, device=dev)
+    need = int(lib.hipo_linear_cross_entropy_bwd_workspace_bytes(
+        _ptr(weight), weight.element_size(), rows, width, vocab, wstride))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _call(lib.hipo_linear_cross_entropy_bwd, what, dev, _ptr(grad), _ptr(hidden), _ptr(weight),
+          hidden.element_size(), _ptr(tokens), tokens.element_size(), _ptr(lse),
+          _optional(grad_lse), _ptr(dhidden), _ptr(dweight), rows, width, vocab, hstride, wstride,
+          float(scale), int(ignore_index), _optional(ws), need)
+    return dhidden, dweight
+
+
 def _error_word(ws: torch.Tensor) -> torch.Tensor:
     raw = ws.view(torch.uint8) if ws.dtype != torch.uint8 else ws
     return raw[BN_ERROR_WORD_OFFSET:BN_ERROR_WORD_OFFSET + 4].view(torch.int32)
@@ -971,4 +1168,5 @@ __all__ = [
     "hold_copy",
     "gelu_erf_bwd_colsum",
     "token_logprobs", "token_logprobs_bwd", "embedding", "embedding_bwd",
+    "block_norms", "block_norms_bwd", "linear_cross_entropy", "linear_cross_entropy_bwd",
 ]

@@ -42,6 +42,8 @@ SOURCES = [
     "gelu_bwd.hip",
     "token_logprobs.hip",
     "embedding.hip",
+    "block_norms.hip",
+    "linear_cross_entropy.hip",
 ]
 
 # Packed-FP32 VALU forms are disabled for all device code (the compiler

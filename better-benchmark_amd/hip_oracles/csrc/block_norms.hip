@@ -1,0 +1,709 @@
+// The norms around a block of a residual network, fused with its gate and the
+// residual sum, and their gradient.
+//
+// With norm(v; w, b) = (v - m) r (offset + w) + b, where r = 1 / sqrt(mean((v -
+// m)^2) + eps) and m is the row's mean (LayerNorm) or 0 (RMSNorm):
+//   n = norm(x; post),  h = residual + scale gate n,  y = norm(h; pre)
+// and backwards, T being the gradient of h from both of its uses:
+//   with u = grad_y (offset + pre), e = (h - m) r:
+//   T = grad_h + r (u - e mean(u e) - mean(u))        (mean(u): LayerNorm only)
+//   dresidual = T,  dpre = sum grad_y e,  dpre_bias = sum grad_y
+//   v = scale gate T,  dgate = scale sum T n,  dpost = sum v f,
+//   dpost_bias = sum v,  with f the normalised x;  dx as T's second term, of v.
+//
+// Both passes read every value once and hold the row in registers between its
+// statistics and its results; HBM bounds them.  A row belongs to a team of
+// lanes: up to 512 columns (one group of 8 values per lane) 1 to 64 lanes of
+// one wave, above that W whole waves with two groups per lane (16-byte
+// accesses of bf16 that cover 1 KiB of a row per wave).
+#include <algorithm>
+
+#include "hipo_common.h"
+
+namespace hipo {
+namespace {
+
+constexpr int kGroup = 8;        // values per lane and step
+constexpr int kSmallCols = 512;  // one wave or less per row
+constexpr int64_t kMostCols = 16384;
+
+struct Vec8 {
+  float v[kGroup];
+};
+
+// 8 values at p, of any element alignment.
+template <typename T>
+__device__ __forceinline__ Vec8 load8(const T* p);
+
+template <>
+__device__ __forceinline__ Vec8 load8<uint16_t>(const uint16_t* p) {
+  const u32x4_t w = *reinterpret_cast<const u32x4_a2_t*>(p);
+  Vec8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r.v[2 * i] = bf16lo(w[i]);
+    r.v[2 * i + 1] = bf16hi(w[i]);
+  }
+  return r;
+}
+
+template <>
+__device__ __forceinline__ Vec8 load8<float>(const float* p) {
+  const f32x4_t a = *reinterpret_cast<const f32x4_a4_t*>(p);
+  const f32x4_t b = *reinterpret_cast<const f32x4_a4_t*>(p + 4);
+  return Vec8{{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
+}
+
+__device__ __forceinline__ void store8(uint16_t* p, const Vec8& r) {
+  u32x4_t w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(r.v[2 * i], r.v[2 * i + 1]);
+  *reinterpret_cast<u32x4_a2_t*>(p) = w;
+}
+
+__device__ __forceinline__ void store8(float* p, const Vec8& r) {
+  *reinterpret_cast<f32x4_a4_t*>(p) = f32x4_t{r.v[0], r.v[1], r.v[2], r.v[3]};
+  *reinterpret_cast<f32x4_a4_t*>(p + 4) = f32x4_t{r.v[4], r.v[5], r.v[6], r.v[7]};
+}
+
+__device__ __forceinline__ float as_stored(float v, const uint16_t*) { return round_bf16(v); }
+__device__ __forceinline__ float as_stored(float v, const float*) { return v; }
+
+__device__ __forceinline__ void store1(uint16_t* p, float v) {
+  *p = static_cast<uint16_t>(pack_bf16x2(v, 0.0f));
+}
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+
+// How a launch is cut: teams of `lanes` lanes, `teams` of them in a workgroup.
+struct Layout {
+  int lanes;  // a power of two up to 64, or a multiple of 64
+  int teams;
+  int threads() const { return lanes * teams; }
+};
+
+inline Layout layout_of(int64_t cols) {
+  const int64_t groups = (cols + kGroup - 1) / kGroup;
+  if (cols <= kSmallCols) {
+    int lanes = 1;
+    while (lanes < groups) lanes *= 2;
+    return Layout{lanes, 512 / lanes};
+  }
+  const int waves = static_cast<int>((groups + 127) / 128);
+  return Layout{waves * kWave, std::max(1, 8 / waves)};
+}
+
+// Where a lane's groups lie.  The group that would cross the row's end is moved
+// back to end there; its first `skip` values belong to the group before, which
+// computes the same bits, and count in no sum.  skip = 8: past the row, owns
+// nothing (and loads what the last group loads).
+template <int U>
+struct Columns {
+  int col[U];
+  int skip[U];
+};
+
+template <int U>
+__device__ __forceinline__ Columns<U> columns_of(int place, int lanes, int cols) {
+  Columns<U> c;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int first = (u * lanes + place) * kGroup;
+    c.col[u] = min(first, cols - kGroup);
+    c.skip[u] = min(first - c.col[u], kGroup);
+  }
+  return c;
+}
+
+// Sums over a team, N at once, every lane receiving them, in an order that the
+// layout fixes.  `slot`: LDS of N floats per wave, other than the last call's.
+template <int N, bool SMALL>
+__device__ __forceinline__ void team_sum(float (&v)[N], int lanes, float* slot) {
+  if (SMALL) {
+    for (int o = 1; o < lanes; o *= 2) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+  const int waves = lanes / kWave;
+  if (waves == 1) return;
+  const int wave = threadIdx.x / kWave;
+  if (lane_id() == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) slot[wave * N + i] = v[i];
+  }
+  __syncthreads();
+  const float* mine = slot + wave / waves * waves * N;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = 0.0f;
+  for (int w = 0; w < waves; ++w) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += mine[w * N + i];
+  }
+}
+
+// Mean and 1 / sqrt(variance + eps) of a team's row.
+template <int U, bool LAYER, bool SMALL>
+__device__ __forceinline__ void row_stats(const Vec8 (&v)[U], const Columns<U>& c, int lanes,
+                                          float inv_cols, float eps, float* slots, float* mean,
+                                          float* rstd) {
+  float s[1] = {0.0f};
+  *mean = 0.0f;
+  if (LAYER) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) s[0] += i >= c.skip[u] ? v[u].v[i] : 0.0f;
+    }
+    team_sum<1, SMALL>(s, lanes, slots);
+    *mean = s[0] * inv_cols;
+    s[0] = 0.0f;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      const float d = v[u].v[i] - *mean;
+      s[0] += i >= c.skip[u] ? d * d : 0.0f;
+    }
+  }
+  team_sum<1, SMALL>(s, lanes, slots + 16);
+  *rstd = 1.0f / sqrtf(s[0] * inv_cols + eps);
+}
+
+struct Forward {
+  const void *x, *residual, *post, *post_bias, *pre, *pre_bias, *gate;
+  void *h, *y;
+  float* stats;
+  int64_t rows;
+  int cols;
+  int64_t rows_per_gate;
+  float scale, offset, eps, inv_cols;
+  int lanes, teams;
+};
+
+template <typename T, int U, bool LAYER, int THREADS>
+__global__ __launch_bounds__(THREADS) void block_norms(Forward a) {
+  constexpr bool kSmall = U == 1;
+  // Two sets of slots, for the rounds in turn: a barrier lies between a read
+  // and the next write of the same set.
+  __shared__ float slots[2][64];
+  const int team = threadIdx.x / a.lanes;
+  const Columns<U> c = columns_of<U>(threadIdx.x % a.lanes, a.lanes, a.cols);
+  int set = 0;
+  const T* post = static_cast<const T*>(a.post);
+  const T* pre = static_cast<const T*>(a.pre);
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * a.teams; first < a.rows;
+       first += static_cast<int64_t>(gridDim.x) * a.teams, set ^= 1) {
+    const bool valid = first + team < a.rows;
+    const int64_t row = valid ? first + team : a.rows - 1;
+    const int64_t at = row * a.cols;
+    Vec8 n[U], h[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) n[u] = load8(static_cast<const T*>(a.x) + at + c.col[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) h[u] = load8(static_cast<const T*>(a.residual) + at + c.col[u]);
+    float mean0 = 0.0f, rstd0 = 1.0f, mean1 = 0.0f, rstd1 = 1.0f;
+    if (post) {
+      row_stats<U, LAYER, kSmall>(n, c, a.lanes, a.inv_cols, a.eps, slots[set], &mean0, &rstd0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const Vec8 w = load8(post + c.col[u]);
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+          n[u].v[i] = (n[u].v[i] - mean0) * rstd0 * (a.offset + w.v[i]);
+        }
+        if (a.post_bias) {
+          const Vec8 b = load8(static_cast<const T*>(a.post_bias) + c.col[u]);
+#pragma unroll
+          for (int i = 0; i < kGroup; ++i) n[u].v[i] += b.v[i];
+        }
+      }
+    }
+    const T* gate =
+        a.gate ? static_cast<const T*>(a.gate) + row / a.rows_per_gate * a.cols : nullptr;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (gate) {
+        const Vec8 g = load8(gate + c.col[u]);
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) n[u].v[i] *= g.v[i];
+      }
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) {
+        h[u].v[i] = as_stored(__builtin_fmaf(a.scale, n[u].v[i], h[u].v[i]), post);
+      }
+      if (valid && c.skip[u] < kGroup) store8(static_cast<T*>(a.h) + at + c.col[u], h[u]);
+    }
+    if (pre) {
+      row_stats<U, LAYER, kSmall>(h, c, a.lanes, a.inv_cols, a.eps, slots[set] + 32, &mean1,
+                                  &rstd1);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const Vec8 w = load8(pre + c.col[u]);
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+          h[u].v[i] = (h[u].v[i] - mean1) * rstd1 * (a.offset + w.v[i]);
+        }
+        if (a.pre_bias) {
+          const Vec8 b = load8(static_cast<const T*>(a.pre_bias) + c.col[u]);
+#pragma unroll
+          for (int i = 0; i < kGroup; ++i) h[u].v[i] += b.v[i];
+        }
+        if (valid && c.skip[u] < kGroup) store8(static_cast<T*>(a.y) + at + c.col[u], h[u]);
+      }
+    }
+    if (valid && threadIdx.x % a.lanes == 0) {
+      *reinterpret_cast<f32x4_a4_t*>(a.stats + row * 4) = f32x4_t{mean0, rstd0, mean1, rstd1};
+    }
+  }
+}
+
+// Column sums of the gradient, in the order of the join's outputs.
+enum Sum { kPre, kPreBias, kPost, kPostBias, kGate, kSums };
+
+struct Backward {
+  const void *grad_h, *grad_y, *x, *h;
+  const float* stats;
+  const void *post, *post_bias, *pre, *gate;
+  void *dx, *dresidual, *dgate;
+  float* part;  // [kSums][blocks][cols], kGate: [2 blocks][cols] at the end
+  int64_t rows;
+  int cols;
+  int64_t rows_per_gate;
+  float scale, offset, inv_cols;
+  int lanes, teams, blocks;
+};
+
+__device__ __forceinline__ int64_t first_row(int64_t rows, int block, int blocks) {
+  return rows * block / blocks;
+}
+
+// A workgroup takes consecutive rows, its teams in turn, and keeps the column
+// sums of all of them in registers; the rows of one gate are a segment, whose
+// sum goes out when the segment ends: as dgate where the segment holds all rows
+// of the gate, else to one of the workgroup's two places for the join (a
+// workgroup has at most two such segments, its first and its last).
+template <typename T, int U, bool LAYER, bool PRE, bool POST, bool GATE, int THREADS>
+__global__ __launch_bounds__(THREADS) void block_norms_bwd(Backward a) {
+  constexpr bool kSmall = U == 1;
+  __shared__ float slots[2][64];
+  extern __shared__ float sums[];  // [teams][cols], where there are several teams
+  const int team = threadIdx.x / a.lanes;
+  const Columns<U> c = columns_of<U>(threadIdx.x % a.lanes, a.lanes, a.cols);
+  const int64_t begin = first_row(a.rows, blockIdx.x, a.blocks);
+  const int64_t end = first_row(a.rows, blockIdx.x + 1, a.blocks);
+  Vec8 acc[kSums][U];
+#pragma unroll
+  for (int k = 0; k < kSums; ++k) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) acc[k][u] = Vec8{};
+  }
+  Vec8 wpre[U], wpost[U], gate[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (PRE) wpre[u] = load8(static_cast<const T*>(a.pre) + c.col[u]);
+    if (POST) wpost[u] = load8(static_cast<const T*>(a.post) + c.col[u]);
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i) {
+      wpre[u].v[i] = PRE ? wpre[u].v[i] + a.offset : 0.0f;
+      wpost[u].v[i] = POST ? wpost[u].v[i] + a.offset : 0.0f;
+      gate[u].v[i] = a.scale;
+    }
+  }
+
+  // The sum over the teams of one accumulator, written by put(column, value).
+  auto flush = [&](Vec8 (&v)[U], auto put) {
+    if (a.teams > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+          if (i >= c.skip[u]) sums[team * a.cols + c.col[u] + i] = v[u].v[i];
+        }
+      }
+      __syncthreads();
+      for (int j = threadIdx.x; j < a.cols; j += blockDim.x) {
+        float s = 0.0f;
+        for (int t = 0; t < a.teams; ++t) s += sums[t * a.cols + j];
+        put(j, s);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+          if (i >= c.skip[u]) put(c.col[u] + i, v[u].v[i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = Vec8{};
+  };
+
+  int set = 0;
+  const bool by_row = GATE && a.rows_per_gate == 1;
+  for (int64_t from = begin; from < end;) {
+    int64_t to = end, which = 0;
+    if (GATE && !by_row) {
+      which = from / a.rows_per_gate;
+      to = min(end, (which + 1) * a.rows_per_gate);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        gate[u] = load8(static_cast<const T*>(a.gate) + which * a.cols + c.col[u]);
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) gate[u].v[i] *= a.scale;
+      }
+    }
+    for (int64_t first = from; first < to; first += a.teams, set ^= 1) {
+      const bool valid = first + team < to;
+      const int64_t row = valid ? first + team : to - 1;
+      const int64_t at = row * a.cols;
+      Vec8 gh[U], gy[U], h[U], x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (PRE) gy[u] = load8(static_cast<const T*>(a.grad_y) + at + c.col[u]);
+        if (PRE) h[u] = load8(static_cast<const T*>(a.h) + at + c.col[u]);
+        if (a.grad_h) {
+          gh[u] = load8(static_cast<const T*>(a.grad_h) + at + c.col[u]);
+        } else {
+          gh[u] = Vec8{};
+        }
+        if (POST || GATE) x[u] = load8(static_cast<const T*>(a.x) + at + c.col[u]);
+      }
+      const f32x4_t st = *reinterpret_cast<const f32x4_a4_t*>(a.stats + row * 4);
+      if (by_row) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          gate[u] = load8(static_cast<const T*>(a.gate) + at + c.col[u]);
+#pragma unroll
+          for (int i = 0; i < kGroup; ++i) gate[u].v[i] *= a.scale;
+        }
+      }
+      // gh becomes T.
+      if (PRE) {
+        float s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+          for (int i = 0; i < kGroup; ++i) {
+            const float e = (h[u].v[i] - st[2]) * st[3];
+            const float g = gy[u].v[i];
+            if (valid) acc[kPre][u].v[i] += g * e;
+            if (LAYER && valid) acc[kPreBias][u].v[i] += g;
+            const float w = i >= c.skip[u] ? g * wpre[u].v[i] : 0.0f;
+            s[0] += w * e;
+            s[1] += w;
+            h[u].v[i] = e;
+          }
+        }
+        team_sum<2, kSmall>(s, a.lanes, slots[set]);
+        s[0] *= a.inv_cols;
+        s[1] = LAYER ? s[1] * a.inv_cols : 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+          for (int i = 0; i < kGroup; ++i) {
+            gh[u].v[i] += st[3] * (gy[u].v[i] * wpre[u].v[i] - h[u].v[i] * s[0] - s[1]);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (valid && c.skip[u] < kGroup) {
+          store8(static_cast<T*>(a.dresidual) + at + c.col[u], gh[u]);
+        }
+      }
+      // gh becomes v = scale gate T, x the normalised x.
+      if (POST || GATE) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          Vec8 b{};
+          if (GATE && POST && LAYER && a.post_bias) {
+            b = load8(static_cast<const T*>(a.post_bias) + c.col[u]);
+          }
+          Vec8 dg;
+#pragma unroll
+          for (int i = 0; i < kGroup; ++i) {
+            float n = x[u].v[i];
+            if (POST) {
+              x[u].v[i] = (n - st[0]) * st[1];
+              n = __builtin_fmaf(x[u].v[i], wpost[u].v[i], b.v[i]);
+            }
+            dg.v[i] = gh[u].v[i] * n * a.scale;
+            if (GATE && valid) acc[kGate][u].v[i] += dg.v[i];
+          }
+          if (by_row && valid && c.skip[u] < kGroup) {
+            store8(static_cast<T*>(a.dgate) + at + c.col[u], dg);
+          }
+        }
+      }
+      float s[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+          gh[u].v[i] *= gate[u].v[i];
+          if (POST) {
+            if (valid) acc[kPost][u].v[i] += gh[u].v[i] * x[u].v[i];
+            if (LAYER && valid) acc[kPostBias][u].v[i] += gh[u].v[i];
+            const float w = i >= c.skip[u] ? gh[u].v[i] * wpost[u].v[i] : 0.0f;
+            s[0] += w * x[u].v[i];
+            s[1] += w;
+          }
+        }
+      }
+      if (POST) {
+        team_sum<2, kSmall>(s, a.lanes, slots[set] + 32);
+        s[0] *= a.inv_cols;
+        s[1] = LAYER ? s[1] * a.inv_cols : 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+          for (int i = 0; i < kGroup; ++i) {
+            gh[u].v[i] = st[1] * (gh[u].v[i] * wpost[u].v[i] - x[u].v[i] * s[0] - s[1]);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (valid && c.skip[u] < kGroup) store8(static_cast<T*>(a.dx) + at + c.col[u], gh[u]);
+      }
+    }
+    if (GATE && !by_row) {
+      const bool whole = from == which * a.rows_per_gate && to == (which + 1) * a.rows_per_gate;
+      if (whole) {
+        T* out = static_cast<T*>(a.dgate) + which * a.cols;
+        flush(acc[kGate], [&](int j, float s) { store1(out + j, s); });
+      } else {
+        float* out = a.part + (static_cast<int64_t>(kGate) * a.blocks + 2 * blockIdx.x +
+                               (from == begin ? 0 : 1)) * a.cols;
+        flush(acc[kGate], [&](int j, float s) { out[j] = s; });
+      }
+    }
+    from = to;
+  }
+  auto put_part = [&](int k, Vec8 (&v)[U]) {
+    float* out = a.part + (static_cast<int64_t>(k) * a.blocks + blockIdx.x) * a.cols;
+    flush(v, [&](int j, float s) { out[j] = s; });
+  };
+  if (PRE) put_part(kPre, acc[kPre]);
+  if (PRE && LAYER) put_part(kPreBias, acc[kPreBias]);
+  if (POST) put_part(kPost, acc[kPost]);
+  if (POST && LAYER) put_part(kPostBias, acc[kPostBias]);
+}
+
+struct Join {
+  const float* part;
+  void* out[kSums];
+  int64_t rows;
+  int cols;
+  int64_t rows_per_gate;
+  int blocks;
+};
+
+// The workgroups' column sums added in their order: 64 columns by 16 parts of
+// the workgroups, the parts joined through LDS.  blockIdx.y: one of the four
+// sums over all rows, or (from 4 on) the gate that a boundary between two
+// workgroups lies in, where it is the first in that gate.
+template <typename T>
+__global__ __launch_bounds__(1024) void join_sums(Join a) {
+  __shared__ float parts[16][64];
+  const int col = blockIdx.x * 64 + threadIdx.x % 64;
+  const int part = threadIdx.x / 64;
+  const int k = min(static_cast<int>(blockIdx.y), static_cast<int>(kGate));
+  if (!a.out[k]) return;
+  int lo = 0, hi = a.blocks;
+  int64_t gate = 0;
+  if (k == kGate) {
+    lo = blockIdx.y - kGate;  // the boundary after workgroup `lo`
+    const int64_t row = first_row(a.rows, lo + 1, a.blocks);
+    gate = row / a.rows_per_gate;
+    const int64_t from = gate * a.rows_per_gate;
+    if (row == from || first_row(a.rows, lo, a.blocks) > from) return;
+    hi = lo + 1;
+    while (hi < a.blocks && first_row(a.rows, hi, a.blocks) < from + a.rows_per_gate) ++hi;
+  }
+  float s = 0.0f;
+  if (col < a.cols) {
+    const float* p = a.part + static_cast<int64_t>(k) * a.blocks * a.cols + col;
+    const int n = hi - lo;
+    const int end = lo + n * (part + 1) / 16;
+    for (int b = lo + n * part / 16; b < end; ++b) {
+      int64_t place = b;
+      if (k == kGate) {
+        place = 2 * b + (first_row(a.rows, b, a.blocks) < gate * a.rows_per_gate ? 1 : 0);
+      }
+      s += p[place * a.cols];
+    }
+  }
+  parts[part][threadIdx.x % 64] = s;
+  __syncthreads();
+  if (part == 0 && col < a.cols) {
+    s = 0.0f;
+    for (int i = 0; i < 16; ++i) s += parts[i][threadIdx.x];
+    store1(static_cast<T*>(a.out[k]) + gate * a.cols + col, s);
+  }
+}
+
+int check_sizes(const char* what, int elem_size, int64_t rows, int64_t cols, int64_t gates,
+                int layer, const void* post, const void* post_bias, const void* pre,
+                const void* pre_bias, const void* gate, float scale, float offset) {
+  HIPO_REQUIRE(elem_size == 2 || elem_size == 4, "%s: elem_size must be 2 or 4", what);
+  HIPO_REQUIRE(rows >= 0 && cols >= 0 && gates >= 0, "%s: negative size", what);
+  HIPO_REQUIRE(cols >= kGroup && cols <= kMostCols, "%s: cols must be from 8 to 16384", what);
+  HIPO_REQUIRE(rows < (int64_t{1} << 31), "%s: rows must be below 2^31", what);
+  HIPO_REQUIRE(layer == 0 || layer == 1, "%s: layer must be 0 or 1", what);
+  HIPO_REQUIRE(post || pre, "%s: a norm is needed before or after the sum", what);
+  HIPO_REQUIRE((post || !post_bias) && (pre || !pre_bias), "%s: a bias needs its norm", what);
+  HIPO_REQUIRE(layer || (!post_bias && !pre_bias), "%s: biases are LayerNorm's", what);
+  HIPO_REQUIRE((gates > 0) == (gate != nullptr), "%s: gate and gate_rows go together", what);
+  HIPO_REQUIRE(gates == 0 || rows % gates == 0, "%s: gate_rows must divide rows", what);
+  HIPO_REQUIRE(__builtin_isfinite(scale) && __builtin_isfinite(offset),
+               "%s: scale and offset must be finite", what);
+  return 0;
+}
+
+template <typename T, int U, int THREADS>
+void launch_fwd(const Forward& a, bool layer, int64_t blocks, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(blocks)), block(a.lanes * a.teams);
+  if (layer) {
+    block_norms<T, U, true, THREADS><<<grid, block, 0, stream>>>(a);
+  } else {
+    block_norms<T, U, false, THREADS><<<grid, block, 0, stream>>>(a);
+  }
+}
+
+template <typename T>
+int run_fwd(const Forward& a, bool layer, hipStream_t stream) {
+  const int64_t blocks = std::min<int64_t>((a.rows + a.teams - 1) / a.teams, int64_t{1} << 20);
+  if (a.cols <= kSmallCols) {
+    launch_fwd<T, 1, 512>(a, layer, blocks, stream);
+  } else if (a.lanes * a.teams <= 512) {
+    launch_fwd<T, 2, 512>(a, layer, blocks, stream);
+  } else {
+    launch_fwd<T, 2, 1024>(a, layer, blocks, stream);
+  }
+  return check_launch("block_norms");
+}
+
+template <typename T, int U, bool LAYER, bool PRE, bool POST, int THREADS>
+void launch_bwd(const Backward& a, hipStream_t stream) {
+  const dim3 grid(a.blocks), block(a.lanes * a.teams);
+  const size_t lds = a.teams > 1 ? sizeof(float) * a.teams * a.cols : 0;
+  if (a.gate) {
+    block_norms_bwd<T, U, LAYER, PRE, POST, true, THREADS><<<grid, block, lds, stream>>>(a);
+  } else {
+    block_norms_bwd<T, U, LAYER, PRE, POST, false, THREADS><<<grid, block, lds, stream>>>(a);
+  }
+}
+
+template <typename T, int U, int THREADS>
+void launch_bwd(const Backward& a, bool layer, hipStream_t stream) {
+  if (a.pre && a.post) {
+    layer ? launch_bwd<T, U, true, true, true, THREADS>(a, stream)
+          : launch_bwd<T, U, false, true, true, THREADS>(a, stream);
+  } else if (a.pre) {
+    layer ? launch_bwd<T, U, true, true, false, THREADS>(a, stream)
+          : launch_bwd<T, U, false, true, false, THREADS>(a, stream);
+  } else {
+    layer ? launch_bwd<T, U, true, false, true, THREADS>(a, stream)
+          : launch_bwd<T, U, false, false, true, THREADS>(a, stream);
+  }
+}
+
+// Workgroups of the gradient: no more than there are rows for their teams.
+int bwd_blocks(int64_t rows, int64_t cols) {
+  const Layout l = layout_of(cols);
+  return static_cast<int>(std::min<int64_t>((rows + l.teams - 1) / l.teams, 512));
+}
+
+template <typename T>
+int run_bwd(const Backward& a, Join j, bool layer, hipStream_t stream) {
+  if (a.cols <= kSmallCols) {
+    launch_bwd<T, 1, 512>(a, layer, stream);
+  } else if (a.lanes * a.teams <= 512) {
+    launch_bwd<T, 2, 512>(a, layer, stream);
+  } else {
+    launch_bwd<T, 2, 1024>(a, layer, stream);
+  }
+  const int rc = check_launch("block_norms_bwd");
+  if (rc != 0) return rc;
+  const bool gates = a.gate && a.rows_per_gate != 1;
+  join_sums<T><<<dim3((a.cols + 63) / 64, kGate + (gates ? a.blocks - 1 : 0)),
+                 1024, 0, stream>>>(j);
+  return check_launch("block_norms_bwd: join_sums");
+}
+
+}  // namespace
+}  // namespace hipo
+
+extern "C" int hipo_block_norms(const void* x, const void* residual, int elem_size,
+                                const void* post, const void* post_bias, const void* pre,
+                                const void* pre_bias, const void* gate, void* h, void* y,
+                                float* stats, int64_t rows, int64_t cols, int64_t gate_rows,
+                                float scale, float offset, float eps, int layer,
+                                hipStream_t stream) {
+  using namespace hipo;
+  clear_error();
+  const int rc = check_sizes("block_norms", elem_size, rows, cols, gate_rows, layer, post,
+                             post_bias, pre, pre_bias, gate, scale, offset);
+  if (rc != 0) return rc;
+  HIPO_REQUIRE(eps >= 0.0f && __builtin_isfinite(eps), "block_norms: eps must be finite, not negative");
+  if (rows == 0) return 0;
+  HIPO_REQUIRE(x && residual && h && stats && (y || !pre), "block_norms: null pointer");
+  const Layout l = layout_of(cols);
+  const Forward a{x, residual, post, post_bias, pre, pre_bias, gate, h, y, stats, rows,
+                  static_cast<int>(cols), gate_rows ? rows / gate_rows : rows, scale, offset, eps,
+                  1.0f / static_cast<float>(cols), l.lanes, l.teams};
+  return elem_size == 2 ? run_fwd<uint16_t>(a, layer != 0, stream)
+                        : run_fwd<float>(a, layer != 0, stream);
+}
+
+extern "C" size_t hipo_block_norms_bwd_workspace_bytes(int64_t rows, int64_t cols) {
+  if (rows <= 0 || cols < hipo::kGroup || cols > hipo::kMostCols) return 0;
+  return sizeof(float) * (hipo::kSums + 1) * hipo::bwd_blocks(rows, cols) * cols;
+}
+
+extern "C" int hipo_block_norms_bwd(const void* grad_h, const void* grad_y, const void* x,
+                                    const void* h, const float* stats, int elem_size,
+                                    const void* post, const void* post_bias, const void* pre,
+                                    const void* pre_bias, const void* gate, void* dx,
+                                    void* dresidual, void* dgate, void* dpost, void* dpost_bias,
+                                    void* dpre, void* dpre_bias, int64_t rows, int64_t cols,
+                                    int64_t gate_rows, float scale, float offset, int layer,
+                                    void* workspace, size_t workspace_bytes,
+                                    hipStream_t stream) {
+  using namespace hipo;
+  clear_error();
+  const char* what = "block_norms_bwd";
+  const int rc = check_sizes(what, elem_size, rows, cols, gate_rows, layer, post, post_bias, pre,
+                             pre_bias, gate, scale, offset);
+  if (rc != 0) return rc;
+  HIPO_REQUIRE((pre || !grad_y) && (pre || grad_h), "%s: grad_y belongs to the norm after the sum",
+               what);
+  HIPO_REQUIRE((dpost != nullptr) == (post != nullptr) && (dpre != nullptr) == (pre != nullptr) &&
+                   (dpost_bias != nullptr) == (post_bias != nullptr) &&
+                   (dpre_bias != nullptr) == (pre_bias != nullptr),
+               "%s: each weight and bias has its gradient", what);
+  if (rows == 0) return 0;
+  HIPO_REQUIRE(stats && dx && dresidual && (x || !(post || gate)) && ((h && grad_y) || !pre) &&
+                   (dgate != nullptr) == (gate != nullptr),
+               "%s: null pointer", what);
+  const size_t need = hipo_block_norms_bwd_workspace_bytes(rows, cols);
+  HIPO_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
+               "%s: workspace of %zu bytes, 16-byte aligned, needed", what, need);
+  const Layout l = layout_of(cols);
+  const int64_t rows_per_gate = gate_rows ? rows / gate_rows : rows;
+  const int blocks = bwd_blocks(rows, cols);
+  const Backward a{grad_h, grad_y, x, h, stats, post, post_bias, pre, gate, dx, dresidual, dgate,
+                   static_cast<float*>(workspace), rows, static_cast<int>(cols), rows_per_gate,
+                   scale, offset, 1.0f / static_cast<float>(cols), l.lanes, l.teams, blocks};
+  const Join j{a.part, {dpre, dpre_bias, dpost, dpost_bias, rows_per_gate == 1 ? nullptr : dgate},
+               rows, a.cols, rows_per_gate, blocks};
+  return elem_size == 2 ? run_bwd<uint16_t>(a, j, layer != 0, stream)
+                        : run_bwd<float>(a, j, layer != 0, stream);
+}

@@ -1,0 +1,921 @@
+// Softmax cross entropy of the output layer without its logits, and its
+// gradients.
+//
+// With s_j = scale hidden weight_j:  lse = ln sum_j e^(s_j),  loss = lse - s_t;
+// d_j = scale ((g + g_lse) e^(s_j - lse) - g [j = t]),  dhidden = d weight,
+// dweight = d^T hidden.
+//
+// All products run through one matrix-product kernel, gemm(), that multiplies
+// rows of two K-contiguous bf16 matrices; what becomes of a tile of the result
+// is its epilogue: a tile's logits are reduced to one maximum and one sum per
+// row (forward), turned into d (backward), or are a tile of a gradient.  Rows
+// that are left out are compacted away first, on the device.  The gradient goes
+// through the vocabulary in pieces, so that d's piece alone is ever in memory.
+//
+// fp32 operands are split into three bf16 parts (8 bits of the significand
+// each) and multiplied as six products of parts, the smallest first; the three
+// left out are below 2^-24 of the largest.
+#include <algorithm>
+
+#include "hipo_common.h"
+
+namespace hipo {
+namespace {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef u32x2_t u32x2_a2_t __attribute__((aligned(2)));
+
+constexpr int kTile = 256;  // rows of either operand that a workgroup multiplies
+constexpr int kStep = 64;   // values of K per round
+constexpr int kThreads = 512;
+constexpr float kLargest = 3.402823466e+38f;
+
+inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// ---------------------------------------------------------------------------
+// Operands: rows that count, and copies in the layout that gemm() reads.
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ int64_t token_at(const void* tokens, int size, int64_t i) {
+  return size == 8 ? static_cast<const int64_t*>(tokens)[i]
+                   : static_cast<const int32_t*>(tokens)[i];
+}
+
+struct Select {
+  const void* tokens;
+  int token_size;
+  int64_t rows, ignore_index;
+  int* kept;      // [rows] the rows that count, in order
+  int* count;     // how many
+  float* target;  // [rows] set to NaN (forward), or null
+  float *loss, *lse;
+};
+
+// One workgroup; rows that do not count get their zeros here.
+__global__ __launch_bounds__(1024) void select_rows(Select a) {
+  __shared__ int waves[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int base = 0;
+  for (int64_t r0 = 0; r0 < a.rows; r0 += 1024) {
+    const int64_t r = r0 + threadIdx.x;
+    const bool keep = r < a.rows && token_at(a.tokens, a.token_size, r) != a.ignore_index;
+    const uint64_t mask = __ballot(keep);
+    if (lane == 0) waves[wave] = __popcll(mask);
+    __syncthreads();
+    int before = base, sum = 0;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) before += waves[w];
+      sum += waves[w];
+    }
+    if (keep) {
+      const int at = before + __popcll(mask & ((uint64_t{1} << lane) - 1));
+      a.kept[at] = static_cast<int>(r);
+      if (a.target) a.target[at] = __builtin_nanf("");
+    } else if (a.loss && r < a.rows) {
+      a.loss[r] = 0.0f;
+      a.lse[r] = 0.0f;
+    }
+    base += sum;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *a.count = base;
+}
+
+// The bf16 parts of x, each the nearest to what the ones before leave; a part
+// that would overflow is cut instead.  What is not finite has no second part.
+__device__ __forceinline__ void split3(float x, uint16_t (&part)[3]) {
+  const uint32_t bits = __float_as_uint(x);
+  uint32_t first = pack_bf16x2(x, 0.0f) & 0xffffu;
+  const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
+  if (finite && (first & 0x7f80u) == 0x7f80u) first = bits >> 16;
+  const float rest = finite ? x - bf16lo(first) : 0.0f;
+  const uint32_t second = pack_bf16x2(rest, 0.0f) & 0xffffu;
+  part[0] = static_cast<uint16_t>(first);
+  part[1] = static_cast<uint16_t>(second);
+  part[2] = static_cast<uint16_t>(pack_bf16x2(rest - bf16lo(second), 0.0f));
+}
+
+struct Pack {
+  const void* src;
+  int64_t ld;       // of src
+  const int* kept;  // rows of src, or null: all
+  const int* count; // how many rows, or null: rows
+  int64_t rows;
+  int cols;
+  uint16_t* dst;
+  int64_t dst_ld, plane;  // of dst, in values
+};
+
+__device__ __forceinline__ float value_at(const uint16_t* p) { return bf16_to_f32(*p); }
+__device__ __forceinline__ float value_at(const float* p) { return *p; }
+
+// dst[plane][row][0 : dst_ld] = the parts of a row of src, zeros past its end.
+template <typename T>
+__global__ __launch_bounds__(256) void pack_rows(Pack a) {
+  const int64_t rows = a.count ? *a.count : a.rows;
+  const int chunks = static_cast<int>(a.dst_ld / 8);
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T* from = static_cast<const T*>(a.src) + (a.kept ? a.kept[row] : row) * a.ld;
+    for (int c = threadIdx.x; c < chunks; c += 256) {
+      uint16_t part[3][8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int col = c * 8 + i;
+        if (sizeof(T) == 2) {
+          part[0][i] = col < a.cols ? reinterpret_cast<const uint16_t*>(from)[col] : 0;
+        } else {
+          uint16_t p[3];
+          split3(col < a.cols ? value_at(from + col) : 0.0f, p);
+          part[0][i] = p[0];
+          part[1][i] = p[1];
+          part[2][i] = p[2];
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < (sizeof(T) == 2 ? 1 : 3); ++p) {
+        u32x4_t w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = part[p][2 * i] | uint32_t{part[p][2 * i + 1]} << 16;
+        *reinterpret_cast<u32x4_t*>(a.dst + p * a.plane + row * a.dst_ld + c * 8) = w;
+      }
+    }
+  }
+}
+
+// dst[plane][col][row] = the parts of src[row][col], zeros from the last row up
+// to a multiple of 64.  A workgroup moves tiles of 64 by 64 through LDS.
+template <typename T>
+__global__ __launch_bounds__(256) void pack_transposed(Pack a) {
+  __shared__ T tile[64][65];
+  const int64_t rows = a.count ? *a.count : a.rows;
+  const int64_t tiles_r = (rows + 63) / 64, tiles_c = (a.cols + 63) / 64;
+  for (int64_t t = blockIdx.x; t < tiles_r * tiles_c; t += gridDim.x) {
+    const int64_t r0 = t / tiles_c * 64;
+    const int c0 = static_cast<int>(t % tiles_c) * 64;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int i = wave; i < 64; i += 4) {
+      const int64_t r = r0 + i;
+      T v = 0;
+      if (r < rows && c0 + lane < a.cols) {
+        v = static_cast<const T*>(a.src)[(a.kept ? a.kept[r] : r) * a.ld + c0 + lane];
+      }
+      tile[i][lane] = v;
+    }
+    __syncthreads();
+    for (int i = wave; i < 64 && c0 + i < a.cols; i += 4) {
+      uint16_t* to = a.dst + (c0 + i) * a.dst_ld + r0 + lane;
+      if (sizeof(T) == 2) {
+        *to = static_cast<uint16_t>(tile[lane][i]);
+      } else {
+        uint16_t p[3];
+        split3(static_cast<float>(tile[lane][i]), p);
+        to[0] = p[0];
+        to[a.plane] = p[1];
+        to[2 * a.plane] = p[2];
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The product of the rows of two matrices
+// ---------------------------------------------------------------------------
+
+enum Epilogue { kReduce, kLogitGrad, kAccumulate, kStore };
+
+struct Product {
+  // out[j][i] = sum_k a[i][k] b[j][k].  a_count, b_count, k_count: read on the
+  // device where they are the number of rows that count.
+  const uint16_t *a, *b;
+  int64_t lda, ldb, a_plane, b_plane;
+  int a_rows, b_rows, k;
+  const int *b_count, *k_count;
+
+  // kReduce, kLogitGrad: a is the vocabulary from `first` on, b the rows.
+  const void* tokens;
+  int token_size;
+  const int* kept;
+  int64_t first;
+  float scale;
+  float2* part;  // [tile of the vocabulary][part_ld] maximum and sum
+  int64_t part_ld, first_tile;
+  float* target;
+  const float *grad, *lse, *grad_lse;
+  uint16_t *d, *dt;  // [rows][d_ld], [piece][dt_ld] and their planes
+  int64_t d_ld, dt_ld, d_plane, dt_plane, vocab;
+
+  // kAccumulate: sums of the pieces [split][rows][sum_ld], K being split among
+  // blockIdx.y (`to_out`: not split, and the last piece).  kStore: out alone.
+  float* sum;
+  int64_t sum_ld, sum_plane;
+  int load_sum, to_out;
+  void* out;
+  int64_t out_ld;
+};
+
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+
+__device__ __forceinline__ void barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// 4 consecutive values of an output row, `n` of them inside.
+__device__ __forceinline__ void store4(uint16_t* p, const f32x4_t& v, int n) {
+  if (n >= 4) {
+    *reinterpret_cast<u32x2_a2_t*>(p) = u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+  } else {
+    for (int i = 0; i < n; ++i) p[i] = static_cast<uint16_t>(pack_bf16x2(v[i], 0.0f));
+  }
+}
+__device__ __forceinline__ void store4(float* p, const f32x4_t& v, int n) {
+  if (n >= 4) {
+    *reinterpret_cast<f32x4_a4_t*>(p) = v;
+  } else {
+    for (int i = 0; i < n; ++i) p[i] = v[i];
+  }
+}
+
+// The parts of a and b that are multiplied, the smallest products first.
+__device__ __forceinline__ int a_part(int pass, int passes) {
+  return passes == 1 ? 0 : (0x001120 >> (4 * pass)) & 3;
+}
+__device__ __forceinline__ int b_part(int pass, int passes) {
+  return passes == 1 ? 0 : (0x010102 >> (4 * pass)) & 3;
+}
+
+template <typename T, Epilogue E>
+__global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
+  constexpr int kPasses = sizeof(T) == 2 ? 1 : 6;
+  __shared__ __attribute__((aligned(16))) uint16_t a0[kTile * kStep], a1[kTile * kStep];
+  __shared__ __attribute__((aligned(16))) uint16_t b0[kTile * kStep], b1[kTile * kStep];
+
+  const int rows_b = p.b_count ? *p.b_count : p.b_rows;
+  const int k = p.k_count ? (*p.k_count + kStep - 1) / kStep * kStep : p.k;
+  // Tiles in an order that keeps an XCD's workgroups on 4 tiles of a by 8 of b.
+  const int tiles_a = (p.a_rows + kTile - 1) / kTile;
+  const int tiles_b = (rows_b + kTile - 1) / kTile;
+  const uint32_t tiles = static_cast<uint32_t>(tiles_a) * tiles_b;
+  if (blockIdx.x >= tiles) return;
+  const uint32_t id = xcd_order(blockIdx.x, tiles);
+  const int band = id / (4 * tiles_b), in_band = id % (4 * tiles_b);
+  const int band_rows = min(4, tiles_a - band * 4);
+  const int tile_a = band * 4 + in_band % band_rows, tile_b = in_band / band_rows;
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int valid_a = min(kTile, p.a_rows - tile_a * kTile);
+  const int valid_b = min(kTile, rows_b - tile_b * kTile);
+
+  // A load moves 8 rows of 64 values straight into LDS, 16 bytes a lane.  The
+  // 16-byte piece c of row r lies at place c ^ (r % 8) of its row, so that the
+  // 16 rows that a matrix instruction reads spread over all banks.
+  const int row_in = lane >> 3, chunk = (lane & 7) ^ row_in;
+  uint32_t from_a[4], from_b[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t row = (q * 8 + wave) * 8 + row_in;
+    from_a[q] = static_cast<uint32_t>(row * p.lda * 2 + chunk * 16);
+    from_b[q] = static_cast<uint32_t>(row * p.ldb * 2 + chunk * 16);
+  }
+  const int bytes_a = static_cast<int>(((valid_a - 1) * p.lda + k) * 2);
+  const int bytes_b = static_cast<int>(((valid_b - 1) * p.ldb + k) * 2);
+
+  auto load = [&](uint16_t* la, uint16_t* lb, int pass, int k0) {
+    const uint16_t* ga = p.a + a_part(pass, kPasses) * p.a_plane + tile_a * p.lda * kTile;
+    const uint16_t* gb = p.b + b_part(pass, kPasses) * p.b_plane + tile_b * p.ldb * kTile;
+    auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(ga), 0, bytes_a, 0x00027000);
+    auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(gb), 0, bytes_b, 0x00027000);
+    // Past K: an offset past the buffer's end, which reads as zero.
+    const uint32_t past = k0 + chunk * 8 < k ? 0u : 0x80000000u;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr_t)(la + (q * 8 + wave) * 512), 16,
+                                               from_a[q] | past, k0 * 2, 0, 0);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr_t)(lb + (q * 8 + wave) * 512), 16,
+                                               from_b[q] | past, k0 * 2, 0, 0);
+    }
+  };
+
+  // 2 by 4 waves of 128 by 64 values each, in tiles of 16 by 16.
+  const int wave_a = (wave >> 2) * 128, wave_b = (wave & 3) * 64;
+  f32x4_t acc[8][4];
+#pragma unroll
+  for (int f = 0; f < 8; ++f) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) acc[f][n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  auto multiply = [&](const uint16_t* la, const uint16_t* lb) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int at = (lane & 15) * kStep + (((s * 4 + (lane >> 4)) ^ (lane & 7)) * 8);
+      bf16x8_t fa[8], fb[4];
+#pragma unroll
+      for (int f = 0; f < 8; ++f) {
+        fa[f] = *reinterpret_cast<const bf16x8_t*>(la + (wave_a + f * 16) * kStep + at);
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        fb[n] = *reinterpret_cast<const bf16x8_t*>(lb + (wave_b + n * 16) * kStep + at);
+      }
+#pragma unroll
+      for (int f = 0; f < 8; ++f) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          acc[f][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[f], fb[n], acc[f][n], 0, 0, 0);
+        }
+      }
+    }
+  };
+
+  // Rounds of K, in pairs, the next one's loads in flight while one is
+  // multiplied.  Rounds past the last (the second of an odd pair, and the one
+  // loaded behind the end) load zeros.
+  int begin = 0, end = (k + kStep - 1) / kStep;
+  if (E == kAccumulate) {
+    const int whole = end;
+    begin = static_cast<int>(static_cast<int64_t>(whole) * blockIdx.y / gridDim.y);
+    end = static_cast<int>(static_cast<int64_t>(whole) * (blockIdx.y + 1) / gridDim.y);
+  }
+  const int rounds = (end - begin) * kPasses;
+  int pass = 0, at = begin;
+  auto next = [&](uint16_t* la, uint16_t* lb) {
+    load(la, lb, pass, pass < kPasses ? at * kStep : k);
+    if (++at >= end) {
+      at = begin;
+      ++pass;
+    }
+  };
+  next(a0, b0);
+  for (int t = 0; t < rounds; t += 2) {
+    next(a1, b1);
+    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    barrier();
+    multiply(a0, b0);
+    barrier();
+    next(a0, b0);
+    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    barrier();
+    multiply(a1, b1);
+    barrier();
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  barrier();
+
+  // acc[f][n][r] is out[j][i] with these.
+  const int i0 = tile_a * kTile + wave_a + (lane >> 4) * 4;  // + 16 f + r
+  const int j0 = tile_b * kTile + wave_b + (lane & 15);      // + 16 n
+
+  if (E == kReduce) {
+    // A row's values are 32 of each of 4 lanes in each of 2 waves.
+    float* both = reinterpret_cast<float*>(a0);  // [wave_a][2][kTile]
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int j = j0 + n * 16;
+      const bool inside = j < rows_b;
+      const int64_t tok = inside ? token_at(p.tokens, p.token_size, p.kept[j]) - p.first : -1;
+      float top = -kLargest;
+#pragma unroll
+      for (int f = 0; f < 8; ++f) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = i0 + f * 16 + r;
+          float s = acc[f][n][r] * p.scale;
+          if (i == tok && i < p.a_rows) p.target[j] = s;
+          if (i >= p.a_rows) s = -INFINITY;
+          acc[f][n][r] = s;
+          top = fmaxf(top, s);
+        }
+      }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      top = fminf(top, kLargest);
+      float sum = 0.0f;
+#pragma unroll
+      for (int f = 0; f < 8; ++f) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum += exp_f32(exp_domain(acc[f][n][r] - top));
+      }
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      if (lane < 16) {
+        both[((wave >> 2) * 2 + 0) * kTile + wave_b + n * 16 + lane] = top;
+        both[((wave >> 2) * 2 + 1) * kTile + wave_b + n * 16 + lane] = sum;
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x < kTile && static_cast<int>(threadIdx.x) < valid_b) {
+      const int j = threadIdx.x;
+      const float t0 = both[j], s0 = both[kTile + j];
+      const float t1 = both[2 * kTile + j], s1 = both[3 * kTile + j];
+      const float top = fmaxf(t0, t1);
+      const float sum = s0 * exp_f32(exp_domain(t0 - top)) + s1 * exp_f32(exp_domain(t1 - top));
+      p.part[(p.first_tile + tile_a) * p.part_ld + tile_b * kTile + j] = make_float2(top, sum);
+    }
+  }
+
+  if (E == kLogitGrad) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int j = j0 + n * 16;
+      const bool inside = j < rows_b;
+      float g = 0.0f, both = 0.0f, lse = 0.0f;
+      int64_t tok = -1;
+      if (inside) {
+        const int row = p.kept[j];
+        tok = token_at(p.tokens, p.token_size, row);
+        g = p.grad[row];
+        if (tok < 0 || tok >= p.vocab) g = __builtin_nanf("");
+        both = p.grad_lse ? g + p.grad_lse[row] : g;
+        lse = p.lse[row];
+        tok -= p.first;
+      }
+#pragma unroll
+      for (int f = 0; f < 8; ++f) {
+        const int i = i0 + f * 16;
+        float v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float e = exp_f32(exp_domain(acc[f][n][r] * p.scale - lse));
+          const float d = (both * e - (i + r == tok ? g : 0.0f)) * p.scale;
+          v[r] = inside && i + r < p.a_rows ? d : 0.0f;
+        }
+        uint16_t part[4][3];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (sizeof(T) == 2) {
+            part[r][0] = static_cast<uint16_t>(pack_bf16x2(v[r], 0.0f));
+          } else {
+            split3(v[r], part[r]);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < (sizeof(T) == 2 ? 1 : 3); ++q) {
+          *reinterpret_cast<u32x2_t*>(p.d + q * p.d_plane + j * p.d_ld + i) =
+              u32x2_t{part[0][q] | uint32_t{part[1][q]} << 16,
+                      part[2][q] | uint32_t{part[3][q]} << 16};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) p.dt[q * p.dt_plane + (i + r) * p.dt_ld + j] = part[r][q];
+        }
+      }
+    }
+  }
+
+  if (E == kAccumulate || E == kStore) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int j = j0 + n * 16;
+      if (j >= rows_b) continue;
+      T* out = static_cast<T*>(p.out) + (E == kStore ? j : (p.to_out ? p.kept[j] : 0)) * p.out_ld;
+#pragma unroll
+      for (int f = 0; f < 8; ++f) {
+        const int i = i0 + f * 16;
+        if (i >= p.a_rows) continue;
+        f32x4_t v = acc[f][n];
+        if (E == kAccumulate) {
+          f32x4_t* sum = reinterpret_cast<f32x4_t*>(p.sum + blockIdx.y * p.sum_plane +
+                                                     j * p.sum_ld + i);
+          if (p.load_sum) v += *sum;
+          if (!p.to_out) {
+            *sum = v;
+            continue;
+          }
+        }
+        store4(out + i, v, p.a_rows - i);
+      }
+    }
+  }
+}
+
+struct JoinLoss {
+  const float2* part;
+  int64_t part_ld;
+  int tiles;
+  const int *kept, *count;
+  const float* target;
+  float *loss, *lse;
+};
+
+// 64 rows by 4 parts of the vocabulary's tiles per workgroup.
+__global__ __launch_bounds__(256) void join_loss(JoinLoss a) {
+  __shared__ float2 parts[4][64];
+  const int count = *a.count;
+  const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * 64; first < count;
+       first += static_cast<int64_t>(gridDim.x) * 64) {
+    const int64_t j = first + lane;
+    float top = -kLargest, sum = 0.0f;
+    if (j < count) {
+      for (int t = part; t < a.tiles; t += 4) {
+        const float2 v = a.part[t * a.part_ld + j];
+        const float m = fmaxf(top, v.x);
+        sum = sum * exp_f32(exp_domain(top - m)) + v.y * exp_f32(exp_domain(v.x - m));
+        top = m;
+      }
+    }
+    parts[part][lane] = make_float2(top, sum);
+    __syncthreads();
+    if (part == 0 && j < count) {
+      for (int q = 1; q < 4; ++q) {
+        const float2 v = parts[q][lane];
+        const float m = fmaxf(top, v.x);
+        sum = sum * exp_f32(exp_domain(top - m)) + v.y * exp_f32(exp_domain(v.x - m));
+        top = m;
+      }
+      const float lse = top + logf(sum);
+      a.lse[a.kept[j]] = lse;
+      a.loss[a.kept[j]] = lse - a.target[j];
+    }
+    __syncthreads();
+  }
+}
+
+// The splits' sums added in order: rows of dhidden.
+template <typename T>
+__global__ __launch_bounds__(256) void join_hidden(const float* sum, int64_t sum_ld,
+                                                   int64_t sum_plane, int splits, const int* kept,
+                                                   const int* count, T* out, int width) {
+  const int chunks = (width + 3) / 4;
+  const int64_t n = static_cast<int64_t>(*count) * chunks;
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; t < n;
+       t += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t j = t / chunks;
+    const int i = static_cast<int>(t % chunks) * 4;
+    const float* from = sum + j * sum_ld + i;
+    f32x4_t v = *reinterpret_cast<const f32x4_t*>(from);
+    for (int q = 1; q < splits; ++q) v += *reinterpret_cast<const f32x4_t*>(from + q * sum_plane);
+    store4(out + kept[j] * static_cast<int64_t>(width) + i, v, width - i);
+  }
+}
+
+// Zeros in the rows of dhidden that do not count.
+template <typename T>
+__global__ __launch_bounds__(256) void zero_rows(const void* tokens, int token_size,
+                                                 int64_t ignore_index, T* out, int64_t rows,
+                                                 int width) {
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    if (token_at(tokens, token_size, r) != ignore_index) continue;
+    for (int c = threadIdx.x; c < width; c += 256) out[r * width + c] = 0;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+
+// Where things lie in the workspace; pieces of the vocabulary are multiples of
+// kTile rows and of one size.
+struct Plan {
+  int64_t rows_pad, k_pad, piece, pieces;
+  int planes;
+  int splits;   // of a piece, for dhidden
+  bool direct;  // weight is read where it lies
+  size_t kept, count, target, part, hidden, weight, hidden_t, weight_t, d, dt, sum, bytes;
+};
+
+constexpr int64_t kCus = 256;
+constexpr int64_t kMostTiles = int64_t{1} << 22;  // 2^31 threads
+constexpr int64_t kMostRows = (int64_t{1} << 22) - kTile;  // a tile's bytes fit 31 bits
+constexpr size_t kForwardBytes = size_t{256} << 20;   // of a copied piece
+constexpr size_t kBackwardBytes = size_t{1536} << 20;  // of a piece's d and copies
+
+Plan plan_of(const void* weight, int elem_size, int64_t rows, int64_t width, int64_t vocab,
+             int64_t weight_ld, bool backward) {
+  Plan p{};
+  p.planes = elem_size == 2 ? 1 : 3;
+  p.direct = elem_size == 2 && aligned16(weight) && weight_ld % 8 == 0 && width % 8 == 0;
+  p.rows_pad = up(rows, kTile);
+  p.k_pad = up(width, kStep);
+  const size_t copy = p.direct ? 0 : sizeof(uint16_t) * p.planes * p.k_pad;
+  const size_t per_row =
+      backward ? copy + sizeof(uint16_t) * p.planes * (2 * p.rows_pad + width) : copy;
+  const size_t most = backward ? kBackwardBytes : kForwardBytes;
+  const int64_t whole = up(vocab, kTile);
+  int64_t piece = whole;
+  if (per_row > 0) {
+    piece = std::min<int64_t>(whole, std::max<int64_t>(kTile, most / per_row / kTile * kTile));
+  }
+  // Tiles of one launch.
+  const int64_t other = std::max(p.rows_pad, up(width, kTile)) / kTile;
+  piece = std::min(piece, std::max<int64_t>(1, kMostTiles / other) * kTile);
+  p.pieces = (vocab + piece - 1) / piece;
+  p.piece = up((vocab + p.pieces - 1) / p.pieces, kTile);
+  p.pieces = (vocab + p.piece - 1) / p.piece;
+  // dhidden has few tiles where there are few rows: the piece is split until
+  // there are as many workgroups as CUs, 8 rounds each at least.
+  const int64_t tiles = p.rows_pad / kTile * (up(width, kTile) / kTile);
+  p.splits = static_cast<int>(
+      std::max<int64_t>(1, std::min<int64_t>(kCus / tiles, p.piece / (8 * kStep))));
+  size_t at = 0;
+  auto take = [&at](size_t bytes) {
+    const size_t here = at;
+    at += up(bytes, 256);
+    return here;
+  };
+  const size_t plane = sizeof(uint16_t) * p.planes;
+  p.kept = take(sizeof(int) * rows);
+  p.count = take(sizeof(int));
+  p.hidden = take(plane * p.rows_pad * p.k_pad);
+  p.weight = take(p.direct ? 0 : plane * p.piece * p.k_pad);
+  if (backward) {
+    p.hidden_t = take(plane * width * p.rows_pad);
+    p.weight_t = take(plane * width * p.piece);
+    p.d = take(plane * p.rows_pad * p.piece);
+    p.dt = take(plane * p.piece * p.rows_pad);
+    p.sum = take(p.pieces * p.splits > 1
+                     ? sizeof(float) * p.splits * p.rows_pad * up(width, 4) : 0);
+  } else {
+    p.target = take(sizeof(float) * rows);
+    p.part = take(sizeof(float2) * (whole / kTile) * p.rows_pad);
+  }
+  p.bytes = at;
+  return p;
+}
+
+bool sizes_fit(int64_t rows, int64_t width, int64_t vocab, int64_t hidden_ld, int64_t weight_ld) {
+  return rows >= 0 && rows <= kMostRows && vocab >= 1 &&
+         vocab <= (int64_t{1} << 31) - 65536 && width >= 1 && width <= (1 << 20) &&
+         hidden_ld >= width && weight_ld >= width && weight_ld <= (1 << 21) &&
+         up(rows, kTile) / kTile * (up(width, kTile) / kTile) <= kMostTiles;
+}
+
+int check_operands(const char* what, int elem_size, int token_size, int64_t rows, int64_t width,
+                   int64_t vocab, int64_t hidden_ld, int64_t weight_ld, float scale) {
+  HIPO_REQUIRE(elem_size == 2 || elem_size == 4, "%s: elem_size must be 2 or 4", what);
+  HIPO_REQUIRE(token_size == 4 || token_size == 8, "%s: token_size must be 4 or 8", what);
+  HIPO_REQUIRE(rows >= 0 && width >= 0 && vocab >= 0, "%s: negative size", what);
+  HIPO_REQUIRE(width >= 1 && width <= (1 << 20), "%s: width must be from 1 to 2^20", what);
+  HIPO_REQUIRE(vocab >= 1, "%s: empty vocabulary", what);
+  HIPO_REQUIRE(hidden_ld >= width && weight_ld >= width, "%s: row_stride below width", what);
+  HIPO_REQUIRE(sizes_fit(rows, width, vocab, hidden_ld, weight_ld),
+               "%s: at most 2^22 - 256 rows, a vocabulary of 2^31 - 65536, a weight_row_stride of "
+               "2^21 and rows * width of 2^38", what);
+  HIPO_REQUIRE(scale >= 0x1p-100f && scale <= 0x1p100f,
+               "%s: scale must be from 2^-100 to 2^100", what);
+  return 0;
+}
+
+template <typename T>
+int pack(const char* what, Pack a, int64_t rows, bool transposed, hipStream_t stream) {
+  if (transposed) {
+    const int64_t tiles = ((rows + 63) / 64) * ((a.cols + 63) / 64);
+    pack_transposed<T><<<static_cast<uint32_t>(std::min<int64_t>(tiles, 1 << 16)), 256, 0,
+                         stream>>>(a);
+  } else {
+    pack_rows<T><<<static_cast<uint32_t>(std::min<int64_t>(rows, 1 << 16)), 256, 0, stream>>>(a);
+  }
+  return check_launch(what);
+}
+
+template <typename T, Epilogue E>
+int multiply(const char* what, const Product& p, int64_t rows_b, hipStream_t stream,
+             int splits = 1) {
+  const int64_t tiles = ((p.a_rows + kTile - 1) / kTile) * ((rows_b + kTile - 1) / kTile);
+  gemm<T, E><<<dim3(static_cast<uint32_t>(tiles), splits), kThreads, 0, stream>>>(p);
+  return check_launch(what);
+}
+
+struct Call {
+  const void *hidden, *weight, *tokens;
+  int token_size;
+  int64_t rows, width, vocab, hidden_ld, weight_ld;
+  float scale;
+  int64_t ignore_index;
+  char* ws;
+  hipStream_t stream;
+
+  template <typename P>
+  P* at(size_t offset) const {
+    return reinterpret_cast<P*>(ws + offset);
+  }
+};
+
+#define HIPO_STEP(call)              \
+  do {                               \
+    const int step_rc = (call);      \
+    if (step_rc != 0) return step_rc; \
+  } while (0)
+
+// The operands of a piece's logits: the vocabulary's rows from `first` on.
+template <typename T>
+int piece_of_weight(const char* what, const Call& c, const Plan& plan, int64_t first, Product* g) {
+  g->a_rows = static_cast<int>(std::min(plan.piece, c.vocab - first));
+  const T* from = static_cast<const T*>(c.weight) + first * c.weight_ld;
+  if (plan.direct) {
+    g->a = reinterpret_cast<const uint16_t*>(from);
+    g->lda = c.weight_ld;
+    g->k = static_cast<int>(c.width);
+  } else {
+    uint16_t* to = c.at<uint16_t>(plan.weight);
+    g->a = to;
+    g->lda = plan.k_pad;
+    g->a_plane = plan.piece * plan.k_pad;
+    g->k = static_cast<int>(plan.k_pad);
+    HIPO_STEP(pack<T>(what, Pack{from, c.weight_ld, nullptr, nullptr, g->a_rows,
+                                 static_cast<int>(c.width), to, plan.k_pad, g->a_plane},
+                      g->a_rows, false, c.stream));
+  }
+  g->first = first;
+  return 0;
+}
+
+template <typename T>
+int select_and_pack(const char* what, const Call& c, const Plan& plan, float* loss, float* lse,
+                    Product* g) {
+  int* kept = c.at<int>(plan.kept);
+  int* count = c.at<int>(plan.count);
+  float* target = loss ? c.at<float>(plan.target) : nullptr;
+  select_rows<<<1, 1024, 0, c.stream>>>(
+      Select{c.tokens, c.token_size, c.rows, c.ignore_index, kept, count, target, loss, lse});
+  HIPO_STEP(check_launch(what));
+  uint16_t* hidden = c.at<uint16_t>(plan.hidden);
+  const int64_t plane = plan.rows_pad * plan.k_pad;
+  HIPO_STEP(pack<T>(what, Pack{c.hidden, c.hidden_ld, kept, count, c.rows,
+                               static_cast<int>(c.width), hidden, plan.k_pad, plane},
+                    c.rows, false, c.stream));
+  g->b = hidden;
+  g->ldb = plan.k_pad;
+  g->b_plane = plane;
+  g->b_count = count;
+  g->tokens = c.tokens;
+  g->token_size = c.token_size;
+  g->kept = kept;
+  g->scale = c.scale;
+  g->vocab = c.vocab;
+  g->target = target;
+  return 0;
+}
+
+template <typename T>
+int run_fwd(const Call& c, const Plan& plan, float* loss, float* lse) {
+  const char* what = "linear_cross_entropy";
+  Product g{};
+  HIPO_STEP(select_and_pack<T>(what, c, plan, loss, lse, &g));
+  g.part = c.at<float2>(plan.part);
+  g.part_ld = plan.rows_pad;
+  for (int64_t i = 0; i < plan.pieces; ++i) {
+    HIPO_STEP(piece_of_weight<T>(what, c, plan, i * plan.piece, &g));
+    g.first_tile = i * plan.piece / kTile;
+    HIPO_STEP((multiply<T, kReduce>(what, g, c.rows, c.stream)));
+  }
+  join_loss<<<static_cast<uint32_t>(std::min<int64_t>((c.rows + 63) / 64, 1 << 16)), 256, 0,
+              c.stream>>>(JoinLoss{g.part, g.part_ld, static_cast<int>(up(c.vocab, kTile) / kTile),
+                                   g.kept, g.b_count, g.target, loss, lse});
+  return check_launch(what);
+}
+
+template <typename T>
+int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse,
+            const float* grad_lse, void* dhidden, void* dweight) {
+  const char* what = "linear_cross_entropy_bwd";
+  Product g{};
+  HIPO_STEP(select_and_pack<T>(what, c, plan, nullptr, nullptr, &g));
+  const int width = static_cast<int>(c.width);
+  uint16_t* hidden_t = c.at<uint16_t>(plan.hidden_t);
+  uint16_t* weight_t = c.at<uint16_t>(plan.weight_t);
+  const int64_t hidden_t_plane = c.width * plan.rows_pad, weight_t_plane = c.width * plan.piece;
+  HIPO_STEP(pack<T>(what, Pack{c.hidden, c.hidden_ld, g.kept, g.b_count, c.rows, width, hidden_t,
+                               plan.rows_pad, hidden_t_plane},
+                    c.rows, true, c.stream));
+  zero_rows<T><<<static_cast<uint32_t>(std::min<int64_t>(c.rows, 1 << 16)), 256, 0, c.stream>>>(
+      c.tokens, c.token_size, c.ignore_index, static_cast<T*>(dhidden), c.rows, width);
+  HIPO_STEP(check_launch(what));
+  g.grad = grad;
+  g.lse = lse;
+  g.grad_lse = grad_lse;
+  g.d = c.at<uint16_t>(plan.d);
+  g.d_ld = plan.piece;
+  g.d_plane = plan.rows_pad * plan.piece;
+  g.dt = c.at<uint16_t>(plan.dt);
+  g.dt_ld = plan.rows_pad;
+  g.dt_plane = plan.piece * plan.rows_pad;
+  for (int64_t i = 0; i < plan.pieces; ++i) {
+    const int64_t first = i * plan.piece;
+    HIPO_STEP(piece_of_weight<T>(what, c, plan, first, &g));
+    HIPO_STEP((multiply<T, kLogitGrad>(what, g, c.rows, c.stream)));
+
+    HIPO_STEP(pack<T>(what, Pack{static_cast<const T*>(c.weight) + first * c.weight_ld,
+                                 c.weight_ld, nullptr, nullptr, g.a_rows, width, weight_t,
+                                 plan.piece, weight_t_plane},
+                      g.a_rows, true, c.stream));
+    Product h{};
+    h.a = weight_t;
+    h.lda = plan.piece;
+    h.a_plane = weight_t_plane;
+    h.a_rows = width;
+    h.b = g.d;
+    h.ldb = g.d_ld;
+    h.b_plane = g.d_plane;
+    h.b_count = g.b_count;
+    h.k = static_cast<int>(up(g.a_rows, kStep));
+    h.kept = g.kept;
+    h.sum = c.at<float>(plan.sum);
+    h.sum_ld = up(c.width, 4);
+    h.sum_plane = plan.rows_pad * h.sum_ld;
+    h.load_sum = i > 0;
+    h.to_out = plan.splits == 1 && i + 1 == plan.pieces;
+    h.out = dhidden;
+    h.out_ld = c.width;
+    HIPO_STEP((multiply<T, kAccumulate>(what, h, c.rows, c.stream, plan.splits)));
+
+    Product w{};
+    w.a = hidden_t;
+    w.lda = plan.rows_pad;
+    w.a_plane = hidden_t_plane;
+    w.a_rows = width;
+    w.b = g.dt;
+    w.ldb = g.dt_ld;
+    w.b_plane = g.dt_plane;
+    w.b_rows = g.a_rows;
+    w.k_count = g.b_count;
+    w.out = static_cast<T*>(dweight) + first * c.width;
+    w.out_ld = c.width;
+    HIPO_STEP((multiply<T, kStore>(what, w, g.a_rows, c.stream)));
+  }
+  if (plan.splits > 1) {
+    const int64_t blocks = (c.rows * ((c.width + 3) / 4) + 255) / 256;
+    join_hidden<T><<<static_cast<uint32_t>(std::min<int64_t>(blocks, 1 << 16)), 256, 0,
+                     c.stream>>>(c.at<float>(plan.sum), up(c.width, 4),
+                                 plan.rows_pad * up(c.width, 4), plan.splits, g.kept, g.b_count,
+                                 static_cast<T*>(dhidden), width);
+    return check_launch(what);
+  }
+  return 0;
+}
+
+}  // namespace
+}  // namespace hipo
+
+extern "C" size_t hipo_linear_cross_entropy_workspace_bytes(const void* weight, int elem_size,
+                                                            int64_t rows, int64_t width,
+                                                            int64_t vocab,
+                                                            int64_t weight_row_stride) {
+  if ((elem_size != 2 && elem_size != 4) || rows == 0 ||
+      !hipo::sizes_fit(rows, width, vocab, width, weight_row_stride)) {
+    return 0;
+  }
+  return hipo::plan_of(weight, elem_size, rows, width, vocab, weight_row_stride, false).bytes;
+}
+
+extern "C" int hipo_linear_cross_entropy(const void* hidden, const void* weight, int elem_size,
+                                         const void* tokens, int token_size, float* loss,
+                                         float* lse, int64_t rows, int64_t width, int64_t vocab,
+                                         int64_t hidden_row_stride, int64_t weight_row_stride,
+                                         float scale, int64_t ignore_index, void* workspace,
+                                         size_t workspace_bytes, hipStream_t stream) {
+  using namespace hipo;
+  clear_error();
+  const char* what = "linear_cross_entropy";
+  HIPO_STEP(check_operands(what, elem_size, token_size, rows, width, vocab, hidden_row_stride,
+                           weight_row_stride, scale));
+  if (rows == 0) return 0;
+  HIPO_REQUIRE(hidden && weight && tokens && loss && lse, "%s: null pointer", what);
+  const Plan plan = plan_of(weight, elem_size, rows, width, vocab, weight_row_stride, false);
+  HIPO_REQUIRE(workspace && workspace_bytes >= plan.bytes && aligned16(workspace),
+               "%s: workspace of %zu bytes, 16-byte aligned, needed", what, plan.bytes);
+  const Call c{hidden, weight, tokens, token_size, rows, width, vocab, hidden_row_stride,
+               weight_row_stride, scale, ignore_index, static_cast<char*>(workspace), stream};
+  return elem_size == 2 ? run_fwd<uint16_t>(c, plan, loss, lse)
+                        : run_fwd<float>(c, plan, loss, lse);
+}
+
+extern "C" size_t hipo_linear_cross_entropy_bwd_workspace_bytes(const void* weight, int elem_size,
+                                                                int64_t rows, int64_t width,
+                                                                int64_t vocab,
+                                                                int64_t weight_row_stride) {
+  if ((elem_size != 2 && elem_size != 4) || rows == 0 ||
+      !hipo::sizes_fit(rows, width, vocab, width, weight_row_stride)) {
+    return 0;
+  }
+  return hipo::plan_of(weight, elem_size, rows, width, vocab, weight_row_stride, true).bytes;
+}
+
+extern "C" int hipo_linear_cross_entropy_bwd(const float* grad, const void* hidden,
+                                             const void* weight, int elem_size,
+                                             const void* tokens, int token_size, const float* lse,
+                                             const float* grad_lse, void* dhidden, void* dweight,
+                                             int64_t rows, int64_t width, int64_t vocab,
+                                             int64_t hidden_row_stride, int64_t weight_row_stride,
+                                             float scale, int64_t ignore_index, void* workspace,
+                                             size_t workspace_bytes, hipStream_t stream) {
+  using namespace hipo;
+  clear_error();
+  const char* what = "linear_cross_entropy_bwd";
+  HIPO_STEP(check_operands(what, elem_size, token_size, rows, width, vocab, hidden_row_stride,
+                           weight_row_stride, scale));
+  if (rows == 0) return 0;
+  HIPO_REQUIRE(grad && hidden && weight && tokens && lse && dhidden && dweight,
+               "%s: null pointer", what);
+  const Plan plan = plan_of(weight, elem_size, rows, width, vocab, weight_row_stride, true);
+  HIPO_REQUIRE(workspace && workspace_bytes >= plan.bytes && aligned16(workspace),
+               "%s: workspace of %zu bytes, 16-byte aligned, needed", what, plan.bytes);
+  const Call c{hidden, weight, tokens, token_size, rows, width, vocab, hidden_row_stride,
+               weight_row_stride, scale, ignore_index, static_cast<char*>(workspace), stream};
+  return elem_size == 2
+             ? run_bwd<uint16_t>(c, plan, grad, lse, grad_lse, dhidden, dweight)
+             : run_bwd<float>(c, plan, grad, lse, grad_lse, dhidden, dweight);
+}

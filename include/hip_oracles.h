@@ -540,6 +540,120 @@ int hipo_embedding_bwd(const void* grad, int elem_size, const void* tokens,
                        int64_t padding_idx, int accumulate, void* workspace,
                        size_t workspace_bytes, hipStream_t stream);
 
+/*
+ * The norms around a block of a residual network, fused with its gate and the
+ * residual sum.  With norm(v; w, b) = (v - m) r (offset + w) + b, r = 1 /
+ * sqrt(mean((v - m)^2) + eps), m the row's mean (layer = 1, LayerNorm) or 0
+ * (layer = 0, RMSNorm, without biases):
+ *   n = post ? norm(x; post, post_bias) : x
+ *   h = residual + scale * gate * n        (one rounding to the tensors' type)
+ *   y = norm(h; pre, pre_bias)             (of h as it is stored; pre only)
+ *   stats[r] = (mean, r) of x, then of h   (0 and 1 where there is no norm)
+ * in fp32.  x, residual, h, y are [rows, cols] contiguous of bf16 (elem_size
+ * 2) or fp32 (4), the vectors [cols] of the same type, all at any element
+ * alignment; cols is from 8 to 16384.  gate is [gate_rows, cols], row r taking
+ * gate row r / (rows / gate_rows): 1 for a vector that all rows share, rows
+ * for a gate per value, between them one per sample (gate_rows divides rows);
+ * NULL with gate_rows 0 for none.  One of post and pre may be NULL, and so may
+ * the biases; y is NULL where pre is.  The outputs overlap no operand.
+ * No counterpart among the reference's oracles; beside
+ * hipo_residual_layernorm_bf16 and hipo_rmsnorm_ex_bf16, which have the second
+ * norm alone.
+ */
+int hipo_block_norms(const void* x, const void* residual, int elem_size,
+                     const void* post, const void* post_bias, const void* pre,
+                     const void* pre_bias, const void* gate, void* h, void* y,
+                     float* stats, int64_t rows, int64_t cols, int64_t gate_rows,
+                     float scale, float offset, float eps, int layer,
+                     hipStream_t stream);
+
+/*
+ * Gradient of hipo_block_norms for grad_h and grad_y, the gradients of h and y
+ * (grad_h may be NULL where pre is not, grad_y is NULL where pre is): with T the
+ * gradient of h from both,
+ *   dresidual = T,  dgate = scale sum(T n) over the rows of each gate row,
+ *   dx, dpost, dpost_bias from scale * gate * T, dpre, dpre_bias from grad_y
+ * of x, h and stats as the forward left them.  fp32 sums in an order that the
+ * sizes and the GPU fix (the same call gives the same bits), one rounding to
+ * the tensors' type.  Sizes and types as in hipo_block_norms; x may be NULL
+ * without post and gate, h without pre; each operand's gradient is given where
+ * the operand is (dpost_bias with post_bias, ...).  The outputs overlap neither
+ * each other nor an operand; with rows == 0 nothing is written.  `workspace`:
+ * at least hipo_block_norms_bwd_workspace_bytes bytes, 16-byte aligned, no
+ * initialisation needed; calls that share one must be ordered.
+ * No counterpart among the reference's oracles.
+ */
+size_t hipo_block_norms_bwd_workspace_bytes(int64_t rows, int64_t cols);
+int hipo_block_norms_bwd(const void* grad_h, const void* grad_y, const void* x,
+                         const void* h, const float* stats, int elem_size,
+                         const void* post, const void* post_bias, const void* pre,
+                         const void* pre_bias, const void* gate, void* dx,
+                         void* dresidual, void* dgate, void* dpost,
+                         void* dpost_bias, void* dpre, void* dpre_bias,
+                         int64_t rows, int64_t cols, int64_t gate_rows, float scale,
+                         float offset, int layer, void* workspace,
+                         size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Softmax cross entropy of the output layer without its logits: with
+ * s_j = scale * sum_k hidden[r, k] weight[j, k],
+ *   lse[r]  = ln sum_j e^(s_j)
+ *   loss[r] = lse[r] - s_t,  t = tokens[r]
+ * in fp32 sums of exact products (fp32 operands: of three bf16 parts each,
+ * products below 2^-24 of the largest left out).  hidden is [rows, width],
+ * weight [vocab, width], with row strides of their own (>= width), both of bf16
+ * (elem_size 2) or fp32 (4), at any element alignment; tokens is [rows] of
+ * int32 (token_size 4) or int64 (8); loss and lse are [rows]; scale is from
+ * 2^-100 to 2^100.  A row whose token is ignore_index is left out, whatever it
+ * holds: 0 and 0.  A token outside [0, vocab) otherwise has loss NaN.  A row
+ * with a NaN logit has lse NaN.  weight that is bf16, 16-byte aligned and whose
+ * row stride is a multiple of 8 is read where it lies; other weights are copied
+ * into the workspace piece by piece.  `workspace`: at least
+ * hipo_linear_cross_entropy_workspace_bytes bytes (weight is looked at for its
+ * alignment only), 16-byte aligned, no initialisation needed; calls that share
+ * one must be ordered.
+ * No counterpart among the reference's oracles; hipo_token_logprobs for logits
+ * that are never in memory.
+ */
+size_t hipo_linear_cross_entropy_workspace_bytes(const void* weight, int elem_size,
+                                                 int64_t rows, int64_t width,
+                                                 int64_t vocab, int64_t weight_row_stride);
+int hipo_linear_cross_entropy(const void* hidden, const void* weight, int elem_size,
+                              const void* tokens, int token_size, float* loss,
+                              float* lse, int64_t rows, int64_t width, int64_t vocab,
+                              int64_t hidden_row_stride, int64_t weight_row_stride,
+                              float scale, int64_t ignore_index, void* workspace,
+                              size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Gradients of hipo_linear_cross_entropy for grad, the gradient of loss, and
+ * grad_lse, of lse (fp32 [rows]; grad_lse may be NULL), lse being the forward's:
+ *   d[r, j]  = scale * ((grad + grad_lse) e^(s_j - lse) - grad [j = t])
+ *   dhidden  = d weight,  dweight = d^T hidden
+ * the logits computed once more in pieces of the vocabulary, the products
+ * accumulated in fp32 and rounded once to the operands' type; d itself is
+ * rounded to bf16 where the operands are bf16 (the matrix cores' type).
+ * dhidden is contiguous [rows, width], dweight [vocab, width]; they overlap
+ * neither each other nor an operand.  Rows of ignore_index are zero in dhidden
+ * and add nothing to dweight, whatever they hold; a row of another token outside
+ * [0, vocab) is NaN and makes dweight NaN.  Operands and workspace as above.
+ * No counterpart among the reference's oracles.
+ */
+size_t hipo_linear_cross_entropy_bwd_workspace_bytes(const void* weight, int elem_size,
+                                                     int64_t rows, int64_t width,
+                                                     int64_t vocab,
+                                                     int64_t weight_row_stride);
+int hipo_linear_cross_entropy_bwd(const float* grad, const void* hidden,
+                                  const void* weight, int elem_size,
+                                  const void* tokens, int token_size,
+                                  const float* lse, const float* grad_lse,
+                                  void* dhidden, void* dweight, int64_t rows,
+                                  int64_t width, int64_t vocab,
+                                  int64_t hidden_row_stride,
+                                  int64_t weight_row_stride, float scale,
+                                  int64_t ignore_index, void* workspace,
+                                  size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

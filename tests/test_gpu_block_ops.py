@@ -1,0 +1,542 @@
+"""The norms around a block and the output layer's cross entropy on the GPU
+against the 64-bit reference, at the sizes, types and options where they could
+go wrong; refusals; streams, graphs and a run of all of them together."""
+import pytest
+import torch
+
+import block_ops_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+NAN, INF, IGNORE = ref.NAN, ref.INF, ref.IGNORE
+DTYPES = [BF16, F32]
+
+
+@pytest.fixture(scope="module")
+def ho():
+    import hip_oracles
+    hip_oracles.load_library()
+    return hip_oracles
+
+
+def shifted(t, shift):
+    """t at `shift` values past an allocation's start, with NaN around it."""
+    if t is None or not shift:
+        return t
+    buf = torch.full((t.numel() + 2 * shift,), NAN, dtype=t.dtype, device=t.device)
+    view = buf[shift:shift + t.numel()].view(t.shape)
+    view.copy_(t)
+    return view
+
+
+# ---------------------------------------------------------------------------
+# Norms
+# ---------------------------------------------------------------------------
+
+def norm_operands(dev, rows, cols, dtype, *, norm, post=True, pre=True, gates=0, seed=0, shift=0,
+                  scale=0.5, offset=1.0, bias=None):
+    g = torch.Generator(device=dev).manual_seed(seed)
+
+    def make(*shape, mean=0.0, std=1.0):
+        t = (mean + std * torch.randn(*shape, generator=g, device=dev)).to(dtype)
+        return shifted(t, shift)
+
+    rowsof = dict(x=make(rows, cols, mean=0.3), residual=make(rows, cols, mean=-1.0, std=3.0))
+    kw = dict(norm=norm, scale=scale, offset=offset)
+    for name, there in (("post", post), ("pre", pre)):
+        if there:
+            kw[name] = make(cols, std=0.3)
+            if norm == "layer" if bias is None else bias:
+                kw[name + "_bias"] = make(cols, std=0.3)
+    if gates:
+        kw["gate"] = make(gates, cols, std=0.7)
+        if gates == 1:
+            kw["gate"] = kw["gate"][0]
+    grads = dict(grad_h=make(rows, cols), grad_y=make(rows, cols) if pre else None)
+    return rowsof, kw, grads
+
+
+def check_norms(ho, rowsof, kw, grads, what, eps=1e-6):
+    h, y, stats = ho.block_norms(**rowsof, **kw, eps=eps)
+    want_h, tol_h, stats0, tol0 = ref.stream(**rowsof, **kw, eps=eps)
+    c = lambda t: t.cpu()  # noqa: E731
+    ref.close(h, c(want_h), c(tol_h), f"{what} h")
+    ref.close(stats[:, :2], c(stats0), c(tol0), f"{what} statistics of x")
+    if "pre" in kw:
+        want_y, tol_y, stats1, tol1 = ref.after(h, **kw, eps=eps)
+        ref.close(y, c(want_y), c(tol_y), f"{what} y")
+        ref.close(stats[:, 2:], c(stats1), c(tol1), f"{what} statistics of h")
+    else:
+        assert y is None
+    args = (grads["grad_h"], grads["grad_y"], rowsof["x"], h if "pre" in kw else None, stats)
+    got = ho.block_norms_bwd(*args, **kw)
+    want = ref.block_norms_bwd(*args, **kw)
+    names = ("dx", "dresidual", "dgate", "dpost", "dpost_bias", "dpre", "dpre_bias")
+    for name, u, v in zip(names, got, want):
+        if v is None:
+            assert u is None, name
+            continue
+        assert u.dtype == rowsof["x"].dtype
+        ref.close(u, c(v[0]), c(v[1]), f"{what} {name}")
+    return (h, y, stats), got
+
+
+SIZES = [(1, 8), (1, 9), (3, 15), (65, 16), (7, 64), (300, 100), (33, 504), (40, 511), (1000, 512),
+         (40, 513), (7, 520), (2, 1001), (515, 1024), (17, 1025), (20, 2880), (9, 4096), (5, 5000),
+         (3, 8192), (3, 8193), (2, 16383), (6, 16384)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("rows,cols", SIZES)
+def test_norms_sizes(rows, cols, norm, dtype, rocm_device, ho):
+    for k, (post, pre, gates, shift) in enumerate(
+            ((True, True, 0, 0), (True, False, 1, 1), (False, True, rows, 3), (True, True, 1, 0))):
+        case = norm_operands(rocm_device, rows, cols, dtype, norm=norm, post=post, pre=pre,
+                             gates=gates, shift=shift, seed=k)
+        if k == 3 and pre:
+            case[2]["grad_h"] = None
+        check_norms(ho, *case, f"[{rows}, {cols}] {dtype} {norm} {k}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [64, 700, 2880])
+@pytest.mark.parametrize("rows,gates", [(6, 2), (6, 3), (4096, 2), (4096, 3), (4096, 7), (4096, 16),
+                                        (4096, 64), (4096, 512), (4096, 1024), (4096, 4096),
+                                        (2050, 41), (8190, 30)])
+def test_gates_of_samples(rows, gates, cols, dtype, rocm_device, ho):
+    """Rows of a gate within a workgroup, over several, and both at once."""
+    rows = rows // gates * gates
+    for norm, post in (("layer", True), ("rms", False)):
+        case = norm_operands(rocm_device, rows, cols, dtype, norm=norm, post=post, gates=gates,
+                             scale=1.0, offset=0.0)
+        check_norms(ho, *case, f"[{rows}, {cols}] {gates} gates {dtype} {norm}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("rows,cols", [(30011, 64), (9001, 1001), (8192, 2048), (700, 8192)])
+def test_norms_of_many_rows(rows, cols, norm, dtype, rocm_device, ho):
+    """The same bits again, biases left out, and rows that are the same in
+    another batch."""
+    for gates in (0, 1):
+        case = norm_operands(rocm_device, rows, cols, dtype, norm=norm, gates=gates,
+                             bias=gates == 0 and norm == "layer")
+        first, grads = check_norms(ho, *case, f"[{rows}, {cols}] {dtype} {norm} {gates}")
+        again = ho.block_norms(**case[0], **case[1])
+        some = slice(rows // 3, rows // 2)
+        part = ho.block_norms(*(v[some].contiguous() for v in case[0].values()), **case[1])
+        for a, b, p in zip(first, again, part):
+            assert torch.equal(a, b) and torch.equal(a[some], p)
+        args = (case[2]["grad_h"], case[2]["grad_y"], case[0]["x"], first[0], first[2])
+        for a, b in zip(grads, ho.block_norms_bwd(*args, **case[1])):
+            assert (a is None and b is None) or torch.equal(a, b)
+        part = ho.block_norms_bwd(*(v[some].contiguous() for v in args), **case[1])
+        assert torch.equal(part[0], grads[0][some]) and torch.equal(part[1], grads[1][some])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [40, 1100])
+def test_norms_of_special_rows(cols, dtype, rocm_device, ho):
+    """Zero and constant rows, NaN, infinities: in their own rows only."""
+    rows = 12
+    for norm in ("rms", "layer"):
+        rowsof, kw, grads = norm_operands(rocm_device, rows, cols, dtype, norm=norm, gates=rows)
+        x, r = rowsof["x"], rowsof["residual"]
+        clean = ho.block_norms(x, r, **kw)
+        x[1] = 0.0
+        x[2] = 1.5
+        r[3] = 0.0
+        x[3] = 0.0
+        x[4, cols // 2] = NAN
+        r[5, 0] = NAN
+        x[6, cols - 1] = INF
+        r[7, cols // 3] = -INF
+        h, y, stats = ho.block_norms(x, r, **kw)
+        for k in (0, 8, 9, 10, 11):
+            assert torch.equal(h[k], clean[0][k]) and torch.equal(y[k], clean[1][k])
+        assert torch.isfinite(y[[1, 2, 3]]).all()
+        assert h[4].isnan().all() and y[4].isnan().all()
+        assert h[5].isnan().sum() == 1 and y[5].isnan().all()
+        assert y[6].isnan().all() and y[7].isnan().any()
+        fine = [0, 1, 2, 3, 8, 9, 10, 11]
+        part = {k: v[fine].contiguous() for k, v in rowsof.items()}
+        kwp = {**kw, "gate": kw["gate"][fine].contiguous()}
+        check_norms(ho, part, kwp, {k: v[fine].contiguous() for k, v in grads.items()},
+                    f"{cols} {dtype} {norm}")
+        got = ho.block_norms_bwd(grads["grad_h"], grads["grad_y"], x, h, stats, **kw)
+        want = ho.block_norms_bwd(*(v[fine].contiguous() for v in (
+            grads["grad_h"], grads["grad_y"], x, h, stats)), **kwp)
+        for k in range(3):  # rows of their own
+            assert torch.equal(got[k][fine], want[k])
+        assert got[0][4].isnan().all() and got[3].isnan().any()
+
+
+def test_norms_beside_those_of_the_library(rocm_device, ho):
+    """Without a norm before the sum, a gate or a scale: residual_layernorm and
+    rmsnorm_ex."""
+    g = torch.Generator(device=rocm_device).manual_seed(1)
+    x, r = (torch.randn(70, 1024, generator=g, device=rocm_device).to(BF16) for _ in range(2))
+    w, b = (torch.randn(1024, generator=g, device=rocm_device).to(BF16) for _ in range(2))
+    h, y, _ = ho.block_norms(x, r, pre=w, pre_bias=b, norm="layer", eps=1e-5)
+    h2, y2, _, _ = ho.residual_layernorm(x, r, w, b, 1e-5)
+    assert torch.equal(h, h2)
+    torch.testing.assert_close(y.float(), y2.float(), rtol=2.0 ** -7, atol=1e-5)
+    h, y, _ = ho.block_norms(x, r, pre=w, eps=1e-5)
+    h2, y2 = ho.rmsnorm_ex(x, w, 1e-5, residual=r, want_h=True)
+    assert torch.equal(h, h2)
+    torch.testing.assert_close(y.float(), y2.float(), rtol=2.0 ** -7, atol=1e-6)
+
+
+def test_norms_without_rows(rocm_device, ho):
+    x = torch.zeros(0, 64, device=rocm_device)
+    w = torch.ones(64, device=rocm_device)
+    h, y, stats = ho.block_norms(x, x, post=w, pre=w, gate=w)
+    assert h.shape == y.shape == (0, 64) and stats.shape == (0, 4)
+    out = ho.block_norms_bwd(x, x, x, h, stats, post=w, pre=w, gate=w)
+    assert out[0].shape == out[1].shape == (0, 64)
+    assert all(not t.any() for t in (out[2], out[3], out[5]))
+
+
+def test_norms_refuse(rocm_device, ho):
+    z = lambda *s, t=BF16: torch.zeros(*s, dtype=t, device=rocm_device)  # noqa: E731
+    x, w, st = z(4, 16), z(16), z(4, 4, t=F32)
+    for call, msg in [
+            (lambda: ho.block_norms(x, x), "norm is needed"),
+            (lambda: ho.block_norms(x.half(), x.half(), pre=w.half()), "bf16 or fp32"),
+            (lambda: ho.block_norms(x, x.float(), pre=w), "one type"),
+            (lambda: ho.block_norms(x, z(4, 8), pre=w), "contiguous"),
+            (lambda: ho.block_norms(z(16, 4).t(), x, pre=w), "contiguous"),
+            (lambda: ho.block_norms(x, x, pre=w.float()), "rows' type"),
+            (lambda: ho.block_norms(x, x, pre=z(32)[::2]), "contiguous"),
+            (lambda: ho.block_norms(x, x, pre=w, gate=z(3, 16)), "divide"),
+            (lambda: ho.block_norms(x, x, pre=w, gate=z(4, 8)), "gate"),
+            (lambda: ho.block_norms(x, x, pre=w, norm="batch"), "norm must be"),
+            (lambda: ho.block_norms_bwd(x, None, x, x, st, pre=w), "go together"),
+            (lambda: ho.block_norms_bwd(x, x, x, None, st, pre=w), "go together"),
+            (lambda: ho.block_norms_bwd(x, x, x, x, st, post=w), "go together"),
+            (lambda: ho.block_norms_bwd(None, None, x, None, st, post=w), "no gradient"),
+            (lambda: ho.block_norms_bwd(x, x, x, x, z(4, 2, t=F32), pre=w), "stats"),
+            (lambda: ho.block_norms_bwd(x, x, x, x, st.double(), pre=w), "stats")]:
+        with pytest.raises((ValueError, RuntimeError), match=msg):
+            call()
+    for kw, msg in [(dict(pre=w, pre_bias=w), "LayerNorm"), (dict(pre=w, scale=INF), "finite"),
+                    (dict(pre=w, eps=-1.0), "eps")]:
+        with pytest.raises(RuntimeError, match=msg):
+            ho.block_norms(x, x, **kw)
+    with pytest.raises(RuntimeError, match="cols"):
+        ho.block_norms(z(4, 7), z(4, 7), pre=z(7))
+    with pytest.raises(RuntimeError, match="cols"):
+        ho.block_norms(z(1, 16385), z(1, 16385), pre=z(16385))
+
+
+# ---------------------------------------------------------------------------
+# Cross entropy
+# ---------------------------------------------------------------------------
+
+def layer_operands(dev, rows, width, vocab, dtype, *, seed=0, pads=(0, 0), shift=0, std=2.5):
+    g = torch.Generator(device=dev).manual_seed(seed)
+
+    def make(n, pad, scale):
+        t = torch.full((n * (width + pad) + shift,), NAN, dtype=dtype, device=dev)
+        t = t[shift:].view(n, width + pad)[:, :width]
+        t.copy_((torch.randn(n, width, generator=g, device=dev) * scale).to(dtype))
+        return t
+
+    hidden, weight = make(rows, pads[0], 1.0), make(vocab, pads[1], std / width ** 0.5)
+    tokens = torch.randint(0, vocab, (rows,), generator=g, device=dev)
+    grads = torch.randn(2, rows, generator=g, device=dev)
+    return hidden, weight, tokens, grads
+
+
+def check_loss(ho, hidden, weight, tokens, grads, what, scale=1.0, wide=True):
+    t = tokens if wide else tokens.to(torch.int32)
+    got = ho.linear_cross_entropy(hidden, weight, t, scale=scale)
+    want = ref.linear_cross_entropy(hidden, weight, tokens, scale)
+    for name, u, (v, tol) in zip(("loss", "lse"), got, want):
+        ref.close(u, v, tol, f"{what} {name}")
+    lse = got[1]
+    for gl in (None, grads[1]):
+        out = ho.linear_cross_entropy_bwd(grads[0], hidden, weight, t, lse, scale=scale,
+                                          grad_lse=gl)
+        wanted = ref.linear_cross_entropy_bwd(grads[0], hidden, weight, tokens, lse, scale,
+                                              grad_lse=gl)
+        for name, u, (v, tol) in zip(("dhidden", "dweight"), out, wanted):
+            assert u.dtype == hidden.dtype and u.is_contiguous()
+            ref.close(u, v, tol, f"{what} {name}")
+    return got, out
+
+
+LAYERS = [(1, 1, 1), (1, 8, 2), (2, 3, 5), (1, 64, 255), (3, 72, 256), (16, 64, 257), (17, 128, 1000),
+          (5, 1001, 3001), (33, 200, 700), (64, 96, 2000), (65, 512, 513), (100, 65, 4097),
+          (129, 64, 1023), (256, 128, 512), (257, 64, 513), (300, 320, 1500), (515, 777, 1030),
+          (1000, 40, 300)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,width,vocab", LAYERS)
+def test_cross_entropy_sizes(rows, width, vocab, dtype, rocm_device, ho):
+    for k, (pads, shift, scale) in enumerate((((0, 0), 0, 1.0), ((8, 16), 0, 0.7),
+                                              ((3, 5), 1, 1.25))):
+        case = layer_operands(rocm_device, rows, width, vocab, dtype, pads=pads, shift=shift,
+                              seed=k)
+        check_loss(ho, *case, f"[{rows}, {width}, {vocab}] {dtype} {k}", scale, wide=k != 1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 2, 20, 70, 300, 1030])
+@pytest.mark.parametrize("kind", ["some", "all", "but one", "first", "last", "unknown"])
+def test_cross_entropy_of_rows_left_out(kind, rows, dtype, rocm_device, ho):
+    """Rows of ignore_index count nowhere, whatever they hold."""
+    hidden, weight, tokens, grads = layer_operands(rocm_device, rows, 72, 600, dtype)
+    out = torch.zeros(rows, dtype=torch.bool, device=rocm_device)
+    if kind == "some":
+        out[::3] = True
+    elif kind == "all":
+        out[:] = True
+    elif kind == "but one":
+        out[:] = True
+        out[rows // 2] = False
+    elif kind == "first":
+        out[:rows // 2] = True
+    elif kind == "last":
+        out[rows // 2:] = True
+    tokens[out] = IGNORE
+    hidden[out] = NAN
+    if rows > 2:
+        hidden[out.nonzero()[:1, 0]] = INF
+    if kind == "unknown":
+        tokens[0], tokens[rows // 2] = 600, -1
+    check_loss(ho, hidden, weight, tokens, grads, f"{kind} {rows} {dtype}")
+    if kind in ("some", "first"):
+        other = ho.linear_cross_entropy(hidden, weight, torch.where(out, 5, tokens), ignore_index=5)
+        kept = ~out & (tokens != 5)
+        assert torch.equal(other[0][kept], ho.linear_cross_entropy(hidden, weight, tokens)[0][kept])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,width,vocab", [(3, 4096, 20011), (1, 2048, 32000), (700, 1024, 9001),
+                                              (2100, 256, 33000), (40, 264, 100003)])
+def test_cross_entropy_of_larger_layers(rows, width, vocab, dtype, rocm_device, ho):
+    case = layer_operands(rocm_device, rows, width, vocab, dtype, std=5.0)
+    what = f"[{rows}, {width}, {vocab}] {dtype}"
+    got, out = check_loss(ho, *case, what, 0.7)
+    hidden, weight, tokens, grads = case
+    again = ho.linear_cross_entropy(hidden, weight, tokens, scale=0.7)
+    assert all(torch.equal(a, b) for a, b in zip(got, again)), what
+    again = ho.linear_cross_entropy_bwd(grads[0], hidden, weight, tokens, got[1], scale=0.7,
+                                        grad_lse=grads[1])
+    assert all(torch.equal(a, b) for a, b in zip(out, again)), what
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [3, 400])
+def test_gradients_over_pieces_of_the_vocabulary(rows, dtype, rocm_device, ho):
+    """More of the vocabulary than one piece of the workspace holds."""
+    width, vocab = 64, 1 << 19 if rows == 400 else 1 << 21
+    vocab += 77
+    hidden, weight, tokens, grads = layer_operands(rocm_device, rows, width, vocab, dtype)
+    loss, lse = ho.linear_cross_entropy(hidden, weight, tokens)
+    logits = hidden.double() @ weight.double().t()
+    want = torch.logsumexp(logits, -1)
+    assert float((lse - want).abs().max()) < 1e-5  # lse below 32: 4 steps of 2^-19
+    dh, dw = ho.linear_cross_entropy_bwd(grads[0], hidden, weight, tokens, lse)
+    # The bound of the sum over the vocabulary is wide; in the mean its roundings
+    # cancel.  A wrong piece shows in the norm of what it holds.
+    d = torch.exp(logits - lse[:, None].double()) * grads[0][:, None].double()
+    del logits
+    d[torch.arange(rows), tokens] -= grads[0].double()
+    least = 2.0 ** -7 if dtype == BF16 else 2.0 ** -18
+    for got, whole in ((dh, d @ weight.double()), (dw, d.t() @ hidden.double())):
+        assert float((got.double() - whole).norm() / whole.norm()) < least
+    part = dw.double().view(-1)[:width * (vocab // 64 * 64)].view(64, -1).norm(dim=-1)
+    whole = (d.t() @ hidden.double())[:vocab // 64 * 64].reshape(64, -1).norm(dim=-1)
+    assert float(((part - whole) / whole).abs().max()) < least
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [6, 300])
+def test_cross_entropy_of_special_values(rows, dtype, rocm_device, ho):
+    """Rows with NaN and infinities are alone with them; logits far from zero and
+    far apart; weights of rows that are NaN."""
+    hidden, weight, tokens, grads = layer_operands(rocm_device, rows, 64, 700, dtype)
+    clean = ho.linear_cross_entropy(hidden, weight, tokens)
+    bad = hidden.clone()
+    bad[1, 5] = NAN
+    bad[2] = INF
+    got = ho.linear_cross_entropy(bad, weight, tokens)
+    keep = [k for k in range(rows) if k not in (1, 2)]
+    for a, b in zip(clean, got):
+        assert torch.equal(a[keep], b[keep])
+        assert b[1].isnan() and not torch.isfinite(b[2])
+    dh, _ = ho.linear_cross_entropy_bwd(grads[0], bad, weight, tokens, got[1])
+    want, _ = ho.linear_cross_entropy_bwd(grads[0], hidden, weight, tokens, clean[1])
+    assert torch.equal(dh[keep], want[keep]) and dh[1].isnan().all()
+    check_loss(ho, hidden * 40, weight, tokens, grads, f"far apart {rows} {dtype}")
+    one = torch.zeros_like(hidden)
+    one[:, 0] = 1.0
+    up = weight.clone()
+    up[:, 0] += 3e4
+    check_loss(ho, one, up, tokens, grads, f"far from zero {rows} {dtype}")
+    check_loss(ho, torch.zeros_like(hidden), weight, tokens, grads, f"equal {rows} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_losses_of_logits_in_memory(dtype, rocm_device, ho):
+    """token_logprobs of the logits, where they are exact: small whole numbers."""
+    g = torch.Generator(device=rocm_device).manual_seed(4)
+    hidden = torch.randint(-2, 3, (90, 24), generator=g, device=rocm_device).to(dtype)
+    weight = torch.randint(-2, 3, (1500, 24), generator=g, device=rocm_device).to(dtype)
+    t = torch.randint(0, 1500, (90,), generator=g, device=rocm_device)
+    t[::9] = IGNORE
+    logits = (hidden.float() @ weight.float().t()).to(dtype)
+    loss, lse = ho.linear_cross_entropy(hidden, weight, t, scale=0.5)
+    lp, lse2 = ho.token_logprobs(logits, t, scale=0.5)
+    assert float((loss + lp).abs().max()) < 2e-5 and float((lse - lse2).abs().max()) < 2e-5
+
+
+def test_cross_entropy_without_rows(rocm_device, ho):
+    h = torch.zeros(0, 16, device=rocm_device)
+    w, t, f = torch.ones(20, 16, device=rocm_device), torch.zeros(
+        0, dtype=torch.int64, device=rocm_device), torch.zeros(0, device=rocm_device)
+    loss, lse = ho.linear_cross_entropy(h, w, t)
+    assert loss.shape == lse.shape == (0,)
+    dh, dw = ho.linear_cross_entropy_bwd(f, h, w, t, f)
+    assert dh.shape == (0, 16) and dw.shape == (20, 16) and not dw.any()
+
+
+def test_cross_entropy_refuses(rocm_device, ho):
+    z = lambda *s, t=BF16: torch.zeros(*s, dtype=t, device=rocm_device)  # noqa: E731
+    h, w, t, f = z(4, 16), z(9, 16), z(4, t=torch.int64), z(4, t=F32)
+    for call, msg in [
+            (dict(hidden=h.half()), "bf16 or fp32"), (dict(weight=w.float()), "hidden's type"),
+            (dict(weight=z(9, 8)), "hidden's type"), (dict(tokens=f), "tokens"),
+            (dict(tokens=t[:3]), "tokens"), (dict(scale=0.0), "scale"),
+            (dict(scale=NAN), "scale"), (dict(weight=z(0, 16)), "empty"),
+            (dict(hidden=z(16, 4).t()), "inner"), (dict(weight=z(16, 9).t()), "inner"),
+            (dict(hidden=z(1, 16).expand(4, 16)), "overlap"),
+            (dict(weight=z(1, 16).expand(9, 16)), "overlap"), (dict(lse=z(4)), "fp32"),
+            (dict(grad=z(3, t=F32)), "fp32"), (dict(grad_lse=z(8, t=F32)[::2]), "fp32")]:
+        args = {"hidden": h, "weight": w, "tokens": t, **call}
+        with pytest.raises(ValueError, match=msg):
+            ho.linear_cross_entropy_bwd(**{"grad": f, "lse": f, **args})
+        if not {"lse", "grad", "grad_lse"} & set(call):
+            with pytest.raises(ValueError, match=msg):
+                ho.linear_cross_entropy(**args)
+
+
+# ---------------------------------------------------------------------------
+# Together
+# ---------------------------------------------------------------------------
+
+class Model:
+    """Two residual blocks (a product each) between an embedding and the loss,
+    weights tied, and their gradients, all through the library."""
+
+    def __init__(self, ho, dev, rows, width, vocab, dtype, seed=0):
+        g = torch.Generator(device=dev).manual_seed(seed)
+        make = lambda *s, std=1.0: (torch.randn(*s, generator=g, device=dev) * std).to(dtype)  # noqa: E731
+        self.ho, self.rows, self.vocab, self.dtype = ho, rows, vocab, dtype
+        self.table = make(vocab, width)
+        self.blocks = [make(width, width, std=width ** -0.5) for _ in range(2)]
+        self.norms = [dict(post=make(width, std=0.1), pre=make(width, std=0.1), gate=make(
+            4, width, std=0.5)) for _ in range(2)]
+        self.ids = torch.randint(0, vocab, (rows,), generator=g, device=dev)
+        self.next = torch.randint(0, vocab, (rows,), generator=g, device=dev)
+        self.next[::5] = IGNORE
+        self.grad = torch.full((rows,), 1.0 / rows, device=dev)
+
+    def step(self):
+        ho, kw = self.ho, dict(offset=1.0, scale=0.7)
+        h = ho.embedding(self.table, self.ids)
+        y, kept = h, []
+        for w, n in zip(self.blocks, self.norms):
+            x = y @ w
+            h, out, stats = ho.block_norms(x, h, **n, **kw)
+            kept.append((y, x, h, stats))
+            y = out
+        width = y.shape[1]
+        loss, lse = ho.linear_cross_entropy(y, self.table, self.next, scale=width ** -0.5)
+        dy, dtable = ho.linear_cross_entropy_bwd(self.grad, y, self.table, self.next, lse,
+                                                 scale=width ** -0.5)
+        dh, out = None, [loss]
+        for (y, x, h, stats), w, n in zip(kept[::-1], self.blocks[::-1], self.norms[::-1]):
+            dx, dh, *dn = ho.block_norms_bwd(dh, dy, x, h, stats, **n, **kw)
+            out += [y.t() @ dx, *(t for t in dn if t is not None)]
+            dy = dx @ w.t()
+        demb = (dh.float() + dy.float()).to(self.dtype)
+        out.append(ho.embedding_bwd(demb, self.ids, self.vocab, into=dtable))
+        return out
+
+    def exact(self):
+        """The same by automatic differentiation in 64 bits."""
+        leaf = lambda t: t.double().requires_grad_()  # noqa: E731
+        table, blocks = leaf(self.table), [leaf(w) for w in self.blocks]
+        norms = [{k: leaf(v) for k, v in n.items()} for n in self.norms]
+        h = table[self.ids]
+        y = h
+        width = h.shape[1]
+        for w, n in zip(blocks, norms):
+            x = y @ w
+            x = torch.nn.functional.rms_norm(x, (width,), 1.0 + n["post"], 1e-6)
+            h = h + 0.7 * x * n["gate"].repeat_interleave(self.rows // 4, 0)
+            y = torch.nn.functional.rms_norm(h, (width,), 1.0 + n["pre"], 1e-6)
+        loss = torch.nn.functional.cross_entropy(y @ table.t() * width ** -0.5, self.next,
+                                                 ignore_index=IGNORE, reduction="none")
+        (loss * self.grad.double()).sum().backward()
+        out = [loss.detach()]
+        for w, n in zip(blocks[::-1], norms[::-1]):
+            out += [w.grad, n["gate"].grad, n["post"].grad, n["pre"].grad]
+        return out + [table.grad]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,width,vocab", [(40, 64, 300), (260, 520, 2003)])
+def test_a_run_of_them_together(rows, width, vocab, dtype, rocm_device, ho):
+    """bf16 values between the calls are off by 2^-8 each, of a chain of some 16
+    roundings; fp32 by 2^-24 of sums of `width` and more terms."""
+    m = Model(ho, rocm_device, rows, width, vocab, dtype)
+    least = 16 * 2.0 ** -8 if dtype == BF16 else 2.0 ** -24 * 16 * width
+    for k, (u, v) in enumerate(zip(m.step(), m.exact())):
+        assert u.shape == v.shape
+        assert float((u.double() - v).norm() / v.norm()) < least, k
+
+
+@pytest.mark.parametrize("rows", [40, 1100])
+def test_the_run_in_a_graph(rows, rocm_device, ho):
+    """Captured once and replayed on new tokens, another number of them left
+    out, with eager work between."""
+    m = Model(ho, rocm_device, rows, 128, 2003, BF16)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        m.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        captured = m.step()
+    for seed in range(4):
+        g = torch.Generator().manual_seed(seed)
+        m.ids.copy_(torch.randint(0, m.vocab, m.ids.shape, generator=g))
+        m.next.copy_(torch.randint(0, m.vocab, m.next.shape, generator=g))
+        m.next[:seed * rows // 3] = IGNORE
+        eager = [v.clone() for v in m.step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        for k, (u, v) in enumerate(zip(captured, eager)):
+            assert torch.equal(u, v), f"replay {seed}, output {k}"
+
+
+def test_two_streams_at_once(rocm_device, ho):
+    models = [Model(ho, rocm_device, 600, 256, 5000, BF16, seed=k) for k in range(2)]
+    want = [[v.clone() for v in m.step()] for m in models]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in models]
+    for _ in range(3):
+        got = []
+        for m, s in zip(models, streams):
+            with torch.cuda.stream(s):
+                got.append(m.step())
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
