@@ -142,42 +142,6 @@ __global__ __launch_bounds__(256) void pack_rows(Pack a) {
   }
 }
 
-// dst[plane][col][row] = the parts of src[row][col], zeros from the last row up
-// to a multiple of 64.  A workgroup moves tiles of 64 by 64 through LDS.
-template <typename T>
-__global__ __launch_bounds__(256) void pack_transposed(Pack a) {
-  __shared__ T tile[64][65];
-  const int64_t rows = a.count ? *a.count : a.rows;
-  const int64_t tiles_r = (rows + 63) / 64, tiles_c = (a.cols + 63) / 64;
-  for (int64_t t = blockIdx.x; t < tiles_r * tiles_c; t += gridDim.x) {
-    const int64_t r0 = t / tiles_c * 64;
-    const int c0 = static_cast<int>(t % tiles_c) * 64;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int i = wave; i < 64; i += 4) {
-      const int64_t r = r0 + i;
-      T v = 0;
-      if (r < rows && c0 + lane < a.cols) {
-        v = static_cast<const T*>(a.src)[(a.kept ? a.kept[r] : r) * a.ld + c0 + lane];
-      }
-      tile[i][lane] = v;
-    }
-    __syncthreads();
-    for (int i = wave; i < 64 && c0 + i < a.cols; i += 4) {
-      uint16_t* to = a.dst + (c0 + i) * a.dst_ld + r0 + lane;
-      if (sizeof(T) == 2) {
-        *to = static_cast<uint16_t>(tile[lane][i]);
-      } else {
-        uint16_t p[3];
-        split3(static_cast<float>(tile[lane][i]), p);
-        to[0] = p[0];
-        to[a.plane] = p[1];
-        to[2 * a.plane] = p[2];
-      }
-    }
-    __syncthreads();
-  }
-}
-
 // ---------------------------------------------------------------------------
 // The product of the rows of two matrices
 // ---------------------------------------------------------------------------
@@ -185,11 +149,12 @@ __global__ __launch_bounds__(256) void pack_transposed(Pack a) {
 enum Epilogue { kReduce, kLogitGrad, kAccumulate, kStore };
 
 struct Product {
-  // out[j][i] = sum_k a[i][k] b[j][k].  a_count, b_count, k_count: read on the
-  // device where they are the number of rows that count.
+  // out[j][i] = sum_k a[i][k] b[j][k], where a and b may lie as [k][i] and [k][j].
+  // `k` values of K, of which a has a_k rows where it lies as [k][i].  b_count,
+  // k_count: read on the device where they are the number of rows that count.
   const uint16_t *a, *b;
   int64_t lda, ldb, a_plane, b_plane;
-  int a_rows, b_rows, k;
+  int a_rows, b_rows, k, a_k;
   const int *b_count, *k_count;
 
   // kReduce, kLogitGrad: a is the vocabulary from `first` on, b the rows.
@@ -202,8 +167,8 @@ struct Product {
   int64_t part_ld, first_tile;
   float* target;
   const float *grad, *lse, *grad_lse;
-  uint16_t *d, *dt;  // [rows][d_ld], [piece][dt_ld] and their planes
-  int64_t d_ld, dt_ld, d_plane, dt_plane, vocab;
+  uint16_t* d;  // [rows][d_ld] and its planes
+  int64_t d_ld, d_plane, vocab;
 
   // kAccumulate: sums of the pieces [split][rows][sum_ld], K being split among
   // blockIdx.y (`to_out`: not split, and the last piece).  kStore: out alone.
@@ -214,11 +179,30 @@ struct Product {
   int64_t out_ld;
 };
 
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
+typedef __attribute__((address_space(3))) const uint16_t* lds_ptr_t;
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4_t;
+typedef int s32x4_t __attribute__((ext_vector_type(4)));
 
+// 16 bytes a lane from byte `from` of the buffer (from its end on: zeros), plus
+// the scalar `offset`, to LDS from byte `to` on, lane after lane.  No register is
+// written; it is waited for by count, in barrier().  (Of the builtin the compiler
+// would wait for every load that might write what an LDS read reads.)  m0 needs
+// one wait state before its use.
+__device__ __forceinline__ void load_to_lds(s32x4_t buffer, uint32_t from, int offset,
+                                            uint32_t to) {
+  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(
+                   from),
+               "s"(buffer), "s"(offset), "s"(to)
+               : "memory");
+}
+
+// All but `Loads` loads of this wave and all its LDS reads are done, in every
+// wave of the workgroup.
+template <int Loads>
 __device__ __forceinline__ void barrier() {
   __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(Loads) : "memory");
   __builtin_amdgcn_sched_barrier(0);
 }
 
@@ -227,14 +211,20 @@ __device__ __forceinline__ void store4(uint16_t* p, const f32x4_t& v, int n) {
   if (n >= 4) {
     *reinterpret_cast<u32x2_a2_t*>(p) = u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
   } else {
-    for (int i = 0; i < n; ++i) p[i] = static_cast<uint16_t>(pack_bf16x2(v[i], 0.0f));
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      if (i < n) p[i] = static_cast<uint16_t>(pack_bf16x2(v[i], 0.0f));
+    }
   }
 }
 __device__ __forceinline__ void store4(float* p, const f32x4_t& v, int n) {
   if (n >= 4) {
     *reinterpret_cast<f32x4_a4_t*>(p) = v;
   } else {
-    for (int i = 0; i < n; ++i) p[i] = v[i];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      if (i < n) p[i] = v[i];
+    }
   }
 }
 
@@ -246,14 +236,125 @@ __device__ __forceinline__ int b_part(int pass, int passes) {
   return passes == 1 ? 0 : (0x010102 >> (4 * pass)) & 3;
 }
 
+// One operand's part of a round: kTile rows by kStep values of K in LDS, moved
+// there straight from memory, 16 bytes a lane, 4 instructions a wave.
+//
+// Of [row][k]: an instruction moves 8 rows of 64 values.  The 16-byte piece c of
+// row r lies at place c ^ (r % 8) of its row, so that the 16 rows that a matrix
+// instruction's operand is read from lie in different banks.
+//
+// Of [k][row] (Across): an instruction moves 2 values of K of 256 rows; the piece
+// c of value k lies at place c ^ (k % 4 * 2), and the operand is read by the
+// LDS's transposing loads, 16 lanes of which take 4 values of K of 16 rows.
+//
+// Two rounds' parts lie one behind the other, from element `first` of the
+// workgroup's LDS on.
+template <bool Across>
+struct Operand {
+  uint32_t from;                // byte of the tile that this lane loads first
+  uint32_t at[Across ? 4 : 2];  // element of the LDS that it reads first
+  uint32_t to;                  // byte of the LDS that this wave writes first
+  int64_t ld, plane;
+  const uint16_t* base;
+  int valid;   // rows
+  int k_rows;  // Across: values of K there are
+  int next;    // bytes between instructions
+
+  __device__ __forceinline__ void init(const uint16_t* m, int64_t m_ld, int64_t m_plane, int tile,
+                                       int rows, int k, int wave, int lane, int wave_row,
+                                       const uint16_t* lds, int first) {
+    ld = m_ld;
+    plane = m_plane;
+    // Across: whole 16-byte pieces, as a load that crosses the buffer's end loses
+    // the 4 bytes that do.  (Rows of memory are whole pieces long.)
+    valid = min(kTile, (Across ? (rows + 7) / 8 * 8 : rows) - tile * kTile);
+    k_rows = k;
+    base = m + static_cast<int64_t>(tile) * kTile * (Across ? 1 : ld);
+    const uint32_t lds_byte = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr_t)lds));
+    to = __builtin_amdgcn_readfirstlane(lds_byte + first * 2 + wave * 1024);
+    const int l = lane & 15, g = lane >> 4;
+    if constexpr (Across) {
+      const int kr = wave * 2 + (lane >> 5);
+      from = static_cast<uint32_t>(kr * ld * 2 + ((lane & 31) ^ ((kr & 3) << 1)) * 16);
+      next = static_cast<int>(16 * ld * 2);
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        at[f] = first + (g * 8 + (l >> 2)) * kTile + wave_row +
+                ((2 * f + ((l & 3) >> 1)) ^ ((l >> 2) << 1)) * 8 + (l & 1) * 4;
+        // (Else `first` joins the reads' offsets, which hold 16 bits.)
+        asm volatile("" : "+v"(at[f]));
+      }
+    } else {
+      const int row = wave * 8 + (lane >> 3);
+      from = static_cast<uint32_t>(row * ld * 2 + ((lane & 7) ^ (lane >> 3)) * 16);
+      next = static_cast<int>(64 * ld * 2);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        at[h] = first + (wave_row + l) * kStep + (((h * 4 + g) ^ (l & 7)) * 8);
+        asm volatile("" : "+v"(at[h]));
+      }
+    }
+  }
+
+  struct Round {
+    s32x4_t buffer;
+    int offset;
+    uint32_t from;
+  };
+
+  // The round of K from k0 on; from k on there are zeros.
+  __device__ __forceinline__ Round round(int part, int k0, int k, int lane) const {
+    const uint16_t* here = base + part * plane;
+    int bytes, offset;
+    uint32_t first = from;
+    if constexpr (Across) {
+      // Rows of K past the last are past the buffer's end, which reads as zero.
+      const int left = min(kStep, k_rows - k0);
+      bytes = max(0, static_cast<int>(((left - 1) * ld + valid) * 2));
+      bytes = left > 0 ? bytes : 0;
+      offset = 0;
+      here += min(k0, k_rows) * ld;
+    } else {
+      bytes = static_cast<int>(((valid - 1) * ld + k) * 2);
+      offset = k0 * 2;
+      first |= k0 + ((lane & 7) ^ (lane >> 3)) * 8 < k ? 0u : 0x80000000u;
+    }
+    const uint64_t address = reinterpret_cast<uint64_t>(here);
+    const s32x4_t r = {__builtin_amdgcn_readfirstlane(static_cast<int>(address)),
+                       __builtin_amdgcn_readfirstlane(static_cast<int>(address >> 32) & 0xffff),
+                       __builtin_amdgcn_readfirstlane(bytes), 0x00027000};
+    return Round{r, __builtin_amdgcn_readfirstlane(offset), first};
+  }
+
+  // A quarter of it.
+  __device__ __forceinline__ void load(int buffer, int q, const Round& r) const {
+    load_to_lds(r.buffer, r.from + q * next, r.offset, to + buffer * kTile * kStep * 2 + q * 8192);
+  }
+
+  // Rows 16 f to 16 f + 15 of the wave's, 32 values of K of half `h`: row l, values
+  // 8 g to 8 g + 7 for lane 16 g + l.
+  __device__ __forceinline__ bf16x8_t fetch(const uint16_t* lds, int buffer, int h, int f) const {
+    if constexpr (Across) {
+      const uint16_t* p = lds + at[f & 3] + buffer * kTile * kStep + (f >> 2) * 64 + h * 32 * kTile;
+      const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)p);
+      const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(p + 4 * kTile));
+      const auto both = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+      return __builtin_bit_cast(bf16x8_t, both);
+    } else {
+      return *reinterpret_cast<const bf16x8_t*>(lds + at[h] + buffer * kTile * kStep +
+                                                f * 16 * kStep);
+    }
+  }
+};
+
 template <typename T, Epilogue E>
 __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
   constexpr int kPasses = sizeof(T) == 2 ? 1 : 6;
-  __shared__ __attribute__((aligned(16))) uint16_t a0[kTile * kStep], a1[kTile * kStep];
-  __shared__ __attribute__((aligned(16))) uint16_t b0[kTile * kStep], b1[kTile * kStep];
+  constexpr bool kAcrossA = E == kAccumulate || E == kStore, kAcrossB = E == kStore;
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[4 * kTile * kStep];
 
   const int rows_b = p.b_count ? *p.b_count : p.b_rows;
-  const int k = p.k_count ? (*p.k_count + kStep - 1) / kStep * kStep : p.k;
+  const int k = p.k_count ? *p.k_count : p.k;
   // Tiles in an order that keeps an XCD's workgroups on 4 tiles of a by 8 of b.
   const int tiles_a = (p.a_rows + kTile - 1) / kTile;
   const int tiles_b = (rows_b + kTile - 1) / kTile;
@@ -265,131 +366,150 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
   const int tile_a = band * 4 + in_band % band_rows, tile_b = in_band / band_rows;
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int valid_a = min(kTile, p.a_rows - tile_a * kTile);
   const int valid_b = min(kTile, rows_b - tile_b * kTile);
-
-  // A load moves 8 rows of 64 values straight into LDS, 16 bytes a lane.  The
-  // 16-byte piece c of row r lies at place c ^ (r % 8) of its row, so that the
-  // 16 rows that a matrix instruction reads spread over all banks.
-  const int row_in = lane >> 3, chunk = (lane & 7) ^ row_in;
-  uint32_t from_a[4], from_b[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const uint32_t row = (q * 8 + wave) * 8 + row_in;
-    from_a[q] = static_cast<uint32_t>(row * p.lda * 2 + chunk * 16);
-    from_b[q] = static_cast<uint32_t>(row * p.ldb * 2 + chunk * 16);
-  }
-  const int bytes_a = static_cast<int>(((valid_a - 1) * p.lda + k) * 2);
-  const int bytes_b = static_cast<int>(((valid_b - 1) * p.ldb + k) * 2);
-
-  auto load = [&](uint16_t* la, uint16_t* lb, int pass, int k0) {
-    const uint16_t* ga = p.a + a_part(pass, kPasses) * p.a_plane + tile_a * p.lda * kTile;
-    const uint16_t* gb = p.b + b_part(pass, kPasses) * p.b_plane + tile_b * p.ldb * kTile;
-    auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(ga), 0, bytes_a, 0x00027000);
-    auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(gb), 0, bytes_b, 0x00027000);
-    // Past K: an offset past the buffer's end, which reads as zero.
-    const uint32_t past = k0 + chunk * 8 < k ? 0u : 0x80000000u;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr_t)(la + (q * 8 + wave) * 512), 16,
-                                               from_a[q] | past, k0 * 2, 0, 0);
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr_t)(lb + (q * 8 + wave) * 512), 16,
-                                               from_b[q] | past, k0 * 2, 0, 0);
-    }
-  };
-
   // 2 by 4 waves of 128 by 64 values each, in tiles of 16 by 16.
   const int wave_a = (wave >> 2) * 128, wave_b = (wave & 3) * 64;
+  Operand<kAcrossA> oa;
+  Operand<kAcrossB> ob;
+  oa.init(p.a, p.lda, p.a_plane, tile_a, p.a_rows, p.k_count ? k : p.a_k, wave, lane, wave_a,
+          lds, 0);
+  ob.init(p.b, p.ldb, p.b_plane, tile_b, rows_b, k, wave, lane, wave_b, lds,
+          2 * kTile * kStep);
+
   f32x4_t acc[8][4];
 #pragma unroll
   for (int f = 0; f < 8; ++f) {
 #pragma unroll
     for (int n = 0; n < 4; ++n) acc[f][n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  auto multiply = [&](const uint16_t* la, const uint16_t* lb) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int at = (lane & 15) * kStep + (((s * 4 + (lane >> 4)) ^ (lane & 7)) * 8);
-      bf16x8_t fa[8], fb[4];
-#pragma unroll
-      for (int f = 0; f < 8; ++f) {
-        fa[f] = *reinterpret_cast<const bf16x8_t*>(la + (wave_a + f * 16) * kStep + at);
-      }
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        fb[n] = *reinterpret_cast<const bf16x8_t*>(lb + (wave_b + n * 16) * kStep + at);
-      }
-#pragma unroll
-      for (int f = 0; f < 8; ++f) {
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          acc[f][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[f], fb[n], acc[f][n], 0, 0, 0);
-        }
-      }
-    }
-  };
+  // A round is two halves of 32 values of K; a half's operands are read from LDS
+  // into one set of registers while the other set is multiplied.
+  bf16x8_t fa[2][8], fb[2][4];
 
-  // Rounds of K, in pairs, the next one's loads in flight while one is
-  // multiplied.  Rounds past the last (the second of an odd pair, and the one
-  // loaded behind the end) load zeros.
+  // Rounds of K, in pairs.  Rounds past the last (the second of an odd pair, and
+  // the two loaded behind the end) load zeros.
   int begin = 0, end = (k + kStep - 1) / kStep;
   if (E == kAccumulate) {
-    const int whole = end;
-    begin = static_cast<int>(static_cast<int64_t>(whole) * blockIdx.y / gridDim.y);
-    end = static_cast<int>(static_cast<int64_t>(whole) * (blockIdx.y + 1) / gridDim.y);
+    // (Divided by lanes: back to scalars, which the loads need.)
+    const int64_t whole = end;
+    begin = __builtin_amdgcn_readfirstlane(static_cast<int>(whole * blockIdx.y / gridDim.y));
+    end = __builtin_amdgcn_readfirstlane(static_cast<int>(whole * (blockIdx.y + 1) / gridDim.y));
   }
   const int rounds = (end - begin) * kPasses;
   int pass = 0, at = begin;
-  auto next = [&](uint16_t* la, uint16_t* lb) {
-    load(la, lb, pass, pass < kPasses ? at * kStep : k);
-    if (++at >= end) {
-      at = begin;
-      ++pass;
+  typename Operand<kAcrossA>::Round ra;
+  typename Operand<kAcrossB>::Round rb;
+  auto prepare = [&]() __attribute__((always_inline)) {
+    const int k0 = pass < kPasses ? at * kStep : max(k, p.a_k);
+    const int now = min(pass, kPasses - 1);
+    ra = oa.round(a_part(now, kPasses), k0, k, lane);
+    rb = ob.round(b_part(now, kPasses), k0, k, lane);
+    const bool wrap = ++at >= end;
+    at = wrap ? begin : at;
+    pass += wrap ? 1 : 0;
+  };
+  // The products of half `half`, in eight groups; with each a part of what the
+  // other half needs is read from LDS and a load of the round after next begins,
+  // so that neither waits in a row for the units that take them.
+  auto multiply = [&](int half, int buffer, bool load) __attribute__((always_inline)) {
+#pragma unroll
+    for (int f = 0; f < 8; ++f) {
+      if (load) {
+        if (f < 4) {
+          oa.load(buffer, f, ra);
+        } else {
+          ob.load(buffer, f - 4, rb);
+        }
+      }
+      const int from = load ? buffer ^ 1 : buffer;
+#pragma unroll
+      for (int m = 2 * f; m < min(2 * f + 2, 12); ++m) {
+        if (m < 4) {
+          fb[half ^ 1][m] = ob.fetch(lds, from, half ^ 1, m);
+        } else {
+          fa[half ^ 1][m - 4] = oa.fetch(lds, from, half ^ 1, m - 4);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        acc[f][n] =
+            __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[half][f], fb[half][n], acc[f][n], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
-  next(a0, b0);
+  // One barrier a round: behind it the round's buffer is read and free for the
+  // round after next, and the next round's loads have arrived.
+  auto round = [&](int buffer) __attribute__((always_inline)) {
+    prepare();
+    multiply(0, buffer, false);
+    barrier<0>();
+    multiply(1, buffer, true);
+  };
+  // (5 wait states from a vector instruction's scalar result to a load.)
+  auto load_all = [&](int buffer) __attribute__((always_inline)) {
+    prepare();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 4");
+#pragma unroll
+    for (int q = 0; q < 4; ++q) oa.load(buffer, q, ra);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) ob.load(buffer, q, rb);
+  };
+  load_all(0);
+  load_all(1);
+  barrier<8>();
+#pragma unroll
+  for (int n = 0; n < 4; ++n) fb[0][n] = ob.fetch(lds, 0, 0, n);
+#pragma unroll
+  for (int f = 0; f < 8; ++f) fa[0][f] = oa.fetch(lds, 0, 0, f);
   for (int t = 0; t < rounds; t += 2) {
-    next(a1, b1);
-    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-    barrier();
-    multiply(a0, b0);
-    barrier();
-    next(a0, b0);
-    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-    barrier();
-    multiply(a1, b1);
-    barrier();
+    round(0);
+    round(1);
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  barrier();
+  barrier<0>();
 
   // acc[f][n][r] is out[j][i] with these.
   const int i0 = tile_a * kTile + wave_a + (lane >> 4) * 4;  // + 16 f + r
   const int j0 = tile_b * kTile + wave_b + (lane & 15);      // + 16 n
 
   if (E == kReduce) {
-    // A row's values are 32 of each of 4 lanes in each of 2 waves.
-    float* both = reinterpret_cast<float*>(a0);  // [wave_a][2][kTile]
+    // A row's values are 32 of each of 4 lanes in each of 2 waves; a maximum and
+    // a sum of e^(s - maximum) of each, in units of the logits without `scale`
+    // (which is positive) up to the end.
+    float* both = reinterpret_cast<float*>(lds);  // [wave_a][2][kTile]
+    const float to_log2 = p.scale * kLog2eHi;
+    if (tile_a + 1 == tiles_a) {
+#pragma unroll
+      for (int f = 0; f < 8; ++f) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (i0 + f * 16 + r >= p.a_rows) acc[f][n][r] = -INFINITY;
+          }
+        }
+      }
+    }
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       const int j = j0 + n * 16;
-      const bool inside = j < rows_b;
-      const int64_t tok = inside ? token_at(p.tokens, p.token_size, p.kept[j]) - p.first : -1;
+      int64_t tok = -1;
+      if (j < rows_b) tok = token_at(p.tokens, p.token_size, p.kept[j]) - p.first - i0;
+      if (tok >= 0 && tok < 116 && i0 + tok < p.a_rows) {
+#pragma unroll
+        for (int f = 0; f < 8; ++f) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (tok == f * 16 + r) p.target[j] = acc[f][n][r] * p.scale;
+          }
+        }
+      }
       float top = -kLargest;
 #pragma unroll
       for (int f = 0; f < 8; ++f) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = i0 + f * 16 + r;
-          float s = acc[f][n][r] * p.scale;
-          if (i == tok && i < p.a_rows) p.target[j] = s;
-          if (i >= p.a_rows) s = -INFINITY;
-          acc[f][n][r] = s;
-          top = fmaxf(top, s);
-        }
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[f][n][r]);
       }
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
@@ -398,12 +518,14 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
 #pragma unroll
       for (int f = 0; f < 8; ++f) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sum += exp_f32(exp_domain(acc[f][n][r] - top));
+        for (int r = 0; r < 4; ++r) {
+          sum += __builtin_amdgcn_exp2f((acc[f][n][r] - top) * to_log2);
+        }
       }
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
       if (lane < 16) {
-        both[((wave >> 2) * 2 + 0) * kTile + wave_b + n * 16 + lane] = top;
+        both[((wave >> 2) * 2 + 0) * kTile + wave_b + n * 16 + lane] = top * p.scale;
         both[((wave >> 2) * 2 + 1) * kTile + wave_b + n * 16 + lane] = sum;
       }
     }
@@ -458,8 +580,6 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
           *reinterpret_cast<u32x2_t*>(p.d + q * p.d_plane + j * p.d_ld + i) =
               u32x2_t{part[0][q] | uint32_t{part[1][q]} << 16,
                       part[2][q] | uint32_t{part[3][q]} << 16};
-#pragma unroll
-          for (int r = 0; r < 4; ++r) p.dt[q * p.dt_plane + (i + r) * p.dt_ld + j] = part[r][q];
         }
       }
     }
@@ -469,6 +589,7 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       const int j = j0 + n * 16;
+      asm volatile("" ::: "memory");  // no loads of later rows ahead of this one's
       if (j >= rows_b) continue;
       T* out = static_cast<T*>(p.out) + (E == kStore ? j : (p.to_out ? p.kept[j] : 0)) * p.out_ld;
 #pragma unroll
@@ -574,7 +695,7 @@ struct Plan {
   int planes;
   int splits;   // of a piece, for dhidden
   bool direct;  // weight is read where it lies
-  size_t kept, count, target, part, hidden, weight, hidden_t, weight_t, d, dt, sum, bytes;
+  size_t kept, count, target, part, hidden, weight, d, sum, bytes;
 };
 
 constexpr int64_t kCus = 256;
@@ -592,7 +713,7 @@ Plan plan_of(const void* weight, int elem_size, int64_t rows, int64_t width, int
   p.k_pad = up(width, kStep);
   const size_t copy = p.direct ? 0 : sizeof(uint16_t) * p.planes * p.k_pad;
   const size_t per_row =
-      backward ? copy + sizeof(uint16_t) * p.planes * (2 * p.rows_pad + width) : copy;
+      backward ? copy + sizeof(uint16_t) * p.planes * p.rows_pad : copy;
   const size_t most = backward ? kBackwardBytes : kForwardBytes;
   const int64_t whole = up(vocab, kTile);
   int64_t piece = whole;
@@ -622,10 +743,7 @@ Plan plan_of(const void* weight, int elem_size, int64_t rows, int64_t width, int
   p.hidden = take(plane * p.rows_pad * p.k_pad);
   p.weight = take(p.direct ? 0 : plane * p.piece * p.k_pad);
   if (backward) {
-    p.hidden_t = take(plane * width * p.rows_pad);
-    p.weight_t = take(plane * width * p.piece);
     p.d = take(plane * p.rows_pad * p.piece);
-    p.dt = take(plane * p.piece * p.rows_pad);
     p.sum = take(p.pieces * p.splits > 1
                      ? sizeof(float) * p.splits * p.rows_pad * up(width, 4) : 0);
   } else {
@@ -660,14 +778,8 @@ int check_operands(const char* what, int elem_size, int token_size, int64_t rows
 }
 
 template <typename T>
-int pack(const char* what, Pack a, int64_t rows, bool transposed, hipStream_t stream) {
-  if (transposed) {
-    const int64_t tiles = ((rows + 63) / 64) * ((a.cols + 63) / 64);
-    pack_transposed<T><<<static_cast<uint32_t>(std::min<int64_t>(tiles, 1 << 16)), 256, 0,
-                         stream>>>(a);
-  } else {
-    pack_rows<T><<<static_cast<uint32_t>(std::min<int64_t>(rows, 1 << 16)), 256, 0, stream>>>(a);
-  }
+int pack(const char* what, Pack a, int64_t rows, hipStream_t stream) {
+  pack_rows<T><<<static_cast<uint32_t>(std::min<int64_t>(rows, 1 << 16)), 256, 0, stream>>>(a);
   return check_launch(what);
 }
 
@@ -717,7 +829,7 @@ int piece_of_weight(const char* what, const Call& c, const Plan& plan, int64_t f
     g->k = static_cast<int>(plan.k_pad);
     HIPO_STEP(pack<T>(what, Pack{from, c.weight_ld, nullptr, nullptr, g->a_rows,
                                  static_cast<int>(c.width), to, plan.k_pad, g->a_plane},
-                      g->a_rows, false, c.stream));
+                      g->a_rows, c.stream));
   }
   g->first = first;
   return 0;
@@ -736,7 +848,7 @@ int select_and_pack(const char* what, const Call& c, const Plan& plan, float* lo
   const int64_t plane = plan.rows_pad * plan.k_pad;
   HIPO_STEP(pack<T>(what, Pack{c.hidden, c.hidden_ld, kept, count, c.rows,
                                static_cast<int>(c.width), hidden, plan.k_pad, plane},
-                    c.rows, false, c.stream));
+                    c.rows, c.stream));
   g->b = hidden;
   g->ldb = plan.k_pad;
   g->b_plane = plane;
@@ -775,12 +887,6 @@ int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse
   Product g{};
   HIPO_STEP(select_and_pack<T>(what, c, plan, nullptr, nullptr, &g));
   const int width = static_cast<int>(c.width);
-  uint16_t* hidden_t = c.at<uint16_t>(plan.hidden_t);
-  uint16_t* weight_t = c.at<uint16_t>(plan.weight_t);
-  const int64_t hidden_t_plane = c.width * plan.rows_pad, weight_t_plane = c.width * plan.piece;
-  HIPO_STEP(pack<T>(what, Pack{c.hidden, c.hidden_ld, g.kept, g.b_count, c.rows, width, hidden_t,
-                               plan.rows_pad, hidden_t_plane},
-                    c.rows, true, c.stream));
   zero_rows<T><<<static_cast<uint32_t>(std::min<int64_t>(c.rows, 1 << 16)), 256, 0, c.stream>>>(
       c.tokens, c.token_size, c.ignore_index, static_cast<T*>(dhidden), c.rows, width);
   HIPO_STEP(check_launch(what));
@@ -790,23 +896,17 @@ int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse
   g.d = c.at<uint16_t>(plan.d);
   g.d_ld = plan.piece;
   g.d_plane = plan.rows_pad * plan.piece;
-  g.dt = c.at<uint16_t>(plan.dt);
-  g.dt_ld = plan.rows_pad;
-  g.dt_plane = plan.piece * plan.rows_pad;
   for (int64_t i = 0; i < plan.pieces; ++i) {
     const int64_t first = i * plan.piece;
     HIPO_STEP(piece_of_weight<T>(what, c, plan, first, &g));
     HIPO_STEP((multiply<T, kLogitGrad>(what, g, c.rows, c.stream)));
 
-    HIPO_STEP(pack<T>(what, Pack{static_cast<const T*>(c.weight) + first * c.weight_ld,
-                                 c.weight_ld, nullptr, nullptr, g.a_rows, width, weight_t,
-                                 plan.piece, weight_t_plane},
-                      g.a_rows, true, c.stream));
     Product h{};
-    h.a = weight_t;
-    h.lda = plan.piece;
-    h.a_plane = weight_t_plane;
+    h.a = g.a;
+    h.lda = g.lda;
+    h.a_plane = g.a_plane;
     h.a_rows = width;
+    h.a_k = g.a_rows;
     h.b = g.d;
     h.ldb = g.d_ld;
     h.b_plane = g.d_plane;
@@ -823,13 +923,13 @@ int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse
     HIPO_STEP((multiply<T, kAccumulate>(what, h, c.rows, c.stream, plan.splits)));
 
     Product w{};
-    w.a = hidden_t;
-    w.lda = plan.rows_pad;
-    w.a_plane = hidden_t_plane;
+    w.a = g.b;
+    w.lda = g.ldb;
+    w.a_plane = g.b_plane;
     w.a_rows = width;
-    w.b = g.dt;
-    w.ldb = g.dt_ld;
-    w.b_plane = g.dt_plane;
+    w.b = g.d;
+    w.ldb = g.d_ld;
+    w.b_plane = g.d_plane;
     w.b_rows = g.a_rows;
     w.k_count = g.b_count;
     w.out = static_cast<T*>(dweight) + first * c.width;
