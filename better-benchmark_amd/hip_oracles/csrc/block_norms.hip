@@ -31,27 +31,55 @@ struct Vec8 {
   float v[kGroup];
 };
 
-// 8 values at p, of any element alignment.
+// 8 values as they lie in memory, at any element alignment.
 template <typename T>
-__device__ __forceinline__ Vec8 load8(const T* p);
+struct Raw8;
 
 template <>
-__device__ __forceinline__ Vec8 load8<uint16_t>(const uint16_t* p) {
-  const u32x4_t w = *reinterpret_cast<const u32x4_a2_t*>(p);
-  Vec8 r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    r.v[2 * i] = bf16lo(w[i]);
-    r.v[2 * i + 1] = bf16hi(w[i]);
+struct Raw8<uint16_t> {
+  u32x4_t w;
+  __device__ __forceinline__ void load(const uint16_t* p) {
+    w = *reinterpret_cast<const u32x4_a2_t*>(p);
   }
-  return r;
-}
+  __device__ __forceinline__ void clear_unless(bool keep) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = keep ? w[i] : 0u;
+  }
+  __device__ __forceinline__ Vec8 values() const {
+    Vec8 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      r.v[2 * i] = bf16lo(w[i]);
+      r.v[2 * i + 1] = bf16hi(w[i]);
+    }
+    return r;
+  }
+};
 
 template <>
-__device__ __forceinline__ Vec8 load8<float>(const float* p) {
-  const f32x4_t a = *reinterpret_cast<const f32x4_a4_t*>(p);
-  const f32x4_t b = *reinterpret_cast<const f32x4_a4_t*>(p + 4);
-  return Vec8{{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
+struct Raw8<float> {
+  f32x4_t a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = *reinterpret_cast<const f32x4_a4_t*>(p);
+    b = *reinterpret_cast<const f32x4_a4_t*>(p + 4);
+  }
+  __device__ __forceinline__ void clear_unless(bool keep) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = keep ? a[i] : 0.0f;
+      b[i] = keep ? b[i] : 0.0f;
+    }
+  }
+  __device__ __forceinline__ Vec8 values() const {
+    return Vec8{{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ Vec8 load8(const T* p) {
+  Raw8<T> r;
+  r.load(p);
+  return r.values();
 }
 
 __device__ __forceinline__ void store8(uint16_t* p, const Vec8& r) {
@@ -81,16 +109,23 @@ struct Layout {
   int threads() const { return lanes * teams; }
 };
 
-inline Layout layout_of(int64_t cols) {
-  const int64_t groups = (cols + kGroup - 1) / kGroup;
+// `groups`: of 8 values per lane, where a row has whole waves.
+inline Layout layout_of(int64_t cols, int groups) {
+  const int64_t pieces = (cols + kGroup - 1) / kGroup;
   if (cols <= kSmallCols) {
     int lanes = 1;
-    while (lanes < groups) lanes *= 2;
+    while (lanes < pieces) lanes *= 2;
     return Layout{lanes, 512 / lanes};
   }
-  const int waves = static_cast<int>((groups + 127) / 128);
+  const int waves = static_cast<int>((pieces + kWave * groups - 1) / (kWave * groups));
   return Layout{waves * kWave, std::max(1, 8 / waves)};
 }
+
+// Groups per lane of the gradient: it holds up to nine rows' worth of registers
+// (four operands, the next row's, up to five sums), and with one group 8 to 16
+// waves fit a CU.  Rows past 4096 columns take two, so that 8 waves hold a row
+// and each lane has 256 registers (with 16 waves it has 128, too few).
+inline int bwd_groups(int64_t cols) { return cols <= 512 * kGroup ? 1 : 2; }
 
 // Where a lane's groups lie.  The group that would cross the row's end is moved
 // back to end there; its first `skip` values belong to the group before, which
@@ -116,8 +151,8 @@ __device__ __forceinline__ Columns<U> columns_of(int place, int lanes, int cols)
 
 // Sums over a team, N at once, every lane receiving them, in an order that the
 // layout fixes.  `slot`: LDS of N floats per wave, other than the last call's.
-template <int N, bool SMALL>
-__device__ __forceinline__ void team_sum(float (&v)[N], int lanes, float* slot) {
+template <int N, bool SMALL, int M>
+__device__ __forceinline__ void team_sum(float (&v)[M], int lanes, float* slot) {
   if (SMALL) {
     for (int o = 1; o < lanes; o *= 2) {
 #pragma unroll
@@ -141,6 +176,32 @@ __device__ __forceinline__ void team_sum(float (&v)[N], int lanes, float* slot) 
   for (int w = 0; w < waves; ++w) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] += mine[w * N + i];
+  }
+}
+
+// s[0] += sum w e and, LAYER, s[1] += sum w over the columns a lane owns.
+template <int U, bool LAYER>
+__device__ __forceinline__ void pair_sum(float (&s)[2], const Vec8 (&w)[U], const Vec8 (&e)[U],
+                                         const Columns<U>& c, bool ragged) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float t[2] = {0.0f, 0.0f};
+    if (ragged) {  // some lane owns a part of its group
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) {
+        const float v = i >= c.skip[u] ? w[u].v[i] : 0.0f;
+        t[0] += v * (i >= c.skip[u] ? e[u].v[i] : 0.0f);
+        if (LAYER) t[1] += v;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) {
+        t[0] += w[u].v[i] * e[u].v[i];
+        if (LAYER) t[1] += w[u].v[i];
+      }
+    }
+    s[0] += c.skip[u] < kGroup ? t[0] : 0.0f;
+    if (LAYER) s[1] += c.skip[u] < kGroup ? t[1] : 0.0f;
   }
 }
 
@@ -286,9 +347,14 @@ __device__ __forceinline__ int64_t first_row(int64_t rows, int block, int blocks
 // sum goes out when the segment ends: as dgate where the segment holds all rows
 // of the gate, else to one of the workgroup's two places for the join (a
 // workgroup has at most two such segments, its first and its last).
-template <typename T, int U, bool LAYER, bool PRE, bool POST, bool GATE, int THREADS>
+// With one group a lane the next row's operands are loaded before the current
+// one's are used.
+enum Gate { kNoGate, kGateOfRows, kGateByRow };  // none, shared by rows, one a row
+
+template <typename T, int U, bool SMALL, bool LAYER, bool PRE, bool POST, Gate GATE, int THREADS>
 __global__ __launch_bounds__(THREADS) void block_norms_bwd(Backward a) {
-  constexpr bool kSmall = U == 1;
+  constexpr bool kSmall = SMALL;
+  constexpr bool kAhead = U == 1;  // with two groups a lane has no registers for it
   __shared__ float slots[2][64];
   extern __shared__ float sums[];  // [teams][cols], where there are several teams
   const int team = threadIdx.x / a.lanes;
@@ -301,11 +367,16 @@ __global__ __launch_bounds__(THREADS) void block_norms_bwd(Backward a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) acc[k][u] = Vec8{};
   }
-  Vec8 wpre[U], wpost[U], gate[U];
+  // (In registers, as a load in the loop would wait for the next row's.)
+  Vec8 wpre[U], wpost[U], bpost[U], gate[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     if (PRE) wpre[u] = load8(static_cast<const T*>(a.pre) + c.col[u]);
     if (POST) wpost[u] = load8(static_cast<const T*>(a.post) + c.col[u]);
+    bpost[u] = Vec8{};
+    if (GATE && POST && LAYER && a.post_bias) {
+      bpost[u] = load8(static_cast<const T*>(a.post_bias) + c.col[u]);
+    }
 #pragma unroll
     for (int i = 0; i < kGroup; ++i) {
       wpre[u].v[i] = PRE ? wpre[u].v[i] + a.offset : 0.0f;
@@ -345,7 +416,8 @@ __global__ __launch_bounds__(THREADS) void block_norms_bwd(Backward a) {
   };
 
   int set = 0;
-  const bool by_row = GATE && a.rows_per_gate == 1;
+  const bool ragged = a.cols % kGroup != 0;
+  constexpr bool by_row = GATE == kGateByRow;
   for (int64_t from = begin; from < end;) {
     int64_t to = end, which = 0;
     if (GATE && !by_row) {
@@ -358,56 +430,74 @@ __global__ __launch_bounds__(THREADS) void block_norms_bwd(Backward a) {
         for (int i = 0; i < kGroup; ++i) gate[u].v[i] *= a.scale;
       }
     }
-    for (int64_t first = from; first < to; first += a.teams, set ^= 1) {
-      const bool valid = first + team < to;
-      const int64_t row = valid ? first + team : to - 1;
+    // All loads without a branch, or the compiler waits for them at its end.
+    const T* grad_h = static_cast<const T*>(a.grad_h ? a.grad_h : a.grad_y);
+    struct Row {
+      Raw8<T> gh[U], gy[U], h[U], x[U], gate[U];
+      float st[4];
+    };
+    auto load = [&](Row& next, int64_t first) __attribute__((always_inline)) {
+      const int64_t row = min(first + team, to - 1);
       const int64_t at = row * a.cols;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (PRE) next.gy[u].load(static_cast<const T*>(a.grad_y) + at + c.col[u]);
+        if (PRE) next.h[u].load(static_cast<const T*>(a.h) + at + c.col[u]);
+        next.gh[u].load(grad_h + at + c.col[u]);
+        if (POST || GATE) next.x[u].load(static_cast<const T*>(a.x) + at + c.col[u]);
+        if (by_row) next.gate[u].load(static_cast<const T*>(a.gate) + at + c.col[u]);
+      }
+      // (What is not used is not loaded: its register would be waited for.)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if ((i < 2 ? POST : PRE) && (LAYER || i % 2 == 1)) next.st[i] = a.stats[row * 4 + i];
+      }
+    };
+    auto step = [&](Row& row, Row& next, int64_t first) __attribute__((always_inline)) {
+      const bool valid = first + team < to;
+      const int64_t at = (first + team) * a.cols;
+      if (!kAhead) load(row, first);
       Vec8 gh[U], gy[U], h[U], x[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (PRE) gy[u] = load8(static_cast<const T*>(a.grad_y) + at + c.col[u]);
-        if (PRE) h[u] = load8(static_cast<const T*>(a.h) + at + c.col[u]);
-        if (a.grad_h) {
-          gh[u] = load8(static_cast<const T*>(a.grad_h) + at + c.col[u]);
-        } else {
-          gh[u] = Vec8{};
-        }
-        if (POST || GATE) x[u] = load8(static_cast<const T*>(a.x) + at + c.col[u]);
-      }
-      const f32x4_t st = *reinterpret_cast<const f32x4_a4_t*>(a.stats + row * 4);
-      if (by_row) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          gate[u] = load8(static_cast<const T*>(a.gate) + at + c.col[u]);
+        // A team past the last row adds nothing: its gradients are 0.
+        row.gy[u].clear_unless(valid);
+        row.gh[u].clear_unless(valid && a.grad_h);
+        if (PRE) gy[u] = row.gy[u].values();
+        if (PRE) h[u] = row.h[u].values();
+        gh[u] = row.gh[u].values();
+        if (POST || GATE) x[u] = row.x[u].values();
+        if (by_row) {
+          gate[u] = row.gate[u].values();
 #pragma unroll
           for (int i = 0; i < kGroup; ++i) gate[u].v[i] *= a.scale;
         }
       }
+      const float st[4] = {row.st[0], row.st[1], row.st[2], row.st[3]};
+      if (kAhead) load(next, min(first + a.teams, to - 1));
       // gh becomes T.
       if (PRE) {
-        float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
           for (int i = 0; i < kGroup; ++i) {
-            const float e = (h[u].v[i] - st[2]) * st[3];
-            const float g = gy[u].v[i];
-            if (valid) acc[kPre][u].v[i] += g * e;
-            if (LAYER && valid) acc[kPreBias][u].v[i] += g;
-            const float w = i >= c.skip[u] ? g * wpre[u].v[i] : 0.0f;
-            s[0] += w * e;
-            s[1] += w;
-            h[u].v[i] = e;
+            h[u].v[i] = (LAYER ? h[u].v[i] - st[2] : h[u].v[i]) * st[3];
+            acc[kPre][u].v[i] += gy[u].v[i] * h[u].v[i];
+            if (LAYER) acc[kPreBias][u].v[i] += gy[u].v[i];
+            gy[u].v[i] *= wpre[u].v[i];
           }
         }
-        team_sum<2, kSmall>(s, a.lanes, slots[set]);
-        s[0] *= a.inv_cols;
-        s[1] = LAYER ? s[1] * a.inv_cols : 0.0f;
+        float s[2] = {0.0f, 0.0f};
+        pair_sum<U, LAYER>(s, gy, h, c, ragged);
+        team_sum<LAYER ? 2 : 1, kSmall>(s, a.lanes, slots[set]);
+        s[0] *= st[3] * a.inv_cols;
+        s[1] *= st[3] * a.inv_cols;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
           for (int i = 0; i < kGroup; ++i) {
-            gh[u].v[i] += st[3] * (gy[u].v[i] * wpre[u].v[i] - h[u].v[i] * s[0] - s[1]);
+            const float rest = LAYER ? gh[u].v[i] - s[1] : gh[u].v[i];
+            gh[u].v[i] = __builtin_fmaf(st[3], gy[u].v[i], __builtin_fmaf(-h[u].v[i], s[0], rest));
           }
         }
       }
@@ -421,50 +511,47 @@ __global__ __launch_bounds__(THREADS) void block_norms_bwd(Backward a) {
       if (POST || GATE) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          Vec8 b{};
-          if (GATE && POST && LAYER && a.post_bias) {
-            b = load8(static_cast<const T*>(a.post_bias) + c.col[u]);
-          }
-          Vec8 dg;
+          Vec8 tn;
 #pragma unroll
           for (int i = 0; i < kGroup; ++i) {
             float n = x[u].v[i];
             if (POST) {
-              x[u].v[i] = (n - st[0]) * st[1];
-              n = __builtin_fmaf(x[u].v[i], wpost[u].v[i], b.v[i]);
+              x[u].v[i] = (LAYER ? n - st[0] : n) * st[1];
+              n = __builtin_fmaf(x[u].v[i], wpost[u].v[i], bpost[u].v[i]);
             }
-            dg.v[i] = gh[u].v[i] * n * a.scale;
-            if (GATE && valid) acc[kGate][u].v[i] += dg.v[i];
+            if (GATE == kGateOfRows) acc[kGate][u].v[i] += gh[u].v[i] * n;
+            tn.v[i] = gh[u].v[i] * n * a.scale;
           }
           if (by_row && valid && c.skip[u] < kGroup) {
-            store8(static_cast<T*>(a.dgate) + at + c.col[u], dg);
+            store8(static_cast<T*>(a.dgate) + at + c.col[u], tn);
           }
         }
       }
-      float s[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int u = 0; u < U; ++u) {
 #pragma unroll
         for (int i = 0; i < kGroup; ++i) {
           gh[u].v[i] *= gate[u].v[i];
           if (POST) {
-            if (valid) acc[kPost][u].v[i] += gh[u].v[i] * x[u].v[i];
-            if (LAYER && valid) acc[kPostBias][u].v[i] += gh[u].v[i];
-            const float w = i >= c.skip[u] ? gh[u].v[i] * wpost[u].v[i] : 0.0f;
-            s[0] += w * x[u].v[i];
-            s[1] += w;
+            acc[kPost][u].v[i] += gh[u].v[i] * x[u].v[i];
+            if (LAYER) acc[kPostBias][u].v[i] += gh[u].v[i];
+            gh[u].v[i] *= wpost[u].v[i];
           }
         }
       }
       if (POST) {
-        team_sum<2, kSmall>(s, a.lanes, slots[set] + 32);
-        s[0] *= a.inv_cols;
-        s[1] = LAYER ? s[1] * a.inv_cols : 0.0f;
+        float s[2] = {0.0f, 0.0f};
+        pair_sum<U, LAYER>(s, gh, x, c, ragged);
+        team_sum<LAYER ? 2 : 1, kSmall>(s, a.lanes, slots[set] + 32);
+        s[0] *= st[1] * a.inv_cols;
+        s[1] *= st[1] * a.inv_cols;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
           for (int i = 0; i < kGroup; ++i) {
-            gh[u].v[i] = st[1] * (gh[u].v[i] * wpost[u].v[i] - x[u].v[i] * s[0] - s[1]);
+            const float rest = x[u].v[i] * -s[0];
+            gh[u].v[i] =
+                __builtin_fmaf(st[1], gh[u].v[i], LAYER ? rest - s[1] : rest);
           }
         }
       }
@@ -472,16 +559,26 @@ __global__ __launch_bounds__(THREADS) void block_norms_bwd(Backward a) {
       for (int u = 0; u < U; ++u) {
         if (valid && c.skip[u] < kGroup) store8(static_cast<T*>(a.dx) + at + c.col[u], gh[u]);
       }
+      set ^= 1;
+    };
+    // Two sets of registers in turn: one would be copied, which waits for it.
+    Row even, odd;
+    if (kAhead) load(even, from);
+    for (int64_t first = from; first < to; first += a.teams) {
+      step(even, odd, first);
+      first += a.teams;
+      if (first >= to) break;
+      step(odd, even, first);
     }
     if (GATE && !by_row) {
       const bool whole = from == which * a.rows_per_gate && to == (which + 1) * a.rows_per_gate;
       if (whole) {
         T* out = static_cast<T*>(a.dgate) + which * a.cols;
-        flush(acc[kGate], [&](int j, float s) { store1(out + j, s); });
+        flush(acc[kGate], [&](int j, float s) { store1(out + j, s * a.scale); });
       } else {
         float* out = a.part + (static_cast<int64_t>(kGate) * a.blocks + 2 * blockIdx.x +
                                (from == begin ? 0 : 1)) * a.cols;
-        flush(acc[kGate], [&](int j, float s) { out[j] = s; });
+        flush(acc[kGate], [&](int j, float s) { out[j] = s * a.scale; });
       }
     }
     from = to;
@@ -503,48 +600,57 @@ struct Join {
   int cols;
   int64_t rows_per_gate;
   int blocks;
+  bool by_boundary;
 };
 
-// The workgroups' column sums added in their order: 64 columns by 16 parts of
+// The workgroup that row `row` falls to.
+__device__ __forceinline__ int block_of(int64_t row, int64_t rows, int blocks) {
+  int b = static_cast<int>(row * blocks / rows);
+  while (b + 1 < blocks && first_row(rows, b + 1, blocks) <= row) ++b;
+  return b;
+}
+
+// The workgroups' column sums added in their order: 32 columns by 32 parts of
 // the workgroups, the parts joined through LDS.  blockIdx.y: one of the four
-// sums over all rows, or (from 4 on) the gate that a boundary between two
-// workgroups lies in, where it is the first in that gate.
+// sums over all rows, or from 4 on a gate: each, or (`by_boundary`, where there
+// are more gates than workgroups) the one that the boundary behind a workgroup
+// lies in, where it is the first in that gate.
 template <typename T>
 __global__ __launch_bounds__(1024) void join_sums(Join a) {
-  __shared__ float parts[16][64];
-  const int col = blockIdx.x * 64 + threadIdx.x % 64;
-  const int part = threadIdx.x / 64;
+  __shared__ float parts[32][33];
+  const int col = blockIdx.x * 32 + threadIdx.x % 32;
+  const int part = threadIdx.x / 32;
   const int k = min(static_cast<int>(blockIdx.y), static_cast<int>(kGate));
   if (!a.out[k]) return;
   int lo = 0, hi = a.blocks;
   int64_t gate = 0;
+  bool second = false;  // whether workgroup `lo` has the gate as its last segment
   if (k == kGate) {
-    lo = blockIdx.y - kGate;  // the boundary after workgroup `lo`
-    const int64_t row = first_row(a.rows, lo + 1, a.blocks);
-    gate = row / a.rows_per_gate;
+    const int at = blockIdx.y - kGate;
+    gate = a.by_boundary ? first_row(a.rows, at + 1, a.blocks) / a.rows_per_gate : at;
     const int64_t from = gate * a.rows_per_gate;
-    if (row == from || first_row(a.rows, lo, a.blocks) > from) return;
-    hi = lo + 1;
-    while (hi < a.blocks && first_row(a.rows, hi, a.blocks) < from + a.rows_per_gate) ++hi;
+    lo = block_of(from, a.rows, a.blocks);
+    hi = block_of(from + a.rows_per_gate - 1, a.rows, a.blocks) + 1;
+    // Within one workgroup: written there.  Another boundary is the gate's first.
+    if (hi == lo + 1 || (a.by_boundary && lo != at)) return;
+    second = first_row(a.rows, lo, a.blocks) < from;
   }
   float s = 0.0f;
   if (col < a.cols) {
+    // kGate: two places a workgroup, the first for the segment it begins with.
+    const int64_t step = k == kGate ? 2 * a.cols : a.cols;
     const float* p = a.part + static_cast<int64_t>(k) * a.blocks * a.cols + col;
-    const int n = hi - lo;
-    const int end = lo + n * (part + 1) / 16;
-    for (int b = lo + n * part / 16; b < end; ++b) {
-      int64_t place = b;
-      if (k == kGate) {
-        place = 2 * b + (first_row(a.rows, b, a.blocks) < gate * a.rows_per_gate ? 1 : 0);
-      }
-      s += p[place * a.cols];
+    const int n = hi - lo, end = n * (part + 1) / 32;
+#pragma unroll 4
+    for (int b = n * part / 32; b < end; ++b) {
+      s += p[(lo + b) * step + (b == 0 && second ? a.cols : 0)];
     }
   }
-  parts[part][threadIdx.x % 64] = s;
+  parts[part][threadIdx.x % 32] = s;
   __syncthreads();
   if (part == 0 && col < a.cols) {
     s = 0.0f;
-    for (int i = 0; i < 16; ++i) s += parts[i][threadIdx.x];
+    for (int i = 0; i < 32; ++i) s += parts[i][threadIdx.x];
     store1(static_cast<T*>(a.out[k]) + gate * a.cols + col, s);
   }
 }
@@ -590,51 +696,61 @@ int run_fwd(const Forward& a, bool layer, hipStream_t stream) {
   return check_launch("block_norms");
 }
 
-template <typename T, int U, bool LAYER, bool PRE, bool POST, int THREADS>
+template <typename T, int U, bool SMALL, bool LAYER, bool PRE, bool POST, int THREADS>
 void launch_bwd(const Backward& a, hipStream_t stream) {
   const dim3 grid(a.blocks), block(a.lanes * a.teams);
   const size_t lds = a.teams > 1 ? sizeof(float) * a.teams * a.cols : 0;
-  if (a.gate) {
-    block_norms_bwd<T, U, LAYER, PRE, POST, true, THREADS><<<grid, block, lds, stream>>>(a);
+  if (!a.gate) {
+    block_norms_bwd<T, U, SMALL, LAYER, PRE, POST, kNoGate, THREADS>
+        <<<grid, block, lds, stream>>>(a);
+  } else if (a.rows_per_gate == 1) {
+    block_norms_bwd<T, U, SMALL, LAYER, PRE, POST, kGateByRow, THREADS>
+        <<<grid, block, lds, stream>>>(a);
   } else {
-    block_norms_bwd<T, U, LAYER, PRE, POST, false, THREADS><<<grid, block, lds, stream>>>(a);
+    block_norms_bwd<T, U, SMALL, LAYER, PRE, POST, kGateOfRows, THREADS>
+        <<<grid, block, lds, stream>>>(a);
   }
 }
 
-template <typename T, int U, int THREADS>
+template <typename T, int U, bool SMALL, int THREADS>
 void launch_bwd(const Backward& a, bool layer, hipStream_t stream) {
   if (a.pre && a.post) {
-    layer ? launch_bwd<T, U, true, true, true, THREADS>(a, stream)
-          : launch_bwd<T, U, false, true, true, THREADS>(a, stream);
+    layer ? launch_bwd<T, U, SMALL, true, true, true, THREADS>(a, stream)
+          : launch_bwd<T, U, SMALL, false, true, true, THREADS>(a, stream);
   } else if (a.pre) {
-    layer ? launch_bwd<T, U, true, true, false, THREADS>(a, stream)
-          : launch_bwd<T, U, false, true, false, THREADS>(a, stream);
+    layer ? launch_bwd<T, U, SMALL, true, true, false, THREADS>(a, stream)
+          : launch_bwd<T, U, SMALL, false, true, false, THREADS>(a, stream);
   } else {
-    layer ? launch_bwd<T, U, true, false, true, THREADS>(a, stream)
-          : launch_bwd<T, U, false, false, true, THREADS>(a, stream);
+    layer ? launch_bwd<T, U, SMALL, true, false, true, THREADS>(a, stream)
+          : launch_bwd<T, U, SMALL, false, false, true, THREADS>(a, stream);
   }
 }
 
 // Workgroups of the gradient: no more than there are rows for their teams.
 int bwd_blocks(int64_t rows, int64_t cols) {
-  const Layout l = layout_of(cols);
-  return static_cast<int>(std::min<int64_t>((rows + l.teams - 1) / l.teams, 512));
+  const Layout l = layout_of(cols, bwd_groups(cols));
+  return static_cast<int>(std::min<int64_t>((rows + l.teams - 1) / l.teams, 256));
 }
 
 template <typename T>
 int run_bwd(const Backward& a, Join j, bool layer, hipStream_t stream) {
   if (a.cols <= kSmallCols) {
-    launch_bwd<T, 1, 512>(a, layer, stream);
+    launch_bwd<T, 1, true, 512>(a, layer, stream);
+  } else if (bwd_groups(a.cols) == 1) {
+    launch_bwd<T, 1, false, 512>(a, layer, stream);
   } else if (a.lanes * a.teams <= 512) {
-    launch_bwd<T, 2, 512>(a, layer, stream);
+    launch_bwd<T, 2, false, 512>(a, layer, stream);
   } else {
-    launch_bwd<T, 2, 1024>(a, layer, stream);
+    launch_bwd<T, 2, false, 1024>(a, layer, stream);
   }
   const int rc = check_launch("block_norms_bwd");
   if (rc != 0) return rc;
-  const bool gates = a.gate && a.rows_per_gate != 1;
-  join_sums<T><<<dim3((a.cols + 63) / 64, kGate + (gates ? a.blocks - 1 : 0)),
-                 1024, 0, stream>>>(j);
+  // Gates whose rows may lie in several workgroups.
+  int64_t gates = a.gate && a.rows_per_gate != 1 ? a.rows / a.rows_per_gate : 0;
+  j.by_boundary = gates > a.blocks;
+  gates = std::min<int64_t>(gates, j.by_boundary ? a.blocks - 1 : gates);
+  join_sums<T><<<dim3((a.cols + 31) / 32, static_cast<uint32_t>(kGate + gates)), 1024, 0,
+                 stream>>>(j);
   return check_launch("block_norms_bwd: join_sums");
 }
 
@@ -655,7 +771,7 @@ extern "C" int hipo_block_norms(const void* x, const void* residual, int elem_si
   HIPO_REQUIRE(eps >= 0.0f && __builtin_isfinite(eps), "block_norms: eps must be finite, not negative");
   if (rows == 0) return 0;
   HIPO_REQUIRE(x && residual && h && stats && (y || !pre), "block_norms: null pointer");
-  const Layout l = layout_of(cols);
+  const Layout l = layout_of(cols, 2);
   const Forward a{x, residual, post, post_bias, pre, pre_bias, gate, h, y, stats, rows,
                   static_cast<int>(cols), gate_rows ? rows / gate_rows : rows, scale, offset, eps,
                   1.0f / static_cast<float>(cols), l.lanes, l.teams};
@@ -696,14 +812,14 @@ extern "C" int hipo_block_norms_bwd(const void* grad_h, const void* grad_y, cons
   const size_t need = hipo_block_norms_bwd_workspace_bytes(rows, cols);
   HIPO_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
                "%s: workspace of %zu bytes, 16-byte aligned, needed", what, need);
-  const Layout l = layout_of(cols);
+  const Layout l = layout_of(cols, bwd_groups(cols));
   const int64_t rows_per_gate = gate_rows ? rows / gate_rows : rows;
   const int blocks = bwd_blocks(rows, cols);
   const Backward a{grad_h, grad_y, x, h, stats, post, post_bias, pre, gate, dx, dresidual, dgate,
                    static_cast<float*>(workspace), rows, static_cast<int>(cols), rows_per_gate,
                    scale, offset, 1.0f / static_cast<float>(cols), l.lanes, l.teams, blocks};
   const Join j{a.part, {dpre, dpre_bias, dpost, dpost_bias, rows_per_gate == 1 ? nullptr : dgate},
-               rows, a.cols, rows_per_gate, blocks};
+               rows, a.cols, rows_per_gate, blocks, false};
   return elem_size == 2 ? run_bwd<uint16_t>(a, j, layer != 0, stream)
                         : run_bwd<float>(a, j, layer != 0, stream);
 }

@@ -81,18 +81,20 @@ __global__ __launch_bounds__(1024) void select_rows(Select a) {
   if (threadIdx.x == 0) *a.count = base;
 }
 
-// The bf16 parts of x, each the nearest to what the ones before leave; a part
-// that would overflow is cut instead.  What is not finite has no second part.
-__device__ __forceinline__ void split3(float x, uint16_t (&part)[3]) {
+// The next bf16 part of x, the nearest one, and what it leaves in x.  A part
+// that would overflow is cut instead; what is not finite leaves 0.
+__device__ __forceinline__ uint16_t next_part(float& x) {
   const uint32_t bits = __float_as_uint(x);
-  uint32_t first = pack_bf16x2(x, 0.0f) & 0xffffu;
+  uint32_t part = pack_bf16x2(x, 0.0f) & 0xffffu;
   const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
-  if (finite && (first & 0x7f80u) == 0x7f80u) first = bits >> 16;
-  const float rest = finite ? x - bf16lo(first) : 0.0f;
-  const uint32_t second = pack_bf16x2(rest, 0.0f) & 0xffffu;
-  part[0] = static_cast<uint16_t>(first);
-  part[1] = static_cast<uint16_t>(second);
-  part[2] = static_cast<uint16_t>(pack_bf16x2(rest - bf16lo(second), 0.0f));
+  if (finite && (part & 0x7f80u) == 0x7f80u) part = bits >> 16;
+  x = finite ? x - bf16lo(part) : 0.0f;
+  return static_cast<uint16_t>(part);
+}
+
+__device__ __forceinline__ void split3(float x, uint16_t (&part)[3]) {
+#pragma unroll
+  for (int q = 0; q < 3; ++q) part[q] = next_part(x);
 }
 
 struct Pack {
@@ -544,54 +546,115 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       const int j = j0 + n * 16;
-      const bool inside = j < rows_b;
-      float g = 0.0f, both = 0.0f, lse = 0.0f;
+      float g = 0.0f, both = 0.0f, lse = 0.0f;  // of rows past the last, whose products are 0
       int64_t tok = -1;
-      if (inside) {
+      if (j < rows_b) {
         const int row = p.kept[j];
         tok = token_at(p.tokens, p.token_size, row);
         g = p.grad[row];
         if (tok < 0 || tok >= p.vocab) g = __builtin_nanf("");
         both = p.grad_lse ? g + p.grad_lse[row] : g;
         lse = p.lse[row];
-        tok -= p.first;
+        tok -= p.first + i0;
       }
+      both *= p.scale;
 #pragma unroll
       for (int f = 0; f < 8; ++f) {
-        const int i = i0 + f * 16;
-        float v[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = exp_f32(exp_domain(acc[f][n][r] * p.scale - lse));
-          const float d = (both * e - (i + r == tok ? g : 0.0f)) * p.scale;
-          v[r] = inside && i + r < p.a_rows ? d : 0.0f;
+          const float ln_p = __builtin_fmaf(acc[f][n][r], p.scale, -lse);
+          acc[f][n][r] = both * __builtin_amdgcn_exp2f(ln_p * kLog2eHi);
         }
-        uint16_t part[4][3];
+      }
+      if (tok >= 0 && tok < 116) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (sizeof(T) == 2) {
-            part[r][0] = static_cast<uint16_t>(pack_bf16x2(v[r], 0.0f));
-          } else {
-            split3(v[r], part[r]);
+        for (int f = 0; f < 8; ++f) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (tok == f * 16 + r) acc[f][n][r] -= g * p.scale;
           }
         }
+      }
+    }
+    if (tile_a + 1 == tiles_a) {
 #pragma unroll
-        for (int q = 0; q < (sizeof(T) == 2 ? 1 : 3); ++q) {
-          *reinterpret_cast<u32x2_t*>(p.d + q * p.d_plane + j * p.d_ld + i) =
-              u32x2_t{part[0][q] | uint32_t{part[1][q]} << 16,
-                      part[2][q] | uint32_t{part[3][q]} << 16};
+      for (int f = 0; f < 8; ++f) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (i0 + f * 16 + r >= p.a_rows) acc[f][n][r] = 0.0f;
+          }
         }
       }
     }
   }
 
-  if (E == kAccumulate || E == kStore) {
+  if constexpr (E == kLogitGrad || (E == kStore && sizeof(T) == 2)) {
+    // bf16 through LDS, so that 32 lanes store 512 consecutive bytes of a row
+    // (straight from the registers a store is 32 bytes of each of 16 rows: the
+    // gradients of 256 x 4096 x 128000 took 0.72 ms for dweight's 1 GB).  The
+    // 16-byte piece c of row j lies at place c ^ (j % 32).
+#pragma unroll
+    for (int q = 0; q < (E == kLogitGrad ? kPasses == 1 ? 1 : 3 : 1); ++q) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int j = wave_b + n * 16 + (lane & 15);
+#pragma unroll
+        for (int f = 0; f < 8; ++f) {
+          const int i = wave_a + f * 16 + (lane >> 4) * 4;
+          u32x2_t v;
+          if (sizeof(T) == 2) {
+            v = u32x2_t{pack_bf16x2(acc[f][n][0], acc[f][n][1]),
+                        pack_bf16x2(acc[f][n][2], acc[f][n][3])};
+          } else {
+            uint32_t part[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              float x = acc[f][n][r];
+              part[r] = next_part(x);
+              acc[f][n][r] = x;
+            }
+            v = u32x2_t{part[0] | part[1] << 16, part[2] | part[3] << 16};
+            asm volatile("" : "+v"(acc[f][n]));  // what is left takes its place: no spills
+          }
+          *reinterpret_cast<u32x2_t*>(lds + j * kTile + (((i >> 3) ^ (j & 31)) << 3) + (i & 7)) = v;
+        }
+      }
+      __syncthreads();
+      const int piece = lane & 31;
+      const int i = tile_a * kTile + piece * 8;
+#pragma unroll 4
+      for (int r = 0; r < 16; ++r) {
+        const int j = r * 16 + wave * 2 + (lane >> 5);
+        const u32x4_t v =
+            *reinterpret_cast<const u32x4_t*>(lds + j * kTile + ((piece ^ (j & 31)) << 3));
+        if (E == kLogitGrad) {
+          *reinterpret_cast<u32x4_t*>(p.d + q * p.d_plane +
+                                      (tile_b * static_cast<int64_t>(kTile) + j) * p.d_ld + i) = v;
+        } else if (j < valid_b) {
+          uint16_t* out = static_cast<uint16_t*>(p.out) +
+                          (tile_b * static_cast<int64_t>(kTile) + j) * p.out_ld + i;
+          if (i + 8 <= p.a_rows) {
+            *reinterpret_cast<u32x4_a2_t*>(out) = v;
+          } else {
+#pragma unroll
+            for (int m = 0; m < 7; ++m) {
+              if (i + m < p.a_rows) out[m] = static_cast<uint16_t>(v[m >> 1] >> (m & 1) * 16);
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+  } else if constexpr (E == kAccumulate || E == kStore) {
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
       const int j = j0 + n * 16;
       asm volatile("" ::: "memory");  // no loads of later rows ahead of this one's
       if (j >= rows_b) continue;
-      T* out = static_cast<T*>(p.out) + (E == kStore ? j : (p.to_out ? p.kept[j] : 0)) * p.out_ld;
+      T* out = static_cast<T*>(p.out) +
+               static_cast<int64_t>(E == kStore ? j : (p.to_out ? p.kept[j] : 0)) * p.out_ld;
 #pragma unroll
       for (int f = 0; f < 8; ++f) {
         const int i = i0 + f * 16;
@@ -621,35 +684,39 @@ struct JoinLoss {
   float *loss, *lse;
 };
 
-// 64 rows by 4 parts of the vocabulary's tiles per workgroup.
+// One tile's maximum and sum joined to the ones so far, and the loss of a row:
+// with the logit's distance from the maximum, which is exact where they are near.
+__device__ __forceinline__ void join_one(float& top, float& sum, float2 v) {
+  const float m = fmaxf(top, v.x);
+  sum = sum * exp_f32(exp_domain(top - m)) + v.y * exp_f32(exp_domain(v.x - m));
+  top = m;
+}
+
+__device__ __forceinline__ void put_loss(float top, float sum, float target, float* loss,
+                                         float* lse) {
+  const float log_sum = logf(sum);
+  *lse = top + log_sum;
+  *loss = log_sum - (target - top);
+}
+
+// 16 rows by 16 parts of the vocabulary's tiles per workgroup.
 __global__ __launch_bounds__(256) void join_loss(JoinLoss a) {
-  __shared__ float2 parts[4][64];
+  __shared__ float2 parts[16][16];
   const int count = *a.count;
-  const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
-  for (int64_t first = static_cast<int64_t>(blockIdx.x) * 64; first < count;
-       first += static_cast<int64_t>(gridDim.x) * 64) {
-    const int64_t j = first + lane;
+  const int row = threadIdx.x & 15, part = threadIdx.x >> 4;
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * 16; first < count;
+       first += static_cast<int64_t>(gridDim.x) * 16) {
+    const int64_t j = first + row;
     float top = -kLargest, sum = 0.0f;
     if (j < count) {
-      for (int t = part; t < a.tiles; t += 4) {
-        const float2 v = a.part[t * a.part_ld + j];
-        const float m = fmaxf(top, v.x);
-        sum = sum * exp_f32(exp_domain(top - m)) + v.y * exp_f32(exp_domain(v.x - m));
-        top = m;
-      }
+#pragma unroll 8
+      for (int t = part; t < a.tiles; t += 16) join_one(top, sum, a.part[t * a.part_ld + j]);
     }
-    parts[part][lane] = make_float2(top, sum);
+    parts[part][row] = make_float2(top, sum);
     __syncthreads();
     if (part == 0 && j < count) {
-      for (int q = 1; q < 4; ++q) {
-        const float2 v = parts[q][lane];
-        const float m = fmaxf(top, v.x);
-        sum = sum * exp_f32(exp_domain(top - m)) + v.y * exp_f32(exp_domain(v.x - m));
-        top = m;
-      }
-      const float lse = top + logf(sum);
-      a.lse[a.kept[j]] = lse;
-      a.loss[a.kept[j]] = lse - a.target[j];
+      for (int q = 1; q < 16; ++q) join_one(top, sum, parts[q][row]);
+      put_loss(top, sum, a.target[j], a.loss + a.kept[j], a.lse + a.kept[j]);
     }
     __syncthreads();
   }
@@ -685,6 +752,222 @@ __global__ __launch_bounds__(256) void zero_rows(const void* tokens, int token_s
 }
 
 // ---------------------------------------------------------------------------
+// Few rows: the vocabulary is read once, as it lies
+// ---------------------------------------------------------------------------
+
+struct Thin {
+  const void *hidden, *weight, *tokens;
+  int token_size, rows, width;
+  int64_t vocab, hidden_ld, weight_ld;
+  float scale;
+  float2* part;  // [rows][tiles] maximum and sum
+  float* target;
+  int64_t tiles;
+};
+
+constexpr int kThinRows = 64;   // at most
+constexpr int kThinTile = 64;   // of the vocabulary
+constexpr int kThinStages = 4;  // loads in flight, in rounds of kStep values of K
+
+// 8 values of a row from column k on, zeros from `width` on.
+template <typename T>
+struct Piece;
+template <>
+struct Piece<uint16_t> {
+  u32x4_t w;
+  __device__ __forceinline__ void load(const uint16_t* row, int k, int width) {
+    if (k + 8 <= width) {
+      w = *reinterpret_cast<const u32x4_a2_t*>(row + k);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = k + 2 * i < width ? row[k + 2 * i] : 0;
+        const uint32_t hi = k + 2 * i + 1 < width ? row[k + 2 * i + 1] : 0;
+        w[i] = lo | hi << 16;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(uint16_t* to, int) const {
+    *reinterpret_cast<u32x4_t*>(to) = w;
+  }
+};
+template <>
+struct Piece<float> {
+  f32x4_t v[2];
+  __device__ __forceinline__ void load(const float* row, int k, int width) {
+    if (k + 8 <= width) {
+      v[0] = *reinterpret_cast<const f32x4_a4_t*>(row + k);
+      v[1] = *reinterpret_cast<const f32x4_a4_t*>(row + k + 4);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = k + i < width ? row[k + i] : 0.0f;
+    }
+  }
+  __device__ __forceinline__ void store(uint16_t* to, int plane) const {
+    uint16_t part[8][3];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) split3(v[i >> 2][i & 3], part[i]);
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+      u32x4_t w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = part[2 * i][q] | uint32_t{part[2 * i + 1][q]} << 16;
+      *reinterpret_cast<u32x4_t*>(to + q * plane) = w;
+    }
+  }
+};
+
+// The logits of up to 16 N rows against 64 of the vocabulary per workgroup, 16 a
+// wave, reduced as gemm()'s.  Both operands go through registers, kThinStages
+// rounds ahead, to LDS (places as in Operand): the weight is read once, at any
+// alignment, fp32 split on the way.  Memory bounds it: the loads in flight
+// (32 KB a workgroup of bf16) and the number of workgroups are what counts.
+template <typename T, int N>
+__global__ __launch_bounds__(256) void thin_logits(Thin a) {
+  constexpr int kPlanes = sizeof(T) == 2 ? 1 : 3, kPasses = kPlanes == 1 ? 1 : 6;
+  constexpr int kPlaneW = kThinTile * kStep, kPlaneH = 16 * N * kStep;
+  constexpr int kPiecesH = (N + 1) / 2;
+  __shared__ __attribute__((aligned(16))) uint16_t weight[2][kPlanes * kPlaneW];
+  __shared__ __attribute__((aligned(16))) uint16_t hidden[2][kPlanes * kPlaneH];
+  __shared__ float2 parts[4][16 * N];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int l = lane & 15, g = lane >> 4;
+  const int row = threadIdx.x >> 3, chunk = threadIdx.x & 7;
+  const int place = row * kStep + ((chunk ^ (row & 7)) * 8);  // and 32 rows on
+  const float to_log2 = a.scale * kLog2eHi;
+  const bool with_h = N > 1 || threadIdx.x < 128;
+  const T* from_h[kPiecesH];
+#pragma unroll
+  for (int q = 0; q < kPiecesH; ++q) {
+    from_h[q] = static_cast<const T*>(a.hidden) +
+                static_cast<int64_t>(min(row + 32 * q, a.rows - 1)) * a.hidden_ld;
+  }
+  for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+    const int64_t first = tile * kThinTile;
+    const T* from_w[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      from_w[q] = static_cast<const T*>(a.weight) +
+                  min(first + row + 32 * q, a.vocab - 1) * a.weight_ld;
+    }
+    Piece<T> w[kThinStages][2], h[kThinStages][kPiecesH];
+    auto load = [&](int stage, int k0) __attribute__((always_inline)) {
+      const int k = k0 + chunk * 8;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) w[stage][q].load(from_w[q], k, a.width);
+      if (with_h) {
+#pragma unroll
+        for (int q = 0; q < kPiecesH; ++q) h[stage][q].load(from_h[q], k, a.width);
+      }
+    };
+    f32x4_t acc[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) acc[n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int s = 0; s < kThinStages; ++s) load(s, s * kStep);
+    for (int k0 = 0; k0 < a.width; k0 += kThinStages * kStep) {
+#pragma unroll
+      for (int s = 0; s < kThinStages; ++s) {
+        if (k0 + s * kStep >= a.width) break;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          w[s][q].store(weight[s & 1] + place + q * 32 * kStep, kPlaneW);
+        }
+        if (with_h) {
+#pragma unroll
+          for (int q = 0; q < kPiecesH; ++q) {
+            h[s][q].store(hidden[s & 1] + place + q * 32 * kStep, kPlaneH);
+          }
+        }
+        load(s, k0 + (s + kThinStages) * kStep);
+        // One barrier a round: a buffer is written again behind the next one's.
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int at = l * kStep + (((half * 4 + g) ^ (l & 7)) * 8);
+          bf16x8_t fw[kPlanes], fh[kPlanes][N];
+#pragma unroll
+          for (int q = 0; q < kPlanes; ++q) {
+            fw[q] = *reinterpret_cast<const bf16x8_t*>(weight[s & 1] + q * kPlaneW +
+                                                       wave * 16 * kStep + at);
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+              fh[q][n] = *reinterpret_cast<const bf16x8_t*>(hidden[s & 1] + q * kPlaneH +
+                                                            n * 16 * kStep + at);
+            }
+          }
+#pragma unroll
+          for (int pass = 0; pass < kPasses; ++pass) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+              acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  fw[a_part(pass, kPasses)], fh[b_part(pass, kPasses)][n], acc[n], 0, 0, 0);
+            }
+          }
+        }
+      }
+    }
+    const int64_t i0 = first + wave * 16 + g * 4;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int j = n * 16 + l;
+      const int64_t tok = j < a.rows ? token_at(a.tokens, a.token_size, j) : -1;
+      float top = -kLargest;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (i0 + r >= a.vocab) acc[n][r] = -INFINITY;
+        if (i0 + r == tok && tok < a.vocab) a.target[j] = acc[n][r] * a.scale;
+        top = fmaxf(top, acc[n][r]);
+      }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      top = fminf(top, kLargest);
+      float sum = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f((acc[n][r] - top) * to_log2);
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      if (g == 0) parts[wave][j] = make_float2(top * a.scale, sum);
+    }
+    __syncthreads();
+    const int j = threadIdx.x;
+    if (j < a.rows) {
+      float top = parts[0][j].x, sum = parts[0][j].y;
+#pragma unroll
+      for (int q = 1; q < 4; ++q) join_one(top, sum, parts[q][j]);
+      a.part[j * a.tiles + tile] = make_float2(top, sum);
+    }
+    __syncthreads();
+  }
+}
+
+// One workgroup a row.
+__global__ __launch_bounds__(256) void join_thin(Thin a, int64_t ignore_index, float* loss,
+                                                 float* lse) {
+  __shared__ float2 parts[4];
+  const int j = blockIdx.x;
+  const int64_t tok = token_at(a.tokens, a.token_size, j);
+  if (tok == ignore_index) {
+    if (threadIdx.x == 0) loss[j] = lse[j] = 0.0f;
+    return;
+  }
+  float top = -kLargest, sum = 0.0f;
+#pragma unroll 4
+  for (int64_t t = threadIdx.x; t < a.tiles; t += 256) join_one(top, sum, a.part[j * a.tiles + t]);
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    join_one(top, sum, make_float2(__shfl_xor(top, o), __shfl_xor(sum, o)));
+  }
+  if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = make_float2(top, sum);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int q = 1; q < 4; ++q) join_one(top, sum, parts[q]);
+    const bool known = tok >= 0 && tok < a.vocab;
+    put_loss(top, sum, known ? a.target[j] : __builtin_nanf(""), loss + j, lse + j);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
 
@@ -701,12 +984,18 @@ struct Plan {
 constexpr int64_t kCus = 256;
 constexpr int64_t kMostTiles = int64_t{1} << 22;  // 2^31 threads
 constexpr int64_t kMostRows = (int64_t{1} << 22) - kTile;  // a tile's bytes fit 31 bits
-constexpr size_t kForwardBytes = size_t{256} << 20;   // of a copied piece
+constexpr size_t kForwardBytes = size_t{1024} << 20;  // of a copied piece
 constexpr size_t kBackwardBytes = size_t{1536} << 20;  // of a piece's d and copies
 
 Plan plan_of(const void* weight, int elem_size, int64_t rows, int64_t width, int64_t vocab,
              int64_t weight_ld, bool backward) {
   Plan p{};
+  if (!backward && rows <= kThinRows) {
+    p.target = 0;
+    p.part = up(sizeof(float) * rows, 256);
+    p.bytes = p.part + sizeof(float2) * rows * (up(vocab, kThinTile) / kThinTile);
+    return p;
+  }
   p.planes = elem_size == 2 ? 1 : 3;
   p.direct = elem_size == 2 && aligned16(weight) && weight_ld % 8 == 0 && width % 8 == 0;
   p.rows_pad = up(rows, kTile);
@@ -863,8 +1152,29 @@ int select_and_pack(const char* what, const Call& c, const Plan& plan, float* lo
 }
 
 template <typename T>
+int run_thin(const Call& c, const Plan& plan, float* loss, float* lse) {
+  const char* what = "linear_cross_entropy";
+  const Thin a{c.hidden,    c.weight,    c.tokens, c.token_size, static_cast<int>(c.rows),
+               static_cast<int>(c.width), c.vocab, c.hidden_ld,  c.weight_ld,
+               c.scale,     c.at<float2>(plan.part), c.at<float>(plan.target),
+               up(c.vocab, kThinTile) / kThinTile};
+  const uint32_t grid = static_cast<uint32_t>(std::min<int64_t>(a.tiles, 1 << 20));
+  if (c.rows <= 16) {
+    thin_logits<T, 1><<<grid, 256, 0, c.stream>>>(a);
+  } else if (c.rows <= 32) {
+    thin_logits<T, 2><<<grid, 256, 0, c.stream>>>(a);
+  } else {
+    thin_logits<T, 4><<<grid, 256, 0, c.stream>>>(a);
+  }
+  HIPO_STEP(check_launch(what));
+  join_thin<<<static_cast<uint32_t>(c.rows), 256, 0, c.stream>>>(a, c.ignore_index, loss, lse);
+  return check_launch(what);
+}
+
+template <typename T>
 int run_fwd(const Call& c, const Plan& plan, float* loss, float* lse) {
   const char* what = "linear_cross_entropy";
+  if (c.rows <= kThinRows) return run_thin<T>(c, plan, loss, lse);
   Product g{};
   HIPO_STEP(select_and_pack<T>(what, c, plan, loss, lse, &g));
   g.part = c.at<float2>(plan.part);
@@ -874,7 +1184,7 @@ int run_fwd(const Call& c, const Plan& plan, float* loss, float* lse) {
     g.first_tile = i * plan.piece / kTile;
     HIPO_STEP((multiply<T, kReduce>(what, g, c.rows, c.stream)));
   }
-  join_loss<<<static_cast<uint32_t>(std::min<int64_t>((c.rows + 63) / 64, 1 << 16)), 256, 0,
+  join_loss<<<static_cast<uint32_t>(std::min<int64_t>((c.rows + 15) / 16, 1 << 16)), 256, 0,
               c.stream>>>(JoinLoss{g.part, g.part_ld, static_cast<int>(up(c.vocab, kTile) / kTile),
                                    g.kept, g.b_count, g.target, loss, lse});
   return check_launch(what);
