@@ -917,25 +917,44 @@ def embedding_bwd(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, scale
 
 def _require_block_norms(what, x, rows_of, post, post_bias, pre, pre_bias, gate, norm):
     """(device, rows, cols, gate rows, layer) of block_norms and its gradient."""
+    # One pass over the operands, whose attributes cost about 0.1 us each; what is
+    # wrong is found again below, for its message.
+    dev, dtype, shape = x.device, x.dtype, x.shape
+    ok = (x.is_cuda and _IS_ROCM and dtype in _FLOATS and len(shape) == 2 and x.is_contiguous()
+          and norm in _NORMS)
+    if ok:
+        rows, cols = shape
+        for t in rows_of:
+            ok = (ok and t.dtype == dtype and t.shape == shape and t.device == dev
+                  and t.is_contiguous())
+        for t in (post, post_bias, pre, pre_bias):
+            ok = ok and (t is None or (t.dtype == dtype and t.shape == (cols,) and t.device == dev
+                                       and t.is_contiguous()))
+        gates = 0
+        if gate is not None and ok:
+            gates = 1 if gate.dim() == 1 else gate.shape[0]
+            ok = (gate.dtype == dtype and gate.dim() in (1, 2) and gate.shape[-1] == cols
+                  and gate.device == dev and gate.is_contiguous() and gates > 0
+                  and rows % gates == 0)
+        if ok:
+            return dev, rows, cols, gates, _NORMS[norm]
     vectors = [t for t in (post, post_bias, pre, pre_bias) if t is not None]
-    dev = _require_rocm(x, *rows_of, *vectors, *(() if gate is None else (gate,)))
-    _require(x.dtype in _FLOATS and x.dim() == 2, f"{what}: 2-D bf16 or fp32 rows required")
-    rows, cols = x.shape
+    _require_rocm(x, *rows_of, *vectors, *(() if gate is None else (gate,)))
+    _require(dtype in _FLOATS and len(shape) == 2, f"{what}: 2-D bf16 or fp32 rows required")
     for t in (x, *rows_of):
-        if not (t.dtype == x.dtype and t.shape == x.shape and t.is_contiguous()):
-            raise ValueError(f"{what}: the rows must be contiguous [R, C] of one type")
+        _require(t.dtype == dtype and t.shape == shape and t.is_contiguous(),
+                 f"{what}: the rows must be contiguous [R, C] of one type")
     for t in vectors:
-        if not (t.dtype == x.dtype and t.shape == (cols,) and t.is_contiguous()):
-            raise ValueError(f"{what}: weights and biases must be contiguous [C] of the rows' type")
-    _require(norm in ("rms", "layer"), f"{what}: norm must be 'rms' or 'layer'")
-    gates = 0
-    if gate is not None:
-        _require(gate.dtype == x.dtype and gate.dim() in (1, 2) and gate.shape[-1] == cols
-                 and gate.is_contiguous(),
-                 f"{what}: gate must be contiguous [C] or [G, C] of the rows' type")
-        gates = gate.shape[0] if gate.dim() == 2 else 1
-        _require(gates > 0 and rows % gates == 0, f"{what}: gate's rows must divide the rows")
-    return dev, rows, cols, gates, 1 if norm == "layer" else 0
+        _require(t.dtype == dtype and t.shape == shape[1:] and t.is_contiguous(),
+                 f"{what}: weights and biases must be contiguous [C] of the rows' type")
+    _require(norm in _NORMS, f"{what}: norm must be 'rms' or 'layer'")
+    _require(gate.dtype == dtype and gate.dim() in (1, 2) and gate.shape[-1] == shape[1]
+             and gate.is_contiguous(),
+             f"{what}: gate must be contiguous [C] or [G, C] of the rows' type")
+    raise ValueError(f"{what}: gate's rows must divide the rows")
+
+
+_NORMS = {"rms": 0, "layer": 1}
 
 
 def _optional(t: torch.Tensor | None) -> int | None:
@@ -994,9 +1013,8 @@ def block_norms_bwd(grad_h: torch.Tensor | None, grad_y: torch.Tensor | None,
     rows_of = [t for t in (grad_h, grad_y, h) if t is not None]
     dev, rows, cols, gates, layer = _require_block_norms(
         what, x, rows_of, post, post_bias, pre, pre_bias, gate, norm)
-    _require_rocm(x, stats)
-    _require(stats.dtype == torch.float32 and stats.shape == (rows, 4) and stats.is_contiguous(),
-             "block_norms_bwd: stats must be contiguous fp32 [R, 4]")
+    _require(stats.device == dev and stats.dtype == torch.float32 and stats.shape == (rows, 4)
+             and stats.is_contiguous(), "block_norms_bwd: stats must be contiguous fp32 [R, 4]")
     dx, dresidual = torch.empty_like(x), torch.empty_like(x)
     made = torch.empty_like if rows else torch.zeros_like  # no rows: nothing is written
     sums = [None if t is None else made(t) for t in (gate, post, post_bias, pre, pre_bias)]
@@ -1010,26 +1028,44 @@ def block_norms_bwd(grad_h: torch.Tensor | None, grad_y: torch.Tensor | None,
     return (dx, dresidual, *sums)
 
 
-def _require_output_layer(what, hidden, weight, tokens, scale):
-    """(rows, width, vocab, row stride of hidden, of weight)."""
-    _require(hidden.dtype in _FLOATS and hidden.dim() == 2,
-             f"{what}: hidden must be 2-D bf16 or fp32")
-    _require(weight.dtype == hidden.dtype and weight.dim() == 2
-             and weight.shape[1] == hidden.shape[1],
+def _require_output_layer(what, hidden, weight, tokens, scale, rows_of=()):
+    """(device, rows, width, vocab, row stride of hidden, of weight)."""
+    # As in _require_block_norms: one pass, and the messages below.
+    dev, dtype, (vocab, _) = hidden.device, hidden.dtype, weight.shape
+    rows, width = hidden.shape
+    hstride, hinner = hidden.stride()
+    wstride, winner = weight.stride()
+    if rows <= 1:
+        hstride = width
+    if vocab <= 1:
+        wstride = width
+    ok = (hidden.is_cuda and _IS_ROCM and dtype in _FLOATS and weight.dtype == dtype
+          and weight.shape[1] == width and weight.device == dev and tokens.device == dev
+          and tokens.dtype in _TOKENS and tokens.shape == (rows,) and tokens.is_contiguous()
+          and vocab > 0 and width > 0 and 2.0 ** -100 <= scale <= 2.0 ** 100
+          and (hinner == winner == 1 or width == 1) and hstride >= width and wstride >= width)
+    for t in rows_of:
+        ok = (ok and t.dtype == torch.float32 and t.shape == (rows,) and t.device == dev
+              and t.is_contiguous())
+    if ok:
+        return dev, rows, width, vocab, hstride, wstride
+    _require_rocm(hidden, weight, tokens, *rows_of)
+    _require(dtype in _FLOATS, f"{what}: hidden must be 2-D bf16 or fp32")
+    _require(weight.dtype == dtype and weight.shape[1] == width,
              f"{what}: weight must be [V, D] of hidden's type")
     _require_tokens(what, tokens)
-    rows, width = hidden.shape
-    vocab = weight.shape[0]
     _require(tokens.shape == (rows,), f"{what}: tokens must be [R]")
     _require(vocab > 0 and width > 0, f"{what}: empty vocabulary or width")
     _require(2.0 ** -100 <= scale <= 2.0 ** 100, f"{what}: scale must be from 2^-100 to 2^100")
-    strides = []
-    for t, n in ((hidden, rows), (weight, vocab)):
-        _require(t.stride(1) == 1 or width == 1, f"{what}: unit inner strides required")
-        stride = t.stride(0) if n > 1 else width
-        _require(stride >= width, f"{what}: rows overlap")
-        strides.append(stride)
-    return rows, width, vocab, *strides
+    _require(hinner == winner == 1 or width == 1, f"{what}: unit inner strides required")
+    _require(hstride >= width and wstride >= width, f"{what}: rows overlap")
+    raise ValueError(f"{what}: grad, lse and grad_lse must be contiguous fp32 [R]")
+
+
+def _two_dimensions(what, hidden, weight):
+    for t in (hidden, weight):
+        if not (isinstance(t, torch.Tensor) and t.dim() == 2):
+            raise ValueError(f"{what}: hidden must be 2-D [R, D], weight [V, D] of hidden's type")
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor, *,
@@ -1044,9 +1080,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, tokens: tor
     NaN.  token_logprobs gives the negative loss of logits that are in memory."""
     lib = _lib or load_library()
     what = "linear_cross_entropy"
-    dev = _require_rocm(hidden, weight, tokens)
-    rows, width, vocab, hstride, wstride = _require_output_layer(what, hidden, weight, tokens,
-                                                                 scale)
+    _two_dimensions(what, hidden, weight)
+    dev, rows, width, vocab, hstride, wstride = _require_output_layer(what, hidden, weight,
+                                                                      tokens, scale)
     loss = torch.empty(rows, dtype=torch.float32, device=dev)
     lse = torch.empty_like(loss)
     need = int(lib.hipo_linear_cross_entropy_workspace_bytes(
@@ -1071,13 +1107,10 @@ def linear_cross_entropy_bwd(grad: torch.Tensor, hidden: torch.Tensor, weight: t
     outside [0, V) is NaN and makes dweight NaN."""
     lib = _lib or load_library()
     what = "linear_cross_entropy_bwd"
-    rows_of = [t for t in (grad, lse, grad_lse) if t is not None]
-    dev = _require_rocm(hidden, weight, tokens, *rows_of)
-    rows, width, vocab, hstride, wstride = _require_output_layer(what, hidden, weight, tokens,
-                                                                 scale)
-    for t in rows_of:
-        if not (t.dtype == torch.float32 and t.shape == (rows,) and t.is_contiguous()):
-            raise ValueError(f"{what}: grad, lse and grad_lse must be contiguous fp32 [R]")
+    _two_dimensions(what, hidden, weight)
+    dev, rows, width, vocab, hstride, wstride = _require_output_layer(
+        what, hidden, weight, tokens, scale,
+        (grad, lse) if grad_lse is None else (grad, lse, grad_lse))
     made = torch.empty if rows else torch.zeros  # no rows: nothing is written
     dhidden = made((rows, width), dtype=hidden.dtype, device=dev)
     dweight = made((vocab, width), dtype=hidden.dtype, device=dev)

@@ -25,9 +25,9 @@ namespace {
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef u32x2_t u32x2_a2_t __attribute__((aligned(2)));
 
-constexpr int kTile = 256;  // rows of either operand that a workgroup multiplies
-constexpr int kStep = 64;   // values of K per round
-constexpr int kThreads = 512;
+constexpr int kTile = 256;       // rows of either operand that a workgroup multiplies,
+constexpr int kSmallTile = 128;  // or where there are too few such tiles
+constexpr int kStep = 64;        // values of K per round
 constexpr float kLargest = 3.402823466e+38f;
 
 inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
@@ -106,6 +106,11 @@ struct Pack {
   int cols;
   uint16_t* dst;
   int64_t dst_ld, plane;  // of dst, in values
+  // Where a row's token is ignore_index, it gets zeros in `zero` (or null).
+  const void* tokens;
+  int token_size;
+  int64_t ignore_index;
+  void* zero;
 };
 
 __device__ __forceinline__ float value_at(const uint16_t* p) { return bf16_to_f32(*p); }
@@ -116,6 +121,14 @@ template <typename T>
 __global__ __launch_bounds__(256) void pack_rows(Pack a) {
   const int64_t rows = a.count ? *a.count : a.rows;
   const int chunks = static_cast<int>(a.dst_ld / 8);
+  if (a.zero) {
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+      if (token_at(a.tokens, a.token_size, row) != a.ignore_index) continue;
+      for (int c = threadIdx.x; c < a.cols; c += 256) {
+        static_cast<T*>(a.zero)[row * a.cols + c] = 0;
+      }
+    }
+  }
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* from = static_cast<const T*>(a.src) + (a.kept ? a.kept[row] : row) * a.ld;
     for (int c = threadIdx.x; c < chunks; c += 256) {
@@ -172,8 +185,9 @@ struct Product {
   uint16_t* d;  // [rows][d_ld] and its planes
   int64_t d_ld, d_plane, vocab;
 
-  // kAccumulate: sums of the pieces [split][rows][sum_ld], K being split among
-  // blockIdx.y (`to_out`: not split, and the last piece).  kStore: out alone.
+  // kAccumulate: sums of the pieces [split][rows][sum_ld], K being split (`to_out`:
+  // not split, and the last piece).  kStore: out alone.
+  int splits;
   float* sum;
   int64_t sum_ld, sum_plane;
   int load_sum, to_out;
@@ -238,21 +252,22 @@ __device__ __forceinline__ int b_part(int pass, int passes) {
   return passes == 1 ? 0 : (0x010102 >> (4 * pass)) & 3;
 }
 
-// One operand's part of a round: kTile rows by kStep values of K in LDS, moved
+// One operand's part of a round: Tile rows by kStep values of K in LDS, moved
 // there straight from memory, 16 bytes a lane, 4 instructions a wave.
 //
 // Of [row][k]: an instruction moves 8 rows of 64 values.  The 16-byte piece c of
 // row r lies at place c ^ (r % 8) of its row, so that the 16 rows that a matrix
 // instruction's operand is read from lie in different banks.
 //
-// Of [k][row] (Across): an instruction moves 2 values of K of 256 rows; the piece
-// c of value k lies at place c ^ (k % 4 * 2), and the operand is read by the
+// Of [k][row] (Across): an instruction moves all rows of 2 (Tile 128: 4) values of
+// K; the piece c of value k lies at place c ^ (k % 4 * 2), and the operand is read by the
 // LDS's transposing loads, 16 lanes of which take 4 values of K of 16 rows.
 //
 // Two rounds' parts lie one behind the other, from element `first` of the
 // workgroup's LDS on.
-template <bool Across>
+template <int Tile, bool Across>
 struct Operand {
+  static constexpr int kWaves = Tile / 32, kPieces = Tile / 8, kValues = 512 / Tile;
   uint32_t from;                // byte of the tile that this lane loads first
   uint32_t at[Across ? 4 : 2];  // element of the LDS that it reads first
   uint32_t to;                  // byte of the LDS that this wave writes first
@@ -269,19 +284,19 @@ struct Operand {
     plane = m_plane;
     // Across: whole 16-byte pieces, as a load that crosses the buffer's end loses
     // the 4 bytes that do.  (Rows of memory are whole pieces long.)
-    valid = min(kTile, (Across ? (rows + 7) / 8 * 8 : rows) - tile * kTile);
+    valid = min(Tile, (Across ? (rows + 7) / 8 * 8 : rows) - tile * Tile);
     k_rows = k;
-    base = m + static_cast<int64_t>(tile) * kTile * (Across ? 1 : ld);
+    base = m + static_cast<int64_t>(tile) * Tile * (Across ? 1 : ld);
     const uint32_t lds_byte = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr_t)lds));
     to = __builtin_amdgcn_readfirstlane(lds_byte + first * 2 + wave * 1024);
     const int l = lane & 15, g = lane >> 4;
     if constexpr (Across) {
-      const int kr = wave * 2 + (lane >> 5);
-      from = static_cast<uint32_t>(kr * ld * 2 + ((lane & 31) ^ ((kr & 3) << 1)) * 16);
-      next = static_cast<int>(16 * ld * 2);
+      const int kr = wave * kValues + lane / kPieces;
+      from = static_cast<uint32_t>(kr * ld * 2 + ((lane % kPieces) ^ ((kr & 3) << 1)) * 16);
+      next = static_cast<int>(kWaves * kValues * ld * 2);
 #pragma unroll
       for (int f = 0; f < 4; ++f) {
-        at[f] = first + (g * 8 + (l >> 2)) * kTile + wave_row +
+        at[f] = first + (g * 8 + (l >> 2)) * Tile + wave_row +
                 ((2 * f + ((l & 3) >> 1)) ^ ((l >> 2) << 1)) * 8 + (l & 1) * 4;
         // (Else `first` joins the reads' offsets, which hold 16 bits.)
         asm volatile("" : "+v"(at[f]));
@@ -289,7 +304,7 @@ struct Operand {
     } else {
       const int row = wave * 8 + (lane >> 3);
       from = static_cast<uint32_t>(row * ld * 2 + ((lane & 7) ^ (lane >> 3)) * 16);
-      next = static_cast<int>(64 * ld * 2);
+      next = static_cast<int>(kWaves * 8 * ld * 2);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         at[h] = first + (wave_row + l) * kStep + (((h * 4 + g) ^ (l & 7)) * 8);
@@ -330,63 +345,66 @@ struct Operand {
 
   // A quarter of it.
   __device__ __forceinline__ void load(int buffer, int q, const Round& r) const {
-    load_to_lds(r.buffer, r.from + q * next, r.offset, to + buffer * kTile * kStep * 2 + q * 8192);
+    load_to_lds(r.buffer, r.from + q * next, r.offset, to + buffer * Tile * kStep * 2 + q * kWaves * 1024);
   }
 
   // Rows 16 f to 16 f + 15 of the wave's, 32 values of K of half `h`: row l, values
   // 8 g to 8 g + 7 for lane 16 g + l.
   __device__ __forceinline__ bf16x8_t fetch(const uint16_t* lds, int buffer, int h, int f) const {
     if constexpr (Across) {
-      const uint16_t* p = lds + at[f & 3] + buffer * kTile * kStep + (f >> 2) * 64 + h * 32 * kTile;
+      const uint16_t* p = lds + at[f & 3] + buffer * Tile * kStep + (f >> 2) * 64 + h * 32 * Tile;
       const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)p);
-      const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(p + 4 * kTile));
+      const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(p + 4 * Tile));
       const auto both = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
       return __builtin_bit_cast(bf16x8_t, both);
     } else {
-      return *reinterpret_cast<const bf16x8_t*>(lds + at[h] + buffer * kTile * kStep +
+      return *reinterpret_cast<const bf16x8_t*>(lds + at[h] + buffer * Tile * kStep +
                                                 f * 16 * kStep);
     }
   }
 };
 
-template <typename T, Epilogue E>
-__global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
+// Tile / 32 waves, 2 by Tile / 64, of Tile / 2 by 64 values each.
+template <typename T, int Tile, Epilogue E>
+__global__ __launch_bounds__(Tile * 2, 2) void gemm(Product p) {
+  constexpr int kWavesB = Tile / 64, kFragments = Tile / 32;
   constexpr int kPasses = sizeof(T) == 2 ? 1 : 6;
   constexpr bool kAcrossA = E == kAccumulate || E == kStore, kAcrossB = E == kStore;
-  __shared__ __attribute__((aligned(1024))) uint16_t lds[4 * kTile * kStep];
+  __shared__ __attribute__((aligned(1024))) uint16_t lds[4 * Tile * kStep];
 
   const int rows_b = p.b_count ? *p.b_count : p.b_rows;
   const int k = p.k_count ? *p.k_count : p.k;
   // Tiles in an order that keeps an XCD's workgroups on 4 tiles of a by 8 of b.
-  const int tiles_a = (p.a_rows + kTile - 1) / kTile;
-  const int tiles_b = (rows_b + kTile - 1) / kTile;
+  const int tiles_a = (p.a_rows + Tile - 1) / Tile;
+  const int tiles_b = (rows_b + Tile - 1) / Tile;
   const uint32_t tiles = static_cast<uint32_t>(tiles_a) * tiles_b;
-  if (blockIdx.x >= tiles) return;
-  const uint32_t id = xcd_order(blockIdx.x, tiles);
+  const uint32_t all = tiles * p.splits;  // an XCD's share of them is of one split or two
+  if (blockIdx.x >= all) return;
+  const uint32_t place = xcd_order(blockIdx.x, all);
+  const uint32_t split = place / tiles, id = place % tiles;
   const int band = id / (4 * tiles_b), in_band = id % (4 * tiles_b);
   const int band_rows = min(4, tiles_a - band * 4);
   const int tile_a = band * 4 + in_band % band_rows, tile_b = in_band / band_rows;
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int valid_b = min(kTile, rows_b - tile_b * kTile);
-  // 2 by 4 waves of 128 by 64 values each, in tiles of 16 by 16.
-  const int wave_a = (wave >> 2) * 128, wave_b = (wave & 3) * 64;
-  Operand<kAcrossA> oa;
-  Operand<kAcrossB> ob;
+  const int valid_b = min(Tile, rows_b - tile_b * Tile);
+  const int wave_a = wave / kWavesB * (Tile / 2), wave_b = wave % kWavesB * 64;
+  Operand<Tile, kAcrossA> oa;
+  Operand<Tile, kAcrossB> ob;
   oa.init(p.a, p.lda, p.a_plane, tile_a, p.a_rows, p.k_count ? k : p.a_k, wave, lane, wave_a,
           lds, 0);
   ob.init(p.b, p.ldb, p.b_plane, tile_b, rows_b, k, wave, lane, wave_b, lds,
-          2 * kTile * kStep);
+          2 * Tile * kStep);
 
-  f32x4_t acc[8][4];
+  f32x4_t acc[kFragments][4];  // of 16 by 16 values
 #pragma unroll
-  for (int f = 0; f < 8; ++f) {
+  for (int f = 0; f < kFragments; ++f) {
 #pragma unroll
     for (int n = 0; n < 4; ++n) acc[f][n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
   // A round is two halves of 32 values of K; a half's operands are read from LDS
   // into one set of registers while the other set is multiplied.
-  bf16x8_t fa[2][8], fb[2][4];
+  bf16x8_t fa[2][kFragments], fb[2][4];
 
   // Rounds of K, in pairs.  Rounds past the last (the second of an odd pair, and
   // the two loaded behind the end) load zeros.
@@ -394,13 +412,13 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
   if (E == kAccumulate) {
     // (Divided by lanes: back to scalars, which the loads need.)
     const int64_t whole = end;
-    begin = __builtin_amdgcn_readfirstlane(static_cast<int>(whole * blockIdx.y / gridDim.y));
-    end = __builtin_amdgcn_readfirstlane(static_cast<int>(whole * (blockIdx.y + 1) / gridDim.y));
+    begin = __builtin_amdgcn_readfirstlane(static_cast<int>(whole * split / p.splits));
+    end = __builtin_amdgcn_readfirstlane(static_cast<int>(whole * (split + 1) / p.splits));
   }
   const int rounds = (end - begin) * kPasses;
   int pass = 0, at = begin;
-  typename Operand<kAcrossA>::Round ra;
-  typename Operand<kAcrossB>::Round rb;
+  typename Operand<Tile, kAcrossA>::Round ra;
+  typename Operand<Tile, kAcrossB>::Round rb;
   auto prepare = [&]() __attribute__((always_inline)) {
     const int k0 = pass < kPasses ? at * kStep : max(k, p.a_k);
     const int now = min(pass, kPasses - 1);
@@ -410,22 +428,26 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
     at = wrap ? begin : at;
     pass += wrap ? 1 : 0;
   };
-  // The products of half `half`, in eight groups; with each a part of what the
-  // other half needs is read from LDS and a load of the round after next begins,
-  // so that neither waits in a row for the units that take them.
+  // The products of half `half`, in groups; with each a part of what the other
+  // half needs is read from LDS and a load of the round after next begins, so that
+  // neither waits in a row for the units that take them.
   auto multiply = [&](int half, int buffer, bool load) __attribute__((always_inline)) {
 #pragma unroll
-    for (int f = 0; f < 8; ++f) {
+    for (int f = 0; f < kFragments; ++f) {
+      constexpr int kLoads = 8 / kFragments, kReads = kFragments == 8 ? 2 : 3;
       if (load) {
-        if (f < 4) {
-          oa.load(buffer, f, ra);
-        } else {
-          ob.load(buffer, f - 4, rb);
+#pragma unroll
+        for (int q = f * kLoads; q < (f + 1) * kLoads; ++q) {
+          if (q < 4) {
+            oa.load(buffer, q, ra);
+          } else {
+            ob.load(buffer, q - 4, rb);
+          }
         }
       }
       const int from = load ? buffer ^ 1 : buffer;
 #pragma unroll
-      for (int m = 2 * f; m < min(2 * f + 2, 12); ++m) {
+      for (int m = kReads * f; m < min(kReads * (f + 1), kFragments + 4); ++m) {
         if (m < 4) {
           fb[half ^ 1][m] = ob.fetch(lds, from, half ^ 1, m);
         } else {
@@ -464,7 +486,7 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
 #pragma unroll
   for (int n = 0; n < 4; ++n) fb[0][n] = ob.fetch(lds, 0, 0, n);
 #pragma unroll
-  for (int f = 0; f < 8; ++f) fa[0][f] = oa.fetch(lds, 0, 0, f);
+  for (int f = 0; f < kFragments; ++f) fa[0][f] = oa.fetch(lds, 0, 0, f);
   for (int t = 0; t < rounds; t += 2) {
     round(0);
     round(1);
@@ -472,18 +494,18 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
   barrier<0>();
 
   // acc[f][n][r] is out[j][i] with these.
-  const int i0 = tile_a * kTile + wave_a + (lane >> 4) * 4;  // + 16 f + r
-  const int j0 = tile_b * kTile + wave_b + (lane & 15);      // + 16 n
+  const int i0 = tile_a * Tile + wave_a + (lane >> 4) * 4;  // + 16 f + r
+  const int j0 = tile_b * Tile + wave_b + (lane & 15);      // + 16 n
 
   if (E == kReduce) {
-    // A row's values are 32 of each of 4 lanes in each of 2 waves; a maximum and
+    // A row's values are 4 kFragments of each of 4 lanes in each of 2 waves; a maximum and
     // a sum of e^(s - maximum) of each, in units of the logits without `scale`
     // (which is positive) up to the end.
-    float* both = reinterpret_cast<float*>(lds);  // [wave_a][2][kTile]
+    float* both = reinterpret_cast<float*>(lds);  // [wave_a][2][Tile]
     const float to_log2 = p.scale * kLog2eHi;
     if (tile_a + 1 == tiles_a) {
 #pragma unroll
-      for (int f = 0; f < 8; ++f) {
+      for (int f = 0; f < kFragments; ++f) {
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
 #pragma unroll
@@ -498,9 +520,9 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
       const int j = j0 + n * 16;
       int64_t tok = -1;
       if (j < rows_b) tok = token_at(p.tokens, p.token_size, p.kept[j]) - p.first - i0;
-      if (tok >= 0 && tok < 116 && i0 + tok < p.a_rows) {
+      if (tok >= 0 && tok < kFragments * 16 - 12 && i0 + tok < p.a_rows) {
 #pragma unroll
-        for (int f = 0; f < 8; ++f) {
+        for (int f = 0; f < kFragments; ++f) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             if (tok == f * 16 + r) p.target[j] = acc[f][n][r] * p.scale;
@@ -509,7 +531,7 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
       }
       float top = -kLargest;
 #pragma unroll
-      for (int f = 0; f < 8; ++f) {
+      for (int f = 0; f < kFragments; ++f) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[f][n][r]);
       }
@@ -518,7 +540,7 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
       top = fminf(top, kLargest);
       float sum = 0.0f;
 #pragma unroll
-      for (int f = 0; f < 8; ++f) {
+      for (int f = 0; f < kFragments; ++f) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           sum += __builtin_amdgcn_exp2f((acc[f][n][r] - top) * to_log2);
@@ -527,18 +549,18 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
       if (lane < 16) {
-        both[((wave >> 2) * 2 + 0) * kTile + wave_b + n * 16 + lane] = top * p.scale;
-        both[((wave >> 2) * 2 + 1) * kTile + wave_b + n * 16 + lane] = sum;
+        both[(wave / kWavesB * 2 + 0) * Tile + wave_b + n * 16 + lane] = top * p.scale;
+        both[(wave / kWavesB * 2 + 1) * Tile + wave_b + n * 16 + lane] = sum;
       }
     }
     __syncthreads();
-    if (threadIdx.x < kTile && static_cast<int>(threadIdx.x) < valid_b) {
+    if (threadIdx.x < Tile && static_cast<int>(threadIdx.x) < valid_b) {
       const int j = threadIdx.x;
-      const float t0 = both[j], s0 = both[kTile + j];
-      const float t1 = both[2 * kTile + j], s1 = both[3 * kTile + j];
+      const float t0 = both[j], s0 = both[Tile + j];
+      const float t1 = both[2 * Tile + j], s1 = both[3 * Tile + j];
       const float top = fmaxf(t0, t1);
       const float sum = s0 * exp_f32(exp_domain(t0 - top)) + s1 * exp_f32(exp_domain(t1 - top));
-      p.part[(p.first_tile + tile_a) * p.part_ld + tile_b * kTile + j] = make_float2(top, sum);
+      p.part[(p.first_tile + tile_a) * p.part_ld + tile_b * Tile + j] = make_float2(top, sum);
     }
   }
 
@@ -559,16 +581,16 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
       }
       both *= p.scale;
 #pragma unroll
-      for (int f = 0; f < 8; ++f) {
+      for (int f = 0; f < kFragments; ++f) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float ln_p = __builtin_fmaf(acc[f][n][r], p.scale, -lse);
           acc[f][n][r] = both * __builtin_amdgcn_exp2f(ln_p * kLog2eHi);
         }
       }
-      if (tok >= 0 && tok < 116) {
+      if (tok >= 0 && tok < kFragments * 16 - 12) {
 #pragma unroll
-        for (int f = 0; f < 8; ++f) {
+        for (int f = 0; f < kFragments; ++f) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             if (tok == f * 16 + r) acc[f][n][r] -= g * p.scale;
@@ -578,7 +600,7 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
     }
     if (tile_a + 1 == tiles_a) {
 #pragma unroll
-      for (int f = 0; f < 8; ++f) {
+      for (int f = 0; f < kFragments; ++f) {
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
 #pragma unroll
@@ -591,17 +613,18 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
   }
 
   if constexpr (E == kLogitGrad || (E == kStore && sizeof(T) == 2)) {
-    // bf16 through LDS, so that 32 lanes store 512 consecutive bytes of a row
-    // (straight from the registers a store is 32 bytes of each of 16 rows: the
+    // bf16 through LDS, so that 32 lanes (Tile 128: 16) store consecutive bytes of
+    // a row (straight from the registers a store is 32 bytes of each of 16 rows: the
     // gradients of 256 x 4096 x 128000 took 0.72 ms for dweight's 1 GB).  The
-    // 16-byte piece c of row j lies at place c ^ (j % 32).
+    // 16-byte piece c of row j lies at place c ^ (j % pieces).
+    constexpr int kPieces = Tile / 8, kValues = 512 / Tile;
 #pragma unroll
     for (int q = 0; q < (E == kLogitGrad ? kPasses == 1 ? 1 : 3 : 1); ++q) {
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const int j = wave_b + n * 16 + (lane & 15);
 #pragma unroll
-        for (int f = 0; f < 8; ++f) {
+        for (int f = 0; f < kFragments; ++f) {
           const int i = wave_a + f * 16 + (lane >> 4) * 4;
           u32x2_t v;
           if (sizeof(T) == 2) {
@@ -618,23 +641,23 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
             v = u32x2_t{part[0] | part[1] << 16, part[2] | part[3] << 16};
             asm volatile("" : "+v"(acc[f][n]));  // what is left takes its place: no spills
           }
-          *reinterpret_cast<u32x2_t*>(lds + j * kTile + (((i >> 3) ^ (j & 31)) << 3) + (i & 7)) = v;
+          *reinterpret_cast<u32x2_t*>(lds + j * Tile + (((i >> 3) ^ (j % kPieces)) << 3) + (i & 7)) = v;
         }
       }
       __syncthreads();
-      const int piece = lane & 31;
-      const int i = tile_a * kTile + piece * 8;
+      const int piece = lane % kPieces;
+      const int i = tile_a * Tile + piece * 8;
 #pragma unroll 4
-      for (int r = 0; r < 16; ++r) {
-        const int j = r * 16 + wave * 2 + (lane >> 5);
+      for (int r = 0; r < Tile; r += kFragments * kValues) {
+        const int j = r + wave * kValues + lane / kPieces;
         const u32x4_t v =
-            *reinterpret_cast<const u32x4_t*>(lds + j * kTile + ((piece ^ (j & 31)) << 3));
+            *reinterpret_cast<const u32x4_t*>(lds + j * Tile + ((piece ^ (j % kPieces)) << 3));
         if (E == kLogitGrad) {
           *reinterpret_cast<u32x4_t*>(p.d + q * p.d_plane +
-                                      (tile_b * static_cast<int64_t>(kTile) + j) * p.d_ld + i) = v;
+                                      (tile_b * static_cast<int64_t>(Tile) + j) * p.d_ld + i) = v;
         } else if (j < valid_b) {
           uint16_t* out = static_cast<uint16_t*>(p.out) +
-                          (tile_b * static_cast<int64_t>(kTile) + j) * p.out_ld + i;
+                          (tile_b * static_cast<int64_t>(Tile) + j) * p.out_ld + i;
           if (i + 8 <= p.a_rows) {
             *reinterpret_cast<u32x4_a2_t*>(out) = v;
           } else {
@@ -656,12 +679,12 @@ __global__ __launch_bounds__(kThreads, 2) void gemm(Product p) {
       T* out = static_cast<T*>(p.out) +
                static_cast<int64_t>(E == kStore ? j : (p.to_out ? p.kept[j] : 0)) * p.out_ld;
 #pragma unroll
-      for (int f = 0; f < 8; ++f) {
+      for (int f = 0; f < kFragments; ++f) {
         const int i = i0 + f * 16;
         if (i >= p.a_rows) continue;
         f32x4_t v = acc[f][n];
         if (E == kAccumulate) {
-          f32x4_t* sum = reinterpret_cast<f32x4_t*>(p.sum + blockIdx.y * p.sum_plane +
+          f32x4_t* sum = reinterpret_cast<f32x4_t*>(p.sum + split * p.sum_plane +
                                                      j * p.sum_ld + i);
           if (p.load_sum) v += *sum;
           if (!p.to_out) {
@@ -737,17 +760,6 @@ __global__ __launch_bounds__(256) void join_hidden(const float* sum, int64_t sum
     f32x4_t v = *reinterpret_cast<const f32x4_t*>(from);
     for (int q = 1; q < splits; ++q) v += *reinterpret_cast<const f32x4_t*>(from + q * sum_plane);
     store4(out + kept[j] * static_cast<int64_t>(width) + i, v, width - i);
-  }
-}
-
-// Zeros in the rows of dhidden that do not count.
-template <typename T>
-__global__ __launch_bounds__(256) void zero_rows(const void* tokens, int token_size,
-                                                 int64_t ignore_index, T* out, int64_t rows,
-                                                 int width) {
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    if (token_at(tokens, token_size, r) != ignore_index) continue;
-    for (int c = threadIdx.x; c < width; c += 256) out[r * width + c] = 0;
   }
 }
 
@@ -971,13 +983,18 @@ __global__ __launch_bounds__(256) void join_thin(Thin a, int64_t ignore_index, f
 // Host
 // ---------------------------------------------------------------------------
 
+inline int64_t tiles_of(int64_t rows_a, int64_t rows_b, int tile) {
+  return (up(rows_a, tile) / tile) * (up(rows_b, tile) / tile);
+}
+
 // Where things lie in the workspace; pieces of the vocabulary are multiples of
 // kTile rows and of one size.
 struct Plan {
   int64_t rows_pad, k_pad, piece, pieces;
   int planes;
-  int splits;   // of a piece, for dhidden
-  bool direct;  // weight is read where it lies
+  int tile, tile_hidden, tile_weight;  // of the logits, dhidden and dweight
+  int splits;                          // of a piece, for dhidden
+  bool direct;                         // weight is read where it lies
   size_t kept, count, target, part, hidden, weight, d, sum, bytes;
 };
 
@@ -986,6 +1003,27 @@ constexpr int64_t kMostTiles = int64_t{1} << 22;  // 2^31 threads
 constexpr int64_t kMostRows = (int64_t{1} << 22) - kTile;  // a tile's bytes fit 31 bits
 constexpr size_t kForwardBytes = size_t{1024} << 20;  // of a copied piece
 constexpr size_t kBackwardBytes = size_t{1536} << 20;  // of a piece's d and copies
+
+// The tile with which a product ends sooner.  256 large tiles run at once (one a
+// CU, for its LDS), or 512 small ones; a round of all takes about 1.5 us, or 1.0
+// (for two thirds of the LDS reads at half the products), and what is around the
+// rounds of a tile about 12 us, or 7.  Measured, large and small: 4096 x 1024 x
+// 32000 (2000 tiles) 304 and 389 us, 512 x 2048 x 8000 (64 tiles) 48 and 28 us.
+struct Work {
+  int64_t tiles, rounds;
+};
+
+int64_t time_of(Work w, int tile) {
+  const int64_t at_once = tile == kTile ? kCus : 2 * kCus;
+  const int64_t waves = (w.tiles + at_once - 1) / at_once;
+  return waves * (tile == kTile ? 15 * w.rounds + 120 : 10 * w.rounds + 70);
+}
+
+template <typename WorkOf>
+int better_tile(WorkOf work_of) {
+  return time_of(work_of(kTile), kTile) <= time_of(work_of(kSmallTile), kSmallTile) ? kTile
+                                                                                    : kSmallTile;
+}
 
 Plan plan_of(const void* weight, int elem_size, int64_t rows, int64_t width, int64_t vocab,
              int64_t weight_ld, bool backward) {
@@ -1015,11 +1053,25 @@ Plan plan_of(const void* weight, int elem_size, int64_t rows, int64_t width, int
   p.pieces = (vocab + piece - 1) / piece;
   p.piece = up((vocab + p.pieces - 1) / p.pieces, kTile);
   p.pieces = (vocab + p.piece - 1) / p.piece;
+  const int64_t passes = elem_size == 2 ? 1 : 6, in_piece = std::min(p.piece, vocab);
+  p.tile = better_tile([&](int tile) {
+    return Work{tiles_of(in_piece, rows, tile), passes * p.k_pad / kStep};
+  });
+  p.tile_weight = better_tile([&](int tile) {
+    return Work{tiles_of(width, in_piece, tile), passes * up(rows, kStep) / kStep};
+  });
   // dhidden has few tiles where there are few rows: the piece is split until
-  // there are as many workgroups as CUs, 8 rounds each at least.
-  const int64_t tiles = p.rows_pad / kTile * (up(width, kTile) / kTile);
-  p.splits = static_cast<int>(
-      std::max<int64_t>(1, std::min<int64_t>(kCus / tiles, p.piece / (8 * kStep))));
+  // there are as many workgroups as run at once, 8 rounds each at least.
+  auto splits_of = [&](int tile) {
+    const int64_t at_once = tile == kTile ? kCus : 2 * kCus;
+    return std::max<int64_t>(1, std::min(at_once / tiles_of(width, rows, tile),
+                                         p.piece / (8 * kStep)));
+  };
+  p.tile_hidden = better_tile([&](int tile) {
+    const int64_t splits = splits_of(tile);
+    return Work{splits * tiles_of(width, rows, tile), passes * p.piece / kStep / splits};
+  });
+  p.splits = static_cast<int>(splits_of(p.tile_hidden));
   size_t at = 0;
   auto take = [&at](size_t bytes) {
     const size_t here = at;
@@ -1037,7 +1089,7 @@ Plan plan_of(const void* weight, int elem_size, int64_t rows, int64_t width, int
                      ? sizeof(float) * p.splits * p.rows_pad * up(width, 4) : 0);
   } else {
     p.target = take(sizeof(float) * rows);
-    p.part = take(sizeof(float2) * (whole / kTile) * p.rows_pad);
+    p.part = take(sizeof(float2) * (up(vocab, p.tile) / p.tile) * p.rows_pad);
   }
   p.bytes = at;
   return p;
@@ -1073,10 +1125,13 @@ int pack(const char* what, Pack a, int64_t rows, hipStream_t stream) {
 }
 
 template <typename T, Epilogue E>
-int multiply(const char* what, const Product& p, int64_t rows_b, hipStream_t stream,
-             int splits = 1) {
-  const int64_t tiles = ((p.a_rows + kTile - 1) / kTile) * ((rows_b + kTile - 1) / kTile);
-  gemm<T, E><<<dim3(static_cast<uint32_t>(tiles), splits), kThreads, 0, stream>>>(p);
+int multiply(const char* what, const Product& p, int tile, int64_t rows_b, hipStream_t stream) {
+  const uint32_t grid = static_cast<uint32_t>(tiles_of(p.a_rows, rows_b, tile) * p.splits);
+  if (tile == kTile) {
+    gemm<T, kTile, E><<<grid, 2 * kTile, 0, stream>>>(p);
+  } else {
+    gemm<T, kSmallTile, E><<<grid, 2 * kSmallTile, 0, stream>>>(p);
+  }
   return check_launch(what);
 }
 
@@ -1117,7 +1172,8 @@ int piece_of_weight(const char* what, const Call& c, const Plan& plan, int64_t f
     g->a_plane = plan.piece * plan.k_pad;
     g->k = static_cast<int>(plan.k_pad);
     HIPO_STEP(pack<T>(what, Pack{from, c.weight_ld, nullptr, nullptr, g->a_rows,
-                                 static_cast<int>(c.width), to, plan.k_pad, g->a_plane},
+                                 static_cast<int>(c.width), to, plan.k_pad, g->a_plane, nullptr, 0, 0,
+                                 nullptr},
                       g->a_rows, c.stream));
   }
   g->first = first;
@@ -1126,7 +1182,7 @@ int piece_of_weight(const char* what, const Call& c, const Plan& plan, int64_t f
 
 template <typename T>
 int select_and_pack(const char* what, const Call& c, const Plan& plan, float* loss, float* lse,
-                    Product* g) {
+                    void* dhidden, Product* g) {
   int* kept = c.at<int>(plan.kept);
   int* count = c.at<int>(plan.count);
   float* target = loss ? c.at<float>(plan.target) : nullptr;
@@ -1136,7 +1192,8 @@ int select_and_pack(const char* what, const Call& c, const Plan& plan, float* lo
   uint16_t* hidden = c.at<uint16_t>(plan.hidden);
   const int64_t plane = plan.rows_pad * plan.k_pad;
   HIPO_STEP(pack<T>(what, Pack{c.hidden, c.hidden_ld, kept, count, c.rows,
-                               static_cast<int>(c.width), hidden, plan.k_pad, plane},
+                               static_cast<int>(c.width), hidden, plan.k_pad, plane, c.tokens,
+                               c.token_size, c.ignore_index, dhidden},
                     c.rows, c.stream));
   g->b = hidden;
   g->ldb = plan.k_pad;
@@ -1145,6 +1202,7 @@ int select_and_pack(const char* what, const Call& c, const Plan& plan, float* lo
   g->tokens = c.tokens;
   g->token_size = c.token_size;
   g->kept = kept;
+  g->splits = 1;
   g->scale = c.scale;
   g->vocab = c.vocab;
   g->target = target;
@@ -1176,16 +1234,16 @@ int run_fwd(const Call& c, const Plan& plan, float* loss, float* lse) {
   const char* what = "linear_cross_entropy";
   if (c.rows <= kThinRows) return run_thin<T>(c, plan, loss, lse);
   Product g{};
-  HIPO_STEP(select_and_pack<T>(what, c, plan, loss, lse, &g));
+  HIPO_STEP(select_and_pack<T>(what, c, plan, loss, lse, nullptr, &g));
   g.part = c.at<float2>(plan.part);
   g.part_ld = plan.rows_pad;
   for (int64_t i = 0; i < plan.pieces; ++i) {
     HIPO_STEP(piece_of_weight<T>(what, c, plan, i * plan.piece, &g));
-    g.first_tile = i * plan.piece / kTile;
-    HIPO_STEP((multiply<T, kReduce>(what, g, c.rows, c.stream)));
+    g.first_tile = i * plan.piece / plan.tile;
+    HIPO_STEP((multiply<T, kReduce>(what, g, plan.tile, c.rows, c.stream)));
   }
   join_loss<<<static_cast<uint32_t>(std::min<int64_t>((c.rows + 15) / 16, 1 << 16)), 256, 0,
-              c.stream>>>(JoinLoss{g.part, g.part_ld, static_cast<int>(up(c.vocab, kTile) / kTile),
+              c.stream>>>(JoinLoss{g.part, g.part_ld, static_cast<int>(up(c.vocab, plan.tile) / plan.tile),
                                    g.kept, g.b_count, g.target, loss, lse});
   return check_launch(what);
 }
@@ -1195,11 +1253,8 @@ int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse
             const float* grad_lse, void* dhidden, void* dweight) {
   const char* what = "linear_cross_entropy_bwd";
   Product g{};
-  HIPO_STEP(select_and_pack<T>(what, c, plan, nullptr, nullptr, &g));
+  HIPO_STEP(select_and_pack<T>(what, c, plan, nullptr, nullptr, dhidden, &g));
   const int width = static_cast<int>(c.width);
-  zero_rows<T><<<static_cast<uint32_t>(std::min<int64_t>(c.rows, 1 << 16)), 256, 0, c.stream>>>(
-      c.tokens, c.token_size, c.ignore_index, static_cast<T*>(dhidden), c.rows, width);
-  HIPO_STEP(check_launch(what));
   g.grad = grad;
   g.lse = lse;
   g.grad_lse = grad_lse;
@@ -1209,7 +1264,7 @@ int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse
   for (int64_t i = 0; i < plan.pieces; ++i) {
     const int64_t first = i * plan.piece;
     HIPO_STEP(piece_of_weight<T>(what, c, plan, first, &g));
-    HIPO_STEP((multiply<T, kLogitGrad>(what, g, c.rows, c.stream)));
+    HIPO_STEP((multiply<T, kLogitGrad>(what, g, plan.tile, c.rows, c.stream)));
 
     Product h{};
     h.a = g.a;
@@ -1226,11 +1281,12 @@ int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse
     h.sum = c.at<float>(plan.sum);
     h.sum_ld = up(c.width, 4);
     h.sum_plane = plan.rows_pad * h.sum_ld;
+    h.splits = plan.splits;
     h.load_sum = i > 0;
     h.to_out = plan.splits == 1 && i + 1 == plan.pieces;
     h.out = dhidden;
     h.out_ld = c.width;
-    HIPO_STEP((multiply<T, kAccumulate>(what, h, c.rows, c.stream, plan.splits)));
+    HIPO_STEP((multiply<T, kAccumulate>(what, h, plan.tile_hidden, c.rows, c.stream)));
 
     Product w{};
     w.a = g.b;
@@ -1242,9 +1298,10 @@ int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse
     w.b_plane = g.d_plane;
     w.b_rows = g.a_rows;
     w.k_count = g.b_count;
+    w.splits = 1;
     w.out = static_cast<T*>(dweight) + first * c.width;
     w.out_ld = c.width;
-    HIPO_STEP((multiply<T, kStore>(what, w, g.a_rows, c.stream)));
+    HIPO_STEP((multiply<T, kStore>(what, w, plan.tile_weight, g.a_rows, c.stream)));
   }
   if (plan.splits > 1) {
     const int64_t blocks = (c.rows * ((c.width + 3) / 4) + 255) / 256;
