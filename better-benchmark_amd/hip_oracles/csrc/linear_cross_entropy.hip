@@ -113,8 +113,53 @@ struct Pack {
   void* zero;
 };
 
-__device__ __forceinline__ float value_at(const uint16_t* p) { return bf16_to_f32(*p); }
-__device__ __forceinline__ float value_at(const float* p) { return *p; }
+// 8 values of a row from column k on, zeros from `width` on.
+template <typename T>
+struct Piece;
+template <>
+struct Piece<uint16_t> {
+  u32x4_t w;
+  __device__ __forceinline__ void load(const uint16_t* row, int k, int width) {
+    if (k + 8 <= width) {
+      w = *reinterpret_cast<const u32x4_a2_t*>(row + k);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = k + 2 * i < width ? row[k + 2 * i] : 0;
+        const uint32_t hi = k + 2 * i + 1 < width ? row[k + 2 * i + 1] : 0;
+        w[i] = lo | hi << 16;
+      }
+    }
+  }
+  __device__ __forceinline__ void store(uint16_t* to, int64_t) const {
+    *reinterpret_cast<u32x4_t*>(to) = w;
+  }
+};
+template <>
+struct Piece<float> {
+  f32x4_t v[2];
+  __device__ __forceinline__ void load(const float* row, int k, int width) {
+    if (k + 8 <= width) {
+      v[0] = *reinterpret_cast<const f32x4_a4_t*>(row + k);
+      v[1] = *reinterpret_cast<const f32x4_a4_t*>(row + k + 4);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = k + i < width ? row[k + i] : 0.0f;
+    }
+  }
+  __device__ __forceinline__ void store(uint16_t* to, int64_t plane) const {
+    uint16_t part[8][3];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) split3(v[i >> 2][i & 3], part[i]);
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+      u32x4_t w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = part[2 * i][q] | uint32_t{part[2 * i + 1][q]} << 16;
+      *reinterpret_cast<u32x4_t*>(to + q * plane) = w;
+    }
+  }
+};
 
 // dst[plane][row][0 : dst_ld] = the parts of a row of src, zeros past its end.
 template <typename T>
@@ -132,27 +177,9 @@ __global__ __launch_bounds__(256) void pack_rows(Pack a) {
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* from = static_cast<const T*>(a.src) + (a.kept ? a.kept[row] : row) * a.ld;
     for (int c = threadIdx.x; c < chunks; c += 256) {
-      uint16_t part[3][8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int col = c * 8 + i;
-        if (sizeof(T) == 2) {
-          part[0][i] = col < a.cols ? reinterpret_cast<const uint16_t*>(from)[col] : 0;
-        } else {
-          uint16_t p[3];
-          split3(col < a.cols ? value_at(from + col) : 0.0f, p);
-          part[0][i] = p[0];
-          part[1][i] = p[1];
-          part[2][i] = p[2];
-        }
-      }
-#pragma unroll
-      for (int p = 0; p < (sizeof(T) == 2 ? 1 : 3); ++p) {
-        u32x4_t w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = part[p][2 * i] | uint32_t{part[p][2 * i + 1]} << 16;
-        *reinterpret_cast<u32x4_t*>(a.dst + p * a.plane + row * a.dst_ld + c * 8) = w;
-      }
+      Piece<T> piece;
+      piece.load(from, c * 8, a.cols);
+      piece.store(a.dst + row * a.dst_ld + c * 8, a.plane);
     }
   }
 }
@@ -758,6 +785,7 @@ __global__ __launch_bounds__(256) void join_hidden(const float* sum, int64_t sum
     const int i = static_cast<int>(t % chunks) * 4;
     const float* from = sum + j * sum_ld + i;
     f32x4_t v = *reinterpret_cast<const f32x4_t*>(from);
+#pragma unroll 8
     for (int q = 1; q < splits; ++q) v += *reinterpret_cast<const f32x4_t*>(from + q * sum_plane);
     store4(out + kept[j] * static_cast<int64_t>(width) + i, v, width - i);
   }
@@ -775,66 +803,24 @@ struct Thin {
   float2* part;  // [rows][tiles] maximum and sum
   float* target;
   int64_t tiles;
+
+  // Of the gradient: the rows that count, and d of the vocabulary from `first` on.
+  const int *kept, *count;
+  const float *grad, *lse, *grad_lse;
+  uint16_t* d;
+  int64_t d_ld, d_plane, first, whole_vocab;
 };
 
 constexpr int kThinRows = 64;   // at most
 constexpr int kThinTile = 64;   // of the vocabulary
 constexpr int kThinStages = 4;  // loads in flight, in rounds of kStep values of K
 
-// 8 values of a row from column k on, zeros from `width` on.
-template <typename T>
-struct Piece;
-template <>
-struct Piece<uint16_t> {
-  u32x4_t w;
-  __device__ __forceinline__ void load(const uint16_t* row, int k, int width) {
-    if (k + 8 <= width) {
-      w = *reinterpret_cast<const u32x4_a2_t*>(row + k);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t lo = k + 2 * i < width ? row[k + 2 * i] : 0;
-        const uint32_t hi = k + 2 * i + 1 < width ? row[k + 2 * i + 1] : 0;
-        w[i] = lo | hi << 16;
-      }
-    }
-  }
-  __device__ __forceinline__ void store(uint16_t* to, int) const {
-    *reinterpret_cast<u32x4_t*>(to) = w;
-  }
-};
-template <>
-struct Piece<float> {
-  f32x4_t v[2];
-  __device__ __forceinline__ void load(const float* row, int k, int width) {
-    if (k + 8 <= width) {
-      v[0] = *reinterpret_cast<const f32x4_a4_t*>(row + k);
-      v[1] = *reinterpret_cast<const f32x4_a4_t*>(row + k + 4);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = k + i < width ? row[k + i] : 0.0f;
-    }
-  }
-  __device__ __forceinline__ void store(uint16_t* to, int plane) const {
-    uint16_t part[8][3];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) split3(v[i >> 2][i & 3], part[i]);
-#pragma unroll
-    for (int q = 0; q < 3; ++q) {
-      u32x4_t w;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = part[2 * i][q] | uint32_t{part[2 * i + 1][q]} << 16;
-      *reinterpret_cast<u32x4_t*>(to + q * plane) = w;
-    }
-  }
-};
-
 // The logits of up to 16 N rows against 64 of the vocabulary per workgroup, 16 a
-// wave, reduced as gemm()'s.  Both operands go through registers, kThinStages
+// wave, reduced or (Grad) turned into d as gemm()'s.  Both operands go through registers, kThinStages
 // rounds ahead, to LDS (places as in Operand): the weight is read once, at any
 // alignment, fp32 split on the way.  Memory bounds it: the loads in flight
 // (32 KB a workgroup of bf16) and the number of workgroups are what counts.
-template <typename T, int N>
+template <typename T, int N, bool Grad>
 __global__ __launch_bounds__(256) void thin_logits(Thin a) {
   constexpr int kPlanes = sizeof(T) == 2 ? 1 : 3, kPasses = kPlanes == 1 ? 1 : 6;
   constexpr int kPlaneW = kThinTile * kStep, kPlaneH = 16 * N * kStep;
@@ -848,11 +834,13 @@ __global__ __launch_bounds__(256) void thin_logits(Thin a) {
   const int place = row * kStep + ((chunk ^ (row & 7)) * 8);  // and 32 rows on
   const float to_log2 = a.scale * kLog2eHi;
   const bool with_h = N > 1 || threadIdx.x < 128;
+  const int rows = Grad ? *a.count : a.rows;
+  if (rows == 0) return;
   const T* from_h[kPiecesH];
 #pragma unroll
   for (int q = 0; q < kPiecesH; ++q) {
-    from_h[q] = static_cast<const T*>(a.hidden) +
-                static_cast<int64_t>(min(row + 32 * q, a.rows - 1)) * a.hidden_ld;
+    const int64_t j = min(row + 32 * q, rows - 1);
+    from_h[q] = static_cast<const T*>(a.hidden) + (Grad ? a.kept[j] : j) * a.hidden_ld;
   }
   for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     const int64_t first = tile * kThinTile;
@@ -920,6 +908,35 @@ __global__ __launch_bounds__(256) void thin_logits(Thin a) {
       }
     }
     const int64_t i0 = first + wave * 16 + g * 4;
+    if constexpr (Grad) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int j = n * 16 + l;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (j < rows) {
+          const int64_t at = a.kept[j], tok = token_at(a.tokens, a.token_size, at);
+          const float grad = tok >= 0 && tok < a.whole_vocab ? a.grad[at] : __builtin_nanf("");
+          const float both = (a.grad_lse ? grad + a.grad_lse[at] : grad) * a.scale;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float ln_p = __builtin_fmaf(acc[n][r], a.scale, -a.lse[at]);
+            v[r] = both * __builtin_amdgcn_exp2f(ln_p * kLog2eHi);
+            if (i0 + r == tok - a.first) v[r] -= grad * a.scale;
+            if (i0 + r >= a.vocab) v[r] = 0.0f;
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < kPlanes; ++q) {
+          uint32_t part[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) part[r] = next_part(v[r]);
+          *reinterpret_cast<u32x2_t*>(a.d + q * a.d_plane + j * a.d_ld + i0) =
+              u32x2_t{part[0] | part[1] << 16, part[2] | part[3] << 16};
+        }
+      }
+      __syncthreads();
+      continue;
+    }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int j = n * 16 + l;
@@ -950,6 +967,136 @@ __global__ __launch_bounds__(256) void thin_logits(Thin a) {
       a.part[j * a.tiles + tile] = make_float2(top, sum);
     }
     __syncthreads();
+  }
+}
+
+struct ThinWeight {
+  const uint16_t *hidden, *d;  // [row][hidden_ld], [row][d_ld] and their planes
+  int64_t hidden_ld, hidden_plane, d_ld, d_plane;
+  const int* count;
+  int width;
+  int64_t vocab;
+  void* out;
+  int64_t out_ld;
+  int chunks;  // of 64 columns, per workgroup
+};
+
+// dweight of up to 64 rows: 64 of the vocabulary per workgroup, 16 a wave, whose
+// d stays in registers while the columns pass, 64 at a time.  The products'
+// operands are [row][...], read across as in Operand.  What is written bounds it,
+// so several workgroups a CU write at once, whole 128-byte pieces of rows.
+template <typename T>
+__global__ __launch_bounds__(256) void thin_weight(ThinWeight a) {
+  constexpr int kPlanes = sizeof(T) == 2 ? 1 : 3, kPasses = kPlanes == 1 ? 1 : 6;
+  constexpr int kPlane = 64 * 64;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2][kPlanes * kPlane];
+  __shared__ __attribute__((aligned(16))) uint16_t stage[4][sizeof(T) == 2 ? 16 * 64 : 8];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int l = lane & 15, g = lane >> 4;
+  const int row = threadIdx.x >> 3, chunk = threadIdx.x & 7;
+  const int place = row * 64 + ((chunk ^ ((row & 3) << 1)) * 8);  // and 32 rows on
+  const int count = *a.count;
+  const int64_t v0 = static_cast<int64_t>(blockIdx.x) * 64;
+  const int begin = blockIdx.y * a.chunks * 64;
+  const int end = min(begin + a.chunks * 64, (a.width + 63) / 64 * 64);
+
+  u32x4_t piece[kPlanes][2];
+  // 64 columns of the rows that count, zeros for the others.
+  auto load = [&](const uint16_t* from, int64_t ld, int64_t plane) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < kPlanes; ++p) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int r = row + 32 * q;
+        piece[p][q] = u32x4_t{0u, 0u, 0u, 0u};
+        if (r < count) {
+          piece[p][q] = *reinterpret_cast<const u32x4_t*>(from + p * plane + r * ld + chunk * 8);
+        }
+      }
+    }
+  };
+  auto store = [&](int buffer) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < kPlanes; ++p) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        *reinterpret_cast<u32x4_t*>(lds[buffer] + p * kPlane + place + q * 32 * 64) = piece[p][q];
+      }
+    }
+  };
+  // Columns 16 f to 16 f + 15, rows 32 h to 32 h + 31: column l, rows 8 g on.
+  auto fetch = [&](int buffer, int p, int h, int f) __attribute__((always_inline)) {
+    const uint16_t* from = lds[buffer] + p * kPlane + (h * 32 + g * 8 + (l >> 2)) * 64 +
+                           ((2 * f + ((l & 3) >> 1)) ^ ((l >> 2) << 1)) * 8 + (l & 1) * 4;
+    const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)from);
+    const s16x4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(from + 4 * 64));
+    return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+
+  load(a.d + v0, a.d_ld, a.d_plane);
+  store(0);
+  load(a.hidden + begin, a.hidden_ld, a.hidden_plane);
+  __syncthreads();
+  bf16x8_t fd[2][kPlanes];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int p = 0; p < kPlanes; ++p) fd[h][p] = fetch(0, p, h, wave);
+  }
+  int buffer = 1;
+  for (int c0 = begin; c0 < end; c0 += 64, buffer ^= 1) {
+    store(buffer);
+    load(a.hidden + min(c0 + 64, end - 64), a.hidden_ld, a.hidden_plane);
+    // One barrier a round: a buffer is written again behind the next one's.
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const int64_t v = v0 + wave * 16;
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+      f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (h * 32 >= count) continue;
+        bf16x8_t fh[kPlanes];
+#pragma unroll
+        for (int p = 0; p < kPlanes; ++p) fh[p] = fetch(buffer, p, h, f);
+#pragma unroll
+        for (int pass = 0; pass < kPasses; ++pass) {
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fh[a_part(pass, kPasses)],
+                                                        fd[h][b_part(pass, kPasses)], acc, 0, 0, 0);
+        }
+      }
+      // acc[r] is row v + l, column c0 + 16 f + 4 g + r.
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<u32x2_t*>(stage[wave] + l * 64 + (((2 * f + (g >> 1)) ^ (l & 7)) * 8) +
+                                    (g & 1) * 4) =
+            u32x2_t{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
+      } else {
+        const int i = c0 + 16 * f + 4 * g;
+        if (v + l < a.vocab && i < a.width) {
+          store4(static_cast<float*>(a.out) + (v + l) * a.out_ld + i, acc, a.width - i);
+        }
+      }
+    }
+    if constexpr (sizeof(T) == 2) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // of this wave's own lanes
+      const int i = c0 + (lane & 7) * 8;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int j = q * 8 + (lane >> 3);
+        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(
+            stage[wave] + j * 64 + (((lane & 7) ^ (j & 7)) * 8));
+        if (v + j >= a.vocab) continue;
+        uint16_t* out = static_cast<uint16_t*>(a.out) + (v + j) * a.out_ld + i;
+        if (i + 8 <= a.width) {
+          *reinterpret_cast<u32x4_a2_t*>(out) = w;
+        } else {
+#pragma unroll
+          for (int m = 0; m < 7; ++m) {
+            if (i + m < a.width) out[m] = static_cast<uint16_t>(w[m >> 1] >> (m & 1) * 16);
+          }
+        }
+      }
+    }
   }
 }
 
@@ -1209,6 +1356,19 @@ int select_and_pack(const char* what, const Call& c, const Plan& plan, float* lo
   return 0;
 }
 
+template <typename T, bool Grad>
+int launch_thin(const char* what, const Thin& a, int64_t rows, hipStream_t stream) {
+  const uint32_t grid = static_cast<uint32_t>(std::min<int64_t>(a.tiles, 1 << 20));
+  if (rows <= 16) {
+    thin_logits<T, 1, Grad><<<grid, 256, 0, stream>>>(a);
+  } else if (rows <= 32) {
+    thin_logits<T, 2, Grad><<<grid, 256, 0, stream>>>(a);
+  } else {
+    thin_logits<T, 4, Grad><<<grid, 256, 0, stream>>>(a);
+  }
+  return check_launch(what);
+}
+
 template <typename T>
 int run_thin(const Call& c, const Plan& plan, float* loss, float* lse) {
   const char* what = "linear_cross_entropy";
@@ -1216,15 +1376,7 @@ int run_thin(const Call& c, const Plan& plan, float* loss, float* lse) {
                static_cast<int>(c.width), c.vocab, c.hidden_ld,  c.weight_ld,
                c.scale,     c.at<float2>(plan.part), c.at<float>(plan.target),
                up(c.vocab, kThinTile) / kThinTile};
-  const uint32_t grid = static_cast<uint32_t>(std::min<int64_t>(a.tiles, 1 << 20));
-  if (c.rows <= 16) {
-    thin_logits<T, 1><<<grid, 256, 0, c.stream>>>(a);
-  } else if (c.rows <= 32) {
-    thin_logits<T, 2><<<grid, 256, 0, c.stream>>>(a);
-  } else {
-    thin_logits<T, 4><<<grid, 256, 0, c.stream>>>(a);
-  }
-  HIPO_STEP(check_launch(what));
+  HIPO_STEP((launch_thin<T, false>(what, a, c.rows, c.stream)));
   join_thin<<<static_cast<uint32_t>(c.rows), 256, 0, c.stream>>>(a, c.ignore_index, loss, lse);
   return check_launch(what);
 }
@@ -1261,10 +1413,36 @@ int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse
   g.d = c.at<uint16_t>(plan.d);
   g.d_ld = plan.piece;
   g.d_plane = plan.rows_pad * plan.piece;
+  const bool thin = c.rows <= kThinRows;
   for (int64_t i = 0; i < plan.pieces; ++i) {
     const int64_t first = i * plan.piece;
     HIPO_STEP(piece_of_weight<T>(what, c, plan, first, &g));
-    HIPO_STEP((multiply<T, kLogitGrad>(what, g, plan.tile, c.rows, c.stream)));
+    if (thin) {
+      Thin t{};
+      t.hidden = c.hidden;
+      t.weight = static_cast<const T*>(c.weight) + first * c.weight_ld;
+      t.tokens = c.tokens;
+      t.token_size = c.token_size;
+      t.width = width;
+      t.vocab = g.a_rows;
+      t.hidden_ld = c.hidden_ld;
+      t.weight_ld = c.weight_ld;
+      t.scale = c.scale;
+      t.tiles = up(g.a_rows, kThinTile) / kThinTile;
+      t.kept = g.kept;
+      t.count = g.b_count;
+      t.grad = grad;
+      t.lse = lse;
+      t.grad_lse = grad_lse;
+      t.d = g.d;
+      t.d_ld = g.d_ld;
+      t.d_plane = g.d_plane;
+      t.first = first;
+      t.whole_vocab = c.vocab;
+      HIPO_STEP((launch_thin<T, true>(what, t, c.rows, c.stream)));
+    } else {
+      HIPO_STEP((multiply<T, kLogitGrad>(what, g, plan.tile, c.rows, c.stream)));
+    }
 
     Product h{};
     h.a = g.a;
@@ -1288,6 +1466,19 @@ int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse
     h.out_ld = c.width;
     HIPO_STEP((multiply<T, kAccumulate>(what, h, plan.tile_hidden, c.rows, c.stream)));
 
+    if (thin) {
+      // Columns in as many parts as it takes to fill the CUs several times.
+      const int64_t strips = up(g.a_rows, 64) / 64, all = up(c.width, 64) / 64;
+      const int64_t parts = std::min<int64_t>(all, std::max<int64_t>(1, 2048 / strips));
+      const int chunks = static_cast<int>((all + parts - 1) / parts);
+      thin_weight<T><<<dim3(static_cast<uint32_t>(strips),
+                            static_cast<uint32_t>((all + chunks - 1) / chunks)),
+                       256, 0, c.stream>>>(
+          ThinWeight{g.b, g.d, g.ldb, g.b_plane, g.d_ld, g.d_plane, g.b_count, width, g.a_rows,
+                     static_cast<T*>(dweight) + first * c.width, c.width, chunks});
+      HIPO_STEP(check_launch(what));
+      continue;
+    }
     Product w{};
     w.a = g.b;
     w.lda = g.ldb;
