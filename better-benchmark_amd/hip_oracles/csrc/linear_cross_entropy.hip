@@ -28,6 +28,7 @@ typedef u32x2_t u32x2_a2_t __attribute__((aligned(2)));
 constexpr int kTile = 256;       // rows of either operand that a workgroup multiplies,
 constexpr int kSmallTile = 128;  // or where there are too few such tiles
 constexpr int kStep = 64;        // values of K per round
+constexpr int kThinRows = 64;    // at most, for the kernels of few rows
 constexpr float kLargest = 3.402823466e+38f;
 
 inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
@@ -81,20 +82,17 @@ __global__ __launch_bounds__(1024) void select_rows(Select a) {
   if (threadIdx.x == 0) *a.count = base;
 }
 
-// The next bf16 part of x, the nearest one, and what it leaves in x.  A part
-// that would overflow is cut instead; what is not finite leaves 0.
-__device__ __forceinline__ uint16_t next_part(float& x) {
-  const uint32_t bits = __float_as_uint(x);
-  uint32_t part = pack_bf16x2(x, 0.0f) & 0xffffu;
-  const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
-  if (finite && (part & 0x7f80u) == 0x7f80u) part = bits >> 16;
-  x = finite ? x - bf16lo(part) : 0.0f;
-  return static_cast<uint16_t>(part);
-}
-
-__device__ __forceinline__ void split3(float x, uint16_t (&part)[3]) {
-#pragma unroll
-  for (int q = 0; q < 3; ++q) part[q] = next_part(x);
+// The next bf16 parts of two values, the nearest ones, and what they leave.  Of
+// three parts the first two are kept finite (a value past the largest bf16 leaves
+// the rest to the next part, an infinity or NaN to the last).
+__device__ __forceinline__ uint32_t next_parts(float& lo, float& hi, bool last) {
+  constexpr float kLargestBf16 = 3.3895313892515355e38f;
+  const uint32_t w = last ? pack_bf16x2(lo, hi)
+                          : pack_bf16x2(__builtin_amdgcn_fmed3f(lo, -kLargestBf16, kLargestBf16),
+                                        __builtin_amdgcn_fmed3f(hi, -kLargestBf16, kLargestBf16));
+  lo -= bf16lo(w);
+  hi -= bf16hi(w);
+  return w;
 }
 
 struct Pack {
@@ -148,14 +146,17 @@ struct Piece<float> {
     }
   }
   __device__ __forceinline__ void store(uint16_t* to, int64_t plane) const {
-    uint16_t part[8][3];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) split3(v[i >> 2][i & 3], part[i]);
+    f32x4_t x[2] = {v[0], v[1]};
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
       u32x4_t w;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = part[2 * i][q] | uint32_t{part[2 * i + 1][q]} << 16;
+      for (int i = 0; i < 4; ++i) {
+        float lo = x[i >> 1][(2 * i) & 3], hi = x[i >> 1][(2 * i + 1) & 3];
+        w[i] = next_parts(lo, hi, q == 2);
+        x[i >> 1][(2 * i) & 3] = lo;
+        x[i >> 1][(2 * i + 1) & 3] = hi;
+      }
       *reinterpret_cast<u32x4_t*>(to + q * plane) = w;
     }
   }
@@ -658,14 +659,9 @@ __global__ __launch_bounds__(Tile * 2, 2) void gemm(Product p) {
             v = u32x2_t{pack_bf16x2(acc[f][n][0], acc[f][n][1]),
                         pack_bf16x2(acc[f][n][2], acc[f][n][3])};
           } else {
-            uint32_t part[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              float x = acc[f][n][r];
-              part[r] = next_part(x);
-              acc[f][n][r] = x;
-            }
-            v = u32x2_t{part[0] | part[1] << 16, part[2] | part[3] << 16};
+            float x[4] = {acc[f][n][0], acc[f][n][1], acc[f][n][2], acc[f][n][3]};
+            v = u32x2_t{next_parts(x[0], x[1], q == 2), next_parts(x[2], x[3], q == 2)};
+            acc[f][n] = f32x4_t{x[0], x[1], x[2], x[3]};
             asm volatile("" : "+v"(acc[f][n]));  // what is left takes its place: no spills
           }
           *reinterpret_cast<u32x2_t*>(lds + j * Tile + (((i >> 3) ^ (j % kPieces)) << 3) + (i & 7)) = v;
@@ -775,8 +771,9 @@ __global__ __launch_bounds__(256) void join_loss(JoinLoss a) {
 // The splits' sums added in order: rows of dhidden.
 template <typename T>
 __global__ __launch_bounds__(256) void join_hidden(const float* sum, int64_t sum_ld,
-                                                   int64_t sum_plane, int splits, const int* kept,
-                                                   const int* count, T* out, int width) {
+                                                   int64_t sum_plane, int splits, bool two_parts,
+                                                   const int* kept, const int* count, T* out,
+                                                   int width) {
   const int chunks = (width + 3) / 4;
   const int64_t n = static_cast<int64_t>(*count) * chunks;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; t < n;
@@ -787,6 +784,11 @@ __global__ __launch_bounds__(256) void join_hidden(const float* sum, int64_t sum
     f32x4_t v = *reinterpret_cast<const f32x4_t*>(from);
 #pragma unroll 8
     for (int q = 1; q < splits; ++q) v += *reinterpret_cast<const f32x4_t*>(from + q * sum_plane);
+    if (two_parts) {
+      from += kThinRows * sum_ld;
+#pragma unroll 8
+      for (int q = 0; q < splits; ++q) v += *reinterpret_cast<const f32x4_t*>(from + q * sum_plane);
+    }
     store4(out + kept[j] * static_cast<int64_t>(width) + i, v, width - i);
   }
 }
@@ -811,9 +813,25 @@ struct Thin {
   int64_t d_ld, d_plane, first, whole_vocab;
 };
 
-constexpr int kThinRows = 64;   // at most
 constexpr int kThinTile = 64;   // of the vocabulary
 constexpr int kThinStages = 4;  // loads in flight, in rounds of kStep values of K
+
+// bf16 parts of d.  Two of bf16 operands, which cost few rows nothing (memory
+// bounds them): with one the gradients of a single row are off by up to twice
+// what their own rounding to bf16 is, where one token's d outweighs the others'.
+template <typename T>
+constexpr int kThinParts = sizeof(T) == 2 ? 2 : 3;
+template <typename T>
+constexpr int kThinPasses = sizeof(T) == 2 ? 2 : 6;
+// The parts of an operand and of d that are multiplied, the smallest products first.
+template <typename T>
+__device__ __forceinline__ int thin_a_part(int pass) {
+  return sizeof(T) == 2 ? 0 : a_part(pass, 6);
+}
+template <typename T>
+__device__ __forceinline__ int thin_d_part(int pass) {
+  return sizeof(T) == 2 ? 1 - pass : b_part(pass, 6);
+}
 
 // The logits of up to 16 N rows against 64 of the vocabulary per workgroup, 16 a
 // wave, reduced or (Grad) turned into d as gemm()'s.  Both operands go through registers, kThinStages
@@ -860,9 +878,10 @@ __global__ __launch_bounds__(256) void thin_logits(Thin a) {
         for (int q = 0; q < kPiecesH; ++q) h[stage][q].load(from_h[q], k, a.width);
       }
     };
-    f32x4_t acc[N];
+    // Two sums, of the halves of the rounds: shorter ones round less.
+    f32x4_t acc[N], other[N];
 #pragma unroll
-    for (int n = 0; n < N; ++n) acc[n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int n = 0; n < N; ++n) acc[n] = other[n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int s = 0; s < kThinStages; ++s) load(s, s * kStep);
     for (int k0 = 0; k0 < a.width; k0 += kThinStages * kStep) {
@@ -900,13 +919,16 @@ __global__ __launch_bounds__(256) void thin_logits(Thin a) {
           for (int pass = 0; pass < kPasses; ++pass) {
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-              acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                  fw[a_part(pass, kPasses)], fh[b_part(pass, kPasses)][n], acc[n], 0, 0, 0);
+              f32x4_t& sum = half == 0 ? acc[n] : other[n];
+              sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  fw[a_part(pass, kPasses)], fh[b_part(pass, kPasses)][n], sum, 0, 0, 0);
             }
           }
         }
       }
     }
+#pragma unroll
+    for (int n = 0; n < N; ++n) acc[n] += other[n];
     const int64_t i0 = first + wave * 16 + g * 4;
     if constexpr (Grad) {
 #pragma unroll
@@ -926,12 +948,10 @@ __global__ __launch_bounds__(256) void thin_logits(Thin a) {
           }
         }
 #pragma unroll
-        for (int q = 0; q < kPlanes; ++q) {
-          uint32_t part[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) part[r] = next_part(v[r]);
-          *reinterpret_cast<u32x2_t*>(a.d + q * a.d_plane + j * a.d_ld + i0) =
-              u32x2_t{part[0] | part[1] << 16, part[2] | part[3] << 16};
+        for (int q = 0; q < kThinParts<T>; ++q) {
+          const bool last = q + 1 == kThinParts<T>;
+          const uint32_t lo = next_parts(v[0], v[1], last), hi = next_parts(v[2], v[3], last);
+          *reinterpret_cast<u32x2_t*>(a.d + q * a.d_plane + j * a.d_ld + i0) = u32x2_t{lo, hi};
         }
       }
       __syncthreads();
@@ -987,9 +1007,9 @@ struct ThinWeight {
 // so several workgroups a CU write at once, whole 128-byte pieces of rows.
 template <typename T>
 __global__ __launch_bounds__(256) void thin_weight(ThinWeight a) {
-  constexpr int kPlanes = sizeof(T) == 2 ? 1 : 3, kPasses = kPlanes == 1 ? 1 : 6;
+  constexpr int kPlanes = sizeof(T) == 2 ? 1 : 3, kParts = kThinParts<T>;
   constexpr int kPlane = 64 * 64;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[2][kPlanes * kPlane];
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2][kParts * kPlane];
   __shared__ __attribute__((aligned(16))) uint16_t stage[4][sizeof(T) == 2 ? 16 * 64 : 8];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l = lane & 15, g = lane >> 4;
@@ -1000,11 +1020,13 @@ __global__ __launch_bounds__(256) void thin_weight(ThinWeight a) {
   const int begin = blockIdx.y * a.chunks * 64;
   const int end = min(begin + a.chunks * 64, (a.width + 63) / 64 * 64);
 
-  u32x4_t piece[kPlanes][2];
-  // 64 columns of the rows that count, zeros for the others.
-  auto load = [&](const uint16_t* from, int64_t ld, int64_t plane) __attribute__((always_inline)) {
+  u32x4_t piece[kParts][2];
+  // 64 columns of the rows that count, zeros for the others, of some planes.
+  auto load = [&](const uint16_t* from, int64_t ld, int64_t plane, int planes)
+                  __attribute__((always_inline)) {
 #pragma unroll
-    for (int p = 0; p < kPlanes; ++p) {
+    for (int p = 0; p < kParts; ++p) {
+      if (p >= planes) continue;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const int r = row + 32 * q;
@@ -1015,9 +1037,10 @@ __global__ __launch_bounds__(256) void thin_weight(ThinWeight a) {
       }
     }
   };
-  auto store = [&](int buffer) __attribute__((always_inline)) {
+  auto store = [&](int buffer, int planes) __attribute__((always_inline)) {
 #pragma unroll
-    for (int p = 0; p < kPlanes; ++p) {
+    for (int p = 0; p < kParts; ++p) {
+      if (p >= planes) continue;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         *reinterpret_cast<u32x4_t*>(lds[buffer] + p * kPlane + place + q * 32 * 64) = piece[p][q];
@@ -1033,20 +1056,20 @@ __global__ __launch_bounds__(256) void thin_weight(ThinWeight a) {
     return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
-  load(a.d + v0, a.d_ld, a.d_plane);
-  store(0);
-  load(a.hidden + begin, a.hidden_ld, a.hidden_plane);
+  load(a.d + v0, a.d_ld, a.d_plane, kParts);
+  store(0, kParts);
+  load(a.hidden + begin, a.hidden_ld, a.hidden_plane, kPlanes);
   __syncthreads();
-  bf16x8_t fd[2][kPlanes];
+  bf16x8_t fd[2][kParts];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
 #pragma unroll
-    for (int p = 0; p < kPlanes; ++p) fd[h][p] = fetch(0, p, h, wave);
+    for (int p = 0; p < kParts; ++p) fd[h][p] = fetch(0, p, h, wave);
   }
   int buffer = 1;
   for (int c0 = begin; c0 < end; c0 += 64, buffer ^= 1) {
-    store(buffer);
-    load(a.hidden + min(c0 + 64, end - 64), a.hidden_ld, a.hidden_plane);
+    store(buffer, kPlanes);
+    load(a.hidden + min(c0 + 64, end - 64), a.hidden_ld, a.hidden_plane, kPlanes);
     // One barrier a round: a buffer is written again behind the next one's.
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const int64_t v = v0 + wave * 16;
@@ -1060,9 +1083,9 @@ __global__ __launch_bounds__(256) void thin_weight(ThinWeight a) {
 #pragma unroll
         for (int p = 0; p < kPlanes; ++p) fh[p] = fetch(buffer, p, h, f);
 #pragma unroll
-        for (int pass = 0; pass < kPasses; ++pass) {
-          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fh[a_part(pass, kPasses)],
-                                                        fd[h][b_part(pass, kPasses)], acc, 0, 0, 0);
+        for (int pass = 0; pass < kThinPasses<T>; ++pass) {
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              fh[thin_a_part<T>(pass)], fd[h][thin_d_part<T>(pass)], acc, 0, 0, 0);
         }
       }
       // acc[r] is row v + l, column c0 + 16 f + 4 g + r.
@@ -1097,6 +1120,129 @@ __global__ __launch_bounds__(256) void thin_weight(ThinWeight a) {
         }
       }
     }
+  }
+}
+
+struct ThinHidden {
+  const void* weight;  // [vocab][weight_ld], as it lies
+  int64_t weight_ld, vocab;
+  int width;
+  const uint16_t* d;  // [row][d_ld] and its planes, zeros past the rows and the vocabulary
+  int64_t d_ld, d_plane;
+  const int* count;
+  float* sum;  // [split][kThinRows][sum_ld]
+  int64_t sum_ld;
+  int load_sum;
+};
+
+// dhidden of up to 16 N rows: 64 columns of a part of the vocabulary per
+// workgroup, 16 a wave, the parts joined by join_hidden().  The weight goes
+// through registers to LDS (as in thin_logits(), read across as in Operand), two
+// rounds of 64 of the vocabulary ahead; its second reading bounds the kernel.
+template <typename T, int N>
+__global__ __launch_bounds__(256) void thin_hidden(ThinHidden a) {
+  constexpr int kPlanes = sizeof(T) == 2 ? 1 : 3, kParts = kThinParts<T>;
+  constexpr int kPlaneW = 64 * 64, kPlaneD = 16 * N * 64, kPiecesD = (N + 1) / 2;
+  __shared__ __attribute__((aligned(16))) uint16_t weight[2][kPlanes * kPlaneW];
+  __shared__ __attribute__((aligned(16))) uint16_t ds[2][kParts * kPlaneD];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int l = lane & 15, g = lane >> 4;
+  const int row = threadIdx.x >> 3, chunk = threadIdx.x & 7;
+  const int place_w = row * 64 + ((chunk ^ ((row & 3) << 1)) * 8);  // and 32 rows on
+  const int place_d = row * 64 + ((chunk ^ (row & 7)) * 8);
+  const bool with_d = N > 1 || threadIdx.x < 128;
+  const int count = *a.count;
+  if (count == 0) return;
+  const int c0 = blockIdx.x * 64;
+  const int64_t rounds = (a.vocab + 63) / 64;
+  const int64_t begin = rounds * blockIdx.y / gridDim.y, end = rounds * (blockIdx.y + 1) / gridDim.y;
+
+  Piece<T> w[2][2];
+  u32x4_t d[2][kParts][kPiecesD];
+  auto load = [&](int stage, int64_t t) __attribute__((always_inline)) {
+    const int64_t v0 = min(t, end - 1) * 64;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      // (Past the vocabulary, and past a row's end, zeros.)
+      const int64_t v = v0 + row + 32 * q;
+      w[stage][q].load(static_cast<const T*>(a.weight) + min(v, a.vocab - 1) * a.weight_ld,
+                       c0 + chunk * 8, v < a.vocab ? a.width : 0);
+    }
+    if (with_d) {
+#pragma unroll
+      for (int p = 0; p < kParts; ++p) {
+#pragma unroll
+        for (int q = 0; q < kPiecesD; ++q) {
+          d[stage][p][q] = *reinterpret_cast<const u32x4_t*>(
+              a.d + p * a.d_plane + (row + 32 * q) * a.d_ld + v0 + chunk * 8);
+        }
+      }
+    }
+  };
+  f32x4_t acc[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) acc[n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  auto round = [&](int s, int64_t t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) w[s][q].store(weight[s] + place_w + q * 32 * 64, kPlaneW);
+    if (with_d) {
+#pragma unroll
+      for (int p = 0; p < kParts; ++p) {
+#pragma unroll
+        for (int q = 0; q < kPiecesD; ++q) {
+          *reinterpret_cast<u32x4_t*>(ds[s] + p * kPlaneD + place_d + q * 32 * 64) = d[s][p][q];
+        }
+      }
+    }
+    load(s, t + 2);
+    // One barrier a round: a buffer is written again behind the next one's.
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      bf16x8_t fw[kPlanes], fd[kParts][N];
+#pragma unroll
+      for (int p = 0; p < kPlanes; ++p) {
+        const uint16_t* from = weight[s] + p * kPlaneW + (h * 32 + g * 8 + (l >> 2)) * 64 +
+                               ((2 * wave + ((l & 3) >> 1)) ^ ((l >> 2) << 1)) * 8 + (l & 1) * 4;
+        const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)from);
+        const s16x4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t)(from + 4 * 64));
+        fw[p] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+      }
+#pragma unroll
+      for (int p = 0; p < kParts; ++p) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          fd[p][n] = *reinterpret_cast<const bf16x8_t*>(
+              ds[s] + p * kPlaneD + (n * 16 + l) * 64 + (((h * 4 + g) ^ (l & 7)) * 8));
+        }
+      }
+#pragma unroll
+      for (int pass = 0; pass < kThinPasses<T>; ++pass) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              fw[thin_a_part<T>(pass)], fd[thin_d_part<T>(pass)][n], acc[n], 0, 0, 0);
+        }
+      }
+    }
+  };
+  if (begin < end) {
+    load(0, begin);
+    load(1, begin + 1);
+  }
+  for (int64_t t = begin; t < end; t += 2) {
+    round(0, t);
+    if (t + 1 >= end) break;
+    round(1, t + 1);
+  }
+  const int i = c0 + wave * 16 + g * 4;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int j = n * 16 + l;
+    if (j >= count || i >= a.width) continue;
+    f32x4_t* sum = reinterpret_cast<f32x4_t*>(
+        a.sum + (static_cast<int64_t>(blockIdx.y) * kThinRows + j) * a.sum_ld + i);
+    *sum = a.load_sum ? acc[n] + *sum : acc[n];
   }
 }
 
@@ -1137,11 +1283,13 @@ inline int64_t tiles_of(int64_t rows_a, int64_t rows_b, int tile) {
 // Where things lie in the workspace; pieces of the vocabulary are multiples of
 // kTile rows and of one size.
 struct Plan {
-  int64_t rows_pad, k_pad, piece, pieces;
-  int planes;
+  int64_t rows_pad, sum_rows, k_pad, piece, pieces;
+  int planes, d_planes;
   int tile, tile_hidden, tile_weight;  // of the logits, dhidden and dweight
   int splits;                          // of a piece, for dhidden
   bool direct;                         // weight is read where it lies
+  bool thin;                           // few rows: the kernels of their own,
+  bool thin_gemm;                      // but for dhidden of aligned bf16
   size_t kept, count, target, part, hidden, weight, d, sum, bytes;
 };
 
@@ -1182,12 +1330,17 @@ Plan plan_of(const void* weight, int elem_size, int64_t rows, int64_t width, int
     return p;
   }
   p.planes = elem_size == 2 ? 1 : 3;
-  p.direct = elem_size == 2 && aligned16(weight) && weight_ld % 8 == 0 && width % 8 == 0;
-  p.rows_pad = up(rows, kTile);
+  const bool aligned = elem_size == 2 && aligned16(weight) && weight_ld % 8 == 0 && width % 8 == 0;
+  p.thin = rows <= kThinRows;
+  p.thin_gemm = p.thin && aligned;
+  p.direct = p.thin || aligned;
+  p.rows_pad = p.thin ? kThinRows : up(rows, kTile);
+  p.d_planes = p.thin && elem_size == 2 ? 2 : p.planes;
+  p.sum_rows = p.thin_gemm ? 2 * kThinRows : p.rows_pad;
   p.k_pad = up(width, kStep);
   const size_t copy = p.direct ? 0 : sizeof(uint16_t) * p.planes * p.k_pad;
   const size_t per_row =
-      backward ? copy + sizeof(uint16_t) * p.planes * p.rows_pad : copy;
+      backward ? copy + sizeof(uint16_t) * p.d_planes * p.rows_pad : copy;
   const size_t most = backward ? kBackwardBytes : kForwardBytes;
   const int64_t whole = up(vocab, kTile);
   int64_t piece = whole;
@@ -1211,14 +1364,19 @@ Plan plan_of(const void* weight, int elem_size, int64_t rows, int64_t width, int
   // there are as many workgroups as run at once, 8 rounds each at least.
   auto splits_of = [&](int tile) {
     const int64_t at_once = tile == kTile ? kCus : 2 * kCus;
-    return std::max<int64_t>(1, std::min(at_once / tiles_of(width, rows, tile),
+    return std::max<int64_t>(1, std::min(at_once / tiles_of(width, p.sum_rows, tile),
                                          p.piece / (8 * kStep)));
   };
   p.tile_hidden = better_tile([&](int tile) {
     const int64_t splits = splits_of(tile);
-    return Work{splits * tiles_of(width, rows, tile), passes * p.piece / kStep / splits};
+    return Work{splits * tiles_of(width, p.sum_rows, tile), passes * p.piece / kStep / splits};
   });
   p.splits = static_cast<int>(splits_of(p.tile_hidden));
+  if (p.thin && !p.thin_gemm) {
+    // Several workgroups a CU, of 2 rounds at least, and not too many to join.
+    p.splits = static_cast<int>(std::max<int64_t>(
+        1, std::min({2048 / (up(width, 64) / 64), int64_t{128}, in_piece / 128})));
+  }
   size_t at = 0;
   auto take = [&at](size_t bytes) {
     const size_t here = at;
@@ -1231,9 +1389,9 @@ Plan plan_of(const void* weight, int elem_size, int64_t rows, int64_t width, int
   p.hidden = take(plane * p.rows_pad * p.k_pad);
   p.weight = take(p.direct ? 0 : plane * p.piece * p.k_pad);
   if (backward) {
-    p.d = take(plane * p.rows_pad * p.piece);
-    p.sum = take(p.pieces * p.splits > 1
-                     ? sizeof(float) * p.splits * p.rows_pad * up(width, 4) : 0);
+    p.d = take(sizeof(uint16_t) * p.d_planes * p.rows_pad * p.piece);
+    p.sum = take(p.thin || p.pieces * p.splits > 1
+                     ? sizeof(float) * p.splits * p.sum_rows * up(width, 4) : 0);
   } else {
     p.target = take(sizeof(float) * rows);
     p.part = take(sizeof(float2) * (up(vocab, p.tile) / p.tile) * p.rows_pad);
@@ -1308,7 +1466,7 @@ template <typename T>
 int piece_of_weight(const char* what, const Call& c, const Plan& plan, int64_t first, Product* g) {
   g->a_rows = static_cast<int>(std::min(plan.piece, c.vocab - first));
   const T* from = static_cast<const T*>(c.weight) + first * c.weight_ld;
-  if (plan.direct) {
+  if (plan.direct) {  // (of few rows at any alignment: gemm() does not read it)
     g->a = reinterpret_cast<const uint16_t*>(from);
     g->lda = c.weight_ld;
     g->k = static_cast<int>(c.width);
@@ -1413,11 +1571,10 @@ int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse
   g.d = c.at<uint16_t>(plan.d);
   g.d_ld = plan.piece;
   g.d_plane = plan.rows_pad * plan.piece;
-  const bool thin = c.rows <= kThinRows;
   for (int64_t i = 0; i < plan.pieces; ++i) {
     const int64_t first = i * plan.piece;
     HIPO_STEP(piece_of_weight<T>(what, c, plan, first, &g));
-    if (thin) {
+    if (plan.thin) {
       Thin t{};
       t.hidden = c.hidden;
       t.weight = static_cast<const T*>(c.weight) + first * c.weight_ld;
@@ -1440,9 +1597,49 @@ int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse
       t.first = first;
       t.whole_vocab = c.vocab;
       HIPO_STEP((launch_thin<T, true>(what, t, c.rows, c.stream)));
-    } else {
-      HIPO_STEP((multiply<T, kLogitGrad>(what, g, plan.tile, c.rows, c.stream)));
+      if (plan.thin_gemm) {
+        // d's two parts as 128 rows, whose sums join_hidden() adds.
+        Product h{};
+        h.a = g.a;
+        h.lda = g.lda;
+        h.a_rows = width;
+        h.a_k = g.a_rows;
+        h.b = g.d;
+        h.ldb = g.d_ld;
+        h.b_rows = 2 * kThinRows;
+        h.k = static_cast<int>(up(g.a_rows, kStep));
+        h.splits = plan.splits;
+        h.sum = c.at<float>(plan.sum);
+        h.sum_ld = up(c.width, 4);
+        h.sum_plane = plan.sum_rows * h.sum_ld;
+        h.load_sum = i > 0;
+        HIPO_STEP((multiply<T, kAccumulate>(what, h, plan.tile_hidden, h.b_rows, c.stream)));
+      } else {
+        const ThinHidden h{t.weight, c.weight_ld, g.a_rows, width, g.d, g.d_ld, g.d_plane,
+                           g.b_count, c.at<float>(plan.sum), up(c.width, 4), i > 0};
+        const dim3 grid(static_cast<uint32_t>(up(c.width, 64) / 64), plan.splits);
+        if (c.rows <= 16) {
+          thin_hidden<T, 1><<<grid, 256, 0, c.stream>>>(h);
+        } else if (c.rows <= 32) {
+          thin_hidden<T, 2><<<grid, 256, 0, c.stream>>>(h);
+        } else {
+          thin_hidden<T, 4><<<grid, 256, 0, c.stream>>>(h);
+        }
+        HIPO_STEP(check_launch(what));
+      }
+      // Columns in as many parts as it takes to fill the CUs several times.
+      const int64_t strips = up(g.a_rows, 64) / 64, all = up(c.width, 64) / 64;
+      const int64_t parts = std::min<int64_t>(all, std::max<int64_t>(1, 2048 / strips));
+      const int chunks = static_cast<int>((all + parts - 1) / parts);
+      thin_weight<T><<<dim3(static_cast<uint32_t>(strips),
+                            static_cast<uint32_t>((all + chunks - 1) / chunks)),
+                       256, 0, c.stream>>>(
+          ThinWeight{g.b, g.d, g.ldb, g.b_plane, g.d_ld, g.d_plane, g.b_count, width, g.a_rows,
+                     static_cast<T*>(dweight) + first * c.width, c.width, chunks});
+      HIPO_STEP(check_launch(what));
+      continue;
     }
+    HIPO_STEP((multiply<T, kLogitGrad>(what, g, plan.tile, c.rows, c.stream)));
 
     Product h{};
     h.a = g.a;
@@ -1466,19 +1663,6 @@ int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse
     h.out_ld = c.width;
     HIPO_STEP((multiply<T, kAccumulate>(what, h, plan.tile_hidden, c.rows, c.stream)));
 
-    if (thin) {
-      // Columns in as many parts as it takes to fill the CUs several times.
-      const int64_t strips = up(g.a_rows, 64) / 64, all = up(c.width, 64) / 64;
-      const int64_t parts = std::min<int64_t>(all, std::max<int64_t>(1, 2048 / strips));
-      const int chunks = static_cast<int>((all + parts - 1) / parts);
-      thin_weight<T><<<dim3(static_cast<uint32_t>(strips),
-                            static_cast<uint32_t>((all + chunks - 1) / chunks)),
-                       256, 0, c.stream>>>(
-          ThinWeight{g.b, g.d, g.ldb, g.b_plane, g.d_ld, g.d_plane, g.b_count, width, g.a_rows,
-                     static_cast<T*>(dweight) + first * c.width, c.width, chunks});
-      HIPO_STEP(check_launch(what));
-      continue;
-    }
     Product w{};
     w.a = g.b;
     w.lda = g.ldb;
@@ -1494,12 +1678,12 @@ int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse
     w.out_ld = c.width;
     HIPO_STEP((multiply<T, kStore>(what, w, plan.tile_weight, g.a_rows, c.stream)));
   }
-  if (plan.splits > 1) {
+  if (plan.thin || plan.splits > 1) {
     const int64_t blocks = (c.rows * ((c.width + 3) / 4) + 255) / 256;
     join_hidden<T><<<static_cast<uint32_t>(std::min<int64_t>(blocks, 1 << 16)), 256, 0,
                      c.stream>>>(c.at<float>(plan.sum), up(c.width, 4),
-                                 plan.rows_pad * up(c.width, 4), plan.splits, g.kept, g.b_count,
-                                 static_cast<T*>(dhidden), width);
+                                 plan.sum_rows * up(c.width, 4), plan.splits, plan.thin_gemm,
+                                 g.kept, g.b_count, static_cast<T*>(dhidden), width);
     return check_launch(what);
   }
   return 0;

@@ -269,7 +269,8 @@ def check_loss(ho, hidden, weight, tokens, grads, what, scale=1.0, wide=True):
 
 
 LAYERS = [(1, 1, 1), (1, 8, 2), (2, 3, 5), (1, 64, 255), (3, 72, 256), (16, 64, 257), (17, 128, 1000),
-          (5, 1001, 3001), (33, 200, 700), (64, 96, 2000), (65, 512, 513), (100, 65, 4097),
+          (5, 1001, 3001), (32, 1032, 777), (33, 200, 700), (48, 2056, 129), (64, 96, 2000),
+          (64, 1024, 1025), (65, 512, 513), (100, 65, 4097), (128, 264, 640), (200, 1000, 260),
           (129, 64, 1023), (256, 128, 512), (257, 64, 513), (300, 320, 1500), (515, 777, 1030),
           (1000, 40, 300)]
 
@@ -331,10 +332,10 @@ def test_cross_entropy_of_larger_layers(rows, width, vocab, dtype, rocm_device, 
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows", [3, 400])
-def test_gradients_over_pieces_of_the_vocabulary(rows, dtype, rocm_device, ho):
-    """More of the vocabulary than one piece of the workspace holds."""
-    width, vocab = 64, 1 << 19 if rows == 400 else 1 << 21
+@pytest.mark.parametrize("rows,width,vocab", [(3, 8, 7 << 20), (3, 9, 7 << 20), (400, 64, 1 << 21)])
+def test_gradients_over_pieces_of_the_vocabulary(rows, width, vocab, dtype, rocm_device, ho):
+    """More of the vocabulary than one piece of the workspace holds: 1.5 GB of d,
+    of few rows and of more."""
     vocab += 77
     hidden, weight, tokens, grads = layer_operands(rocm_device, rows, width, vocab, dtype)
     loss, lse = ho.linear_cross_entropy(hidden, weight, tokens)
@@ -353,6 +354,31 @@ def test_gradients_over_pieces_of_the_vocabulary(rows, dtype, rocm_device, ho):
     part = dw.double().view(-1)[:width * (vocab // 64 * 64)].view(64, -1).norm(dim=-1)
     whole = (d.t() @ hidden.double())[:vocab // 64 * 64].reshape(64, -1).norm(dim=-1)
     assert float(((part - whole) / whole).abs().max()) < least
+
+
+def test_losses_over_pieces_of_the_vocabulary(rocm_device, ho):
+    """More fp32 weights than the 1 GB of copies that one piece of the workspace is."""
+    hidden, weight, tokens, _ = layer_operands(rocm_device, 70, 1024, 180001, F32)
+    got = ho.linear_cross_entropy(hidden, weight, tokens, scale=0.7)
+    for name, u, (v, tol) in zip(("loss", "lse"), got, ref.linear_cross_entropy(
+            hidden, weight, tokens, 0.7)):
+        ref.close(u, v, tol, name)
+
+
+@pytest.mark.parametrize("rows,width", [(1, 64), (1, 65), (3, 200), (20, 72), (64, 131)])
+def test_gradients_of_few_rows_are_rounded_once(rows, width, rocm_device, ho):
+    """Up to 64 rows d has two bf16 parts, so that bf16 gradients are off by their
+    own rounding alone: half a step, and 2^-15 of the sums of absolute products
+    for the parts' and the sums' own."""
+    hidden, weight, tokens, grads = layer_operands(rocm_device, rows, width, 1500, BF16)
+    _, lse = ho.linear_cross_entropy(hidden, weight, tokens)
+    got = ho.linear_cross_entropy_bwd(grads[0], hidden, weight, tokens, lse)
+    h, w = hidden.double(), weight.double()
+    d = torch.exp(h @ w.t() - lse[:, None].double()) * grads[0][:, None].double()
+    d[torch.arange(rows), tokens] -= grads[0].double()
+    for u, v, size in ((got[0], d @ w, d.abs() @ w.abs()),
+                       (got[1], d.t() @ h, d.abs().t() @ h.abs())):
+        ref.close(u, v.cpu(), (v.abs() * 2.0 ** -8 + size * 2.0 ** -15).cpu(), f"{rows} {width}")
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
