@@ -1101,8 +1101,8 @@ def linear_cross_entropy_bwd(grad: torch.Tensor, hidden: torch.Tensor, weight: t
     operands' type: grad and grad_lse (fp32 [R]) are the gradients of its loss and
     lse (1 / R each of the mean loss, 2 c lse / R of a penalty c lse^2), lse is
     its result.  The logits are computed once more, in pieces of the vocabulary;
-    with bf16 operands their gradients are rounded to bf16 for the products with
-    hidden and weight, whose sums are fp32.  Rows of ignore_index have gradient
+    with bf16 operands their gradients are rounded to bf16 (up to 64 rows: to two
+    bf16 parts) for the products with hidden and weight, whose sums are fp32.  Rows of ignore_index have gradient
     zero and add nothing to dweight, whatever they hold; a row of another token
     outside [0, V) is NaN and makes dweight NaN."""
     lib = _lib or load_library()

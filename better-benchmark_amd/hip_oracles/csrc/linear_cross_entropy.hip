@@ -5,16 +5,25 @@
 // d_j = scale ((g + g_lse) e^(s_j - lse) - g [j = t]),  dhidden = d weight,
 // dweight = d^T hidden.
 //
-// All products run through one matrix-product kernel, gemm(), that multiplies
-// rows of two K-contiguous bf16 matrices; what becomes of a tile of the result
-// is its epilogue: a tile's logits are reduced to one maximum and one sum per
-// row (forward), turned into d (backward), or are a tile of a gradient.  Rows
-// that are left out are compacted away first, on the device.  The gradient goes
-// through the vocabulary in pieces, so that d's piece alone is ever in memory.
+// Of more than 64 rows all products run through one matrix-product kernel,
+// gemm(), of bf16 operands; what becomes of a tile of the result is its epilogue: a
+// tile's logits are reduced to one maximum and one sum per row (forward), turned
+// into d (backward), or are a tile of a gradient.  Rows that are left out are
+// compacted away first, on the device.  The gradient goes through the vocabulary in
+// pieces, so that d's piece alone is ever in memory.  The matrix cores bound it:
+// 8192 x 4096 x 65536 takes 3.06 ms forward (1.44 PFLOP/s; the library's product
+// alone of 8192 x 4096 x 64000: 1.43) and 9.7 backward (1.36).  Up to 64 rows the
+// weight's bytes bound everything, and kernels of their own read it as it lies.
 //
-// fp32 operands are split into three bf16 parts (8 bits of the significand
-// each) and multiplied as six products of parts, the smallest first; the three
-// left out are below 2^-24 of the largest.
+// fp32 operands are split into three bf16 parts (8 bits of the significand each)
+// and multiplied as six products of parts, the smallest first; the three left out
+// are below 2^-24 of the largest.  (The fp32 matrix instructions reach a sixteenth
+// of the bf16 rate, six products 2.7 times as much.)
+//
+// d of bf16 operands is rounded to bf16 for its products with them, which the
+// matrix cores take of one type: each value is off by half a step (2^-9 of it on
+// average), as much again as the gradients' own rounding (relative 2-norms 0.0024
+// where gradients rounded from exact d have 0.0017); sums are fp32 throughout.
 #include <algorithm>
 
 #include "hipo_common.h"
@@ -29,6 +38,7 @@ constexpr int kTile = 256;       // rows of either operand that a workgroup mult
 constexpr int kSmallTile = 128;  // or where there are too few such tiles
 constexpr int kStep = 64;        // values of K per round
 constexpr int kThinRows = 64;    // at most, for the kernels of few rows
+constexpr int64_t kCus = 256;
 constexpr float kLargest = 3.402823466e+38f;
 
 inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
@@ -393,6 +403,15 @@ struct Operand {
 };
 
 // Tile / 32 waves, 2 by Tile / 64, of Tile / 2 by 64 values each.
+//
+// What it took (8192 x 4096 x 65536, eighth of the rows left out, forward): loads to
+// LDS a round ahead with two barriers a round 1.14 PFLOP/s; the operands of half a
+// round in registers ahead and one barrier 1.29; loads and LDS reads spread among
+// the matrix instructions 1.45.  LDS reads of the 256 tile take 1536 of a round's
+// 2048 cycles; 131 KB of LDS and 240 registers leave one workgroup a CU.  At 1.8 GHz,
+// where the card's power holds it, the matrix cores were busy 65 % of the cycles
+// before the last step.  No gain: s_setprio around the products, bands of 8 tiles
+// instead of 4 for an XCD, rows of copies and of d padded off powers of two.
 template <typename T, int Tile, Epilogue E>
 __global__ __launch_bounds__(Tile * 2, 2) void gemm(Product p) {
   constexpr int kWavesB = Tile / 64, kFragments = Tile / 32;
@@ -834,26 +853,35 @@ __device__ __forceinline__ int thin_d_part(int pass) {
 }
 
 // The logits of up to 16 N rows against 64 of the vocabulary per workgroup, 16 a
-// wave, reduced or (Grad) turned into d as gemm()'s.  Both operands go through registers, kThinStages
-// rounds ahead, to LDS (places as in Operand): the weight is read once, at any
-// alignment, fp32 split on the way.  Memory bounds it: the loads in flight
-// (32 KB a workgroup of bf16) and the number of workgroups are what counts.
-template <typename T, int N, bool Grad>
-__global__ __launch_bounds__(256) void thin_logits(Thin a) {
+// wave, reduced or (Grad) turned into d as gemm()'s.  Both operands go through
+// registers, kThinStages rounds ahead, to LDS (places as in Operand): the weight is
+// read once, at any alignment, fp32 split on the way.  Memory bounds it (1 x 4096 x
+// 128000 bf16: 203 us, 5.2 TB/s; fp32 460 us, 4.6): the loads in flight (32 KB a
+// workgroup of bf16) and the number of workgroups are what counts.  Where there are
+// few, K is split among `Groups` groups of four waves, whose sums are
+// added through LDS.
+template <typename T, int N, bool Grad, int Groups>
+__global__ __launch_bounds__(256 * Groups) void thin_logits(Thin a) {
   constexpr int kPlanes = sizeof(T) == 2 ? 1 : 3, kPasses = kPlanes == 1 ? 1 : 6;
   constexpr int kPlaneW = kThinTile * kStep, kPlaneH = 16 * N * kStep;
   constexpr int kPiecesH = (N + 1) / 2;
-  __shared__ __attribute__((aligned(16))) uint16_t weight[2][kPlanes * kPlaneW];
-  __shared__ __attribute__((aligned(16))) uint16_t hidden[2][kPlanes * kPlaneH];
+  __shared__ __attribute__((aligned(16))) uint16_t weights[Groups][2][kPlanes * kPlaneW];
+  __shared__ __attribute__((aligned(16))) uint16_t hiddens[Groups][2][kPlanes * kPlaneH];
   __shared__ float2 parts[4][16 * N];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int group = threadIdx.x >> 8, thread = threadIdx.x & 255;
+  uint16_t(&weight)[2][kPlanes * kPlaneW] = weights[group];
+  uint16_t(&hidden)[2][kPlanes * kPlaneH] = hiddens[group];
+  const int lane = thread & 63, wave = thread >> 6;
   const int l = lane & 15, g = lane >> 4;
-  const int row = threadIdx.x >> 3, chunk = threadIdx.x & 7;
+  const int row = thread >> 3, chunk = thread & 7;
   const int place = row * kStep + ((chunk ^ (row & 7)) * 8);  // and 32 rows on
   const float to_log2 = a.scale * kLog2eHi;
-  const bool with_h = N > 1 || threadIdx.x < 128;
+  const bool with_h = N > 1 || thread < 128;
   const int rows = Grad ? *a.count : a.rows;
   if (rows == 0) return;
+  // This group's columns: from `begin` to `end`, `length` at most.
+  const int length = ((a.width + kStep - 1) / kStep + Groups - 1) / Groups * kStep;
+  const int begin = group * length, end = min(a.width, begin + length);
   const T* from_h[kPiecesH];
 #pragma unroll
   for (int q = 0; q < kPiecesH; ++q) {
@@ -870,12 +898,12 @@ __global__ __launch_bounds__(256) void thin_logits(Thin a) {
     }
     Piece<T> w[kThinStages][2], h[kThinStages][kPiecesH];
     auto load = [&](int stage, int k0) __attribute__((always_inline)) {
-      const int k = k0 + chunk * 8;
+      const int k = begin + k0 + chunk * 8;
 #pragma unroll
-      for (int q = 0; q < 2; ++q) w[stage][q].load(from_w[q], k, a.width);
+      for (int q = 0; q < 2; ++q) w[stage][q].load(from_w[q], k, end);
       if (with_h) {
 #pragma unroll
-        for (int q = 0; q < kPiecesH; ++q) h[stage][q].load(from_h[q], k, a.width);
+        for (int q = 0; q < kPiecesH; ++q) h[stage][q].load(from_h[q], k, end);
       }
     };
     // Two sums, of the halves of the rounds: shorter ones round less.
@@ -884,10 +912,10 @@ __global__ __launch_bounds__(256) void thin_logits(Thin a) {
     for (int n = 0; n < N; ++n) acc[n] = other[n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int s = 0; s < kThinStages; ++s) load(s, s * kStep);
-    for (int k0 = 0; k0 < a.width; k0 += kThinStages * kStep) {
+    for (int k0 = 0; k0 < length; k0 += kThinStages * kStep) {
 #pragma unroll
       for (int s = 0; s < kThinStages; ++s) {
-        if (k0 + s * kStep >= a.width) break;
+        if (k0 + s * kStep >= length) break;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           w[s][q].store(weight[s & 1] + place + q * 32 * kStep, kPlaneW);
@@ -929,10 +957,29 @@ __global__ __launch_bounds__(256) void thin_logits(Thin a) {
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) acc[n] += other[n];
+    if constexpr (Groups > 1) {
+      __syncthreads();
+      // In LDS that the group itself has read.
+      f32x4_t* sums = reinterpret_cast<f32x4_t*>(weights[group]);
+      if (group > 0) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) sums[n * 256 + thread] = acc[n];
+      }
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll
+        for (int q = 1; q < Groups; ++q) {
+          const f32x4_t* from = reinterpret_cast<const f32x4_t*>(weights[q]);
+#pragma unroll
+          for (int n = 0; n < N; ++n) acc[n] += from[n * 256 + thread];
+        }
+      }
+    }
     const int64_t i0 = first + wave * 16 + g * 4;
     if constexpr (Grad) {
 #pragma unroll
       for (int n = 0; n < N; ++n) {
+        if (group > 0) break;
         const int j = n * 16 + l;
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (j < rows) {
@@ -959,6 +1006,7 @@ __global__ __launch_bounds__(256) void thin_logits(Thin a) {
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
+      if (group > 0) break;
       const int j = n * 16 + l;
       const int64_t tok = j < a.rows ? token_at(a.tokens, a.token_size, j) : -1;
       float top = -kLargest;
@@ -1004,7 +1052,8 @@ struct ThinWeight {
 // dweight of up to 64 rows: 64 of the vocabulary per workgroup, 16 a wave, whose
 // d stays in registers while the columns pass, 64 at a time.  The products'
 // operands are [row][...], read across as in Operand.  What is written bounds it,
-// so several workgroups a CU write at once, whole 128-byte pieces of rows.
+// so several workgroups a CU write at once, whole 128-byte pieces of rows (1 x 4096
+// x 128000: 264 us for 1.05 GB, where gemm()'s tiles of one or two rounds took 360).
 template <typename T>
 __global__ __launch_bounds__(256) void thin_weight(ThinWeight a) {
   constexpr int kPlanes = sizeof(T) == 2 ? 1 : 3, kParts = kThinParts<T>;
@@ -1138,7 +1187,9 @@ struct ThinHidden {
 // dhidden of up to 16 N rows: 64 columns of a part of the vocabulary per
 // workgroup, 16 a wave, the parts joined by join_hidden().  The weight goes
 // through registers to LDS (as in thin_logits(), read across as in Operand), two
-// rounds of 64 of the vocabulary ahead; its second reading bounds the kernel.
+// rounds of 64 of the vocabulary ahead; its second reading bounds the kernel.  (Of
+// aligned bf16 gemm() is quicker, d's parts as 128 rows: 64 x 4096 x 128000 205 us
+// against 318.)
 template <typename T, int N>
 __global__ __launch_bounds__(256) void thin_hidden(ThinHidden a) {
   constexpr int kPlanes = sizeof(T) == 2 ? 1 : 3, kParts = kThinParts<T>;
@@ -1293,7 +1344,6 @@ struct Plan {
   size_t kept, count, target, part, hidden, weight, d, sum, bytes;
 };
 
-constexpr int64_t kCus = 256;
 constexpr int64_t kMostTiles = int64_t{1} << 22;  // 2^31 threads
 constexpr int64_t kMostRows = (int64_t{1} << 22) - kTile;  // a tile's bytes fit 31 bits
 constexpr size_t kForwardBytes = size_t{1024} << 20;  // of a copied piece
@@ -1517,12 +1567,20 @@ int select_and_pack(const char* what, const Call& c, const Plan& plan, float* lo
 template <typename T, bool Grad>
 int launch_thin(const char* what, const Thin& a, int64_t rows, hipStream_t stream) {
   const uint32_t grid = static_cast<uint32_t>(std::min<int64_t>(a.tiles, 1 << 20));
+  // No more workgroups than CUs: K split, as far as LDS and registers reach (4 x
+  // 3584 x 3968 bf16, 62 workgroups: 22.1 -> 15.2 us; 1 x 2048 x 32000, 500
+  // workgroups: 23.9 -> 30.5, so not there).
+  const bool few = a.tiles <= kCus;
+  constexpr int kMany = sizeof(T) == 2 ? 4 : 2, kWide = sizeof(T) == 2 ? 2 : 1;
   if (rows <= 16) {
-    thin_logits<T, 1, Grad><<<grid, 256, 0, stream>>>(a);
+    few ? thin_logits<T, 1, Grad, kMany><<<grid, 256 * kMany, 0, stream>>>(a)
+        : thin_logits<T, 1, Grad, 1><<<grid, 256, 0, stream>>>(a);
   } else if (rows <= 32) {
-    thin_logits<T, 2, Grad><<<grid, 256, 0, stream>>>(a);
+    few ? thin_logits<T, 2, Grad, kMany><<<grid, 256 * kMany, 0, stream>>>(a)
+        : thin_logits<T, 2, Grad, 1><<<grid, 256, 0, stream>>>(a);
   } else {
-    thin_logits<T, 4, Grad><<<grid, 256, 0, stream>>>(a);
+    few ? thin_logits<T, 4, Grad, kWide><<<grid, 256 * kWide, 0, stream>>>(a)
+        : thin_logits<T, 4, Grad, 1><<<grid, 256, 0, stream>>>(a);
   }
   return check_launch(what);
 }

@@ -604,14 +604,17 @@ int hipo_block_norms_bwd(const void* grad_h, const void* grad_y, const void* x,
  * weight [vocab, width], with row strides of their own (>= width), both of bf16
  * (elem_size 2) or fp32 (4), at any element alignment; tokens is [rows] of
  * int32 (token_size 4) or int64 (8); loss and lse are [rows]; scale is from
- * 2^-100 to 2^100.  A row whose token is ignore_index is left out, whatever it
- * holds: 0 and 0.  A token outside [0, vocab) otherwise has loss NaN.  A row
- * with a NaN logit has lse NaN.  weight that is bf16, 16-byte aligned and whose
- * row stride is a multiple of 8 is read where it lies; other weights are copied
- * into the workspace piece by piece.  `workspace`: at least
- * hipo_linear_cross_entropy_workspace_bytes bytes (weight is looked at for its
- * alignment only), 16-byte aligned, no initialisation needed; calls that share
- * one must be ordered.
+ * 2^-100 to 2^100.  At most 2^22 - 256 rows, width 2^20, weight_row_stride 2^21,
+ * a vocabulary of 2^31 - 65536, and rows * width 2^38.  A row whose token is
+ * ignore_index is left out, whatever it holds: 0 and 0.  A token outside [0,
+ * vocab) otherwise has loss NaN.  A row with a NaN logit has lse NaN, one with an
+ * infinite logit no finite lse.  Up to 64 rows weight is read where it lies, and so
+ * is one that is bf16, 16-byte aligned, of a width and a row stride that are
+ * multiples of 8; others are copied into the workspace piece by piece.
+ * `workspace`: at least hipo_linear_cross_entropy_workspace_bytes bytes (weight is
+ * looked at for its alignment only), 16-byte aligned, no initialisation needed;
+ * calls that share one must be ordered.  The same call gives the same bits; a row's
+ * may differ in the last ones between batches of other sizes.
  * No counterpart among the reference's oracles; hipo_token_logprobs for logits
  * that are never in memory.
  */
@@ -632,7 +635,8 @@ int hipo_linear_cross_entropy(const void* hidden, const void* weight, int elem_s
  *   dhidden  = d weight,  dweight = d^T hidden
  * the logits computed once more in pieces of the vocabulary, the products
  * accumulated in fp32 and rounded once to the operands' type; d itself is
- * rounded to bf16 where the operands are bf16 (the matrix cores' type).
+ * rounded to bf16 where the operands are bf16 (the matrix cores' type; up to 64
+ * rows to two bf16 parts, some 2^-17 of it).
  * dhidden is contiguous [rows, width], dweight [vocab, width]; they overlap
  * neither each other nor an operand.  Rows of ignore_index are zero in dhidden
  * and add nothing to dweight, whatever they hold; a row of another token outside
