@@ -1397,6 +1397,7 @@ Plan plan_of(const void* weight, int elem_size, int64_t rows, int64_t width, int
   if (per_row > 0) {
     piece = std::min<int64_t>(whole, std::max<int64_t>(kTile, most / per_row / kTile * kTile));
   }
+  piece = std::min(piece, kMostRows);  // a row of d
   // Tiles of one launch.
   const int64_t other = std::max(p.rows_pad, up(width, kTile)) / kTile;
   piece = std::min(piece, std::max<int64_t>(1, kMostTiles / other) * kTile);

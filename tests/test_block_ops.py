@@ -186,6 +186,8 @@ def test_cross_entropy_can_be_launched(launches):
 @pytest.mark.parametrize("call", [
     ("block_norms", 300, 700, 0, 2, 0), ("block_norms_bwd", 300, 700, 1, 2, 0),
     ("linear_cross_entropy", 300, 200, 3000, 2), ("linear_cross_entropy", 3, 200, 3000, 4),
+    ("linear_cross_entropy_bwd", 3, 200, 3000, 2), ("linear_cross_entropy_bwd", 40, 201, 3000, 2),
+    ("linear_cross_entropy_bwd", 3, 200, 3000, 4),
     ("linear_cross_entropy_bwd", 300, 200, 3000, 2), ("linear_cross_entropy_bwd", 8192, 4096,
                                                       128000, 4)])
 def test_a_refused_launch_ends_the_call(call, launches):
