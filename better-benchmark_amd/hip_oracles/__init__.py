@@ -932,7 +932,7 @@ def _require_block_norms(what, x, rows_of, post, post_bias, pre, pre_bias, gate,
                                        and t.is_contiguous()))
         gates = 0
         if gate is not None and ok:
-            gates = 1 if gate.dim() == 1 else gate.shape[0]
+            gates = gate.shape[0] if gate.dim() == 2 else 1
             ok = (gate.dtype == dtype and gate.dim() in (1, 2) and gate.shape[-1] == cols
                   and gate.device == dev and gate.is_contiguous() and gates > 0
                   and rows % gates == 0)

@@ -212,6 +212,8 @@ def test_norms_refuse(rocm_device, ho):
             (lambda: ho.block_norms(x, x, pre=z(32)[::2]), "contiguous"),
             (lambda: ho.block_norms(x, x, pre=w, gate=z(3, 16)), "divide"),
             (lambda: ho.block_norms(x, x, pre=w, gate=z(4, 8)), "gate"),
+            (lambda: ho.block_norms(x, x, pre=w, gate=z(())), "gate"),
+            (lambda: ho.block_norms(x, x, pre=w, gate=z(2, 2, 16)), "gate"),
             (lambda: ho.block_norms(x, x, pre=w, norm="batch"), "norm must be"),
             (lambda: ho.block_norms_bwd(x, None, x, x, st, pre=w), "go together"),
             (lambda: ho.block_norms_bwd(x, x, x, None, st, pre=w), "go together"),
