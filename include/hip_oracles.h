@@ -600,7 +600,8 @@ int hipo_block_norms_bwd(const void* grad_h, const void* grad_y, const void* x,
  *   lse[r]  = ln sum_j e^(s_j)
  *   loss[r] = lse[r] - s_t,  t = tokens[r]
  * in fp32 sums of exact products (fp32 operands: of three bf16 parts each,
- * products below 2^-24 of the largest left out).  hidden is [rows, width],
+ * products below 2^-24 of the largest left out; parts end at 2^-133, so values
+ * below 2^-110 are held to fewer bits than 24).  hidden is [rows, width],
  * weight [vocab, width], with row strides of their own (>= width), both of bf16
  * (elem_size 2) or fp32 (4), at any element alignment; tokens is [rows] of
  * int32 (token_size 4) or int64 (8); loss and lse are [rows]; scale is from
