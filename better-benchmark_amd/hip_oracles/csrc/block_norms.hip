@@ -145,7 +145,7 @@ inline Layout layout_of(int64_t cols, int groups) {
 // Groups per lane of the gradient: it holds up to nine rows' worth of registers
 // (four operands, the next row's, up to five sums), and with one group 8 to 16
 // waves fit a CU.  Rows past 4096 columns take two, so that 8 waves hold a row
-// and each lane has 256 registers (with 16 waves it has 128, too few).
+// and each lane has 256 registers; past 8192 columns 16 waves do, of 128.
 inline int bwd_groups(int64_t cols) { return cols <= 512 * kGroup ? 1 : 2; }
 
 // Where a lane's groups lie.  The group that would cross the row's end is moved
@@ -376,35 +376,73 @@ template <typename T, int U, bool SMALL, bool LAYER, bool PRE, bool POST, Gate G
 __global__ __launch_bounds__(THREADS) void block_norms_bwd(Backward a) {
   constexpr bool kSmall = SMALL;
   constexpr bool kAhead = U == 1;  // with two groups a lane has no registers for it
+  // 16 waves leave a lane 128 registers.  The two weights' sums then lie in LDS, 128
+  // KB of it, read and written once a row (16 bytes of a lane beside the next's), and
+  // weights and gate are loaded where they are used: [4096, 12288] bf16 297 -> 151 us,
+  // of 512 threads (8192 x 5120) 122 -> 129, so not there.
+  constexpr bool kFewRegisters = THREADS == 1024;
   __shared__ float slots[2][64];
+  __shared__ f32x4_t held[kFewRegisters ? 2 * U * 2 * THREADS : 1];
   extern __shared__ float sums[];  // [teams][cols], where there are several teams
   const int team = threadIdx.x / a.lanes;
   const Columns<U> c = columns_of<U>(threadIdx.x % a.lanes, a.lanes, a.cols);
   const int64_t begin = first_row(a.rows, blockIdx.x, a.blocks);
   const int64_t end = first_row(a.rows, blockIdx.x + 1, a.blocks);
   Vec8 acc[kSums][U];
+  auto sum_of = [&](int k, int u) __attribute__((always_inline)) {
+    if (!kFewRegisters || (k != kPre && k != kPost)) return acc[k][u];
+    const f32x4_t* at = held + ((k == kPost) * U + u) * 2 * THREADS + threadIdx.x;
+    const f32x4_t v = at[0], w = at[THREADS];
+    return Vec8{{v[0], v[1], v[2], v[3], w[0], w[1], w[2], w[3]}};
+  };
+  auto set_sum = [&](int k, int u, const Vec8& v) __attribute__((always_inline)) {
+    if (!kFewRegisters || (k != kPre && k != kPost)) {
+      acc[k][u] = v;
+      return;
+    }
+    f32x4_t* at = held + ((k == kPost) * U + u) * 2 * THREADS + threadIdx.x;
+    at[0] = f32x4_t{v.v[0], v.v[1], v.v[2], v.v[3]};
+    at[THREADS] = f32x4_t{v.v[4], v.v[5], v.v[6], v.v[7]};
+  };
 #pragma unroll
   for (int k = 0; k < kSums; ++k) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) acc[k][u] = Vec8{};
+    for (int u = 0; u < U; ++u) set_sum(k, u, Vec8{});
   }
-  // (In registers, as a load in the loop would wait for the next row's.)
+  // (In registers where there is room, as a load in the loop would wait for the next
+  // row's.)
   Vec8 wpre[U], wpost[U], bpost[U], gate[U];
+  auto vector = [&](Vec8 (&w)[U], const void* from, float plus) __attribute__((always_inline)) {
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (PRE) wpre[u] = load8(static_cast<const T*>(a.pre) + c.col[u]);
-    if (POST) wpost[u] = load8(static_cast<const T*>(a.post) + c.col[u]);
-    bpost[u] = Vec8{};
-    if (GATE && POST && LAYER && a.post_bias) {
-      bpost[u] = load8(static_cast<const T*>(a.post_bias) + c.col[u]);
-    }
+    for (int u = 0; u < U; ++u) {
+      w[u] = load8(static_cast<const T*>(from) + c.col[u]);
 #pragma unroll
-    for (int i = 0; i < kGroup; ++i) {
-      wpre[u].v[i] = PRE ? wpre[u].v[i] + a.offset : 0.0f;
-      wpost[u].v[i] = POST ? wpost[u].v[i] + a.offset : 0.0f;
-      gate[u].v[i] = a.scale;
+      for (int i = 0; i < kGroup; ++i) w[u].v[i] += plus;
     }
-  }
+  };
+  auto load_pre = [&]() __attribute__((always_inline)) { vector(wpre, a.pre, a.offset); };
+  auto load_post = [&]() __attribute__((always_inline)) {
+    vector(wpost, a.post, a.offset);
+    if (GATE && LAYER) {
+      if (a.post_bias) {
+        vector(bpost, a.post_bias, 0.0f);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) bpost[u] = Vec8{};
+      }
+    }
+  };
+  // scale * gate of one of its rows.
+  auto load_gate = [&](int64_t which) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      gate[u] = load8(static_cast<const T*>(a.gate) + which * a.cols + c.col[u]);
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) gate[u].v[i] *= a.scale;
+    }
+  };
+  if (!kFewRegisters && PRE) load_pre();
+  if (!kFewRegisters && POST) load_post();
 
   // The sum over the teams of one accumulator, written by put(column, value).
   auto flush = [&](Vec8 (&v)[U], auto put) {
@@ -444,12 +482,7 @@ __global__ __launch_bounds__(THREADS) void block_norms_bwd(Backward a) {
     if (GATE && !by_row) {
       which = from / a.rows_per_gate;
       to = min(end, (which + 1) * a.rows_per_gate);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        gate[u] = load8(static_cast<const T*>(a.gate) + which * a.cols + c.col[u]);
-#pragma unroll
-        for (int i = 0; i < kGroup; ++i) gate[u].v[i] *= a.scale;
-      }
+      if (!kFewRegisters) load_gate(which);
     }
     // All loads without a branch, or the compiler waits for them at its end.
     const T* grad_h = static_cast<const T*>(a.grad_h ? a.grad_h : a.grad_y);
@@ -466,7 +499,9 @@ __global__ __launch_bounds__(THREADS) void block_norms_bwd(Backward a) {
         if (PRE) next.h[u].load_once(static_cast<const T*>(a.h) + at + c.col[u]);
         next.gh[u].load_once(grad_h + at + c.col[u]);
         if (POST || GATE) next.x[u].load_once(static_cast<const T*>(a.x) + at + c.col[u]);
-        if (by_row) next.gate[u].load_once(static_cast<const T*>(a.gate) + at + c.col[u]);
+        if (by_row && !kFewRegisters) {
+          next.gate[u].load_once(static_cast<const T*>(a.gate) + at + c.col[u]);
+        }
       }
       // (What is not used is not loaded: its register would be waited for.)
 #pragma unroll
@@ -487,8 +522,7 @@ __global__ __launch_bounds__(THREADS) void block_norms_bwd(Backward a) {
         if (PRE) gy[u] = row.gy[u].values();
         if (PRE) h[u] = row.h[u].values();
         gh[u] = row.gh[u].values();
-        if (POST || GATE) x[u] = row.x[u].values();
-        if (by_row) {
+        if (by_row && !kFewRegisters) {
           gate[u] = row.gate[u].values();
 #pragma unroll
           for (int i = 0; i < kGroup; ++i) gate[u].v[i] *= a.scale;
@@ -498,15 +532,19 @@ __global__ __launch_bounds__(THREADS) void block_norms_bwd(Backward a) {
       if (kAhead) load(next, min(first + a.teams, to - 1));
       // gh becomes T.
       if (PRE) {
+        if (kFewRegisters) load_pre();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+          Vec8 dw = sum_of(kPre, u), db = sum_of(kPreBias, u);
 #pragma unroll
           for (int i = 0; i < kGroup; ++i) {
             h[u].v[i] = (LAYER ? h[u].v[i] - st[2] : h[u].v[i]) * st[3];
-            acc[kPre][u].v[i] += gy[u].v[i] * h[u].v[i];
-            if (LAYER) acc[kPreBias][u].v[i] += gy[u].v[i];
+            dw.v[i] += gy[u].v[i] * h[u].v[i];
+            db.v[i] += gy[u].v[i];
             gy[u].v[i] *= wpre[u].v[i];
           }
+          set_sum(kPre, u, dw);
+          if (LAYER) set_sum(kPreBias, u, db);
         }
         float s[2] = {0.0f, 0.0f};
         pair_sum<U, LAYER>(s, gy, h, c, ragged);
@@ -529,16 +567,20 @@ __global__ __launch_bounds__(THREADS) void block_norms_bwd(Backward a) {
         }
       }
       // gh becomes v = scale gate T, x the normalised x.
+      if (kFewRegisters && POST) load_post();
+      if (kFewRegisters && GATE) load_gate(by_row ? min(first + team, to - 1) : which);
       if (POST || GATE) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           Vec8 tn;
+          x[u] = row.x[u].values();
 #pragma unroll
           for (int i = 0; i < kGroup; ++i) {
             float n = x[u].v[i];
             if (POST) {
               x[u].v[i] = (LAYER ? n - st[0] : n) * st[1];
-              n = __builtin_fmaf(x[u].v[i], wpost[u].v[i], bpost[u].v[i]);
+              n = x[u].v[i] * wpost[u].v[i];
+              if (LAYER) n = __builtin_fmaf(x[u].v[i], wpost[u].v[i], bpost[u].v[i]);
             }
             if (GATE == kGateOfRows) acc[kGate][u].v[i] += gh[u].v[i] * n;
             tn.v[i] = gh[u].v[i] * n * a.scale;
@@ -550,15 +592,18 @@ __global__ __launch_bounds__(THREADS) void block_norms_bwd(Backward a) {
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
+        Vec8 dw = sum_of(kPost, u), db = sum_of(kPostBias, u);
 #pragma unroll
         for (int i = 0; i < kGroup; ++i) {
-          gh[u].v[i] *= gate[u].v[i];
+          gh[u].v[i] *= GATE ? gate[u].v[i] : a.scale;
           if (POST) {
-            acc[kPost][u].v[i] += gh[u].v[i] * x[u].v[i];
-            if (LAYER) acc[kPostBias][u].v[i] += gh[u].v[i];
+            dw.v[i] += gh[u].v[i] * x[u].v[i];
+            db.v[i] += gh[u].v[i];
             gh[u].v[i] *= wpost[u].v[i];
           }
         }
+        if (POST) set_sum(kPost, u, dw);
+        if (POST && LAYER) set_sum(kPostBias, u, db);
       }
       if (POST) {
         float s[2] = {0.0f, 0.0f};
@@ -604,14 +649,17 @@ __global__ __launch_bounds__(THREADS) void block_norms_bwd(Backward a) {
     }
     from = to;
   }
-  auto put_part = [&](int k, Vec8 (&v)[U]) {
+  auto put_part = [&](int k) __attribute__((always_inline)) {
+    Vec8 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = sum_of(k, u);
     float* out = a.part + (static_cast<int64_t>(k) * a.blocks + blockIdx.x) * a.cols;
     flush(v, [&](int j, float s) { out[j] = s; });
   };
-  if (PRE) put_part(kPre, acc[kPre]);
-  if (PRE && LAYER) put_part(kPreBias, acc[kPreBias]);
-  if (POST) put_part(kPost, acc[kPost]);
-  if (POST && LAYER) put_part(kPostBias, acc[kPostBias]);
+  if (PRE) put_part(kPre);
+  if (PRE && LAYER) put_part(kPreBias);
+  if (POST) put_part(kPost);
+  if (POST && LAYER) put_part(kPostBias);
 }
 
 struct Join {

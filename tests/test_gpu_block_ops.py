@@ -115,8 +115,16 @@ def test_gates_of_samples(rows, gates, cols, dtype, rocm_device, ho):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,gates,cols", [(600, 7, 9001), (600, 600, 12288), (1024, 16, 16384),
+                                             (1024, 512, 8200)])
+def test_gates_of_wide_samples(rows, gates, cols, dtype, rocm_device, ho):
+    test_gates_of_samples(rows, gates, cols, dtype, rocm_device, ho)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("norm", ["rms", "layer"])
-@pytest.mark.parametrize("rows,cols", [(30011, 64), (9001, 1001), (8192, 2048), (700, 8192)])
+@pytest.mark.parametrize("rows,cols", [(30011, 64), (9001, 1001), (8192, 2048), (700, 8192),
+                                       (777, 9001), (520, 16384)])
 def test_norms_of_many_rows(rows, cols, norm, dtype, rocm_device, ho):
     """The same bits again, biases left out, and rows that are the same in
     another batch."""
