@@ -127,9 +127,11 @@ struct Piece;
 template <>
 struct Piece<uint16_t> {
   u32x4_t w;
+  template <bool Once = false>
   __device__ __forceinline__ void load(const uint16_t* row, int k, int width) {
     if (k + 8 <= width) {
-      w = *reinterpret_cast<const u32x4_a2_t*>(row + k);
+      const u32x4_a2_t* at = reinterpret_cast<const u32x4_a2_t*>(row + k);
+      w = Once ? __builtin_nontemporal_load(at) : *at;
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -146,6 +148,7 @@ struct Piece<uint16_t> {
 template <>
 struct Piece<float> {
   f32x4_t v[2];
+  template <bool Once = false>
   __device__ __forceinline__ void load(const float* row, int k, int width) {
     if (k + 8 <= width) {
       v[0] = *reinterpret_cast<const f32x4_a4_t*>(row + k);
@@ -701,7 +704,9 @@ __global__ __launch_bounds__(Tile * 2, 2) void gemm(Product p) {
           uint16_t* out = static_cast<uint16_t*>(p.out) +
                           (tile_b * static_cast<int64_t>(Tile) + j) * p.out_ld + i;
           if (i + 8 <= p.a_rows) {
-            *reinterpret_cast<u32x4_a2_t*>(out) = v;
+            // (Of no use in the caches: 256 x 4096 x 128000 1034 -> 971 us, with the
+            // rows of few-row calls 732 -> 690.)
+            __builtin_nontemporal_store(v, reinterpret_cast<u32x4_a2_t*>(out));
           } else {
 #pragma unroll
             for (int m = 0; m < 7; ++m) {
@@ -856,11 +861,11 @@ __device__ __forceinline__ int thin_d_part(int pass) {
 // wave, reduced or (Grad) turned into d as gemm()'s.  Both operands go through
 // registers, kThinStages rounds ahead, to LDS (places as in Operand): the weight is
 // read once, at any alignment, fp32 split on the way.  Memory bounds it (1 x 4096 x
-// 128000 bf16: 203 us, 5.2 TB/s; fp32 460 us, 4.6): the loads in flight (32 KB a
+// 128000 bf16: 192 us, 5.5 TB/s; fp32 460 us, 4.6): the loads in flight (32 KB a
 // workgroup of bf16) and the number of workgroups are what counts.  Where there are
-// few, K is split among `Groups` groups of four waves, whose sums are
-// added through LDS.
-template <typename T, int N, bool Grad, int Groups>
+// few, K is split among `Groups` groups of four waves, whose sums are added
+// through LDS.  Once: the weight takes no place in the caches.
+template <typename T, int N, bool Grad, int Groups, bool Once = false>
 __global__ __launch_bounds__(256 * Groups) void thin_logits(Thin a) {
   constexpr int kPlanes = sizeof(T) == 2 ? 1 : 3, kPasses = kPlanes == 1 ? 1 : 6;
   constexpr int kPlaneW = kThinTile * kStep, kPlaneH = 16 * N * kStep;
@@ -900,7 +905,7 @@ __global__ __launch_bounds__(256 * Groups) void thin_logits(Thin a) {
     auto load = [&](int stage, int k0) __attribute__((always_inline)) {
       const int k = begin + k0 + chunk * 8;
 #pragma unroll
-      for (int q = 0; q < 2; ++q) w[stage][q].load(from_w[q], k, end);
+      for (int q = 0; q < 2; ++q) w[stage][q].template load<Once>(from_w[q], k, end);
       if (with_h) {
 #pragma unroll
         for (int q = 0; q < kPiecesH; ++q) h[stage][q].load(from_h[q], k, end);
@@ -1160,7 +1165,7 @@ __global__ __launch_bounds__(256) void thin_weight(ThinWeight a) {
         if (v + j >= a.vocab) continue;
         uint16_t* out = static_cast<uint16_t*>(a.out) + (v + j) * a.out_ld + i;
         if (i + 8 <= a.width) {
-          *reinterpret_cast<u32x4_a2_t*>(out) = w;
+          __builtin_nontemporal_store(w, reinterpret_cast<u32x4_a2_t*>(out));
         } else {
 #pragma unroll
           for (int m = 0; m < 7; ++m) {
@@ -1573,15 +1578,26 @@ int launch_thin(const char* what, const Thin& a, int64_t rows, hipStream_t strea
   // workgroups: 23.9 -> 30.5, so not there).
   const bool few = a.tiles <= kCus;
   constexpr int kMany = sizeof(T) == 2 ? 4 : 2, kWide = sizeof(T) == 2 ? 2 : 1;
+  // Rows that are whole 128-byte lines, read once: past the caches, which hold other
+  // layers' weights by the next call (1 x 4096 x 128000 207 -> 192 us, 1 x 2048 x 32000
+  // among other states 36.7 -> 33.3; the same 131 MB at once again 26.8 -> 32.0).  Of
+  // other rows (3 x 1000 x 20001) 17.4 -> 20.3, as two rows' reads meet in a line; the
+  // gradient reads the weight twice (8 x 2048 x 32000 117 -> 119).
+  constexpr bool kOnce = sizeof(T) == 2 && !Grad;
+  const bool once = kOnce && reinterpret_cast<uintptr_t>(a.weight) % 128 == 0 &&
+                    a.weight_ld % 64 == 0;
   if (rows <= 16) {
-    few ? thin_logits<T, 1, Grad, kMany><<<grid, 256 * kMany, 0, stream>>>(a)
-        : thin_logits<T, 1, Grad, 1><<<grid, 256, 0, stream>>>(a);
+    few    ? thin_logits<T, 1, Grad, kMany><<<grid, 256 * kMany, 0, stream>>>(a)
+    : once ? thin_logits<T, 1, Grad, 1, kOnce><<<grid, 256, 0, stream>>>(a)
+           : thin_logits<T, 1, Grad, 1><<<grid, 256, 0, stream>>>(a);
   } else if (rows <= 32) {
-    few ? thin_logits<T, 2, Grad, kMany><<<grid, 256 * kMany, 0, stream>>>(a)
-        : thin_logits<T, 2, Grad, 1><<<grid, 256, 0, stream>>>(a);
+    few    ? thin_logits<T, 2, Grad, kMany><<<grid, 256 * kMany, 0, stream>>>(a)
+    : once ? thin_logits<T, 2, Grad, 1, kOnce><<<grid, 256, 0, stream>>>(a)
+           : thin_logits<T, 2, Grad, 1><<<grid, 256, 0, stream>>>(a);
   } else {
-    few ? thin_logits<T, 4, Grad, kWide><<<grid, 256 * kWide, 0, stream>>>(a)
-        : thin_logits<T, 4, Grad, 1><<<grid, 256, 0, stream>>>(a);
+    few    ? thin_logits<T, 4, Grad, kWide><<<grid, 256 * kWide, 0, stream>>>(a)
+    : once ? thin_logits<T, 4, Grad, 1, kOnce><<<grid, 256, 0, stream>>>(a)
+           : thin_logits<T, 4, Grad, 1><<<grid, 256, 0, stream>>>(a);
   }
   return check_launch(what);
 }
