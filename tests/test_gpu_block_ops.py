@@ -328,7 +328,8 @@ def test_cross_entropy_of_rows_left_out(kind, rows, dtype, rocm_device, ho):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,width,vocab", [(3, 4096, 20011), (1, 2048, 32000), (700, 1024, 9001),
-                                              (2100, 256, 33000), (40, 264, 100003)])
+                                              (2100, 256, 33000), (40, 264, 100003),
+                                              (20, 512, 17001), (64, 192, 24000)])
 def test_cross_entropy_of_larger_layers(rows, width, vocab, dtype, rocm_device, ho):
     case = layer_operands(rocm_device, rows, width, vocab, dtype, std=5.0)
     what = f"[{rows}, {width}, {vocab}] {dtype}"
