@@ -296,7 +296,7 @@ def test_cross_entropy_sizes(rows, width, vocab, dtype, rocm_device, ho):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows", [1, 2, 20, 70, 300, 1030])
+@pytest.mark.parametrize("rows", [1, 2, 20, 70, 300, 1030, 2500])
 @pytest.mark.parametrize("kind", ["some", "all", "but one", "first", "last", "unknown"])
 def test_cross_entropy_of_rows_left_out(kind, rows, dtype, rocm_device, ho):
     """Rows of ignore_index count nowhere, whatever they hold."""
