@@ -121,6 +121,12 @@ _SIGNATURES = {
         ctypes.c_int,
         [_c_ptr, _c_ptr, _c_ptr, ctypes.c_int, _c_ptr, ctypes.c_int] + [_c_ptr] * 4
         + [_c_i64] * 5 + [_c_f32, _c_i64, _c_ptr, ctypes.c_size_t, _c_ptr]),
+    "hipo_linear_cross_entropy_bwd_two_parts_workspace_bytes": (
+        ctypes.c_size_t, [_c_ptr, ctypes.c_int] + [_c_i64] * 4),
+    "hipo_linear_cross_entropy_bwd_two_parts": (
+        ctypes.c_int,
+        [_c_ptr, _c_ptr, _c_ptr, ctypes.c_int, _c_ptr, ctypes.c_int] + [_c_ptr] * 4
+        + [_c_i64] * 5 + [_c_f32, _c_i64, _c_ptr, ctypes.c_size_t, _c_ptr]),
 }
 
 _lib = None
@@ -1096,15 +1102,21 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, tokens: tor
 
 def linear_cross_entropy_bwd(grad: torch.Tensor, hidden: torch.Tensor, weight: torch.Tensor,
                              tokens: torch.Tensor, lse: torch.Tensor, *, scale: float = 1.0,
-                             ignore_index: int = -100, grad_lse: torch.Tensor | None = None):
+                             ignore_index: int = -100, grad_lse: torch.Tensor | None = None,
+                             two_parts: bool = False):
     """Gradients (dhidden [R, D], dweight [V, D]) of linear_cross_entropy, of the
     operands' type: grad and grad_lse (fp32 [R]) are the gradients of its loss and
     lse (1 / R each of the mean loss, 2 c lse / R of a penalty c lse^2), lse is
-    its result.  The logits are computed once more, in pieces of the vocabulary;
-    with bf16 operands their gradients are rounded to bf16 (up to 64 rows: to two
-    bf16 parts) for the products with hidden and weight, whose sums are fp32.  Rows of ignore_index have gradient
-    zero and add nothing to dweight, whatever they hold; a row of another token
-    outside [0, V) is NaN and makes dweight NaN."""
+    its result.  The logits are computed once more, in pieces of the vocabulary.
+    Rows of ignore_index have gradient zero and add nothing to dweight, whatever
+    they hold; a row of another token outside [0, V) is NaN and makes dweight NaN.
+
+    With bf16 operands the logits' gradients are rounded to bf16 for the products
+    with hidden and weight, whose sums are fp32: the results are off by as much
+    again as by their own rounding.  With two_parts (and always up to 64 rows)
+    they are held in two bf16 parts, and the results are off by their own rounding
+    alone, at twice the products of dhidden and dweight.  fp32 operands have three
+    parts either way."""
     lib = _lib or load_library()
     what = "linear_cross_entropy_bwd"
     _two_dimensions(what, hidden, weight)
@@ -1114,13 +1126,17 @@ def linear_cross_entropy_bwd(grad: torch.Tensor, hidden: torch.Tensor, weight: t
     made = torch.empty if rows else torch.zeros  # no rows: nothing is written
     dhidden = made((rows, width), dtype=hidden.dtype, device=dev)
     dweight = made((vocab, width), dtype=hidden.dtype, device=dev)
-    need = int(lib.hipo_linear_cross_entropy_bwd_workspace_bytes(
-        _ptr(weight), weight.element_size(), rows, width, vocab, wstride))
+    bwd = lib.hipo_linear_cross_entropy_bwd
+    bytes_of = lib.hipo_linear_cross_entropy_bwd_workspace_bytes
+    if two_parts:
+        bwd = lib.hipo_linear_cross_entropy_bwd_two_parts
+        bytes_of = lib.hipo_linear_cross_entropy_bwd_two_parts_workspace_bytes
+    need = int(bytes_of(_ptr(weight), weight.element_size(), rows, width, vocab, wstride))
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(lib.hipo_linear_cross_entropy_bwd, what, dev, _ptr(grad), _ptr(hidden), _ptr(weight),
-          hidden.element_size(), _ptr(tokens), tokens.element_size(), _ptr(lse),
-          _optional(grad_lse), _ptr(dhidden), _ptr(dweight), rows, width, vocab, hstride, wstride,
-          float(scale), int(ignore_index), _optional(ws), need)
+    _call(bwd, what, dev, _ptr(grad), _ptr(hidden), _ptr(weight), hidden.element_size(),
+          _ptr(tokens), tokens.element_size(), _ptr(lse), _optional(grad_lse), _ptr(dhidden),
+          _ptr(dweight), rows, width, vocab, hstride, wstride, float(scale), int(ignore_index),
+          _optional(ws), need)
     return dhidden, dweight
 
 

@@ -24,6 +24,9 @@
 // matrix cores take of one type: each value is off by half a step (2^-9 of it on
 // average), as much again as the gradients' own rounding (relative 2-norms 0.0024
 // where gradients rounded from exact d have 0.0017); sums are fp32 throughout.
+// Where the caller asks for two parts (and always up to 64 rows) d is held in two
+// bf16 parts, some 2^-17 of it, each multiplied: 0.0017 again, at twice the products
+// of dhidden and dweight (8192 x 4096 x 128000 16.8 -> 28.9 ms).
 #include <algorithm>
 
 #include "hipo_common.h"
@@ -93,9 +96,9 @@ __global__ __launch_bounds__(1024) void select_rows(Select a) {
   if (threadIdx.x == 0) *a.count = base;
 }
 
-// The next bf16 parts of two values, the nearest ones, and what they leave.  Of
-// three parts the first two are kept finite (a value past the largest bf16 leaves
-// the rest to the next part, an infinity or NaN to the last).
+// The next bf16 parts of two values, the nearest ones, and what they leave.  All
+// but the last are kept finite (a value past the largest bf16 leaves the rest to
+// the next part, an infinity or NaN to the last).
 __device__ __forceinline__ uint32_t next_parts(float& lo, float& hi, bool last) {
   constexpr float kLargestBf16 = 3.3895313892515355e38f;
   const uint32_t w = last ? pack_bf16x2(lo, hi)
@@ -326,12 +329,13 @@ __device__ __forceinline__ void store4(float* p, const f32x4_t& v, int n) {
   }
 }
 
-// The parts of a and b that are multiplied, the smallest products first.
+// The parts of a and b that are multiplied, the smallest products first: six of
+// three parts each, or those of b alone.
 __device__ __forceinline__ int a_part(int pass, int passes) {
-  return passes == 1 ? 0 : (0x001120 >> (4 * pass)) & 3;
+  return passes == 6 ? (0x001120 >> (4 * pass)) & 3 : 0;
 }
 __device__ __forceinline__ int b_part(int pass, int passes) {
-  return passes == 1 ? 0 : (0x010102 >> (4 * pass)) & 3;
+  return passes == 6 ? (0x010102 >> (4 * pass)) & 3 : passes == 2 ? 1 - pass : 0;
 }
 
 // One operand's part of a round: Tile rows by kStep values of K in LDS, moved
@@ -456,11 +460,14 @@ struct Operand {
 // where the card's power holds it, the matrix cores were busy 65 % of the cycles
 // before the last step.  No gain: s_setprio around the products, bands of 8 tiles
 // instead of 4 for an XCD, rows of copies and of d padded off powers of two.
-template <typename T, int Tile, Epilogue E>
+//
+// Parts: of d, which kLogitGrad writes and the gradients' products read as b.
+template <typename T, int Tile, Epilogue E, int Parts = sizeof(T) == 2 ? 1 : 3>
 __global__ __launch_bounds__(Tile * 2, 2) void gemm(Product p) {
   constexpr int kWavesB = Tile / 64, kFragments = Tile / 32;
-  constexpr int kPasses = sizeof(T) == 2 ? 1 : 6;
-  constexpr bool kAcrossA = E == kAccumulate || E == kStore, kAcrossB = E == kStore;
+  constexpr bool kOfD = E == kAccumulate || E == kStore;
+  constexpr int kPasses = sizeof(T) == 4 ? 6 : kOfD ? Parts : 1;
+  constexpr bool kAcrossA = kOfD, kAcrossB = E == kStore;
   __shared__ __attribute__((aligned(1024))) uint16_t lds[4 * Tile * kStep];
 
   const int rows_b = p.b_count ? *p.b_count : p.b_rows;
@@ -710,7 +717,7 @@ __global__ __launch_bounds__(Tile * 2, 2) void gemm(Product p) {
     // 16-byte piece c of row j lies at place c ^ (j % pieces).
     constexpr int kPieces = Tile / 8, kValues = 512 / Tile;
 #pragma unroll
-    for (int q = 0; q < (E == kLogitGrad ? kPasses == 1 ? 1 : 3 : 1); ++q) {
+    for (int q = 0; q < (E == kLogitGrad ? Parts : 1); ++q) {
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const int j = wave_b + n * 16 + (lane & 15);
@@ -718,12 +725,13 @@ __global__ __launch_bounds__(Tile * 2, 2) void gemm(Product p) {
         for (int f = 0; f < kFragments; ++f) {
           const int i = wave_a + f * 16 + (lane >> 4) * 4;
           u32x2_t v;
-          if (sizeof(T) == 2) {
+          if (E == kStore || Parts == 1) {
             v = u32x2_t{pack_bf16x2(acc[f][n][0], acc[f][n][1]),
                         pack_bf16x2(acc[f][n][2], acc[f][n][3])};
           } else {
             float x[4] = {acc[f][n][0], acc[f][n][1], acc[f][n][2], acc[f][n][3]};
-            v = u32x2_t{next_parts(x[0], x[1], q == 2), next_parts(x[2], x[3], q == 2)};
+            constexpr int kLast = Parts - 1;
+            v = u32x2_t{next_parts(x[0], x[1], q == kLast), next_parts(x[2], x[3], q == kLast)};
             acc[f][n] = f32x4_t{x[0], x[1], x[2], x[3]};
             asm volatile("" : "+v"(acc[f][n]));  // what is left takes its place: no spills
           }
@@ -1387,6 +1395,7 @@ struct Plan {
   bool direct;                         // weight is read where it lies
   bool thin;                           // few rows: the kernels of their own,
   bool thin_gemm;                      // but for dhidden of aligned bf16
+  bool two_parts;                      // of bf16 operands' d, of more rows
   size_t kept, count, target, part, hidden, weight, d, sum, bytes;
 };
 
@@ -1417,7 +1426,7 @@ int better_tile(WorkOf work_of) {
 }
 
 Plan plan_of(const void* weight, int elem_size, int64_t rows, int64_t width, int64_t vocab,
-             int64_t weight_ld, bool backward) {
+             int64_t weight_ld, bool backward, bool two_parts) {
   Plan p{};
   if (!backward && rows <= kThinRows) {
     p.target = 0;
@@ -1431,7 +1440,8 @@ Plan plan_of(const void* weight, int elem_size, int64_t rows, int64_t width, int
   p.thin_gemm = p.thin && aligned;
   p.direct = p.thin || aligned;
   p.rows_pad = p.thin ? kThinRows : up(rows, kTile);
-  p.d_planes = p.thin && elem_size == 2 ? 2 : p.planes;
+  p.two_parts = two_parts && elem_size == 2 && !p.thin;
+  p.d_planes = (p.thin && elem_size == 2) || p.two_parts ? 2 : p.planes;
   p.sum_rows = p.thin_gemm ? 2 * kThinRows : p.rows_pad;
   p.k_pad = up(width, kStep);
   const size_t copy = p.direct ? 0 : sizeof(uint16_t) * p.planes * p.k_pad;
@@ -1451,11 +1461,12 @@ Plan plan_of(const void* weight, int elem_size, int64_t rows, int64_t width, int
   p.piece = up((vocab + p.pieces - 1) / p.pieces, kTile);
   p.pieces = (vocab + p.piece - 1) / p.piece;
   const int64_t passes = elem_size == 2 ? 1 : 6, in_piece = std::min(p.piece, vocab);
+  const int64_t passes_d = p.two_parts ? 2 : passes;
   p.tile = better_tile([&](int tile) {
     return Work{tiles_of(in_piece, rows, tile), passes * p.k_pad / kStep};
   });
   p.tile_weight = better_tile([&](int tile) {
-    return Work{tiles_of(width, in_piece, tile), passes * up(rows, kStep) / kStep};
+    return Work{tiles_of(width, in_piece, tile), passes_d * up(rows, kStep) / kStep};
   });
   // dhidden has few tiles where there are few rows: the piece is split until
   // there are as many workgroups as run at once, 8 rounds each at least.
@@ -1466,7 +1477,7 @@ Plan plan_of(const void* weight, int elem_size, int64_t rows, int64_t width, int
   };
   p.tile_hidden = better_tile([&](int tile) {
     const int64_t splits = splits_of(tile);
-    return Work{splits * tiles_of(width, p.sum_rows, tile), passes * p.piece / kStep / splits};
+    return Work{splits * tiles_of(width, p.sum_rows, tile), passes_d * p.piece / kStep / splits};
   });
   p.splits = static_cast<int>(splits_of(p.tile_hidden));
   if (p.thin && !p.thin_gemm) {
@@ -1526,15 +1537,25 @@ int pack(const char* what, Pack a, int64_t rows, hipStream_t stream) {
   return check_launch(what);
 }
 
-template <typename T, Epilogue E>
+template <typename T, Epilogue E, int Parts = sizeof(T) == 2 ? 1 : 3>
 int multiply(const char* what, const Product& p, int tile, int64_t rows_b, hipStream_t stream) {
   const uint32_t grid = static_cast<uint32_t>(tiles_of(p.a_rows, rows_b, tile) * p.splits);
   if (tile == kTile) {
-    gemm<T, kTile, E><<<grid, 2 * kTile, 0, stream>>>(p);
+    gemm<T, kTile, E, Parts><<<grid, 2 * kTile, 0, stream>>>(p);
   } else {
-    gemm<T, kSmallTile, E><<<grid, 2 * kSmallTile, 0, stream>>>(p);
+    gemm<T, kSmallTile, E, Parts><<<grid, 2 * kSmallTile, 0, stream>>>(p);
   }
   return check_launch(what);
+}
+
+// Of d, in one part or two where the operands are bf16.
+template <typename T, Epilogue E>
+int multiply_d(const char* what, const Product& p, int tile, int64_t rows_b, bool two_parts,
+               hipStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    if (two_parts) return multiply<T, E, 2>(what, p, tile, rows_b, stream);
+  }
+  return multiply<T, E>(what, p, tile, rows_b, stream);
 }
 
 struct Call {
@@ -1680,9 +1701,8 @@ int run_fwd(const Call& c, const Plan& plan, float* loss, float* lse) {
 }
 
 template <typename T>
-int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse,
-            const float* grad_lse, void* dhidden, void* dweight) {
-  const char* what = "linear_cross_entropy_bwd";
+int run_bwd(const char* what, const Call& c, const Plan& plan, const float* grad,
+            const float* lse, const float* grad_lse, void* dhidden, void* dweight) {
   Product g{};
   HIPO_STEP(select_and_pack<T>(what, c, plan, nullptr, nullptr, dhidden, &g));
   const int width = static_cast<int>(c.width);
@@ -1760,7 +1780,7 @@ int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse
       HIPO_STEP(check_launch(what));
       continue;
     }
-    HIPO_STEP((multiply<T, kLogitGrad>(what, g, plan.tile, c.rows, c.stream)));
+    HIPO_STEP((multiply_d<T, kLogitGrad>(what, g, plan.tile, c.rows, plan.two_parts, c.stream)));
 
     Product h{};
     h.a = g.a;
@@ -1782,7 +1802,8 @@ int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse
     h.to_out = plan.splits == 1 && i + 1 == plan.pieces;
     h.out = dhidden;
     h.out_ld = c.width;
-    HIPO_STEP((multiply<T, kAccumulate>(what, h, plan.tile_hidden, c.rows, c.stream)));
+    HIPO_STEP((multiply_d<T, kAccumulate>(what, h, plan.tile_hidden, c.rows, plan.two_parts,
+                                          c.stream)));
 
     Product w{};
     w.a = g.b;
@@ -1797,7 +1818,8 @@ int run_bwd(const Call& c, const Plan& plan, const float* grad, const float* lse
     w.splits = 1;
     w.out = static_cast<T*>(dweight) + first * c.width;
     w.out_ld = c.width;
-    HIPO_STEP((multiply<T, kStore>(what, w, plan.tile_weight, g.a_rows, c.stream)));
+    HIPO_STEP((multiply_d<T, kStore>(what, w, plan.tile_weight, g.a_rows, plan.two_parts,
+                                     c.stream)));
   }
   if (plan.thin || plan.splits > 1) {
     const int64_t blocks = (c.rows * ((c.width + 3) / 4) + 255) / 256;
@@ -1821,7 +1843,8 @@ extern "C" size_t hipo_linear_cross_entropy_workspace_bytes(const void* weight, 
       !hipo::sizes_fit(rows, width, vocab, width, weight_row_stride)) {
     return 0;
   }
-  return hipo::plan_of(weight, elem_size, rows, width, vocab, weight_row_stride, false).bytes;
+  return hipo::plan_of(weight, elem_size, rows, width, vocab, weight_row_stride, false, false)
+      .bytes;
 }
 
 extern "C" int hipo_linear_cross_entropy(const void* hidden, const void* weight, int elem_size,
@@ -1837,7 +1860,8 @@ extern "C" int hipo_linear_cross_entropy(const void* hidden, const void* weight,
                            weight_row_stride, scale));
   if (rows == 0) return 0;
   HIPO_REQUIRE(hidden && weight && tokens && loss && lse, "%s: null pointer", what);
-  const Plan plan = plan_of(weight, elem_size, rows, width, vocab, weight_row_stride, false);
+  const Plan plan = plan_of(weight, elem_size, rows, width, vocab, weight_row_stride, false,
+                            false);
   HIPO_REQUIRE(workspace && workspace_bytes >= plan.bytes && aligned16(workspace),
                "%s: workspace of %zu bytes, 16-byte aligned, needed", what, plan.bytes);
   const Call c{hidden, weight, tokens, token_size, rows, width, vocab, hidden_row_stride,
@@ -1846,15 +1870,44 @@ extern "C" int hipo_linear_cross_entropy(const void* hidden, const void* weight,
                         : run_fwd<float>(c, plan, loss, lse);
 }
 
-extern "C" size_t hipo_linear_cross_entropy_bwd_workspace_bytes(const void* weight, int elem_size,
-                                                                int64_t rows, int64_t width,
-                                                                int64_t vocab,
-                                                                int64_t weight_row_stride) {
+namespace hipo {
+namespace {
+
+size_t bwd_workspace_bytes(const void* weight, int elem_size, int64_t rows, int64_t width,
+                           int64_t vocab, int64_t weight_ld, bool two_parts) {
   if ((elem_size != 2 && elem_size != 4) || rows == 0 ||
-      !hipo::sizes_fit(rows, width, vocab, width, weight_row_stride)) {
+      !sizes_fit(rows, width, vocab, width, weight_ld)) {
     return 0;
   }
-  return hipo::plan_of(weight, elem_size, rows, width, vocab, weight_row_stride, true).bytes;
+  return plan_of(weight, elem_size, rows, width, vocab, weight_ld, true, two_parts).bytes;
+}
+
+int bwd(const char* what, const float* grad, int elem_size, const float* lse,
+        const float* grad_lse, void* dhidden, void* dweight, const Call& c,
+        size_t workspace_bytes, bool two_parts) {
+  clear_error();
+  HIPO_STEP(check_operands(what, elem_size, c.token_size, c.rows, c.width, c.vocab, c.hidden_ld,
+                           c.weight_ld, c.scale));
+  if (c.rows == 0) return 0;
+  HIPO_REQUIRE(grad && c.hidden && c.weight && c.tokens && lse && dhidden && dweight,
+               "%s: null pointer", what);
+  const Plan plan = plan_of(c.weight, elem_size, c.rows, c.width, c.vocab, c.weight_ld, true,
+                            two_parts);
+  HIPO_REQUIRE(c.ws && workspace_bytes >= plan.bytes && aligned16(c.ws),
+               "%s: workspace of %zu bytes, 16-byte aligned, needed", what, plan.bytes);
+  return elem_size == 2
+             ? run_bwd<uint16_t>(what, c, plan, grad, lse, grad_lse, dhidden, dweight)
+             : run_bwd<float>(what, c, plan, grad, lse, grad_lse, dhidden, dweight);
+}
+
+}  // namespace
+}  // namespace hipo
+
+extern "C" size_t hipo_linear_cross_entropy_bwd_workspace_bytes(
+    const void* weight, int elem_size, int64_t rows, int64_t width, int64_t vocab,
+    int64_t weight_row_stride) {
+  return hipo::bwd_workspace_bytes(weight, elem_size, rows, width, vocab, weight_row_stride,
+                                   false);
 }
 
 extern "C" int hipo_linear_cross_entropy_bwd(const float* grad, const void* hidden,
@@ -1865,20 +1918,28 @@ extern "C" int hipo_linear_cross_entropy_bwd(const float* grad, const void* hidd
                                              int64_t hidden_row_stride, int64_t weight_row_stride,
                                              float scale, int64_t ignore_index, void* workspace,
                                              size_t workspace_bytes, hipStream_t stream) {
-  using namespace hipo;
-  clear_error();
-  const char* what = "linear_cross_entropy_bwd";
-  HIPO_STEP(check_operands(what, elem_size, token_size, rows, width, vocab, hidden_row_stride,
-                           weight_row_stride, scale));
-  if (rows == 0) return 0;
-  HIPO_REQUIRE(grad && hidden && weight && tokens && lse && dhidden && dweight,
-               "%s: null pointer", what);
-  const Plan plan = plan_of(weight, elem_size, rows, width, vocab, weight_row_stride, true);
-  HIPO_REQUIRE(workspace && workspace_bytes >= plan.bytes && aligned16(workspace),
-               "%s: workspace of %zu bytes, 16-byte aligned, needed", what, plan.bytes);
-  const Call c{hidden, weight, tokens, token_size, rows, width, vocab, hidden_row_stride,
-               weight_row_stride, scale, ignore_index, static_cast<char*>(workspace), stream};
-  return elem_size == 2
-             ? run_bwd<uint16_t>(c, plan, grad, lse, grad_lse, dhidden, dweight)
-             : run_bwd<float>(c, plan, grad, lse, grad_lse, dhidden, dweight);
+  return hipo::bwd("linear_cross_entropy_bwd", grad, elem_size, lse, grad_lse, dhidden, dweight,
+                   {hidden, weight, tokens, token_size, rows, width, vocab, hidden_row_stride,
+                    weight_row_stride, scale, ignore_index, static_cast<char*>(workspace), stream},
+                   workspace_bytes, false);
+}
+
+extern "C" size_t hipo_linear_cross_entropy_bwd_two_parts_workspace_bytes(
+    const void* weight, int elem_size, int64_t rows, int64_t width, int64_t vocab,
+    int64_t weight_row_stride) {
+  return hipo::bwd_workspace_bytes(weight, elem_size, rows, width, vocab, weight_row_stride,
+                                   true);
+}
+
+extern "C" int hipo_linear_cross_entropy_bwd_two_parts(
+    const float* grad, const void* hidden, const void* weight, int elem_size,
+    const void* tokens, int token_size, const float* lse, const float* grad_lse, void* dhidden,
+    void* dweight, int64_t rows, int64_t width, int64_t vocab, int64_t hidden_row_stride,
+    int64_t weight_row_stride, float scale, int64_t ignore_index, void* workspace,
+    size_t workspace_bytes, hipStream_t stream) {
+  return hipo::bwd("linear_cross_entropy_bwd_two_parts", grad, elem_size, lse, grad_lse, dhidden,
+                   dweight,
+                   {hidden, weight, tokens, token_size, rows, width, vocab, hidden_row_stride,
+                    weight_row_stride, scale, ignore_index, static_cast<char*>(workspace), stream},
+                   workspace_bytes, true);
 }

@@ -637,7 +637,9 @@ int hipo_linear_cross_entropy(const void* hidden, const void* weight, int elem_s
  * the logits computed once more in pieces of the vocabulary, the products
  * accumulated in fp32 and rounded once to the operands' type; d itself is
  * rounded to bf16 where the operands are bf16 (the matrix cores' type; up to 64
- * rows to two bf16 parts, some 2^-17 of it).
+ * rows to two bf16 parts, some 2^-17 of it; so with _two_parts at any number of
+ * rows, for gradients that are off by their own rounding alone, at twice the
+ * products of dhidden and dweight).
  * dhidden is contiguous [rows, width], dweight [vocab, width]; they overlap
  * neither each other nor an operand.  Rows of ignore_index are zero in dhidden
  * and add nothing to dweight, whatever they hold; a row of another token outside
@@ -658,6 +660,16 @@ int hipo_linear_cross_entropy_bwd(const float* grad, const void* hidden,
                                   int64_t weight_row_stride, float scale,
                                   int64_t ignore_index, void* workspace,
                                   size_t workspace_bytes, hipStream_t stream);
+size_t hipo_linear_cross_entropy_bwd_two_parts_workspace_bytes(
+    const void* weight, int elem_size, int64_t rows, int64_t width, int64_t vocab,
+    int64_t weight_row_stride);
+int hipo_linear_cross_entropy_bwd_two_parts(
+    const float* grad, const void* hidden, const void* weight, int elem_size,
+    const void* tokens, int token_size, const float* lse, const float* grad_lse,
+    void* dhidden, void* dweight, int64_t rows, int64_t width, int64_t vocab,
+    int64_t hidden_row_stride, int64_t weight_row_stride, float scale,
+    int64_t ignore_index, void* workspace, size_t workspace_bytes,
+    hipStream_t stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */

@@ -29,6 +29,9 @@ int hipo_linear_cross_entropy_bwd(const float*, const void*, const void*, int, c
                                   const float*, const float*, void*, void*, int64_t, int64_t,
                                   int64_t, int64_t, int64_t, float, int64_t, void*, size_t,
                                   void*);
+decltype(hipo_linear_cross_entropy_bwd_workspace_bytes)
+    hipo_linear_cross_entropy_bwd_two_parts_workspace_bytes;
+decltype(hipo_linear_cross_entropy_bwd) hipo_linear_cross_entropy_bwd_two_parts;
 }
 
 namespace {
@@ -57,6 +60,12 @@ int call(const std::string& op, const std::vector<int64_t>& n) {
     return hipo_linear_cross_entropy_bwd(
         f, p, p, e, p, 8, f, nullptr, p, p, n[0], n[1], n[2], n[1], n[1], 1.0f, -100, p,
         hipo_linear_cross_entropy_bwd_workspace_bytes(p, e, n[0], n[1], n[2], n[1]), nullptr);
+  }
+  if (op == "linear_cross_entropy_bwd_two_parts") {
+    return hipo_linear_cross_entropy_bwd_two_parts(
+        f, p, p, e, p, 8, f, nullptr, p, p, n[0], n[1], n[2], n[1], n[1], 1.0f, -100, p,
+        hipo_linear_cross_entropy_bwd_two_parts_workspace_bytes(p, e, n[0], n[1], n[2], n[1]),
+        nullptr);
   }
   return 2;
 }

@@ -198,6 +198,47 @@ def test_a_refused_launch_ends_the_call(call, launches):
         assert rc == 9 and again == made[:n + 1]
 
 
+TWO_PARTS = "linear_cross_entropy_bwd_two_parts"
+
+
+def test_two_parts_can_be_launched(launches):
+    sizes = ((1, 1, 1), (65, 1, 1), (8192, 4096, 128000), (257, 1001, 50001),
+             ((1 << 22) - 256, 8, 70000), (65, 8, (1 << 31) - 65536),
+             ((1 << 22) - 256, 1 << 16, 300), (65, 1 << 20, 70000))
+    calls = [(-1, TWO_PARTS, *size, elem) for size in sizes for elem in (2, 4)]
+    for call, (made, rc) in zip(calls, launches(*calls)):
+        assert rc == 0 and made, call
+        assert_launchable(made)
+
+
+def test_a_refused_launch_of_two_parts_ends_the_call(launches):
+    call = (TWO_PARTS, 300, 200, 3000, 2)
+    (made, rc), = launches((-1, *call))
+    assert rc == 0
+    for n, (again, rc) in enumerate(launches(*((n, *call) for n in range(len(made))))):
+        assert rc == 9 and again == made[:n + 1]
+
+
+def test_two_parts_check_their_arguments(lib):
+    def call(es=2, rows=100, wb=1 << 50, g=P):
+        return lib.hipo_linear_cross_entropy_bwd_two_parts(
+            g, P, P, es, P, 8, P, None, P, P, rows, 8, 8, 8, 8, 1.0, -100, P, wb, None)
+
+    need = lib.hipo_linear_cross_entropy_bwd_two_parts_workspace_bytes
+    for kw, msg in ((dict(es=3), b"elem_size"), (dict(rows=-1), b"negative"),
+                    (dict(g=None), b"null"), (dict(wb=need(P, 2, 100, 8, 8, 8) - 1),
+                                              b"workspace")):
+        assert call(**kw) == HIPO_EINVAL
+        assert msg in lib.hipo_last_error() and b"_two_parts" in lib.hipo_last_error()
+    assert call(rows=0) == 0 and need(P, 2, 0, 8, 8, 8) == 0
+    one = lib.hipo_linear_cross_entropy_bwd_workspace_bytes
+    for rows, elem, more in ((64, 2, False), (65, 2, True), (8192, 2, False), (65, 4, False)):
+        # (Of 8192 rows the pieces are smaller.)
+        two = need(P, elem, rows, 4096, 32000, 4096)
+        assert (two > one(P, elem, rows, 4096, 32000, 4096)) == more or rows == 8192
+        assert two <= (2 << 30) + 12 * max(256, rows) * (4096 + 64)
+
+
 # ---------------------------------------------------------------------------
 # The reference
 # ---------------------------------------------------------------------------

@@ -577,3 +577,52 @@ def test_two_streams_at_once(rocm_device, ho):
         torch.cuda.synchronize()
         for a, b in zip(want, got):
             assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def gradients_in_64_bits(grad, hidden, weight, tokens, lse, scale=1.0):
+    """[(dhidden or dweight, the sums of its absolute products)] of one lse."""
+    h, w = hidden.double(), weight.double()
+    keep = tokens != IGNORE
+    d = torch.exp(h @ w.t() * scale - lse[:, None].double()) * grad[:, None].double()
+    d[keep.nonzero()[:, 0], tokens[keep]] -= grad[keep].double()
+    d *= scale * keep[:, None]
+    return [(d @ w, d.abs() @ w.abs()), (d.t() @ h, d.abs().t() @ h.abs())]
+
+
+@pytest.mark.parametrize("rows,width,vocab", [
+    (64, 264, 1500), (65, 264, 1500), (65, 65, 1501), (200, 1000, 260), (700, 768, 9001),
+    (1030, 72, 4000), (2500, 520, 8000), (400, 64, (1 << 20) + 77)])
+def test_gradients_of_two_parts_are_rounded_once(rows, width, vocab, rocm_device, ho):
+    """With two_parts bf16 gradients are off by their own rounding alone: half a
+    step of each, and in the 2-norm what rounding the 64-bit gradients is off by.
+    d's two parts leave 2^-16 of it at most, so 2^-15 of the sums of absolute
+    products with the sums' own roundings; in the norm, where these have either
+    sign, 2^-14 of the gradient, a twentieth of the 2^-9.2 that the rounding is.
+    One part is off by as much as the rounding, 1.4 times as much in all.  (The
+    last size is two pieces of the vocabulary.)"""
+    hidden, weight, tokens, grads = layer_operands(rocm_device, rows, width, vocab, BF16)
+    tokens[::9] = IGNORE
+    _, lse = ho.linear_cross_entropy(hidden, weight, tokens)
+    args = (grads[0], hidden, weight, tokens, lse)
+    want = gradients_in_64_bits(*args)
+    got = ho.linear_cross_entropy_bwd(*args, two_parts=True)
+    again = ho.linear_cross_entropy_bwd(*args, two_parts=True)
+    one = ho.linear_cross_entropy_bwd(*args)
+    for name, u, a, o, (v, size) in zip(("dhidden", "dweight"), got, again, one, want):
+        what = f"[{rows}, {width}, {vocab}] {name}"
+        assert torch.equal(u, a), what
+        own = float((v.to(BF16).double() - v).norm())
+        off = float((u.double() - v).norm())
+        assert off <= 1.05 * own, f"{what}: {off / own:.3f} of the rounding"
+        if rows <= 64:
+            assert torch.equal(u, o), what
+        over = (u.double() - v).abs() - v.abs() * 2.0 ** -8 - size * 2.0 ** -15
+        assert float(over.max()) <= 2.0 ** -133, what
+
+
+def test_two_parts_of_fp32_are_three(rocm_device, ho):
+    hidden, weight, tokens, grads = layer_operands(rocm_device, 100, 72, 900, F32)
+    _, lse = ho.linear_cross_entropy(hidden, weight, tokens)
+    got = [ho.linear_cross_entropy_bwd(grads[0], hidden, weight, tokens, lse, two_parts=k)
+           for k in (False, True)]
+    assert all(torch.equal(a, b) for a, b in zip(*got))
