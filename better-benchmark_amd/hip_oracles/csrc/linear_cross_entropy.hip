@@ -289,14 +289,19 @@ typedef int s32x4_t __attribute__((ext_vector_type(4)));
 // the scalar `offset`, to LDS from byte `to` on, lane after lane.  No register is
 // written; it is waited for by count, in barrier().  (Of the builtin the compiler
 // would wait for every load that might write what an LDS read reads.)  m0 needs
-// one wait state before its use.
+// one wait state before its use.  The compiler keeps nothing in m0 from one
+// instruction to another and warns of its name below; but it merges settings of m0
+// that it takes to be alike, which this one must end.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(s32x4_t buffer, uint32_t from, int offset,
                                             uint32_t to) {
   asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(
                    from),
                "s"(buffer), "s"(offset), "s"(to)
-               : "memory");
+               : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // All but `Loads` loads of this wave and all its LDS reads are done, in every
 // wave of the workgroup.

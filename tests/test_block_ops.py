@@ -1,6 +1,7 @@
 """The norms around a block and the output layer's cross entropy without a GPU:
 argument checks of the entry points, empty calls, launches, and the 64-bit
 reference against automatic differentiation and differences."""
+import re
 import subprocess
 
 import pytest
@@ -237,6 +238,17 @@ def test_two_parts_check_their_arguments(lib):
         two = need(P, elem, rows, 4096, 32000, 4096)
         assert (two > one(P, elem, rows, 4096, 32000, 4096)) == more or rows == 8192
         assert two <= (2 << 30) + 12 * max(256, rows) * (4096 + 64)
+
+
+def test_assembly_names_the_registers_that_it_writes():
+    """m0 is no operand: a statement that sets it has to say so."""
+    found = 0
+    for path in sorted((ROOT / "better-benchmark_amd" / "hip_oracles" / "csrc").iterdir()):
+        for asm in re.findall(r"asm volatile\s*\((.*?)\);", path.read_text(), re.S):
+            if re.search(r"\bs_\w+ m0,", asm):
+                found += 1
+                assert '"m0"' in asm.rpartition(":")[2], f"{path.name}: {asm}"
+    assert found
 
 
 # ---------------------------------------------------------------------------
