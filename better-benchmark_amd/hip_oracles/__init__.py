@@ -1123,9 +1123,8 @@ def linear_cross_entropy_bwd(grad: torch.Tensor, hidden: torch.Tensor, weight: t
     dev, rows, width, vocab, hstride, wstride = _require_output_layer(
         what, hidden, weight, tokens, scale,
         (grad, lse) if grad_lse is None else (grad, lse, grad_lse))
-    made = torch.empty if rows else torch.zeros  # no rows: nothing is written
-    dhidden = made((rows, width), dtype=hidden.dtype, device=dev)
-    dweight = made((vocab, width), dtype=hidden.dtype, device=dev)
+    dhidden = torch.empty((rows, width), dtype=hidden.dtype, device=dev)
+    dweight = torch.empty((vocab, width), dtype=hidden.dtype, device=dev)
     bwd = lib.hipo_linear_cross_entropy_bwd
     bytes_of = lib.hipo_linear_cross_entropy_bwd_workspace_bytes
     if two_parts:

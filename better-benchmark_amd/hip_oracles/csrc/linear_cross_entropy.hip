@@ -1356,6 +1356,18 @@ __global__ __launch_bounds__(256) void thin_hidden(ThinHidden a) {
   }
 }
 
+// dweight of no rows, as 16-bit values.
+__global__ __launch_bounds__(256) void zero_weight(uint16_t* out, int64_t n) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256 * 8;
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8; i < n; i += step) {
+    if (i + 8 <= n) {
+      *reinterpret_cast<u32x4_a2_t*>(out + i) = u32x4_t{0u, 0u, 0u, 0u};
+    } else {
+      for (int64_t m = i; m < n; ++m) out[m] = 0;
+    }
+  }
+}
+
 // One workgroup a row.
 __global__ __launch_bounds__(256) void join_thin(Thin a, int64_t ignore_index, float* loss,
                                                  float* lse) {
@@ -1893,7 +1905,13 @@ int bwd(const char* what, const float* grad, int elem_size, const float* lse,
   clear_error();
   HIPO_STEP(check_operands(what, elem_size, c.token_size, c.rows, c.width, c.vocab, c.hidden_ld,
                            c.weight_ld, c.scale));
-  if (c.rows == 0) return 0;
+  if (c.rows == 0) {
+    if (!dweight) return 0;
+    const int64_t n = c.vocab * c.width * (elem_size / 2);
+    zero_weight<<<static_cast<uint32_t>(std::min<int64_t>(up(n, 2048) / 2048, 1 << 16)), 256, 0,
+                  c.stream>>>(static_cast<uint16_t*>(dweight), n);
+    return check_launch(what);
+  }
   HIPO_REQUIRE(grad && c.hidden && c.weight && c.tokens && lse && dhidden && dweight,
                "%s: null pointer", what);
   const Plan plan = plan_of(c.weight, elem_size, c.rows, c.width, c.vocab, c.weight_ld, true,

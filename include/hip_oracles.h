@@ -643,7 +643,9 @@ int hipo_linear_cross_entropy(const void* hidden, const void* weight, int elem_s
  * dhidden is contiguous [rows, width], dweight [vocab, width]; they overlap
  * neither each other nor an operand.  Rows of ignore_index are zero in dhidden
  * and add nothing to dweight, whatever they hold; a row of another token outside
- * [0, vocab) is NaN and makes dweight NaN.  Operands and workspace as above.
+ * [0, vocab) is NaN and makes dweight NaN.  With rows == 0 dweight (where it is
+ * given) is zero and no other pointer is looked at.  Operands and workspace as
+ * above.
  * No counterpart among the reference's oracles.
  */
 size_t hipo_linear_cross_entropy_bwd_workspace_bytes(const void* weight, int elem_size,

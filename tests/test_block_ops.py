@@ -220,10 +220,21 @@ def test_a_refused_launch_of_two_parts_ends_the_call(launches):
         assert rc == 9 and again == made[:n + 1]
 
 
+def test_the_gradient_of_no_rows_is_written(launches):
+    calls = [(-1, op, 0, width, vocab, elem)
+             for op in ("linear_cross_entropy_bwd", TWO_PARTS) for elem in (2, 4)
+             for width, vocab in ((1, 1), (65, 1001), (1 << 20, (1 << 31) - 65536))]
+    for call, (made, rc) in zip(calls, launches(*calls)):
+        assert rc == 0 and len(made) == 1 and "zero_weight" in made[0][0], call
+        assert_launchable(made)
+    (made, rc), = launches((0, "linear_cross_entropy_bwd", 0, 8, 8, 2))
+    assert rc == 9 and len(made) == 1
+
+
 def test_two_parts_check_their_arguments(lib):
-    def call(es=2, rows=100, wb=1 << 50, g=P):
+    def call(es=2, rows=100, wb=1 << 50, g=P, dw=P):
         return lib.hipo_linear_cross_entropy_bwd_two_parts(
-            g, P, P, es, P, 8, P, None, P, P, rows, 8, 8, 8, 8, 1.0, -100, P, wb, None)
+            g, P, P, es, P, 8, P, None, P, dw, rows, 8, 8, 8, 8, 1.0, -100, P, wb, None)
 
     need = lib.hipo_linear_cross_entropy_bwd_two_parts_workspace_bytes
     for kw, msg in ((dict(es=3), b"elem_size"), (dict(rows=-1), b"negative"),
@@ -231,7 +242,7 @@ def test_two_parts_check_their_arguments(lib):
                                               b"workspace")):
         assert call(**kw) == HIPO_EINVAL
         assert msg in lib.hipo_last_error() and b"_two_parts" in lib.hipo_last_error()
-    assert call(rows=0) == 0 and need(P, 2, 0, 8, 8, 8) == 0
+    assert call(rows=0, dw=None) == 0 and need(P, 2, 0, 8, 8, 8) == 0
     one = lib.hipo_linear_cross_entropy_bwd_workspace_bytes
     for rows, elem, more in ((64, 2, False), (65, 2, True), (8192, 2, False), (65, 4, False)):
         # (Of 8192 rows the pieces are smaller.)

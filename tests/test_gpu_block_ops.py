@@ -626,3 +626,19 @@ def test_two_parts_of_fp32_are_three(rocm_device, ho):
     got = [ho.linear_cross_entropy_bwd(grads[0], hidden, weight, tokens, lse, two_parts=k)
            for k in (False, True)]
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("elem,dtype", [(2, BF16), (4, F32)])
+@pytest.mark.parametrize("width,vocab", [(1, 1), (7, 3), (65, 1001), (264, 2000)])
+def test_the_gradient_of_no_rows_is_zero(width, vocab, elem, dtype, rocm_device, ho):
+    """As of rows that are all left out, and no value beside dweight is written."""
+    lib = ho.load_library()
+    for bwd in (lib.hipo_linear_cross_entropy_bwd, lib.hipo_linear_cross_entropy_bwd_two_parts):
+        for shift in (64, 65):
+            buf = torch.full((width * vocab + 2 * shift,), NAN, dtype=dtype, device=rocm_device)
+            rc = bwd(None, None, None, elem, None, 8, None, None, None,
+                     buf.data_ptr() + shift * elem, 0, width, vocab, width, width, 1.0, IGNORE,
+                     None, 0, torch.cuda.current_stream().cuda_stream)
+            assert rc == 0
+            assert not buf[shift:-shift].any()
+            assert buf[:shift].isnan().all() and buf[-shift:].isnan().all()
