@@ -184,13 +184,15 @@ _IS_ROCM = torch.version.hip is not None
 
 
 def _require_rocm(*tensors: torch.Tensor) -> torch.device:
-    dev = tensors[0].device
+    dev = None
     for t in tensors:
         if not isinstance(t, torch.Tensor):
-            raise ValueError("expected tensors")
+            raise ValueError(f"expected tensors, got {type(t).__name__}")
         if not t.is_cuda:
             raise ValueError(f"hip_oracles runs on the ROCm device only, got a {t.device} tensor")
-        if t.device != dev:
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
             raise ValueError("all operands must be on one device")
     _require(_IS_ROCM, "torch is not a ROCm build")
     return dev
@@ -924,28 +926,32 @@ def embedding_bwd(grad: torch.Tensor, tokens: torch.Tensor, vocab: int, *, scale
 def _require_block_norms(what, x, rows_of, post, post_bias, pre, pre_bias, gate, norm):
     """(device, rows, cols, gate rows, layer) of block_norms and its gradient."""
     # One pass over the operands, whose attributes cost about 0.1 us each; what is
-    # wrong is found again below, for its message.
-    dev, dtype, shape = x.device, x.dtype, x.shape
-    ok = (x.is_cuda and _IS_ROCM and dtype in _FLOATS and len(shape) == 2 and x.is_contiguous()
-          and norm in _NORMS)
-    if ok:
-        rows, cols = shape
-        for t in rows_of:
-            ok = (ok and t.dtype == dtype and t.shape == shape and t.device == dev
-                  and t.is_contiguous())
-        for t in (post, post_bias, pre, pre_bias):
-            ok = ok and (t is None or (t.dtype == dtype and t.shape == (cols,) and t.device == dev
-                                       and t.is_contiguous()))
-        gates = 0
-        if gate is not None and ok:
-            gates = gate.shape[0] if gate.dim() == 2 else 1
-            ok = (gate.dtype == dtype and gate.dim() in (1, 2) and gate.shape[-1] == cols
-                  and gate.device == dev and gate.is_contiguous() and gates > 0
-                  and rows % gates == 0)
+    # wrong (no tensor at all, for one) is found again below, for its message.
+    try:
+        dev, dtype, shape = x.device, x.dtype, x.shape
+        ok = (x.is_cuda and _IS_ROCM and dtype in _FLOATS and len(shape) == 2
+              and x.is_contiguous() and norm in _NORMS)
         if ok:
-            return dev, rows, cols, gates, _NORMS[norm]
+            rows, cols = shape
+            for t in rows_of:
+                ok = (ok and t.dtype == dtype and t.shape == shape and t.device == dev
+                      and t.is_contiguous())
+            for t in (post, post_bias, pre, pre_bias):
+                ok = ok and (t is None or (t.dtype == dtype and t.shape == (cols,)
+                                           and t.device == dev and t.is_contiguous()))
+            gates = 0
+            if gate is not None and ok:
+                gates = gate.shape[0] if gate.dim() == 2 else 1
+                ok = (gate.dtype == dtype and gate.dim() in (1, 2) and gate.shape[-1] == cols
+                      and gate.device == dev and gate.is_contiguous() and gates > 0
+                      and rows % gates == 0)
+            if ok:
+                return dev, rows, cols, gates, _NORMS[norm]
+    except AttributeError:
+        pass
     vectors = [t for t in (post, post_bias, pre, pre_bias) if t is not None]
     _require_rocm(x, *rows_of, *vectors, *(() if gate is None else (gate,)))
+    dtype, shape = x.dtype, x.shape
     _require(dtype in _FLOATS and len(shape) == 2, f"{what}: 2-D bf16 or fp32 rows required")
     for t in (x, *rows_of):
         _require(t.dtype == dtype and t.shape == shape and t.is_contiguous(),
@@ -1019,7 +1025,8 @@ def block_norms_bwd(grad_h: torch.Tensor | None, grad_y: torch.Tensor | None,
     rows_of = [t for t in (grad_h, grad_y, h) if t is not None]
     dev, rows, cols, gates, layer = _require_block_norms(
         what, x, rows_of, post, post_bias, pre, pre_bias, gate, norm)
-    _require(stats.device == dev and stats.dtype == torch.float32 and stats.shape == (rows, 4)
+    _require(isinstance(stats, torch.Tensor) and stats.device == dev
+             and stats.dtype == torch.float32 and stats.shape == (rows, 4)
              and stats.is_contiguous(), "block_norms_bwd: stats must be contiguous fp32 [R, 4]")
     dx, dresidual = torch.empty_like(x), torch.empty_like(x)
     made = torch.empty_like if rows else torch.zeros_like  # no rows: nothing is written
@@ -1045,16 +1052,20 @@ def _require_output_layer(what, hidden, weight, tokens, scale, rows_of=()):
         hstride = width
     if vocab <= 1:
         wstride = width
-    ok = (hidden.is_cuda and _IS_ROCM and dtype in _FLOATS and weight.dtype == dtype
-          and weight.shape[1] == width and weight.device == dev and tokens.device == dev
-          and tokens.dtype in _TOKENS and tokens.shape == (rows,) and tokens.is_contiguous()
-          and vocab > 0 and width > 0 and 2.0 ** -100 <= scale <= 2.0 ** 100
-          and (hinner == winner == 1 or width == 1) and hstride >= width and wstride >= width)
-    for t in rows_of:
-        ok = (ok and t.dtype == torch.float32 and t.shape == (rows,) and t.device == dev
-              and t.is_contiguous())
-    if ok:
-        return dev, rows, width, vocab, hstride, wstride
+    try:
+        ok = (hidden.is_cuda and _IS_ROCM and dtype in _FLOATS and weight.dtype == dtype
+              and weight.shape[1] == width and weight.device == dev and tokens.device == dev
+              and tokens.dtype in _TOKENS and tokens.shape == (rows,) and tokens.is_contiguous()
+              and vocab > 0 and width > 0 and 2.0 ** -100 <= scale <= 2.0 ** 100
+              and (hinner == winner == 1 or width == 1) and hstride >= width
+              and wstride >= width)
+        for t in rows_of:
+            ok = (ok and t.dtype == torch.float32 and t.shape == (rows,) and t.device == dev
+                  and t.is_contiguous())
+        if ok:
+            return dev, rows, width, vocab, hstride, wstride
+    except AttributeError:
+        pass
     _require_rocm(hidden, weight, tokens, *rows_of)
     _require(dtype in _FLOATS, f"{what}: hidden must be 2-D bf16 or fp32")
     _require(weight.dtype == dtype and weight.shape[1] == width,

@@ -4,6 +4,7 @@ reference against automatic differentiation and differences."""
 import re
 import subprocess
 
+import numpy as np
 import pytest
 import torch
 
@@ -122,6 +123,20 @@ def test_wrappers_refuse_cpu_tensors():
                  lambda: hip_oracles.linear_cross_entropy_bwd(f, x, x, t, f)):
         with pytest.raises(ValueError, match="ROCm device only"):
             call()
+
+
+def test_wrappers_refuse_what_is_no_tensor():
+    x, w, f = torch.zeros(2, 8), torch.zeros(8), torch.zeros(2)
+    t = torch.zeros(2, dtype=torch.int64)
+    for bad in (None, [0.0], 1.0, np.zeros((2, 8))):
+        for call in (lambda: hip_oracles.block_norms(bad, x, pre=w),
+                     lambda: hip_oracles.block_norms_bwd(x, x, bad, x, torch.zeros(2, 4), pre=w),
+                     lambda: hip_oracles.linear_cross_entropy(bad, x, t),
+                     lambda: hip_oracles.linear_cross_entropy_bwd(f, x, bad, t, f),
+                     lambda: hip_oracles.embedding(bad, t),
+                     lambda: hip_oracles.row_mean(bad)):
+            with pytest.raises(ValueError):
+                call()
 
 
 # ---------------------------------------------------------------------------

@@ -642,3 +642,28 @@ def test_the_gradient_of_no_rows_is_zero(width, vocab, elem, dtype, rocm_device,
             assert rc == 0
             assert not buf[shift:-shift].any()
             assert buf[:shift].isnan().all() and buf[-shift:].isnan().all()
+
+
+@pytest.mark.parametrize("bad", [1.0, [0.0], "x"])
+def test_what_is_no_tensor_is_refused(bad, rocm_device, ho):
+    z = lambda *s, t=BF16: torch.zeros(*s, dtype=t, device=rocm_device)  # noqa: E731
+    x, w, st = z(4, 16), z(16), z(4, 4, t=F32)
+    t, f = z(4, t=torch.int64), z(4, t=F32)
+    layer = dict(norm="layer", post=w, pre=w)
+    calls = [lambda kw=kw: ho.block_norms(**{"x": x, "residual": x, **layer, **kw})
+             for kw in (dict(x=bad), dict(residual=bad), dict(post=bad), dict(post_bias=bad),
+                        dict(pre=bad), dict(pre_bias=bad), dict(gate=bad))]
+    given = dict(grad_h=x, grad_y=x, x=x, h=x, stats=st)
+    calls += [lambda kw=kw: ho.block_norms_bwd(**{**given, **layer, **kw})
+              for kw in [{k: bad} for k in (*given, "post", "post_bias", "pre", "pre_bias",
+                                            "gate")]]
+    loss = dict(hidden=x, weight=x, tokens=t)
+    calls += [lambda kw=kw: ho.linear_cross_entropy(**{**loss, **kw})
+              for kw in [{k: bad} for k in loss]]
+    loss_bwd = dict(loss, grad=f, lse=f, grad_lse=f)
+    calls += [lambda kw=kw: ho.linear_cross_entropy_bwd(**{**loss_bwd, **kw})
+              for kw in [{k: bad} for k in loss_bwd]]
+    for k, call in enumerate(calls):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {k}")
