@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import block_ops_reference as ref
+import fp32_parts_reference as parts
 import hip_oracles
 from conftest import ROOT
 
@@ -382,3 +383,74 @@ def test_cross_entropy_reference(in_64_bits):
                                                     scale, grad_lse=grads[1])
     torch.testing.assert_close(dh, h.grad, rtol=1e-11, atol=1e-11)
     torch.testing.assert_close(dw, w.grad, rtol=1e-11, atol=1e-11)
+
+
+# ---------------------------------------------------------------------------
+# Products of fp32 values
+# ---------------------------------------------------------------------------
+
+def test_sizes_of_the_parts_tests_take_every_kernel(launches):
+    calls = [(-1, op, *size, 4) for size in parts.SIZES
+             for op in ("linear_cross_entropy", "linear_cross_entropy_bwd")]
+    names = {name for made, _ in launches(*calls) for name, _, _ in made}
+    names = subprocess.run(["c++filt"], input="\n".join(names), capture_output=True, check=True,
+                           text=True).stdout.replace("hipo::(anonymous namespace)::", "")
+    for tile in (128, 256):
+        for epilogue in range(4):
+            assert f"gemm<float, {tile}, (Epilogue){epilogue}, 3>" in names
+    for n in (1, 2, 4):
+        assert f"thin_hidden<float, {n}>" in names
+        for grad in ("false", "true"):
+            for groups in ((1,) if n == 4 else (1, 2)):
+                assert f"thin_logits<float, {n}, {grad}, {groups}, false>" in names
+    assert "thin_weight<float>" in names
+
+
+def off_by(got, a, b):
+    """The share of the products that are off by more than the bound."""
+    want = a.double() * b.double()
+    return float(((got - want).abs() > parts.TOL * want.abs()).double().mean())
+
+
+@pytest.mark.parametrize("without", parts.PASSES)
+def test_a_product_that_is_left_out_shows(without):
+    """Of the operands that the kernels are tested with: with all six passes every
+    product is within the bound, with five most are not."""
+    for size in parts.SIZES[:8]:
+        _, _, _, (h, w) = parts.one_logit_a_row(*size, "cpu")
+        grad, hidden, weight, tokens, _ = parts.one_value_of_d_a_row(*size, "cpu")
+        for a, b in ((w, h), (weight[tokens], -grad[:, None]), (hidden, -grad[:, None])):
+            assert off_by(parts.product(a, b), a, b) == 0
+            least = 0.5 if a.numel() > 100 else 0.3
+            assert off_by(parts.product(a, b, without), a, b) > least, (size, without)
+
+
+@pytest.mark.parametrize("without", parts.PASSES)
+def test_a_logit_without_a_product_shows_in_its_probability(without):
+    """e^(s - lse) where lse is s rounded, as the gradient's logits are tested."""
+    for size in parts.SIZES:
+        _, _, _, (h, w) = parts.one_logit_a_row(*size, "cpu")
+        s = h.double() * w.double()
+        lse = s.float().double()
+        full, less = (torch.exp(parts.product(w, h, k) - lse) for k in (None, without))
+        p = torch.exp(s - lse)
+        tol = p * torch.expm1(parts.TOL * s.abs() + 2.0 ** -20)
+        assert ((full - p).abs() <= tol).all()
+        assert float(((less - p).abs() > tol).double().mean()) > 0.5 or size[0] < 10
+
+
+@pytest.mark.parametrize("size", parts.SIZES[:8])
+def test_operands_of_the_parts_tests(size):
+    """They are what they say, by the 64-bit formulas."""
+    hidden, weight, tokens, (h, w) = parts.one_logit_a_row(*size, "cpu")
+    logits = hidden.double() @ weight.double().t()
+    s = h.double() * w.double()
+    rows = torch.arange(len(s))
+    assert torch.equal(logits[rows, tokens], s)
+    assert torch.equal(torch.logsumexp(logits, -1), s)
+    grad, hidden, weight, tokens, lse = parts.one_value_of_d_a_row(*size, "cpu")
+    (dh, _), (dw, _) = ref.linear_cross_entropy_bwd(grad, hidden, weight, tokens, lse)
+    assert torch.equal(dh, -grad.double()[:, None] * weight.double()[tokens])
+    want = torch.zeros_like(dw)
+    want[tokens] = -grad.double()[:, None] * hidden.double()
+    assert torch.equal(dw, want)

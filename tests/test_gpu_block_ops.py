@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import block_ops_reference as ref
+import fp32_parts_reference as parts
 
 pytestmark = pytest.mark.gpu
 
@@ -667,3 +668,46 @@ def test_what_is_no_tensor_is_refused(bad, rocm_device, ho):
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {k}")
+
+
+# ---------------------------------------------------------------------------
+# Products of fp32 values: every part of every value counts
+# ---------------------------------------------------------------------------
+
+def assert_near(got, want, tol, what):
+    over = (got.double() - want).abs() - tol
+    assert float(over.max()) <= 0, (
+        f"{what}: {float((over > 0).double().mean()):.2%} of the values are over the bound, "
+        f"{float(((got.double() - want).abs() / tol.clamp(min=1e-300)).max()):.2f} times it")
+
+
+@pytest.mark.parametrize("size", parts.SIZES)
+def test_parts_of_fp32_logits(size, rocm_device, ho):
+    """lse is the row's one logit; the gradient's e^(s - lse) shows its own s."""
+    hidden, weight, tokens, (h, w) = parts.one_logit_a_row(*size, rocm_device)
+    s = h.double() * w.double()
+    _, got = ho.linear_cross_entropy(hidden, weight, tokens)
+    assert_near(got, s, parts.TOL * s.abs(), f"{size} lse")
+    lse = s.float()
+    p = torch.exp(s - lse.double())
+    zero, one = torch.zeros_like(lse), torch.ones_like(lse)
+    dh, _ = ho.linear_cross_entropy_bwd(zero, hidden, weight, tokens, lse, grad_lse=one)
+    want = p[:, None] * weight[tokens].double()
+    # Of e^: s's own bound, half a step of s - lse, below 2^-4, and of its product,
+    # and a step of the exponential: 2^-22 in all, 2^-20 with the product's.
+    tol = want.abs() * torch.expm1(parts.TOL * s.abs() + 2.0 ** -20)[:, None]
+    assert_near(dh, want, tol, f"{size} dhidden")
+
+
+@pytest.mark.parametrize("size", parts.SIZES)
+def test_parts_of_fp32_gradients(size, rocm_device, ho):
+    grad, hidden, weight, tokens, lse = parts.one_value_of_d_a_row(*size, rocm_device)
+    dh, dw = ho.linear_cross_entropy_bwd(grad, hidden, weight, tokens, lse)
+    d = -grad.double()[:, None]
+    want = d * weight[tokens].double()
+    assert_near(dh, want, parts.TOL * want.abs(), f"{size} dhidden")
+    want = d * hidden.double()
+    assert_near(dw[tokens], want, parts.TOL * want.abs(), f"{size} dweight")
+    rest = torch.ones(size[2], dtype=torch.bool, device=rocm_device)
+    rest[tokens] = False
+    assert not dw[rest].any(), f"{size}: dweight of other tokens"
