@@ -711,3 +711,113 @@ def test_parts_of_fp32_gradients(size, rocm_device, ho):
     rest = torch.ones(size[2], dtype=torch.bool, device=rocm_device)
     rest[tokens] = False
     assert not dw[rest].any(), f"{size}: dweight of other tokens"
+
+
+# ---------------------------------------------------------------------------
+# Nothing is written beside the outputs and the workspace
+# ---------------------------------------------------------------------------
+
+class Fenced:
+    """Memory of exactly the size asked for, `past` bytes behind a 16-byte
+    boundary, full of NaN, with a pattern before and behind it."""
+    FENCE, BYTE = 1 << 16, 0xA5
+
+    def __init__(self, dev, size, past=0):
+        self.from_, self.size = self.FENCE + past, size
+        self.all = torch.full((size + 2 * self.FENCE + past,), self.BYTE, dtype=torch.uint8,
+                              device=dev)
+        self.all[self.from_:self.from_ + size] = 0xFF
+        assert self.all.data_ptr() % 16 == 0
+
+    def ptr(self):
+        return self.all.data_ptr() + self.from_
+
+    def holds(self, want):
+        """Whether it has want's bits, and the pattern is as it was."""
+        inside = self.all[self.from_:self.from_ + self.size]
+        return torch.equal(inside, want.contiguous().view(-1).view(torch.uint8))
+
+    def intact(self):
+        before, behind = self.all[:self.from_], self.all[self.from_ + self.size:]
+        return bool((before == self.BYTE).all() and (behind == self.BYTE).all())
+
+
+def fenced_call(ho, fn, what, outputs, before, after, need, dev, past):
+    """fn(*before, *outputs, *after[, workspace, its size], stream) with the outputs
+    (tensors of what they should be, or None) fenced."""
+    outs = [None if t is None else Fenced(dev, t.numel() * t.element_size(), past) for t in outputs]
+    ws = None if need is None else Fenced(dev, need)
+    args = [*before, *(None if f is None else f.ptr() for f in outs), *after]
+    if ws is not None:
+        args += [ws.ptr(), need]
+    rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, (what, ho.load_library().hipo_last_error())
+    torch.cuda.synchronize()
+    for k, (f, t) in enumerate(zip(outs, outputs)):
+        if f is not None:
+            assert f.intact(), f"{what}: written beside output {k}"
+            assert f.holds(t), f"{what}: output {k}"
+    assert ws is None or ws.intact(), f"{what}: written beside the workspace"
+
+
+def address(t):
+    return None if t is None else t.data_ptr()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 8), (3, 9), (5, 15), (40, 511), (33, 520), (600, 700),
+                                       (7, 1001), (17, 1025), (9, 2880), (3, 5000), (2, 8193),
+                                       (2, 16383), (300, 16384)])
+def test_norms_write_their_outputs_alone(rows, cols, dtype, rocm_device, ho):
+    lib, elem = ho.load_library(), torch.finfo(dtype).bits // 8
+    for k, (norm, post, pre, gates) in enumerate((
+            ("layer", True, True, rows), ("rms", True, False, 1), ("layer", False, True, 0),
+            ("rms", True, True, 1 if rows % 3 else rows // 3))):
+        rowsof, kw, grads = norm_operands(rocm_device, rows, cols, dtype, norm=norm, post=post,
+                                          pre=pre, gates=gates, seed=k)
+        what, layer = f"[{rows}, {cols}] {dtype} {k}", int(norm == "layer")
+        out = ho.block_norms(**rowsof, **kw)
+        vectors = [address(kw.get(n)) for n in ("post", "post_bias", "pre", "pre_bias", "gate")]
+        past = elem * k
+        fenced_call(ho, lib.hipo_block_norms, what, out,
+                    [address(rowsof["x"]), address(rowsof["residual"]), elem, *vectors],
+                    [rows, cols, gates, kw["scale"], kw["offset"], 1e-6, layer], None,
+                    rocm_device, past)
+        h = out[0] if pre else None
+        got = ho.block_norms_bwd(grads["grad_h"], grads["grad_y"], rowsof["x"], h, out[2], **kw)
+        fenced_call(ho, lib.hipo_block_norms_bwd, f"{what} gradient", got,
+                    [address(grads["grad_h"]), address(grads["grad_y"]), address(rowsof["x"]),
+                     address(h), address(out[2]), elem, *vectors],
+                    [rows, cols, gates, kw["scale"], kw["offset"], layer],
+                    lib.hipo_block_norms_bwd_workspace_bytes(rows, cols), rocm_device, past)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,width,vocab", [
+    (1, 1, 1), (3, 72, 256), (5, 1001, 3001), (16, 64, 17000), (33, 200, 700), (64, 96, 2000),
+    (64, 131, 20001), (65, 512, 513), (100, 65, 4097), (129, 64, 1023), (257, 64, 513),
+    (515, 777, 1030), (2100, 100, 3001), (2100, 1000, 9000), (70, 1024, 180001),
+    (400, 64, (1 << 21) + 77)])
+def test_cross_entropy_writes_its_outputs_alone(rows, width, vocab, dtype, rocm_device, ho):
+    lib, elem = ho.load_library(), torch.finfo(dtype).bits // 8
+    for k, pads in enumerate(((0, 0), (3, 5))):
+        hidden, weight, tokens, grads = layer_operands(rocm_device, rows, width, vocab, dtype,
+                                                       pads=pads)
+        tokens[::7] = IGNORE
+        what, past = f"[{rows}, {width}, {vocab}] {dtype} {k}", elem * (3 * k)
+        sizes = [rows, width, vocab, width + pads[0], width + pads[1], 0.7, IGNORE]
+        given = [address(hidden), address(weight), elem, address(tokens), 8]
+        asked = (address(weight), elem, rows, width, vocab, width + pads[1])
+        loss, lse = ho.linear_cross_entropy(hidden, weight, tokens, scale=0.7)
+        fenced_call(ho, lib.hipo_linear_cross_entropy, what, (loss, lse), given, sizes,
+                    lib.hipo_linear_cross_entropy_workspace_bytes(*asked), rocm_device, 4 * k)
+        for two_parts, fn, bytes_of in (
+                (False, lib.hipo_linear_cross_entropy_bwd,
+                 lib.hipo_linear_cross_entropy_bwd_workspace_bytes),
+                (True, lib.hipo_linear_cross_entropy_bwd_two_parts,
+                 lib.hipo_linear_cross_entropy_bwd_two_parts_workspace_bytes)):
+            got = ho.linear_cross_entropy_bwd(grads[0], hidden, weight, tokens, lse, scale=0.7,
+                                              grad_lse=grads[1], two_parts=two_parts)
+            fenced_call(ho, fn, f"{what} gradient {two_parts}", got,
+                        [address(grads[0]), *given, address(lse), address(grads[1])], sizes,
+                        bytes_of(*asked), rocm_device, past)
