@@ -821,3 +821,108 @@ def test_cross_entropy_writes_its_outputs_alone(rows, width, vocab, dtype, rocm_
             fenced_call(ho, fn, f"{what} gradient {two_parts}", got,
                         [address(grads[0]), *given, address(lse), address(grads[1])], sizes,
                         bytes_of(*asked), rocm_device, past)
+
+
+# ---------------------------------------------------------------------------
+# Pieces of the gradients, row strides far above the width, every call of a run
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,width,vocab", [*LAYERS, (2100, 100, 3001), (2100, 1000, 9000),
+                                              (300, 264, 20001), (40, 264, 20001)])
+def test_gradients_row_by_row(rows, width, vocab, dtype, rocm_device, ho):
+    """Of d = g_lse p with probabilities near one another, so that a piece of d
+    that is missing or wrong shows in the 2-norm of a row of dhidden (64 of 2000
+    tokens: a sixth of it) and of 64 rows of dweight, whose worst-case bounds
+    would hide it.  bf16: half a step, 2^-8, of d and of the result.  fp32: ln p,
+    below 16, is off by half a step, 2^-21, and so is its product, 2^-20.5; with
+    the logits' and the sums' own 2^-19."""
+    hidden, weight, tokens, grads = layer_operands(rocm_device, rows, width, vocab, dtype, std=0.5)
+    _, lse = ho.linear_cross_entropy(hidden, weight, tokens)
+    zero = torch.zeros_like(lse)
+    h, w = hidden.double(), weight.double()
+    d = torch.exp(h @ w.t() - lse[:, None].double()) * grads[1][:, None].double()
+    want = d @ w, d.t() @ h
+    least = 2.0 ** -7 if dtype == BF16 else 2.0 ** -18
+    for two_parts in (False, True):
+        got = ho.linear_cross_entropy_bwd(zero, hidden, weight, tokens, lse, grad_lse=grads[1],
+                                          two_parts=two_parts)
+        for name, u, v, strip in zip(("dhidden", "dweight"), got, want, (1, 64)):
+            for first in range(0, len(v), strip * 4096):
+                some = slice(first, first + strip * 4096)
+                off, size = ((u.double() - v)[some], v[some])
+                off, size = (torch.stack([p.norm() for p in t.split(strip)]) if strip > 1
+                             else t.norm(dim=-1) for t in (off, size))
+                worst = float((off / size).max())
+                assert worst <= least, f"[{rows}, {width}, {vocab}] {dtype} {name}: {worst:.2e}"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,width,vocab,more", [(3, 65, 300, 9), (5, 72, 1000, 0),
+                                                   (40, 72, 300, 0), (100, 72, 300, 0),
+                                                   (260, 264, 600, 0), (100, 72, 300, 8)])
+def test_row_strides_far_above_the_width(rows, width, vocab, more, dtype, rocm_device, ho):
+    """Up to the largest of the weight, 2^21, and past 2^31 bytes of hidden."""
+    pads = (2 ** 31 // (2 * rows) + 5 + more - width, 2 ** 21 - more - width)
+    hidden, weight, tokens, grads = layer_operands(rocm_device, rows, width, vocab, dtype,
+                                                   pads=pads)
+    assert weight.stride(0) == 2 ** 21 - more and hidden.stride(0) * rows * 2 > 2 ** 31
+    got = ho.linear_cross_entropy(hidden, weight, tokens)
+    near = [t.contiguous() for t in (hidden, weight)]
+    check_loss(ho, *near, tokens, grads, f"[{rows}, {width}, {vocab}] {dtype}")
+    for k, (u, (v, tol)) in enumerate(zip(got, ref.linear_cross_entropy(*near, tokens))):
+        ref.close(u, v, tol, f"[{rows}, {width}, {vocab}] {dtype} {k}")
+    lse = got[1]
+    for two_parts in (False, True):
+        kw = dict(grad_lse=grads[1], two_parts=two_parts)
+        a = ho.linear_cross_entropy_bwd(grads[0], hidden, weight, tokens, lse, **kw)
+        wanted = ref.linear_cross_entropy_bwd(grads[0], *near, tokens, lse, grad_lse=grads[1])
+        for name, u, (v, tol) in zip(("dhidden", "dweight"), a, wanted):
+            ref.close(u, v, tol, f"[{rows}, {width}, {vocab}] {dtype} {name}")
+
+
+class Checked:
+    """The library, each call's results held to the 64-bit formulas of the
+    operands that it had."""
+
+    def __init__(self, ho):
+        self.ho, self.calls = ho, 0
+        self.embedding, self.embedding_bwd = ho.embedding, ho.embedding_bwd
+
+    def close(self, names, got, want):
+        self.calls += 1
+        for name, u, v in zip(names, got, want):
+            if v is not None:
+                ref.close(u, v[0].cpu(), v[1].cpu(), f"call {self.calls} {name}")
+
+    def block_norms(self, x, residual, **kw):
+        h, y, stats = self.ho.block_norms(x, residual, **kw)
+        want_h, tol_h, _, _ = ref.stream(x, residual, **kw)
+        want_y, tol_y, _, _ = ref.after(h, **kw)
+        self.close(("h", "y"), (h, y), ((want_h, tol_h), (want_y, tol_y)))
+        return h, y, stats
+
+    def block_norms_bwd(self, *args, **kw):
+        got = self.ho.block_norms_bwd(*args, **kw)
+        self.close(("dx", "dresidual", "dgate", "dpost", "dpost_bias", "dpre", "dpre_bias"), got,
+                   ref.block_norms_bwd(*args, **kw))
+        return got
+
+    def linear_cross_entropy(self, *args, scale):
+        got = self.ho.linear_cross_entropy(*args, scale=scale)
+        self.close(("loss", "lse"), got, ref.linear_cross_entropy(*args, scale))
+        return got
+
+    def linear_cross_entropy_bwd(self, *args, scale):
+        got = self.ho.linear_cross_entropy_bwd(*args, scale=scale)
+        self.close(("dhidden", "dweight"), got, ref.linear_cross_entropy_bwd(*args, scale))
+        return got
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,width,vocab", [(40, 64, 300), (260, 520, 2003), (2100, 264, 5001)])
+def test_every_call_of_a_run(rows, width, vocab, dtype, rocm_device, ho):
+    """What a run's roundings between its calls would hide."""
+    checked = Checked(ho)
+    Model(checked, rocm_device, rows, width, vocab, dtype).step()
+    assert checked.calls == 6
