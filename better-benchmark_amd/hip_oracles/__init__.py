@@ -1094,7 +1094,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, tokens: tor
 
     A row whose token is ignore_index is left out, whatever it holds: 0 and 0.
     Any other token outside [0, V) has loss NaN; a row with a NaN logit has both
-    NaN.  token_logprobs gives the negative loss of logits that are in memory."""
+    NaN, one with a logit of +infinity no finite lse; a logit of -infinity adds
+    nothing.  token_logprobs gives the negative loss of logits that are in memory."""
     lib = _lib or load_library()
     what = "linear_cross_entropy"
     _two_dimensions(what, hidden, weight)

@@ -608,8 +608,11 @@ int hipo_block_norms_bwd(const void* grad_h, const void* grad_y, const void* x,
  * 2^-100 to 2^100.  At most 2^22 - 256 rows, width 2^20, weight_row_stride 2^21,
  * a vocabulary of 2^31 - 65536, and rows * width 2^38.  A row whose token is
  * ignore_index is left out, whatever it holds: 0 and 0.  A token outside [0,
- * vocab) otherwise has loss NaN.  A row with a NaN logit has lse NaN, one with an
- * infinite logit no finite lse.  Up to 64 rows weight is read where it lies, and so
+ * vocab) otherwise has loss NaN.  A row with a NaN logit has lse NaN, one with a
+ * logit of +infinity no finite lse; a logit of -infinity adds nothing to the sum,
+ * and is a loss of +infinity for its own token (an infinite value in fp32 operands:
+ * where those that it is multiplied with are below 128, else the logit may be NaN).
+ * Up to 64 rows weight is read where it lies, and so
  * is one that is bf16, 16-byte aligned, of a width and a row stride that are
  * multiples of 8; others are copied into the workspace piece by piece.
  * `workspace`: at least hipo_linear_cross_entropy_workspace_bytes bytes (weight is

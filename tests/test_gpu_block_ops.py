@@ -926,3 +926,41 @@ def test_every_call_of_a_run(rows, width, vocab, dtype, rocm_device, ho):
     checked = Checked(ho)
     Model(checked, rocm_device, rows, width, vocab, dtype).step()
     assert checked.calls == 6
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,width,vocab", [(3, 20, 300), (20, 72, 20001), (50, 72, 300),
+                                              (100, 72, 700), (2100, 100, 33000)])
+def test_infinite_logits(rows, width, vocab, dtype, rocm_device, ho):
+    """-infinity adds nothing and is a loss of +infinity for its own token;
+    dhidden is NaN in the columns where 0 is multiplied with an infinite weight
+    and as without that token in the others, and dweight is finite."""
+    hidden, weight, tokens, grads = layer_operands(rocm_device, rows, width, vocab, dtype)
+    hidden = hidden.abs() + 0.125  # (no 0, and all of one sign)
+    weight = weight.clone()
+    gone = [0, vocab // 2, vocab - 1]
+    weight[gone, 7] = -INF
+    tokens = torch.where(torch.isin(tokens, torch.tensor(gone, device=rocm_device)), 1, tokens)
+    tokens[1] = gone[1]
+    got = ho.linear_cross_entropy(hidden, weight, tokens)
+    left = torch.ones(vocab, dtype=torch.bool, device=rocm_device)
+    left[gone] = False
+    place = torch.cumsum(left, 0) - 1
+    there = torch.where(torch.arange(rows, device=rocm_device) == 1, -1, place[tokens])
+    assert got[0][1] == INF and torch.isfinite(got[1]).all()
+    wanted = ref.linear_cross_entropy(hidden, weight[left], there)
+    for name, u, (v, tol) in zip(("loss", "lse"), got, wanted):
+        u = u.clone()
+        u[1], v[1] = (0.0, 0.0) if name == "loss" else (u[1], v[1])
+        ref.close(u, v, tol, f"[{rows}, {width}, {vocab}] {dtype} {name}")
+    tokens[1] = 1
+    dh, dw = ho.linear_cross_entropy_bwd(grads[0], hidden, weight, tokens, got[1])
+    want = ref.linear_cross_entropy_bwd(grads[0], hidden, weight[left], place[tokens], got[1])
+    rest = [c for c in range(width) if c != 7]
+    assert dh[:, 7].isnan().all()
+    ref.close(dh[:, rest], want[0][0][:, rest], want[0][1][:, rest], f"{rows} {dtype} dhidden")
+    ref.close(dw[left], *want[1], f"{rows} {dtype} dweight")
+    assert not dw[gone].any()
+    weight[vocab // 3, 7] = INF
+    got = ho.linear_cross_entropy(hidden, weight, tokens)
+    assert not torch.isfinite(got[1]).any() and not torch.isfinite(got[0]).any()
