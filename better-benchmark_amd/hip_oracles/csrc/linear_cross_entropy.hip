@@ -1659,9 +1659,13 @@ int launch_thin(const char* what, const Thin& a, int64_t rows, hipStream_t strea
   const uint32_t grid = static_cast<uint32_t>(std::min<int64_t>(a.tiles, 1 << 20));
   // No more workgroups than CUs: K split, as far as LDS and registers reach (4 x
   // 3584 x 3968 bf16, 62 workgroups: 22.1 -> 15.2 us; 1 x 2048 x 32000, 500
-  // workgroups: 23.9 -> 30.5, so not there).
+  // workgroups: 23.9 -> 30.5, so not there).  Four groups leave a lane 128 registers:
+  // of 17 to 32 rows the forward spills with them (24 x 2048 x 16000: 22.2 us, two
+  // groups 19.5; 32 x 3584 x 3968: 21.0, 20.9), the gradient does not (24 x 2048 x
+  // 16000: 67.4, 66.4; 32 x 4096 x 8000: 62.6, 63.9).
   const bool few = a.tiles <= kCus;
   constexpr int kMany = sizeof(T) == 2 ? 4 : 2, kWide = sizeof(T) == 2 ? 2 : 1;
+  constexpr int kMiddle = Grad ? kMany : 2;
   // Rows that are whole 128-byte lines, read once: past the caches, which hold other
   // layers' weights by the next call (1 x 4096 x 128000 207 -> 192 us, 1 x 2048 x 32000
   // among other states 36.7 -> 33.3; the same 131 MB at once again 26.8 -> 32.0).  Of
@@ -1675,7 +1679,7 @@ int launch_thin(const char* what, const Thin& a, int64_t rows, hipStream_t strea
     : once ? thin_logits<T, 1, Grad, 1, kOnce><<<grid, 256, 0, stream>>>(a)
            : thin_logits<T, 1, Grad, 1><<<grid, 256, 0, stream>>>(a);
   } else if (rows <= 32) {
-    few    ? thin_logits<T, 2, Grad, kMany><<<grid, 256 * kMany, 0, stream>>>(a)
+    few    ? thin_logits<T, 2, Grad, kMiddle><<<grid, 256 * kMiddle, 0, stream>>>(a)
     : once ? thin_logits<T, 2, Grad, 1, kOnce><<<grid, 256, 0, stream>>>(a)
            : thin_logits<T, 2, Grad, 1><<<grid, 256, 0, stream>>>(a);
   } else {

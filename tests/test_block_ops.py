@@ -218,6 +218,20 @@ def test_a_refused_launch_ends_the_call(call, launches):
 TWO_PARTS = "linear_cross_entropy_bwd_two_parts"
 
 
+@pytest.mark.parametrize("rows,elem,threads", [(16, 2, (1024, 1024)), (17, 2, (512, 1024)),
+                                               (32, 2, (512, 1024)), (33, 2, (512, 512)),
+                                               (16, 4, (512, 512)), (32, 4, (512, 512)),
+                                               (33, 4, (256, 256))])
+def test_groups_of_few_rows_by_the_registers_they_leave(rows, elem, threads, launches):
+    """1024 threads leave a lane 128 registers, which the forward of 17 to 32 rows
+    does not fit."""
+    calls = [(-1, op, rows, 2048, 16000, elem)
+             for op in ("linear_cross_entropy", "linear_cross_entropy_bwd")]
+    for want, (made, _) in zip(threads, launches(*calls)):
+        (_, _, block), = [m for m in made if "thin_logits" in m[0]]
+        assert block == (want, 1, 1)
+
+
 def test_two_parts_can_be_launched(launches):
     sizes = ((1, 1, 1), (65, 1, 1), (8192, 4096, 128000), (257, 1001, 50001),
              ((1 << 22) - 256, 8, 70000), (65, 8, (1 << 31) - 65536),
