@@ -990,7 +990,10 @@ def block_norms(x: torch.Tensor, residual: torch.Tensor, *, post: torch.Tensor |
     [R, 4] for block_norms_bwd (mean and 1 / deviation of x and of h, 0 and 1
     where there is no norm).  One of post and pre at least; weights, biases and
     gate are of the rows' type.  gate: [C], or [G, C] where G divides R, for
-    R / G consecutive rows each (a sample's, or G = R)."""
+    R / G consecutive rows each (a sample's, or G = R).
+
+    bf16 with the second norm alone, no gate and no gradient to come is
+    residual_layernorm's or rmsnorm_ex's, which are quicker."""
     lib = _lib or load_library()
     what = "block_norms"
     dev, rows, cols, gates, layer = _require_block_norms(

@@ -13,9 +13,10 @@
 //
 // Both passes read every value once and hold the row in registers between its
 // statistics and its results; HBM bounds them.  A row belongs to a team of
-// lanes: up to 512 columns (one group of 8 values per lane) 1 to 64 lanes of
-// one wave, above that W whole waves with two groups per lane (16-byte
-// accesses of bf16 that cover 1 KiB of a row per wave).
+// lanes with groups of 8 values (16-byte accesses of bf16, 1 KiB of a row per
+// wave): up to 512 columns 1 to 64 lanes of one wave with one group each, above
+// that whole waves, forwards with two groups a lane, backwards with one up to
+// 4096 columns (bwd_groups()).
 #include <algorithm>
 
 #include "hipo_common.h"
@@ -286,7 +287,9 @@ __global__ __launch_bounds__(THREADS) void block_norms(Forward a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) n[u] = load8_once(static_cast<const T*>(a.x) + at + c.col[u]);
 #pragma unroll
-    for (int u = 0; u < U; ++u) h[u] = load8_once(static_cast<const T*>(a.residual) + at + c.col[u]);
+    for (int u = 0; u < U; ++u) {
+      h[u] = load8_once(static_cast<const T*>(a.residual) + at + c.col[u]);
+    }
     float mean0 = 0.0f, rstd0 = 1.0f, mean1 = 0.0f, rstd1 = 1.0f;
     if (post) {
       row_stats<U, LAYER, kSmall>(n, c, a.lanes, a.inv_cols, a.eps, slots[set], &mean0, &rstd0);
@@ -378,8 +381,13 @@ __global__ __launch_bounds__(THREADS) void block_norms_bwd(Backward a) {
   constexpr bool kAhead = U == 1;  // with two groups a lane has no registers for it
   // 16 waves leave a lane 128 registers.  The two weights' sums then lie in LDS, 128
   // KB of it, read and written once a row (16 bytes of a lane beside the next's), and
-  // weights and gate are loaded where they are used: [4096, 12288] bf16 297 -> 151 us,
-  // of 512 threads (8192 x 5120) 122 -> 129, so not there.
+  // weights and gate are loaded where they are used: [4096, 12288] bf16 297 -> 151 us.
+  // Of 512 threads not: [8192, 5120] 115 -> 125 us (122 with the next row's loads ahead,
+  // for which there is room then), [8192, 8192] 148 -> 153 (159), with a gate a row
+  // 216 -> 218 (241).  Biases' and gates' sums still spill: of LayerNorm before and
+  // after the sum 52 registers a lane, with a gate a row 88, with one that rows share
+  // 194 ([4096, 16384] with 16 gates 607 us, where RMSNorm without a gate, which spills
+  // none, takes 177); of 512 threads the last alone, 29 ([8192, 8192] 245 and 148).
   constexpr bool kFewRegisters = THREADS == 1024;
   __shared__ float slots[2][64];
   __shared__ f32x4_t held[kFewRegisters ? 2 * U * 2 * THREADS : 1];
@@ -795,7 +803,11 @@ void launch_bwd(const Backward& a, bool layer, hipStream_t stream) {
   }
 }
 
-// Workgroups of the gradient: no more than there are rows for their teams.
+// Workgroups of the gradient: no more than there are rows for their teams, and one a
+// CU.  Two were, RMSNorm before and after the sum of 8192 rows: of 1280 columns 32.1 ->
+// 31.1 us, 2560 55.7 -> 53.2, 2880 61.1 -> 60.7, but 3584 69.2 -> 72.3, 4096 74.3 ->
+// 78.5, 5120 115 -> 123, 8192 148 -> 167, and 16384 x 2880 with 16 gates 126 -> 138:
+// twice the sums to write and join, and few variants fit a CU twice.
 int bwd_blocks(int64_t rows, int64_t cols) {
   const Layout l = layout_of(cols, bwd_groups(cols));
   return static_cast<int>(std::min<int64_t>((rows + l.teams - 1) / l.teams, 256));
@@ -837,7 +849,8 @@ extern "C" int hipo_block_norms(const void* x, const void* residual, int elem_si
   const int rc = check_sizes("block_norms", elem_size, rows, cols, gate_rows, layer, post,
                              post_bias, pre, pre_bias, gate, scale, offset);
   if (rc != 0) return rc;
-  HIPO_REQUIRE(eps >= 0.0f && __builtin_isfinite(eps), "block_norms: eps must be finite, not negative");
+  HIPO_REQUIRE(eps >= 0.0f && __builtin_isfinite(eps),
+               "block_norms: eps must be finite, not negative");
   if (rows == 0) return 0;
   HIPO_REQUIRE(x && residual && h && stats && (y || !pre), "block_norms: null pointer");
   const Layout l = layout_of(cols, 2);

@@ -436,7 +436,8 @@ struct Operand {
 
   // A quarter of it.
   __device__ __forceinline__ void load(int buffer, int q, const Round& r) const {
-    load_to_lds(r.buffer, r.from + q * next, r.offset, to + buffer * Tile * kStep * 2 + q * kWaves * 1024);
+    load_to_lds(r.buffer, r.from + q * next, r.offset,
+                to + buffer * Tile * kStep * 2 + q * kWaves * 1024);
   }
 
   // Rows 16 f to 16 f + 15 of the wave's, 32 values of K of half `h`: row l, values
@@ -740,7 +741,8 @@ __global__ __launch_bounds__(Tile * 2, 2) void gemm(Product p) {
             acc[f][n] = f32x4_t{x[0], x[1], x[2], x[3]};
             asm volatile("" : "+v"(acc[f][n]));  // what is left takes its place: no spills
           }
-          *reinterpret_cast<u32x2_t*>(lds + j * Tile + (((i >> 3) ^ (j % kPieces)) << 3) + (i & 7)) = v;
+          *reinterpret_cast<u32x2_t*>(lds + j * Tile + (((i >> 3) ^ (j % kPieces)) << 3) +
+                                      (i & 7)) = v;
         }
       }
       __syncthreads();
@@ -915,7 +917,7 @@ __device__ __forceinline__ int thin_d_part(int pass) {
 // wave, reduced or (Grad) turned into d as gemm()'s.  Both operands go through
 // registers, kThinStages rounds ahead, to LDS (places as in Operand): the weight is
 // read once, at any alignment, fp32 split on the way.  Memory bounds it (1 x 4096 x
-// 128000 bf16: 192 us, 5.5 TB/s; fp32 460 us, 4.6): the loads in flight (32 KB a
+// 128000 bf16: 188 us, 5.6 TB/s; fp32 452 us, 4.6): the loads in flight (32 KB a
 // workgroup of bf16) and the number of workgroups are what counts.  Where there are
 // few, K is split among `Groups` groups of four waves, whose sums are added
 // through LDS.  Once: the weight takes no place in the caches.
@@ -1265,7 +1267,8 @@ __global__ __launch_bounds__(256) void thin_hidden(ThinHidden a) {
   if (count == 0) return;
   const int c0 = blockIdx.x * 64;
   const int64_t rounds = (a.vocab + 63) / 64;
-  const int64_t begin = rounds * blockIdx.y / gridDim.y, end = rounds * (blockIdx.y + 1) / gridDim.y;
+  const int64_t begin = rounds * blockIdx.y / gridDim.y;
+  const int64_t end = rounds * (blockIdx.y + 1) / gridDim.y;
 
   Piece<T> w[2][2];
   u32x4_t d[2][kParts][kPiecesD];
@@ -1611,10 +1614,9 @@ int piece_of_weight(const char* what, const Call& c, const Plan& plan, int64_t f
     g->lda = plan.k_pad;
     g->a_plane = plan.piece * plan.k_pad;
     g->k = static_cast<int>(plan.k_pad);
-    HIPO_STEP(pack<T>(what, Pack{from, c.weight_ld, nullptr, nullptr, g->a_rows,
-                                 static_cast<int>(c.width), to, plan.k_pad, g->a_plane, nullptr, 0, 0,
-                                 nullptr},
-                      g->a_rows, c.stream));
+    const Pack all{from, c.weight_ld, nullptr, nullptr, g->a_rows, static_cast<int>(c.width),
+                   to, plan.k_pad, g->a_plane, nullptr, 0, 0, nullptr};
+    HIPO_STEP(pack<T>(what, all, g->a_rows, c.stream));
   }
   g->first = first;
   return 0;
@@ -1667,8 +1669,8 @@ int launch_thin(const char* what, const Thin& a, int64_t rows, hipStream_t strea
   constexpr int kMany = sizeof(T) == 2 ? 4 : 2, kWide = sizeof(T) == 2 ? 2 : 1;
   constexpr int kMiddle = Grad ? kMany : 2;
   // Rows that are whole 128-byte lines, read once: past the caches, which hold other
-  // layers' weights by the next call (1 x 4096 x 128000 207 -> 192 us, 1 x 2048 x 32000
-  // among other states 36.7 -> 33.3; the same 131 MB at once again 26.8 -> 32.0).  Of
+  // layers' weights by the next call (1 x 4096 x 128000 203 -> 187 us, 1 x 2048 x 32000
+  // among other states 37.8 -> 33.9; the same 131 MB at once again 26.8 -> 32.0).  Of
   // other rows (3 x 1000 x 20001) 17.4 -> 20.3, as two rows' reads meet in a line; the
   // gradient reads the weight twice (8 x 2048 x 32000 117 -> 119).
   constexpr bool kOnce = sizeof(T) == 2 && !Grad;
@@ -1715,9 +1717,10 @@ int run_fwd(const Call& c, const Plan& plan, float* loss, float* lse) {
     g.first_tile = i * plan.piece / plan.tile;
     HIPO_STEP((multiply<T, kReduce>(what, g, plan.tile, c.rows, c.stream)));
   }
+  const int tiles = static_cast<int>(up(c.vocab, plan.tile) / plan.tile);
   join_loss<<<static_cast<uint32_t>(std::min<int64_t>((c.rows + 15) / 16, 1 << 16)), 256, 0,
-              c.stream>>>(JoinLoss{g.part, g.part_ld, static_cast<int>(up(c.vocab, plan.tile) / plan.tile),
-                                   g.kept, g.b_count, g.target, loss, lse});
+              c.stream>>>(
+      JoinLoss{g.part, g.part_ld, tiles, g.kept, g.b_count, g.target, loss, lse});
   return check_launch(what);
 }
 

@@ -558,7 +558,8 @@ int hipo_embedding_bwd(const void* grad, int elem_size, const void* tokens,
  * the biases; y is NULL where pre is.  The outputs overlap no operand.
  * No counterpart among the reference's oracles; beside
  * hipo_residual_layernorm_bf16 and hipo_rmsnorm_ex_bf16, which have the second
- * norm alone.
+ * norm alone, of bf16, and are quicker where that is all and no gradient follows
+ * ([8192, 4096] 46 and 45 us, here 53 and 47; [16, 2048] 11 and 8, here 11 and 10).
  */
 int hipo_block_norms(const void* x, const void* residual, int elem_size,
                      const void* post, const void* post_bias, const void* pre,
@@ -638,11 +639,12 @@ int hipo_linear_cross_entropy(const void* hidden, const void* weight, int elem_s
  *   d[r, j]  = scale * ((grad + grad_lse) e^(s_j - lse) - grad [j = t])
  *   dhidden  = d weight,  dweight = d^T hidden
  * the logits computed once more in pieces of the vocabulary, the products
- * accumulated in fp32 and rounded once to the operands' type; d itself is
- * rounded to bf16 where the operands are bf16 (the matrix cores' type; up to 64
- * rows to two bf16 parts, some 2^-17 of it; so with _two_parts at any number of
- * rows, for gradients that are off by their own rounding alone, at twice the
- * products of dhidden and dweight).
+ * accumulated in fp32 and rounded once to the operands' type; e^(s_j - lse) of
+ * the fp32 lse is off by a factor of about 1 + |lse| 2^-24.  d itself is rounded to
+ * bf16 where the operands are bf16 (the matrix cores' type): up to 64 rows, and
+ * with _two_parts at any number of rows, to two bf16 parts, some 2^-17 of it, so
+ * that the gradients are off by their own rounding alone, at twice the products of
+ * dhidden and dweight.
  * dhidden is contiguous [rows, width], dweight [vocab, width]; they overlap
  * neither each other nor an operand.  Rows of ignore_index are zero in dhidden
  * and add nothing to dweight, whatever they hold; a row of another token outside
