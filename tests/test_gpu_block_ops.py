@@ -964,3 +964,60 @@ def test_infinite_logits(rows, width, vocab, dtype, rocm_device, ho):
     weight[vocab // 3, 7] = INF
     got = ho.linear_cross_entropy(hidden, weight, tokens)
     assert not torch.isfinite(got[1]).any() and not torch.isfinite(got[0]).any()
+
+
+@pytest.mark.parametrize("rows", [3, 70, 300, 2500])
+@pytest.mark.parametrize("kind", ["some", "all", "but one", "unknown", "nan"])
+def test_two_parts_of_rows_left_out(kind, rows, rocm_device, ho):
+    """Rows of ignore_index count nowhere, whatever they hold; NaN where one part
+    has NaN, and the others' values near those of one part."""
+    hidden, weight, tokens, grads = layer_operands(rocm_device, rows, 72, 600, BF16)
+    out = torch.zeros(rows, dtype=torch.bool, device=rocm_device)
+    if kind == "some":
+        out[::3] = True
+    elif kind in ("all", "but one"):
+        out[:] = True
+        out[rows // 2] = kind == "all"
+    tokens[out] = IGNORE
+    hidden[out] = NAN
+    if kind == "unknown":
+        tokens[0], tokens[rows // 2] = 600, -1
+    if kind == "nan":
+        hidden[rows // 2, 5] = NAN
+    _, lse = ho.linear_cross_entropy(hidden, weight, tokens)
+    one, two = (ho.linear_cross_entropy_bwd(grads[0], hidden, weight, tokens, lse,
+                                            grad_lse=grads[1], two_parts=k) for k in (False, True))
+    for u, v in zip(one, two):
+        assert torch.equal(u.isnan(), v.isnan())
+        fine = ~u.isnan()
+        assert float((u - v)[fine].double().norm()) <= 2.0 ** -7 * float(u[fine].double().norm())
+    assert not two[0][out].any()
+    if kind in ("unknown", "nan"):
+        assert two[0][rows // 2].isnan().all() and two[1].isnan().all()
+    if kind == "all":
+        assert not two[1].any()
+
+
+def test_two_parts_in_a_graph(rocm_device, ho):
+    """Replayed on new tokens, another number of them left out, with eager work
+    between."""
+    hidden, weight, tokens, grads = layer_operands(rocm_device, 300, 264, 2003, BF16)
+    lse = torch.full_like(grads[0], 9.0)
+    call = lambda: ho.linear_cross_entropy_bwd(  # noqa: E731
+        grads[0], hidden, weight, tokens, lse, grad_lse=grads[1], two_parts=True)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        captured = call()
+    for seed in range(4):
+        g = torch.Generator().manual_seed(seed)
+        tokens.copy_(torch.randint(0, 2003, (300,), generator=g))
+        tokens[:seed * 100] = IGNORE
+        eager = [v.clone() for v in call()]
+        graph.replay()
+        torch.cuda.synchronize()
+        for u, v in zip(captured, eager):
+            assert torch.equal(u, v), f"replay {seed}"
