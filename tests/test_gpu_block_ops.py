@@ -1021,3 +1021,84 @@ def test_two_parts_in_a_graph(rocm_device, ho):
         torch.cuda.synchronize()
         for u, v in zip(captured, eager):
             assert torch.equal(u, v), f"replay {seed}"
+
+
+# ---------------------------------------------------------------------------
+# Offsets past 32 bits
+# ---------------------------------------------------------------------------
+
+def normal(dev, *shape, seed=0, std=1.0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    t = torch.empty(*shape, dtype=BF16, device=dev)
+    for part in t.split(1 << 18):
+        part.normal_(0.0, std, generator=g)
+    return t
+
+
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+def test_norms_of_more_rows_than_workgroups(norm, rocm_device, ho):
+    """2^20 workgroups of one row each and a few rows more, of 4.3e9 values: the
+    rows are as in a call of their own."""
+    rows, cols = (1 << 20) + 5, 4099
+    x, r, gh, gy = (normal(rocm_device, rows, cols, seed=k) for k in range(4))
+    w, v = (normal(rocm_device, cols, seed=k) for k in (5, 6))
+    kw = dict(post=w, pre=v, gate=w, norm=norm, scale=0.5, offset=1.0)
+    h, y, stats = ho.block_norms(x, r, **kw)
+    got = ho.block_norms_bwd(gh, gy, x, h, stats, **kw)
+    assert all(torch.isfinite(t).all() for t in got[2:] if t is not None)
+    for some in (slice(0, 9), slice(rows // 2, rows // 2 + 9), slice(rows - 9, rows)):
+        part = [t[some].contiguous() for t in (x, r, gh, gy)]
+        for u, own in zip((h, y, stats), ho.block_norms(*part[:2], **kw)):
+            assert torch.equal(u[some], own)
+        own = ho.block_norms_bwd(*part[2:], part[0], h[some].contiguous(),
+                                 stats[some].contiguous(), **kw)
+        assert torch.equal(got[0][some], own[0]) and torch.equal(got[1][some], own[1])
+
+
+@pytest.mark.parametrize("rows", [3, 70])
+def test_output_layers_of_more_than_32_bits(rows, rocm_device, ho):
+    """A weight and its gradient of 4.3e9 values, in the kernels of few rows and in
+    the products; d = g_lse p, every row of the weight counting about as much."""
+    width, vocab = 2056, (1 << 21) + 100
+    weight = normal(rocm_device, vocab, width, std=0.5 / width ** 0.5)
+    hidden = normal(rocm_device, rows, width, seed=1)
+    tokens = torch.linspace(0, vocab - 1, rows, device=rocm_device).round().long()
+    loss, lse = ho.linear_cross_entropy(hidden, weight, tokens)
+    h = hidden.double()
+    s = torch.cat([h @ w.double().t() for w in weight.split(1 << 17)], 1)
+    want = torch.logsumexp(s, -1)
+    # Of values below 16: a few steps of 2^-20.
+    assert float((lse - want).abs().max()) < 2.0 ** -17
+    assert float((loss - (want - s.gather(1, tokens[:, None])[:, 0])).abs().max()) < 2.0 ** -17
+    one, zero = torch.ones_like(lse), torch.zeros_like(lse)
+    p = torch.exp(s - lse.double()[:, None])
+    dh_want = sum(q @ w.double() for q, w in zip(p.split(1 << 17, 1), weight.split(1 << 17)))
+    for two_parts in (False, True):
+        dh, dw = ho.linear_cross_entropy_bwd(zero, hidden, weight, tokens, lse, grad_lse=one,
+                                             two_parts=two_parts)
+        off = (dh.double() - dh_want).norm(dim=-1) / dh_want.norm(dim=-1)
+        assert float(off.max()) <= 2.0 ** -7
+        for some in (slice(0, 300), slice(vocab // 2, vocab // 2 + 300), slice(vocab - 300, vocab)):
+            v = p[:, some].t() @ h
+            off = (dw[some].double() - v).norm(dim=-1) / v.norm(dim=-1)
+            assert float(off.max()) <= 2.0 ** -7, some
+
+
+def test_hidden_states_of_more_than_32_bits(rocm_device, ho):
+    """4.3e9 values of hidden and dhidden: rows as in a call of their own, to what
+    other tiles' sums may differ by."""
+    rows, width, vocab = (1 << 22) - 256, 1032, 70
+    hidden = normal(rocm_device, rows, width)
+    weight = normal(rocm_device, vocab, width, seed=1, std=0.5 / width ** 0.5)
+    tokens = torch.arange(rows, device=rocm_device) % vocab
+    tokens[::5] = IGNORE
+    loss, lse = ho.linear_cross_entropy(hidden, weight, tokens)
+    grad = torch.ones(rows, device=rocm_device)
+    dh, dw = ho.linear_cross_entropy_bwd(grad, hidden, weight, tokens, lse)
+    assert torch.isfinite(dw).all() and torch.isfinite(loss).all()
+    for some in (slice(0, 500), slice(rows // 2, rows // 2 + 500), slice(rows - 500, rows)):
+        args = (hidden[some], weight, tokens[some])
+        for u, (v, tol) in zip((loss, lse), ref.linear_cross_entropy(*args)):
+            ref.close(u[some], v, tol, f"{some}")
+        v, tol = ref.linear_cross_entropy_bwd(grad[some], *args, lse[some])[0]
+        ref.close(dh[some], v, tol, f"{some} dhidden")
